@@ -1,7 +1,8 @@
 /*
  * moda_hip.h -- C ABI of libmoda_hip.so: fused sequence+depth attention
  * (MoDA) for AMD MI355X (gfx950), forward and backward, plus the depth-KV
- * cache reorganisation.
+ * cache reorganisation; rotary positions, a paged key/value cache and the
+ * attention of new tokens over it.
  *
  * Every pointer that names tensor data is a DEVICE pointer.  Strides are in
  * elements; the innermost (head-dim) stride is always 1.  For the matrix-core
@@ -333,6 +334,88 @@ int moda_hip_block_tail(const moda_hip_block_tail_args* args, void* stream);
  */
 int moda_hip_attend_block_tail(const moda_hip_desc* desc, const void* q, const void* k, const void* v, const void* kd, const void* vd,
                                const moda_hip_block_tail_args* args, void* stream);
+
+/*
+ * Rotary positions.  The first `dim` elements of a head's row (the rest are copied) turn in pairs -- (2i, 2i + 1) where
+ * interleaved, else (i, i + dim / 2) -- by the angle 2 pi * position * rates[i]:
+ *   y0 = amplitude * (x0 cos - x1 sin), y1 = amplitude * (x0 sin + x1 cos).
+ * rates: DEVICE array of dim / 2 values in 64 bits, in turns per position (product and fraction are taken in 64 bits).  dim
+ * even, at most the head dim.  inverse: by the opposite angle, which makes the gradient of x from that of y.
+ *
+ * moda_hip_rotary_rows: up to three tensors [B, T * rows_per_token, heads, D] -> the same shape, for one set of positions: row r
+ * is at position positions[b * position_stride + r / rows_per_token] (int32, or int64 where positions64; position_stride 0:
+ * shared by the batch; positions NULL: 0, 1, .. T - 1).  y may be x where their strides agree.  Any strides (the inner
+ * one 1); rows on 16-byte boundaries with dim a multiple of 16 (fp32: 8) move by 16 bytes, others element by element.
+ */
+typedef struct moda_hip_rotary {
+  const double* rates;
+  int64_t dim;
+  float amplitude;
+  int32_t interleaved, inverse, reserved;
+} moda_hip_rotary;
+typedef struct moda_hip_rotary_part {
+  const void* x;
+  void* y;
+  moda_hip_strides sx, sy;
+  int64_t rows_per_token, heads;
+} moda_hip_rotary_part;
+int moda_hip_rotary_rows(int32_t dtype, int64_t B, int64_t T, int64_t D, const moda_hip_rotary_part* parts, int32_t n_parts,
+                         const void* positions, int32_t positions64, int64_t position_stride, const moda_hip_rotary* rotary,
+                         void* stream);
+
+/*
+ * A paged key/value cache: k_pages [n_pages, page_size, H, D], v_pages [n_pages, page_size, H, Dv] with element strides
+ * {page, token in the page, head} and unit inner stride, rows on 16-byte boundaries (base and strides; MODA_HIP_EALIGN
+ * otherwise), page_size a power of two, n_pages * page_size and max_pages * page_size below 2^31.  DEVICE arrays: position p of
+ * sequence b lies in page table[b * table_stride + p / page_size], max_pages entries a sequence; past[b] tokens of it were there
+ * before the call; of its T new tokens new_lens[b] are real (NULL: T).  Counts are taken as at least 0 and past + new tokens as at
+ * most max_pages * page_size; a table entry outside [0, n_pages) names no page: its tokens are not stored and not seen.
+ *
+ * moda_hip_paged_append: new token i of sequence b -- k, v rows [B, T, H, *] -- to position past[b] + i.  With cu_seqlens
+ * (DEVICE, B + 1 offsets) the new tokens are packed, [1, total_tokens, H, *], sequence b owning cu[b] .. cu[b + 1] - 1; T is then not
+ * read and new_lens NULL; rows behind the last sequence go nowhere (q: as they are).  k (with `rotary`) is rotated by its position
+ * on the way, and so is q [B, T * G, Hq, D] (or NULL) to q_out, padded rows included.  kd, vd (or NULL): the token's k and
+ * v, as stored, also go to slot `slot` of the depth caches [B, T * L, H, *].  A page that is written belongs to one sequence: two tokens
+ * for the same place leave either of them, piece by piece.
+ * moda_hip_paged_attend: row (t, g) of sequence b attends over positions <= past[b] + t, that is, the new tokens are in the cache already,
+ * and over the L_valid first slots (0: all L) of its own token in kd, vd [B, T * L, H, *].  q, o: [B, T * G, H, *], rows t * G + g,
+ * lse [B, T * G, H] fp32 base 2; with `plain` [B, T, H * G, *], heads h * G + g, lse [B, T, H * G].  Rows that see nothing, padded
+ * ones among them, have o = 0 and lse = -inf.  cu_seqlens NULL.  All rows on 16-byte boundaries.
+ * Head dims up to 256, multiples of 8 (fp32: of 4); MODA_HIP_EUNSUPPORTED otherwise.
+ */
+typedef struct moda_hip_paged_cache {
+  int32_t struct_size, dtype;
+  int64_t B, T, H, D, Dv;
+  int64_t n_pages, page_size, max_pages;
+  void *k_pages, *v_pages;
+  moda_hip_strides k, v;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t *past, *new_lens, *cu_seqlens;
+  int64_t total_tokens;
+} moda_hip_paged_cache;
+typedef struct moda_hip_paged_append_args {
+  int32_t struct_size, reserved;
+  const void *k, *v, *q;
+  void *q_out, *kd, *vd;
+  moda_hip_strides sk, sv, sq, sq_out, skd, svd;
+  int64_t G, Hq, L, slot;
+} moda_hip_paged_append_args;
+int moda_hip_paged_append(const moda_hip_paged_cache* cache, const moda_hip_paged_append_args* args, const moda_hip_rotary* rotary,
+                          void* stream);
+typedef struct moda_hip_paged_attend_args {
+  int32_t struct_size, plain;
+  const void *q, *kd, *vd;
+  void* o;
+  float* lse;
+  moda_hip_strides sq, skd, svd, so;
+  int64_t G, L, L_valid;
+  float scale;
+  int32_t reserved;
+} moda_hip_paged_attend_args;
+size_t moda_hip_paged_attend_workspace_bytes(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_args* args);
+int moda_hip_paged_attend(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_args* args, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 /*
  * Which kernels a descriptor runs on: 1 = the matrix-core kernels (tensor rows must then be 16-byte aligned, see

@@ -26,6 +26,8 @@ from .ops import (  # noqa: F401
     set_fp32_compute,
 )
 from .depth_cache import build_depth_cache, stack_depth, DepthCache  # noqa: F401
+from .rotary import Rotary, RotaryFunction, apply_rotary  # noqa: F401
+from .paged import paged_append, paged_attn, paged_attn_fwd, paged_moda, paged_moda_fwd, PagedKVCache  # noqa: F401
 from .modules import DepthStream, MoDAAttention, MoDAStack  # noqa: F401
 
 __all__ = [
@@ -47,6 +49,14 @@ __all__ = [
     "build_depth_cache",
     "stack_depth",
     "DepthCache",
+    "Rotary",
+    "apply_rotary",
+    "paged_append",
+    "paged_attn",
+    "paged_attn_fwd",
+    "paged_moda",
+    "paged_moda_fwd",
+    "PagedKVCache",
     "DepthStream",
     "MoDAAttention",
     "MoDAStack",

@@ -36,6 +36,10 @@ EXPORTS = (
     "moda_hip_pack_weights_and_norm",
     "moda_hip_block_tail",
     "moda_hip_attend_block_tail",
+    "moda_hip_rotary_rows",
+    "moda_hip_paged_append",
+    "moda_hip_paged_attend_workspace_bytes",
+    "moda_hip_paged_attend",
     "moda_hip_uses_matrix_cores",
     "moda_hip_strerror",
     "moda_hip_version",

@@ -9,6 +9,7 @@
 #include "../../include/moda_hip.h"
 #include "geometry.h"
 #include "kargs.h"
+#include "paged.h"
 #include "tuning.h"
 
 namespace moda {
@@ -30,6 +31,8 @@ hipError_t launch_layer_norm(int dtype, int64_t rows, int64_t dim, const void* x
 hipError_t launch_pack_weights(const moda_hip_weight* w, int n, float* gelu_table, const moda_hip_norm_rows* norm, hipStream_t stream);
 hipError_t launch_block_tail(const moda_hip_block_tail_args* args, int compute_units, hipStream_t stream);
 hipError_t launch_attend_tail(const moda_hip_block_tail_args* args, const KArgs& attention, hipStream_t stream);
+hipError_t launch_rows(RowArgs& a, int dtype, bool vec, bool inter, bool paged, hipStream_t stream);
+hipError_t launch_paged_attend(const PagedAttendArgs& a, int dtype, hipStream_t stream);
 }  // namespace moda
 
 using moda::KArgs;
@@ -703,6 +706,212 @@ int moda_hip_attend_block_tail(const moda_hip_desc* d, const void* q, const void
   if ((rc = check_device(&a.compute_units))) return rc;
   if (!moda::attend_tail_takes(t->width, (int64_t)a.Hkv * a.Gf, a.Hkv, moda::block_tail_rows(t->rows, a.compute_units))) return MODA_HIP_EUNSUPPORTED;
   return moda::launch_attend_tail(t, a, (hipStream_t)stream) == hipSuccess ? MODA_HIP_OK : MODA_HIP_ELAUNCH;
+}
+
+namespace {
+bool known_dtype(int32_t dtype) { return dtype >= MODA_HIP_BF16 && dtype <= MODA_HIP_FP32; }
+void copy_strides(int64_t (&to)[3], const moda_hip_strides& s) {
+  to[0] = s.b;
+  to[1] = s.t;
+  to[2] = s.h;
+}
+bool is_power_of_two(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
+
+int check_rotary(const moda_hip_rotary* r, int64_t D) {
+  if (!r->rates || r->dim <= 0 || r->dim % 2 != 0 || r->dim > D) return MODA_HIP_EINVAL;
+  return (uintptr_t)r->rates % sizeof(double) == 0 ? MODA_HIP_OK : MODA_HIP_EALIGN;
+}
+void set_rotary(const moda_hip_rotary* r, moda::RowArgs& a) {
+  a.rates = r->rates;
+  a.rot = (int)r->dim;
+  a.amplitude = r->amplitude;
+  a.sign = r->inverse ? -1.f : 1.f;
+}
+
+// the geometry of a paged cache, and its arrays
+int fill_cache(const moda_hip_paged_cache* c, moda::PagedKV& to) {
+  if (!c || c->struct_size != (int32_t)sizeof(*c) || !known_dtype(c->dtype)) return MODA_HIP_EINVAL;
+  if (c->B < 0 || c->T < 0 || c->H <= 0 || c->D <= 0 || c->Dv <= 0 || c->n_pages <= 0 || c->max_pages <= 0 || c->page_size <= 0 ||
+      c->total_tokens < 0 || c->table_stride < 0 || (c->cu_seqlens && c->new_lens))
+    return MODA_HIP_EINVAL;
+  const int64_t step = c->dtype == MODA_HIP_FP32 ? 4 : 8, most = 1ll << 31;
+  if (c->D > 256 || c->Dv > 256 || c->D % step != 0 || c->Dv % step != 0 || !is_power_of_two(c->page_size)) return MODA_HIP_EUNSUPPORTED;
+  if (c->n_pages >= most || c->max_pages >= most || c->page_size >= most || c->n_pages * c->page_size >= most ||
+      c->max_pages * c->page_size >= most || c->B >= (1 << 20) || c->T >= (1 << 24) || c->H >= (1 << 16) || c->B * c->T >= most ||
+      c->total_tokens >= most)
+    return MODA_HIP_EUNSUPPORTED;
+  if (!c->k_pages || !c->v_pages || !c->table || !c->past) return MODA_HIP_EINVAL;
+  if (!aligned(c->k_pages, c->k, elem_size(c->dtype), true) || !aligned(c->v_pages, c->v, elem_size(c->dtype), true)) return MODA_HIP_EALIGN;
+  for (const void* p : {c->table, c->past, c->new_lens, c->cu_seqlens})
+    if ((uintptr_t)p % sizeof(int32_t) != 0) return MODA_HIP_EALIGN;
+  to.k = (char*)c->k_pages;
+  to.v = (char*)c->v_pages;
+  copy_strides(to.sk, c->k);
+  copy_strides(to.sv, c->v);
+  to.table = c->table;
+  to.table_stride = c->table_stride;
+  to.past = c->past;
+  to.new_lens = c->new_lens;
+  to.cu = c->cu_seqlens;
+  to.B = (int)c->B;
+  to.T = (int)c->T;
+  to.H = (int)c->H;
+  to.n_pages = (int)c->n_pages;
+  to.max_pages = (int)c->max_pages;
+  to.page_shift = __builtin_ctzll((unsigned long long)c->page_size);
+  return MODA_HIP_OK;
+}
+}  // namespace
+
+int moda_hip_rotary_rows(int32_t dtype, int64_t B, int64_t T, int64_t D, const moda_hip_rotary_part* parts, int32_t n_parts,
+                         const void* positions, int32_t positions64, int64_t position_stride, const moda_hip_rotary* rotary, void* stream) {
+  if (!known_dtype(dtype) || B < 0 || T < 0 || D <= 0 || !parts || n_parts < 1 || n_parts > 3 || !rotary || position_stride < 0)
+    return MODA_HIP_EINVAL;
+  int rc = check_rotary(rotary, D);
+  if (rc) return rc;
+  if (B >= (1ll << 31) || T >= (1ll << 31) || B * T >= (1ll << 31) || D > 4096) return MODA_HIP_EUNSUPPORTED;
+  const int es = elem_size(dtype), step = 16 / es;
+  bool vec = rotary->dim % (2 * step) == 0 && D % step == 0;
+  moda::RowArgs a = {};
+  for (int i = 0; i < n_parts; i++) {
+    const moda_hip_rotary_part& p = parts[i];
+    if (p.rows_per_token <= 0 || p.heads <= 0) return MODA_HIP_EINVAL;
+    if (p.rows_per_token >= (1 << 15) || p.heads >= (1 << 15) || p.rows_per_token * p.heads >= (1 << 15)) return MODA_HIP_EUNSUPPORTED;
+    if (B * T > 0 && (!p.x || !p.y)) return MODA_HIP_EINVAL;
+    if (!aligned(p.x, p.sx, es, false) || !aligned(p.y, p.sy, es, false)) return MODA_HIP_EALIGN;
+    vec = vec && aligned(p.x, p.sx, es, true) && aligned(p.y, p.sy, es, true);
+    moda::RowPart& to = a.part[i];
+    to.x = (const char*)p.x;
+    to.y = (char*)p.y;
+    copy_strides(to.sx, p.sx);
+    copy_strides(to.sy, p.sy);
+    to.rows = (int)p.rows_per_token;
+    to.heads = (int)p.heads;
+    to.dim = (int)D;
+    to.rotated = 1;
+  }
+  if ((uintptr_t)positions % (positions64 ? 8 : 4) != 0) return MODA_HIP_EALIGN;
+  if (B * T == 0) return MODA_HIP_OK;
+  if ((rc = check_device())) return rc;
+  a.n_parts = n_parts;
+  a.tokens = B * T;
+  a.T = (int)T;
+  a.positions = positions;
+  a.positions64 = positions64;
+  a.position_stride = position_stride;
+  set_rotary(rotary, a);
+  return moda::launch_rows(a, dtype, vec, rotary->interleaved, false, (hipStream_t)stream) == hipSuccess ? MODA_HIP_OK : MODA_HIP_ELAUNCH;
+}
+
+int moda_hip_paged_append(const moda_hip_paged_cache* cache, const moda_hip_paged_append_args* t, const moda_hip_rotary* rotary, void* stream) {
+  moda::RowArgs a = {};
+  int rc = fill_cache(cache, a.cache);
+  if (rc) return rc;
+  if (!t || t->struct_size != (int32_t)sizeof(*t) || (!t->kd) != (!t->vd) || (t->q && (t->G <= 0 || t->Hq <= 0))) return MODA_HIP_EINVAL;
+  if (t->kd && (t->L <= 0 || t->slot < 0 || t->slot >= t->L)) return MODA_HIP_EINVAL;
+  if (rotary && (rc = check_rotary(rotary, cache->D))) return rc;
+  a.tokens = cache->cu_seqlens ? cache->total_tokens : cache->B * cache->T;
+  if (a.tokens == 0) return MODA_HIP_OK;
+  if (!t->k || !t->v || (t->q && !t->q_out)) return MODA_HIP_EINVAL;
+  if ((t->kd && (t->L >= (1 << 20) || a.tokens * t->L >= (1ll << 40))) ||
+      (t->q && (t->G >= (1 << 15) || t->Hq >= (1 << 15) || t->G * t->Hq >= (1 << 15))) || cache->H >= (1 << 15))
+    return MODA_HIP_EUNSUPPORTED;
+  const int es = elem_size(cache->dtype), step = 16 / es;
+  bool vec = !rotary || rotary->dim % (2 * step) == 0;
+  const struct {
+    const void* p;
+    const moda_hip_strides& s;
+  } at[6] = {{t->k, t->sk}, {t->v, t->sv}, {t->q, t->sq}, {t->q ? t->q_out : nullptr, t->sq_out}, {t->kd, t->skd}, {t->vd, t->svd}};
+  for (const auto& x : at) {
+    if (!x.p) continue;
+    if (!aligned(x.p, x.s, es, false)) return MODA_HIP_EALIGN;
+    vec = vec && aligned(x.p, x.s, es, true);
+  }
+  if ((rc = check_device())) return rc;
+  a.n_parts = t->q ? 3 : 2;
+  for (int i = 0; i < a.n_parts; i++) {
+    moda::RowPart& to = a.part[i];
+    to.x = (const char*)(i == 0 ? t->k : i == 1 ? t->v : t->q);
+    copy_strides(to.sx, i == 0 ? t->sk : i == 1 ? t->sv : t->sq);
+    to.rows = i == 2 ? (int)t->G : 1;
+    to.heads = i == 2 ? (int)t->Hq : (int)cache->H;
+    to.dim = (int)(i == 1 ? cache->Dv : cache->D);
+    to.rotated = rotary && i != 1;
+    to.values = i == 1;
+    if (i == 2) {
+      to.y = (char*)t->q_out;
+      copy_strides(to.sy, t->sq_out);
+    } else {
+      to.depth = (char*)(i == 0 ? t->kd : t->vd);
+      copy_strides(to.sd, i == 0 ? t->skd : t->svd);
+    }
+  }
+  a.T = (int)(cache->cu_seqlens ? cache->total_tokens : cache->T);
+  a.L = (int)t->L;
+  a.slot = (int)t->slot;
+  if (rotary) set_rotary(rotary, a);
+  return moda::launch_rows(a, cache->dtype, vec, rotary && rotary->interleaved, true, (hipStream_t)stream) == hipSuccess ? MODA_HIP_OK
+                                                                                                                         : MODA_HIP_ELAUNCH;
+}
+
+namespace {
+int fill_attend(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_args* t, moda::PagedAttendArgs& a) {
+  int rc = fill_cache(cache, a.cache);
+  if (rc) return rc;
+  if (!t || t->struct_size != (int32_t)sizeof(*t) || cache->cu_seqlens || t->G <= 0 || t->L < 0 || t->L_valid < 0 || t->L_valid > t->L ||
+      (t->plain && t->L > 0))
+    return MODA_HIP_EINVAL;
+  if (t->G >= (1 << 15) || cache->T * t->G >= (1 << 24) || t->L >= (1 << 20) || cache->T * t->L >= (1 << 30) ||
+      cache->B * cache->T * t->G * cache->H >= (1ll << 31))
+    return MODA_HIP_EUNSUPPORTED;
+  a.G = (int)t->G;
+  a.D = (int)cache->D;
+  a.Dv = (int)cache->Dv;
+  a.L = (int)t->L;
+  a.Lv = (int)(t->L_valid > 0 ? t->L_valid : t->L);
+  a.scale = (float)(t->scale * 1.4426950408889634);
+  a.q = (const char*)t->q;
+  a.kd = (const char*)t->kd;
+  a.vd = (const char*)t->vd;
+  a.o = (char*)t->o;
+  a.lse = t->lse;
+  // {batch, token, row of the group, head}: folded rows are t * G + g, plain heads h * G + g
+  const auto rows = [&](int64_t(&to)[4], const moda_hip_strides& s) {
+    to[0] = s.b;
+    to[1] = t->plain ? s.t : s.t * t->G;
+    to[2] = t->plain ? s.h : s.t;
+    to[3] = t->plain ? s.h * t->G : s.h;
+  };
+  rows(a.sq, t->sq);
+  rows(a.so, t->so);
+  const int64_t heads = cache->H * (t->plain ? t->G : 1), n = cache->T * (t->plain ? 1 : t->G);
+  rows(a.slse, moda_hip_strides{n * heads, heads, 1});
+  copy_strides(a.skd, t->skd);
+  copy_strides(a.svd, t->svd);
+  return MODA_HIP_OK;
+}
+}  // namespace
+
+size_t moda_hip_paged_attend_workspace_bytes(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_args* t) {
+  moda::PagedAttendArgs a = {};
+  return fill_attend(cache, t, a) ? 0 : 4;
+}
+
+int moda_hip_paged_attend(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_args* t, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  moda::PagedAttendArgs a = {};
+  int rc = fill_attend(cache, t, a);
+  if (rc) return rc;
+  if (cache->B * cache->T == 0) return MODA_HIP_OK;
+  if (!t->q || !t->o || !t->lse || (t->L > 0 && (!t->kd || !t->vd))) return MODA_HIP_EINVAL;
+  const int es = elem_size(cache->dtype);
+  if (!aligned(t->q, t->sq, es, true) || !aligned(t->o, t->so, es, true) || (uintptr_t)t->lse % 4 != 0) return MODA_HIP_EALIGN;
+  if (t->L > 0 && (!aligned(t->kd, t->skd, es, true) || !aligned(t->vd, t->svd, es, true))) return MODA_HIP_EALIGN;
+  if (!workspace || workspace_bytes < moda_hip_paged_attend_workspace_bytes(cache, t)) return MODA_HIP_EWORKSPACE;
+  if ((uintptr_t)workspace % 16 != 0) return MODA_HIP_EALIGN;
+  if ((rc = check_device())) return rc;
+  a.work = (float*)workspace;
+  return moda::launch_paged_attend(a, cache->dtype, (hipStream_t)stream) == hipSuccess ? MODA_HIP_OK : MODA_HIP_ELAUNCH;
 }
 
 int moda_hip_uses_matrix_cores(const moda_hip_desc* d) {

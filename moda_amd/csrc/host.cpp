@@ -900,6 +900,305 @@ std::optional<Tensor> stack_forward(const Tensor& x_in, const std::vector<Block>
   return x;
 }
 
+// ------------------------------------------------------------------------------------------------------------------
+// rotary positions (moda_amd/rotary.py)
+// ------------------------------------------------------------------------------------------------------------------
+
+// What a rotation is besides its tensors.
+struct Rotation : c10::intrusive_ptr_target {
+  int64_t dim = 0, G = 1;
+  double amplitude = 1.0;
+  bool interleaved = false, inverse = false;
+};
+
+void check_rates(const Tensor& rates, int64_t dim, const Tensor& x) {
+  CONTRACT(rates.dim() == 1 && rates.scalar_type() == at::kDouble && rates.is_contiguous() && dim > 0 && rates.size(0) * 2 == dim,
+           "the rates of a rotation are a vector of dim / 2 values in 64 bits");
+  CONTRACT(rates.device() == x.device(), "rates and tensors must be on one device");
+}
+
+// one launch for both tensors (either may be undefined): q [B, T * G, Hq, D], k [B, T, H, D]
+std::pair<Tensor, Tensor> rotate(const Rotation& r, const Tensor& rates, const Tensor& q_in, const Tensor& k_in, const Tensor& positions_in) {
+  const Tensor& any = q_in.defined() ? q_in : k_in;
+  CONTRACT(any.defined() && any.dim() == 4 && (!k_in.defined() || k_in.dim() == 4), "q, k must be [B, rows, heads, D]");
+  CONTRACT(r.G >= 1, "moda_group_num must be positive");
+  const int64_t B = any.size(0), T = k_in.defined() ? k_in.size(1) : q_in.size(1) / r.G, D = any.size(3);
+  CONTRACT(!q_in.defined() || q_in.size(1) == T * r.G, "q holds ", q_in.defined() ? q_in.size(1) : 0, " rows, expected T*moda_group_num = ", T * r.G);
+  CONTRACT(!q_in.defined() || !k_in.defined() || (k_in.size(0) == B && k_in.size(3) == D), "q and k must share batch size and head dim");
+  CONTRACT(r.dim <= D, "the rotation turns ", r.dim, " elements of a head, which has ", D);
+  check_device(any);
+  same_dtype({&q_in, &k_in});
+  CONTRACT(!q_in.defined() || !k_in.defined() || q_in.device() == k_in.device(), "q and k must be on one device");
+  check_rates(rates, r.dim, any);
+  const int dt = dtype_code(any);
+  Tensor positions = positions_in;
+  if (positions.defined()) {
+    CONTRACT(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, "positions must be int32 or int64");
+    CONTRACT(positions.device() == any.device(), "positions must be on the tensors' device");
+    CONTRACT(has_shape(positions, {T}) || has_shape(positions, {B, T}), "positions must be [T] or [B, T] = ", shape_text({B, T}));
+    if (positions.size(-1) > 1 && positions.stride(-1) != 1) positions = positions.contiguous();
+  }
+  std::array<Tensor, 2> in = {q_in, k_in}, out;
+  moda_hip_rotary_part parts[2];
+  int n = 0;
+  for (int i = 0; i < 2; i++) {
+    if (!in[i].defined()) continue;
+    in[i] = usable(in[i], false);
+    out[i] = at::empty(in[i].sizes(), in[i].options());
+    if (in[i].numel() == 0) continue;
+    parts[n++] = {in_ptr(in[i]), out_ptr(out[i]), strides_of(in[i]), strides_of(out[i]), i == 0 ? r.G : 1, in[i].size(2)};
+  }
+  if (n == 0) return {out[0], out[1]};
+  const moda_hip_rotary how = {rates.const_data_ptr<double>(), r.dim, (float)r.amplitude, r.interleaved, r.inverse, 0};
+  c10::OptionalDeviceGuard guard(any.device());
+  check_rc(moda_hip_rotary_rows(dt, B, T, D, parts, n, in_ptr(positions), positions.defined() && positions.scalar_type() == at::kLong,
+                                positions.defined() && positions.dim() == 2 ? positions.stride(0) : 0, &how, stream_of(any)),
+           "moda_hip_rotary_rows");
+  return {out[0], out[1]};
+}
+
+// The gradient of a rotation is the rotation by the opposite angle: the node's backward is the node itself.
+struct Rotate : torch::autograd::Function<Rotate> {
+  static variable_list forward(AutogradContext* ctx, const OptTensor& q, const OptTensor& k, const Tensor& rates, const OptTensor& positions,
+                               const c10::intrusive_ptr<Rotation>& how) {
+    auto r = rotate(*how, rates, value(q), value(k), value(positions));
+    ctx->save_for_backward({rates, value(positions)});
+    ctx->saved_data["state"] = owning(how);
+    ctx->saved_data["q"] = q.has_value();
+    ctx->saved_data["k"] = k.has_value();
+    ctx->set_materialize_grads(false);
+    return outputs(q.has_value(), k.has_value(), r.first, r.second);
+  }
+  // a node's outputs are defined: those of the inputs there are, in their order
+  static variable_list outputs(bool q, bool k, const Tensor& first, const Tensor& second) {
+    variable_list r;
+    if (q) r.push_back(first);
+    if (k) r.push_back(second);
+    return r;
+  }
+  static std::pair<Tensor, Tensor> pair(bool q, bool k, const variable_list& r) { return {q ? r[0] : Tensor(), k ? r[q] : Tensor()}; }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return in_engine([&] {
+      const variable_list s = ctx->get_saved_variables();
+      auto back = c10::make_intrusive<Rotation>(*owned<Rotation>(ctx));
+      back->inverse = !back->inverse;
+      const auto g = pair(ctx->saved_data["q"].toBool(), ctx->saved_data["k"].toBool(), grads);
+      if (!g.first.defined() && !g.second.defined()) return variable_list(5);
+      const auto r = pair(g.first.defined(), g.second.defined(), apply(optional(g.first), optional(g.second), s[0], optional(s[1]), back));
+      return variable_list{r.first, r.second, Tensor(), Tensor(), Tensor()};
+    });
+  }
+};
+
+std::pair<OptTensor, OptTensor> apply_rotary(const OptTensor& q, const OptTensor& k, const Tensor& rates, int64_t dim, double amplitude,
+                                             bool interleaved, const OptTensor& positions, int64_t G, bool inverse, bool differentiable) {
+  py::gil_scoped_release nogil;
+  auto how = c10::make_intrusive<Rotation>();
+  how->dim = dim;
+  how->G = G;
+  how->amplitude = amplitude;
+  how->interleaved = interleaved;
+  how->inverse = inverse;
+  if (!differentiable) {
+    const auto r = rotate(*how, rates, value(q), value(k), value(positions));
+    return {optional(r.first), optional(r.second)};
+  }
+  const auto r = Rotate::pair(q.has_value(), k.has_value(), Rotate::apply(q, k, rates, positions, how));
+  return {optional(r.first), optional(r.second)};
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// paged key/value cache (moda_amd/paged.py)
+// ------------------------------------------------------------------------------------------------------------------
+
+void no_gradients(std::initializer_list<const Tensor*> xs, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* x : xs)
+    CONTRACT(!x->defined() || !x->requires_grad(), what, " has no backward pass: call it under torch.no_grad()");
+}
+
+const int32_t* counts(const Tensor& x, const char* name, std::initializer_list<int64_t> shape, const Tensor& cache) {
+  CONTRACT(x.scalar_type() == at::kInt && x.device() == cache.device() && has_shape(x, shape) && x.is_contiguous(), name,
+           " must be a contiguous int32 tensor ", shape_text(shape), " on the cache's device");
+  return x.const_data_ptr<int32_t>();
+}
+
+// Pages cannot be copied into another layout: what the kernels do not take is refused.
+moda_hip_strides page_strides(const Tensor& x, const char* name, bool written) {
+  const int64_t m = 16 / x.element_size();
+  bool ok = x.stride(3) == 1 && (uintptr_t)x.const_data_ptr() % 16 == 0;
+  for (int i = 0; i < 3; i++) ok = ok && x.stride(i) >= 0 && x.stride(i) % m == 0 && !(written && x.stride(i) == 0 && x.size(i) > 1);
+  CONTRACT(ok, name, " must have unit inner stride, rows on 16-byte boundaries", written ? " and no two places in one" : "");
+  return {x.stride(0), x.stride(1), x.stride(2)};
+}
+
+// `B`, `T`: sequences and new tokens of the call
+moda_hip_paged_cache describe_cache(const Tensor& ck, const Tensor& cv, const Tensor& table, const Tensor& past, const Tensor& new_lens,
+                                    int64_t B, int64_t T, bool written) {
+  CONTRACT(ck.dim() == 4 && cv.dim() == 4, "cache_k, cache_v must be [n_pages, page_size, H, D]");
+  CONTRACT(ck.size(0) == cv.size(0) && ck.size(1) == cv.size(1) && ck.size(2) == cv.size(2), "cache_k and cache_v must agree in pages, page size and heads");
+  check_device(ck);
+  same_dtype({&ck, &cv});
+  CONTRACT(ck.device() == cv.device(), "cache_k and cache_v must be on one device");
+  const int64_t P = ck.size(1);
+  CONTRACT(P > 0 && (P & (P - 1)) == 0, "the page size must be a power of two, got ", P);
+  CONTRACT(ck.size(0) > 0, "the cache has no pages");
+  CONTRACT(table.dim() == 2 && table.scalar_type() == at::kInt && table.device() == ck.device() && table.size(0) == B && table.size(1) > 0 &&
+               (table.stride(1) == 1 || table.size(1) == 1) && table.stride(0) >= 0,
+           "page_table must be an int32 tensor [", B, ", pages of a sequence] with unit inner stride on the cache's device");
+  moda_hip_paged_cache c = {};
+  c.struct_size = sizeof(c);
+  c.dtype = dtype_code(ck);
+  c.B = B;
+  c.T = T;
+  c.H = ck.size(2);
+  c.D = ck.size(3);
+  c.Dv = cv.size(3);
+  c.n_pages = ck.size(0);
+  c.page_size = P;
+  c.max_pages = table.size(1);
+  c.k = page_strides(ck, "cache_k", written);
+  c.v = page_strides(cv, "cache_v", written);
+  c.k_pages = const_cast<void*>(in_ptr(ck));
+  c.v_pages = const_cast<void*>(in_ptr(cv));
+  c.table = table.const_data_ptr<int32_t>();
+  c.table_stride = table.stride(0);
+  c.past = counts(past, "past", {B}, ck);
+  if (new_lens.defined()) c.new_lens = counts(new_lens, "new_lens", {B}, ck);
+  return c;
+}
+
+void same_place(std::initializer_list<const Tensor*> xs, const Tensor& cache) {
+  for (const Tensor* x : xs)
+    if (x->defined()) CONTRACT(x->scalar_type() == cache.scalar_type() && x->device() == cache.device(), "tensors and cache must share dtype and device");
+}
+
+OptTensor paged_append(const Tensor& k_in, const Tensor& v_in, const Tensor& ck, const Tensor& cv, const Tensor& table, const Tensor& past,
+                       const OptTensor& new_lens, const OptTensor& cu_seqlens, const OptTensor& q_opt, const OptTensor& rates, int64_t dim,
+                       double amplitude, bool interleaved, int64_t G, const OptTensor& cached_k, const OptTensor& cached_v, int64_t slot) {
+  py::gil_scoped_release nogil;
+  const Tensor q_in = value(q_opt), kd = value(cached_k), vd = value(cached_v), cu = value(cu_seqlens);
+  CONTRACT(k_in.dim() == 4 && v_in.dim() == 4, "k, v must be [B, T, H, D]");
+  const int64_t tb = k_in.size(0), T = k_in.size(1), H = k_in.size(2), D = k_in.size(3), Dv = v_in.size(3);
+  CONTRACT(has_shape(v_in, {tb, T, H, Dv}), "k and v must agree in batch size, tokens and heads");
+  no_gradients({&k_in, &v_in, &q_in, &kd, &vd}, "paged_append");
+  CONTRACT(!cu.defined() || (tb == 1 && cu.dim() == 1 && cu.size(0) >= 1), "with cu_seqlens all new tokens share one packed axis: batch size must be 1, offsets [n+1]");
+  CONTRACT(!cu.defined() || !new_lens.has_value(), "new tokens are counted by cu_seqlens or by new_lens, not both");
+  const int64_t B = cu.defined() ? cu.size(0) - 1 : tb;
+  moda_hip_paged_cache c = describe_cache(ck, cv, table, past, value(new_lens), B, cu.defined() ? 0 : T, true);
+  CONTRACT(H == c.H && D == c.D && Dv == c.Dv, "k, v must have the cache's heads and head dims");
+  same_place({&k_in, &v_in, &q_in, &kd, &vd}, ck);
+  if (cu.defined()) {
+    c.cu_seqlens = counts(cu, "cu_seqlens", {B + 1}, ck);
+    c.total_tokens = T;
+  }
+  CONTRACT(kd.defined() == vd.defined(), "depth k and v must be given together");
+  moda_hip_paged_append_args a = {};
+  a.struct_size = sizeof(a);
+  if (kd.defined()) {
+    CONTRACT(kd.dim() == 4 && T > 0 && kd.size(1) % T == 0 && kd.size(1) > 0, "depth k/v must be [B, T*L, H, D]");
+    a.L = kd.size(1) / T;
+    a.slot = slot;
+    CONTRACT(has_shape(kd, {tb, T * a.L, H, D}) && has_shape(vd, {tb, T * a.L, H, Dv}), "depth k/v must be [B, T*L, H, D]");
+    CONTRACT(slot >= 0 && slot < a.L, "slots out of range");
+    for (const Tensor* x : {&kd, &vd})
+      CONTRACT(x->stride(3) == 1 && x->is_non_overlapping_and_dense(), "the depth caches must be dense with unit inner stride");
+    a.kd = out_ptr(kd);
+    a.vd = out_ptr(vd);
+    a.skd = strides_of(kd);
+    a.svd = strides_of(vd);
+  }
+  Tensor q, q_out;
+  if (q_in.defined()) {
+    CONTRACT(rates.has_value(), "q is rotated, and there is no rotation: pass rotary, or keep q");
+    CONTRACT(q_in.dim() == 4 && q_in.size(0) == tb && q_in.size(1) == T * G && q_in.size(3) == D, "q must be [B, T*moda_group_num, heads, D]");
+    q = usable(q_in, false);
+    q_out = at::empty(q.sizes(), q.options());
+    a.q = in_ptr(q);
+    a.q_out = out_ptr(q_out);
+    a.sq = strides_of(q);
+    a.sq_out = strides_of(q_out);
+    a.G = G;
+    a.Hq = q.size(2);
+  }
+  moda_hip_rotary how = {};
+  if (rates.has_value()) {
+    check_rates(*rates, dim, ck);
+    CONTRACT(dim <= D, "the rotation turns ", dim, " elements of a head, which has ", D);
+    how = {rates->const_data_ptr<double>(), dim, (float)amplitude, interleaved, 0, 0};
+  }
+  if (tb * T == 0) return optional(q_out);
+  const Tensor k = usable(k_in, false), v = usable(v_in, false);
+  a.k = in_ptr(k);
+  a.v = in_ptr(v);
+  a.sk = strides_of(k);
+  a.sv = strides_of(v);
+  c10::OptionalDeviceGuard guard(ck.device());
+  check_rc(moda_hip_paged_append(&c, &a, rates.has_value() ? &how : nullptr, stream_of(ck)), "moda_hip_paged_append");
+  // written outside of autograd's sight: what keeps a view or a saved version of a cache has to know
+  for (const Tensor* x : {&ck, &cv, &kd, &vd})
+    if (x->defined() && !x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+  return optional(q_out);
+}
+
+std::pair<Tensor, Tensor> paged_attend(const Tensor& q_in, const Tensor& ck, const Tensor& cv, const Tensor& table, const Tensor& past,
+                                       const OptTensor& new_lens, std::optional<double> scale, const OptTensor& cached_k,
+                                       const OptTensor& cached_v, std::optional<int64_t> depth_valid, int64_t G, bool plain) {
+  py::gil_scoped_release nogil;
+  Tensor kd = value(cached_k), vd = value(cached_v);
+  if (!kd.defined() || !vd.defined()) kd = vd = Tensor();  // one without the other counts as none
+  CONTRACT(q_in.dim() == 4, "q must be [B, rows, heads, D]");
+  no_gradients({&q_in, &ck, &cv, &kd, &vd}, "attention over a paged cache");
+  CONTRACT(ck.dim() == 4, "cache_k, cache_v must be [n_pages, page_size, H, D]");
+  const int64_t B = q_in.size(0), H = ck.size(2);
+  if (plain) {
+    CONTRACT(H > 0 && q_in.size(2) > 0 && q_in.size(2) % H == 0, "plain GQA: q must be [B, T, H*G, D]");
+    G = q_in.size(2) / H;
+  }
+  CONTRACT(G > 0, "moda_group_num must be positive");
+  CONTRACT(plain || q_in.size(2) == H, "folded layout: q and the cache must have the same number of heads");
+  CONTRACT(plain || q_in.size(1) % G == 0, "query rows must be a multiple of moda_group_num");
+  const int64_t T = plain ? q_in.size(1) : q_in.size(1) / G;
+  const moda_hip_paged_cache c = describe_cache(ck, cv, table, past, value(new_lens), B, T, false);
+  CONTRACT(q_in.size(3) == c.D, "q and the cache must share the head dim");
+  same_place({&q_in, &kd, &vd}, ck);
+  moda_hip_paged_attend_args a = {};
+  a.struct_size = sizeof(a);
+  a.plain = plain;
+  a.G = G;
+  a.scale = (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)c.D));
+  Tensor o = at::empty({B, q_in.size(1), q_in.size(2), c.Dv}, q_in.options());
+  Tensor lse = at::empty({B, q_in.size(1), q_in.size(2)}, q_in.options().dtype(at::kFloat));
+  if (o.numel() == 0) return {o, lse};
+  if (kd.defined()) {
+    CONTRACT(kd.dim() == 4 && kd.size(1) % T == 0, "depth rows must be T * L");
+    a.L = kd.size(1) / T;
+    CONTRACT(has_shape(kd, {B, T * a.L, H, c.D}) && has_shape(vd, {B, T * a.L, H, c.Dv}), "depth k/v must be [B, T*L, H, D]");
+    if (a.L > 0 && depth_valid.has_value()) {
+      CONTRACT(*depth_valid >= 1 && *depth_valid <= a.L, "depth_valid must be in [1, ", a.L, "], got ", *depth_valid);
+      a.L_valid = *depth_valid;
+    }
+  }
+  const Tensor q = usable(q_in, true);
+  if (a.L > 0) {
+    kd = usable(kd, true);
+    vd = usable(vd, true);
+    a.kd = in_ptr(kd);
+    a.vd = in_ptr(vd);
+    a.skd = strides_of(kd);
+    a.svd = strides_of(vd);
+  }
+  a.q = in_ptr(q);
+  a.o = out_ptr(o);
+  a.lse = (float*)out_ptr(lse);
+  a.sq = strides_of(q);
+  a.so = strides_of(o);
+  c10::OptionalDeviceGuard guard(ck.device());
+  Tensor ws = at::empty({std::max<int64_t>((int64_t)moda_hip_paged_attend_workspace_bytes(&c, &a), 4)}, q.options().dtype(at::kByte));
+  check_rc(moda_hip_paged_attend(&c, &a, out_ptr(ws), (size_t)ws.nbytes(), stream_of(ck)), "moda_hip_paged_attend");
+  return {o, lse};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -921,6 +1220,9 @@ PYBIND11_MODULE(_host, m) {
       .def_readonly("host", &Packed::host);
   py::class_<TrainStream>(m, "TrainStream").def(py::init<int64_t>()).def("attend", &TrainStream::attend).def("push", &TrainStream::push);
   m.def("depth_push", &depth_push);
+  m.def("apply_rotary", &apply_rotary);
+  m.def("paged_append", &paged_append);
+  m.def("paged_attend", &paged_attend);
   m.def("stack_forward", [](const Tensor& x, const std::vector<std::vector<OptTensor>>& params, const std::vector<std::array<double, 2>>& eps,
                             int64_t heads, int64_t kv_heads, bool is_causal, int64_t chunk_tokens, bool post_norm) {
     std::vector<Block> blocks;

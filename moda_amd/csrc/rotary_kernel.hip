@@ -1,0 +1,191 @@
+// Rows of query and key heads rotated by their token's position, and the same on the way into a paged cache.
+//
+// Pair i of a row at position p turns by the angle 2 pi frac(p * rate_i): product and fraction in 64 bits (a position of
+// 10^6 leaves 32-bit angles with four correct digits), sine and cosine of the rest in 32 bits, once for all heads that
+// a thread has of its token.  y0 = A (x0 cos - x1 sin), y1 = A (x0 sin + x1 cos); the gradient of x is the rotation of
+// the gradient of y by the opposite angle, so the backward pass is this kernel with the other sign.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "paged.h"
+#include "../../include/moda_hip.h"
+
+namespace moda {
+
+struct Bf16 {
+  typedef uint16_t bits;
+  __device__ static float widen(bits x) { return __uint_as_float((uint32_t)x << 16); }
+  __device__ static bits narrow(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+};
+struct Fp16 {
+  typedef uint16_t bits;
+  __device__ static float widen(bits x) { return (float)__builtin_bit_cast(_Float16, x); }
+  __device__ static bits narrow(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+};
+struct Fp32 {
+  typedef uint32_t bits;
+  __device__ static float widen(bits x) { return __uint_as_float(x); }
+  __device__ static bits narrow(float x) { return __float_as_uint(x); }
+};
+
+// sequence of token n of a packed axis (B: behind the last one)
+__device__ __forceinline__ int sequence_of(const int32_t* cu, int B, int64_t n) {
+  int lo = 0, hi = B;  // cu[lo] <= n < cu[hi], hi = B standing for any
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid + 1] <= n)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// A thread has chunk c of VEC pairs (or, past the rotated elements, of VEC elements) of every `groups`-th (row, head) item of
+// one token.  VEC elements are 16 bytes, or one where rows do not lie on that grid.
+template <typename E, int VEC, bool INTER, bool PAGED>
+__global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
+  typedef typename E::bits bits;
+  typedef bits vec __attribute__((ext_vector_type(VEC)));
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, unit = id >> a.lane_shift;
+  const int c0 = (int)(id & ((1 << a.lane_shift) - 1));
+  const int64_t n = unit / a.groups;
+  if (n >= a.tokens) return;
+  const int group = (int)(unit - n * a.groups);
+
+  int64_t tb = n / a.T, tt = n - tb * a.T;  // batch and token of the tensors
+  int64_t pos = tt;
+  int page = -1, b = (int)tb;
+  bool turn = true, stored = false;  // whether q, k are rotated; whether the token goes to the cache
+  if (PAGED) {
+    if (a.cache.cu) {
+      b = sequence_of(a.cache.cu, a.cache.B, n);
+      turn = b < a.cache.B;
+      pos = turn ? n - a.cache.cu[b] : 0;
+      stored = turn;
+    } else {
+      stored = tt < a.cache.new_of(b);
+    }
+    if (turn) pos += a.cache.past_of(b);
+    if (stored && pos < a.cache.capacity()) page = a.cache.page_of(b, (int)pos);
+  } else if (a.positions) {
+    const int64_t at = tb * a.position_stride + tt;
+    pos = a.positions64 ? ((const int64_t*)a.positions)[at] : ((const int32_t*)a.positions)[at];
+  }
+
+  const int n_rot = a.rot / (2 * VEC);
+  float cs[VEC], sn[VEC];
+  if (c0 < n_rot) {
+#pragma unroll
+    for (int i = 0; i < VEC; i++) {
+      const double t = (double)pos * a.rates[c0 * VEC + i];
+      float s, c;
+      sincospif(2.f * (float)(t - rint(t)), &s, &c);
+      cs[i] = turn ? c * a.amplitude : 1.f;
+      sn[i] = turn ? s * a.amplitude * a.sign : 0.f;
+    }
+  }
+
+  int first = 0;
+  for (int p = 0; p < a.n_parts; p++) {
+    const RowPart& part = a.part[p];
+    const int count = part.rows * part.heads, rot = part.rotated ? n_rot : 0, rot_elems = rot * 2 * VEC;
+    const int chunks = rot + (part.dim - rot_elems) / VEC;
+    const bits* x = (const bits*)part.x + tb * part.sx[0] + tt * part.rows * part.sx[1];
+    bits *y = nullptr, *depth = nullptr;
+    if (part.y) {
+      y = (bits*)part.y + tb * part.sy[0] + tt * part.rows * part.sy[1];
+    } else if (PAGED) {
+      if (page >= 0)
+        y = part.values ? (bits*)a.cache.v + a.cache.offset(a.cache.sv, page, (int)pos, 0)
+                        : (bits*)a.cache.k + a.cache.offset(a.cache.sk, page, (int)pos, 0);
+      if (part.depth && stored) depth = (bits*)part.depth + tb * part.sd[0] + (tt * a.L + a.slot) * part.sd[1];
+    }
+    const int64_t y_head = part.y ? part.sy[2] : part.values ? a.cache.sv[2] : a.cache.sk[2];
+    // the items of all parts are dealt out in turn: a part goes on where the one before it stopped
+    int item = group - first % a.groups;
+    if (item < 0) item += a.groups;
+    first += count;
+    if (!y && !depth) continue;
+    for (; item < count; item += a.groups) {
+      const int r = part.heads_magic ? (int)__umulhi((unsigned)item, part.heads_magic) : item, h = item - r * part.heads;
+      const bits* xr = x + r * part.sx[1] + h * part.sx[2];
+      bits* yr = y + (part.y ? r * part.sy[1] : 0) + h * y_head;
+      bits* dr = depth + h * part.sd[2];
+      for (int c = c0; c < chunks; c += 1 << a.lane_shift) {
+        if (c < rot) {
+          const int e0 = INTER ? 2 * c * VEC : c * VEC, e1 = INTER ? e0 + VEC : a.rot / 2 + e0;
+          const vec u = *(const vec*)(xr + e0), v = *(const vec*)(xr + e1);
+          vec yu, yv;
+#pragma unroll
+          for (int i = 0; i < VEC; i++) {
+            // interleaved: pair i is elements 2i, 2i + 1 of the two vectors together
+            const float x0 = E::widen(!INTER ? u[i] : 2 * i < VEC ? u[2 * i % VEC] : v[2 * i % VEC]);
+            const float x1 = E::widen(!INTER ? v[i] : 2 * i + 1 < VEC ? u[(2 * i + 1) % VEC] : v[(2 * i + 1) % VEC]);
+            const bits y0 = E::narrow(x0 * cs[i] - x1 * sn[i]), y1 = E::narrow(x0 * sn[i] + x1 * cs[i]);
+            if (!INTER) {
+              yu[i] = y0;
+              yv[i] = y1;
+            } else {
+              (2 * i < VEC ? yu : yv)[2 * i % VEC] = y0;
+              (2 * i + 1 < VEC ? yu : yv)[(2 * i + 1) % VEC] = y1;
+            }
+          }
+          if (y) {
+            *(vec*)(yr + e0) = yu;
+            *(vec*)(yr + e1) = yv;
+          }
+          if (PAGED && depth) {
+            *(vec*)(dr + e0) = yu;
+            *(vec*)(dr + e1) = yv;
+          }
+        } else {
+          const int e = rot_elems + (c - rot) * VEC;
+          const vec u = *(const vec*)(xr + e);
+          if (y) *(vec*)(yr + e) = u;
+          if (PAGED && depth) *(vec*)(dr + e) = u;
+        }
+      }
+    }
+  }
+}
+
+template <typename E, int VEC, bool PAGED>
+static void launch_rows_as(const RowArgs& a, bool inter, int64_t blocks, hipStream_t stream) {
+  if (inter)
+    rows_kernel<E, VEC, true, PAGED><<<(unsigned)blocks, 256, 0, stream>>>(a);
+  else
+    rows_kernel<E, VEC, false, PAGED><<<(unsigned)blocks, 256, 0, stream>>>(a);
+}
+
+// `vec`: all rows lie on the 16-byte grid and the rotated elements are whole vectors of pairs
+hipError_t launch_rows(RowArgs& a, int dtype, bool vec, bool inter, bool paged, hipStream_t stream) {
+  const int v = !vec ? 1 : dtype == MODA_HIP_FP32 ? 4 : 8;
+  int most = 1;
+  a.items = 0;
+  for (int p = 0; p < a.n_parts; p++) {
+    RowPart& part = a.part[p];
+    const int rot = part.rotated ? a.rot / (2 * v) : 0, chunks = rot + (part.dim - 2 * rot * v) / v;
+    most = max(most, part.rotated ? chunks : (chunks + 1) / 2);  // copies: two chunks a thread, as many bytes as a rotated one
+    part.heads_magic = part.heads == 1 ? 0 : (unsigned)((1ull << 32) / part.heads) + 1;
+    a.items += part.rows * part.heads;
+  }
+  a.lane_shift = 0;
+  while ((1 << a.lane_shift) < most && a.lane_shift < 8) a.lane_shift++;
+  // one item a thread until the machine is full (256 compute units of 2048 threads), more after that: the angles are then shared
+  const int64_t full = 256 * 2048, lanes = a.tokens << a.lane_shift;
+  a.groups = (int)max((int64_t)1, min((int64_t)a.items, full / max(lanes, (int64_t)1)));
+  const int64_t blocks = (lanes * a.groups + 255) / 256;
+  if (blocks >= (1ll << 31)) return hipErrorInvalidValue;
+#define MODA_ROWS(E, V) paged ? launch_rows_as<E, V, true>(a, inter, blocks, stream) : launch_rows_as<E, V, false>(a, inter, blocks, stream)
+  if (dtype == MODA_HIP_FP32)
+    vec ? (MODA_ROWS(Fp32, 4)) : (MODA_ROWS(Fp32, 1));
+  else if (dtype == MODA_HIP_FP16)
+    vec ? (MODA_ROWS(Fp16, 8)) : (MODA_ROWS(Fp16, 1));
+  else
+    vec ? (MODA_ROWS(Bf16, 8)) : (MODA_ROWS(Bf16, 1));
+#undef MODA_ROWS
+  return hipGetLastError();
+}
+
+}  // namespace moda
