@@ -32,6 +32,7 @@ hipError_t launch_pack_weights(const moda_hip_weight* w, int n, float* gelu_tabl
 hipError_t launch_block_tail(const moda_hip_block_tail_args* args, int compute_units, hipStream_t stream);
 hipError_t launch_attend_tail(const moda_hip_block_tail_args* args, const KArgs& attention, hipStream_t stream);
 hipError_t launch_rows(RowArgs& a, int dtype, bool vec, bool inter, bool paged, hipStream_t stream);
+size_t plan_paged_attend(PagedAttendArgs& a, int dtype);
 hipError_t launch_paged_attend(const PagedAttendArgs& a, int dtype, hipStream_t stream);
 }  // namespace moda
 
@@ -894,7 +895,7 @@ int fill_attend(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_a
 
 size_t moda_hip_paged_attend_workspace_bytes(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_args* t) {
   moda::PagedAttendArgs a = {};
-  return fill_attend(cache, t, a) ? 0 : 4;
+  return fill_attend(cache, t, a) || cache->B * cache->T == 0 ? 0 : moda::plan_paged_attend(a, cache->dtype);
 }
 
 int moda_hip_paged_attend(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_args* t, void* workspace, size_t workspace_bytes,
@@ -907,7 +908,7 @@ int moda_hip_paged_attend(const moda_hip_paged_cache* cache, const moda_hip_page
   const int es = elem_size(cache->dtype);
   if (!aligned(t->q, t->sq, es, true) || !aligned(t->o, t->so, es, true) || (uintptr_t)t->lse % 4 != 0) return MODA_HIP_EALIGN;
   if (t->L > 0 && (!aligned(t->kd, t->skd, es, true) || !aligned(t->vd, t->svd, es, true))) return MODA_HIP_EALIGN;
-  if (!workspace || workspace_bytes < moda_hip_paged_attend_workspace_bytes(cache, t)) return MODA_HIP_EWORKSPACE;
+  if (!workspace || workspace_bytes < moda::plan_paged_attend(a, cache->dtype)) return MODA_HIP_EWORKSPACE;
   if ((uintptr_t)workspace % 16 != 0) return MODA_HIP_EALIGN;
   if ((rc = check_device())) return rc;
   a.work = (float*)workspace;

@@ -76,6 +76,8 @@ struct PagedAttendArgs {
   int G, D, Dv, L, Lv;
   float scale;  // of logits in base 2
   float* work;
+  // how the work is cut (plan_paged_attend)
+  int waves, least_tiles, row_tiles, part_rows, part_width;
 };
 
 }  // namespace moda

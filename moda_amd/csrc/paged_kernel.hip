@@ -2,81 +2,723 @@
 //
 // Row (t, g) of sequence b sees positions j <= past[b] + t and slots l < Lv of its token:
 //   s = scale <q, key>,  o = sum 2^(s - m) value / sum 2^(s - m),  lse = m + log2(sum)
-// with the running maximum m and both sums in 32 bits.  A row that sees nothing has o = 0 and lse = -inf.
-#include <hip/hip_runtime.h>
-#include <stdint.h>
-
+// in one pass over keys and values with the running maximum m, the sum and o in 32 bits.  A row that sees nothing has
+// o = 0 and lse = -inf.
+//
+// What bounds it is the stream of keys and values from HBM: each is read once for all rows of its key/value head, four rows
+// make 4 FLOP of a byte, the matrix instruction does a hundred times that.  So the work is cut for the stream alone.  All
+// tiles of 32 keys -- of every sequence, key/value head and 16 (32, 64) rows -- stand on one axis, sequences with
+// their lengths as they are on the device; each of a fixed number of waves, as many as keep the card's loads in flight, takes an equal
+// run of it, whatever the lengths are, and the host needs to know none of them (a captured launch follows them as they grow).
+// A wave is a workgroup by itself: it fetches its tiles into a ring of its own and waits for nobody.  Runs that begin or end
+// inside a segment (one sequence, head and row tile) leave maximum, sum and o in the workspace, at most two of them a
+// wave; a second launch joins them in the order of the axis, so that results do not depend on who came first.
 #include "paged.h"
+#include "tile16.h"
 #include "../../include/moda_hip.h"
 
 namespace moda {
 
 namespace {
 
-__device__ __forceinline__ float load_as_float(const char* p, int64_t i, int dtype) {
-  if (dtype == MODA_HIP_FP32) return ((const float*)p)[i];
-  const uint16_t x = ((const uint16_t*)p)[i];
-  return dtype == MODA_HIP_FP16 ? (float)__builtin_bit_cast(_Float16, x) : __uint_as_float((uint32_t)x << 16);
+constexpr int kTileKeys = 32;
+
+// what invalid rows and chunks past a head dim read
+__device__ __align__(64) uint32_t zero_line[16];
+
+__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor((long long)x, d, 64);
+  return x;
 }
 
-// One wave per query row and head, a lane every 64th element of the head.
-__global__ __launch_bounds__(64) void paged_attend_kernel(const PagedAttendArgs a, int dtype) {
-  const PagedKV& c = a.cache;
-  const int lane = threadIdx.x;
-  int64_t at = blockIdx.x;
-  const int h = (int)(at % c.H);
-  at /= c.H;
-  const int g = (int)(at % a.G);
-  at /= a.G;
-  const int t = (int)(at % c.T), b = (int)(at / c.T);
+// Sequence b on the axis: positions that its last new token sees, tiles of them and of its new tokens' depth slots.
+struct Seq {
+  int past, fresh, len, seq_tiles, tiles;
+  __device__ __forceinline__ Seq(const PagedAttendArgs& a, int b) {
+    fresh = a.cache.new_of(b);
+    past = a.cache.past_of(b);
+    len = fresh > 0 ? min(past + fresh, a.cache.capacity()) : 0;
+    seq_tiles = (len + kTileKeys - 1) / kTileKeys;
+    tiles = seq_tiles + (fresh * a.Lv + kTileKeys - 1) / kTileKeys;
+  }
+};
 
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  const int64_t q0 = b * a.sq[0] + t * a.sq[1] + g * a.sq[2] + h * a.sq[3];
-  for (int i = 0; i < 4; i++) q[i] = lane + 64 * i < a.D ? load_as_float(a.q, q0 + lane + 64 * i, dtype) : 0.f;
-  auto see = [&](const char* kp, int64_t k0, const char* vp, int64_t v0) {
-    float s = 0.f;
-    for (int i = 0; i < 4; i++)
-      if (lane + 64 * i < a.D) s += q[i] * load_as_float(kp, k0 + lane + 64 * i, dtype);
-    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
-    s *= a.scale;
-    const float top = fmaxf(m, s), from = top == -INFINITY ? 0.f : top;
-    const float shrink = exp2f(m - from), p = exp2f(s - from);
-    m = top;
-    l = l * shrink + p;
-    for (int i = 0; i < 4; i++)
-      if (lane + 64 * i < a.Dv) o[i] = o[i] * shrink + p * load_as_float(vp, v0 + lane + 64 * i, dtype);
-  };
-  if (t < c.new_of(b)) {
-    const int end = min(c.past_of(b) + t + 1, c.capacity());
-    for (int j = 0; j < end; j++) {
-      const int page = c.page_of(b, j);
-      if (page >= 0) see(c.k, c.offset(c.sk, page, j, h), c.v, c.offset(c.sv, page, j, h));
+// Tiles on the whole axis, and how many of them a wave takes.
+struct Plan {
+  int64_t total, per;
+  __device__ __forceinline__ Plan(const PagedAttendArgs& a, int lane) {
+    int64_t sum = 0;
+    for (int b = lane; b < a.cache.B; b += 64) sum += Seq(a, b).tiles;
+    total = wave_sum(sum) * (a.cache.H * a.row_tiles);
+    per = max((total + a.waves - 1) / a.waves, (int64_t)a.least_tiles);
+  }
+};
+
+// One 16-byte (or 4-byte) piece a lane, global -> LDS, lane l to lds + l * BYTES.  Inline assembly as in tile.h (lds_dma): the
+// compiler does not see these loads and so puts no waits between them and later LDS reads; whoever reads the tile
+// waits by count.  Addresses of its own for every lane: pages lie anywhere in memory.
+template <int BYTES>
+__device__ __forceinline__ void global_to_lds(uint32_t lds, uint64_t address) {
+  const uint32_t m0v = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+  if (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0v), "v"(address) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, off" : : "s"(m0v), "v"(address) : "memory", "m0");
+}
+template <int K>
+__device__ __forceinline__ void wait_but() {
+  WaveTileLoader<64>::wait_but<K>();
+}
+
+// A part of a segment that a wave has: its row statistics and sums, row n of 16 (NR times) on lane n = lane & 15, elements
+// 16 c + 4 q + i of o[c] on lane group q = lane >> 4 (MAP: 64 (c / 4) + 16 q + 4 i + c % 4, the order of the fp32 kernel).
+struct PartAt {
+  float *ml, *o;
+  __device__ __forceinline__ PartAt(const PagedAttendArgs& a, int64_t slot) {
+    ml = a.work + slot * a.part_rows * 2;
+    o = a.work + (int64_t)2 * a.waves * a.part_rows * 2 + slot * a.part_rows * a.part_width;
+  }
+};
+
+template <typename E>
+__device__ __forceinline__ void store_element(char* p, int64_t i, float x) {
+  ((typename E::elem*)p)[i] = (typename E::elem)x;
+}
+struct FP32 {
+  typedef float elem;
+};
+
+// the row of the call that row r of a row tile is
+struct RowOf {
+  int t, g;
+  bool real;
+  __device__ __forceinline__ RowOf(const PagedAttendArgs& a, int rt, int rows, int r) {
+    const int row = rt * rows + r;
+    real = row < a.cache.T * a.G;
+    t = row / a.G;
+    g = row - t * a.G;
+  }
+};
+
+template <typename E, int W, int NR, bool MAP>
+__device__ void store_part(const PagedAttendArgs& a, const Seq& seq, int b, int h, int rt, bool whole, int64_t slot, const f32x4 (&o)[W / 16][NR],
+                           const float (&m)[NR], const float (&l_lane)[NR], int lane) {
+  const int n = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int nr = 0; nr < NR; nr++) {
+    const RowOf row(a, rt, 16 * NR, 16 * nr + n);
+    const float l = quad_sum(l_lane[nr]);
+    if (!row.real) continue;
+    const bool padded = row.t >= seq.fresh;
+    if (!whole) {
+      const PartAt part(a, slot);
+      const int r = 16 * nr + n;
+      if (q == 0) {
+        part.ml[2 * r] = padded ? kNegInf : m[nr];
+        part.ml[2 * r + 1] = padded ? 0.f : l;
+      }
+#pragma unroll
+      for (int c = 0; c < W / 16; c++) {
+        float* to = part.o + (int64_t)r * W;
+        if (!MAP) {
+          *(f32x4*)(to + 16 * c + 4 * q) = o[c][nr];
+        } else if (c % 4 == 0) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) *(f32x4*)(to + 16 * c + 16 * q + 4 * i) = f32x4{o[c][nr][i], o[c + 1][nr][i], o[c + 2][nr][i], o[c + 3][nr][i]};
+        }
+      }
+      continue;
     }
-    for (int s = 0; s < a.Lv; s++) {
-      const int64_t row = (int64_t)t * a.L + s;
-      see(a.kd, b * a.skd[0] + row * a.skd[1] + h * a.skd[2], a.vd, b * a.svd[0] + row * a.svd[1] + h * a.svd[2]);
+    const bool empty = padded || l == 0.f;
+    const float inv = empty ? 0.f : 1.f / l;
+    const int64_t to = b * a.so[0] + row.t * a.so[1] + row.g * a.so[2] + h * a.so[3];
+#pragma unroll
+    for (int c = 0; c < W / 16; c++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int e = MAP ? 64 * (c / 4) + 16 * q + 4 * i + c % 4 : 16 * c + 4 * q + i;
+        if (e < a.Dv) store_element<E>(a.o, to + e, empty ? 0.f : o[c][nr][i] * inv);
+      }
+    if (q == 0)
+      a.lse[b * a.slse[0] + row.t * a.slse[1] + row.g * a.slse[2] + h * a.slse[3]] = empty ? kNegInf : m[nr] + __builtin_amdgcn_logf(l);
+  }
+}
+
+// Which keys row `nr` of a lane sees in a tile: indices [lo, hi) of the sequence's positions, or of its depth columns.
+struct Window {
+  int lo, hi;
+};
+
+// The running softmax of one tile: x = logits in base 2 (what is not seen: -inf) -> probabilities against the new maximum; the
+// sums so far are brought to it.  In lanes of one row (four) the maximum agrees, the sum is the lane's own.
+template <int N, int MB, int NR>
+__device__ __forceinline__ void softmax_step(float (&x)[N], float& m, float& l, f32x4 (&o)[MB][NR], int nr) {
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < N; i++) top = fmaxf(top, x[i]);
+  top = fmaxf(m, quad_max(top));
+  const float from = top == kNegInf ? 0.f : top;
+  if (__any(top != m)) {  // (a NaN never equals itself: the sums become NaN with it)
+    const float shrink = fast_exp2(m - from);
+    l *= shrink;
+#pragma unroll
+    for (int c = 0; c < MB; c++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[c][nr][i] *= shrink;
+    m = top;
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    x[i] = fast_exp2(x[i] - from);
+    l += x[i];
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// 16-bit types
+// ------------------------------------------------------------------------------------------------------------------
+
+// LDS of a wave: NS stages of a K and a V tile; table entries of the tiles to come (2 NS tiles); addresses of the rows of one
+// tile; which keys of a tile are there.
+template <int W, int NS>
+struct WaveLds {
+  static constexpr int kTile = kTileKeys * W * 2, kStage = 2 * kTile;
+  static constexpr int kTable = NS * kStage, kRows = kTable + 2 * NS * 256, kMask = kRows + kTileKeys * 16, kBytes = kMask + 16 * NS;
+};
+
+template <typename T, int W, int NR, int NS>
+struct PagedWave {
+  typedef WaveLds<W, NS> Lds;
+  static constexpr int CH = W / 8, RPW = 64 / CH, NL = kTileKeys / RPW, KS = W / 32, MB = W / 16;
+  const PagedAttendArgs& a;
+  const int lane;
+  const uint32_t lds;  // byte address
+  Operand16<W> oa;
+  i32x4 q[NR][KS];
+  f32x4 o[MB][NR];
+  float m[NR], l[NR];
+  // the segment
+  int b, h, rt;
+  const Seq* seq;
+  uint64_t zero;
+
+  __device__ __forceinline__ PagedWave(const PagedAttendArgs& args, int lane_, uint32_t lds_) : a(args), lane(lane_), lds(lds_) {
+    oa.init(lane);
+    zero = (uint64_t)&zero_line[0];
+  }
+  template <typename P>
+  __device__ __forceinline__ MODA_LDS P* at(int byte) const {
+    return (MODA_LDS P*)(uintptr_t)(lds + byte);
+  }
+
+  // table entries of a tile's positions (lanes r and r + 32: row r)
+  __device__ __forceinline__ void fetch_table(int tile, int ring) const {
+    const int j = tile * kTileKeys + (lane & 31);
+    const bool in = tile < seq->seq_tiles && j < seq->len;
+    const uint64_t p = (uint64_t)(a.cache.table + b * a.cache.table_stride + (j >> a.cache.page_shift));
+    global_to_lds<4>(lds + Lds::kTable + ring * 256, in ? p : zero);
+  }
+  // where the rows of a tile lie, from its table entries; an address of zero: nowhere
+  __device__ __forceinline__ void find_rows(int tile, int ring, int stage) const {
+    const int r = lane & 31;
+    uint64_t kp = 0, vp = 0;
+    if (tile < seq->seq_tiles) {
+      const int j = tile * kTileKeys + r, page = *at<int>(Lds::kTable + ring * 256 + 4 * lane);
+      if (j < seq->len && (unsigned)page < (unsigned)a.cache.n_pages) {
+        kp = (uint64_t)(a.cache.k + 2 * a.cache.offset(a.cache.sk, page, j, h));
+        vp = (uint64_t)(a.cache.v + 2 * a.cache.offset(a.cache.sv, page, j, h));
+      }
+    } else {
+      const int col = (tile - seq->seq_tiles) * kTileKeys + r, t = col / a.Lv;
+      if (t < seq->fresh) {
+        const int64_t row = (int64_t)t * a.L + (col - t * a.Lv);
+        kp = (uint64_t)(a.kd + 2 * (b * a.skd[0] + row * a.skd[1] + h * a.skd[2]));
+        vp = (uint64_t)(a.vd + 2 * (b * a.svd[0] + row * a.svd[1] + h * a.svd[2]));
+      }
+    }
+    const uint32_t there = (uint32_t)__ballot(kp != 0);
+    if (lane < 32) {
+      *at<uint64_t>(Lds::kRows + 16 * r) = kp;
+      *at<uint64_t>(Lds::kRows + 16 * r + 8) = vp;
+    }
+    if (lane == 0) *at<uint32_t>(Lds::kMask + 4 * stage) = there;
+  }
+  // a K (0) or V (1) tile, from the rows found last
+  __device__ __forceinline__ void fetch_tile(int which, int stage) const {
+    const int prow = lane / CH, pch = lane % CH, dim = which ? a.Dv : a.D;
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+      const int row = i * RPW + prow, chunk = pch ^ Tile<W>::swz(row);
+      const uint64_t p = *at<uint64_t>(Lds::kRows + 16 * row + 8 * which);
+      global_to_lds<16>(lds + stage * Lds::kStage + which * Lds::kTile + i * 1024, p != 0 && chunk * 8 < dim ? p + chunk * 16 : zero);
     }
   }
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  const int64_t o0 = b * a.so[0] + t * a.so[1] + g * a.so[2] + h * a.so[3];
-  for (int i = 0; i < 4; i++)
-    if (lane + 64 * i < a.Dv) {
-      const float x = o[i] * inv;
-      if (dtype == MODA_HIP_FP32)
-        ((float*)a.o)[o0 + lane + 64 * i] = x;
-      else
-        ((uint16_t*)a.o)[o0 + lane + 64 * i] =
-            dtype == MODA_HIP_FP16 ? __builtin_bit_cast(uint16_t, (_Float16)x) : __builtin_bit_cast(uint16_t, (__bf16)x);
+
+  // Values of a tile that not every row sees, one of them not finite: 0 x inf would reach rows that do not see it, so each row adds up
+  // what it sees, key by key.  p: the lane's probabilities (zero where unseen, and where they underflow).
+  __device__ void add_key_by_key(const float (&p)[8], int nr, Window win, int first, uint32_t there, lds_cptr tile) {
+    const int n = lane & 15, g = lane >> 4;
+    for (int key = 0; key < kTileKeys; key++) {
+      const int low = key & 15, from = (low >> 2) == 0 ? 0 : (low >> 2) == 1 ? 3 : (low >> 2) == 2 ? 1 : 2;  // slot_base(from) = low & 12
+      float x = p[0];
+#pragma unroll
+      for (int i = 1; i < 8; i++) x = i == (key >> 4) * 4 + (key & 3) ? p[i] : x;
+      x = __shfl(x, n + 16 * from, 64);
+      const bool seen = (there >> key & 1) && first + key >= win.lo && first + key < win.hi;
+      if (!seen) continue;
+#pragma unroll
+      for (int c = 0; c < MB; c++) {
+        const int e = 16 * c + 4 * g;
+        const i32x2 v = *(MODA_LDS const i32x2*)(tile + Tile<W>::off(key, e >> 3) + (e & 7));
+        float v0, v1, v2, v3;
+        unpack2<T>(v[0], v0, v1);
+        unpack2<T>(v[1], v2, v3);
+        o[c][nr][0] += x * v0;
+        o[c][nr][1] += x * v1;
+        o[c][nr][2] += x * v2;
+        o[c][nr][3] += x * v3;
+      }
     }
-  if (lane == 0) a.lse[b * a.slse[0] + t * a.slse[1] + g * a.slse[2] + h * a.slse[3]] = l > 0.f || l != l ? m + log2f(l) : -INFINITY;
+  }
+
+  // tiles [t0, t1) of the segment
+  __device__ void run(int t0, int t1) {
+    const int n = lane & 15, g = lane >> 4, tiles = t1 - t0;
+    const bool one_token = a.cache.T == 1;
+    Window seq_win[NR], depth_win[NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+      const RowOf row(a, rt, 16 * NR, 16 * nr + n);
+      const int64_t from = b * a.sq[0] + row.t * a.sq[1] + row.g * a.sq[2] + h * a.sq[3];
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        const int e = 32 * ks + 8 * g;
+        i32x4 x = {0, 0, 0, 0};
+        if (row.real && e < a.D) x = *(const i32x4*)(a.q + 2 * (from + e));
+        q[nr][ks] = x;
+      }
+      seq_win[nr] = {0, seq->past + row.t + 1};
+      depth_win[nr] = {row.t * a.Lv, row.t * a.Lv + a.Lv};
+      m[nr] = kNegInf;
+      l[nr] = 0.f;
+#pragma unroll
+      for (int c = 0; c < MB; c++) o[c][nr] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // the rows have to be here before the tiles are sent for: the compiler would wait for everything behind them as well
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(q[nr][ks]));
+    const int first_t = rt * 16 * NR / a.G;  // of the row tile's tokens
+
+#pragma unroll
+    for (int j = 0; j < NS; j++) fetch_table(t0 + j, j);
+    wait_but<0>();
+#pragma unroll
+    for (int j = 0; j < NS; j++)
+      if (j < tiles) {
+        fetch_table(t0 + j + NS, NS + j);
+        find_rows(t0 + j, j, j);
+        fetch_tile(0, j);
+        fetch_tile(1, j);
+      }
+    // loads behind a tile's K when NS - 1 more tiles are on their way, and behind its V when the next K is as well
+    constexpr int kBehindK = NL + (NS - 1) * (2 * NL + 1), kBehindV = (NS - 1) * (2 * NL + 1) + NL + 1;
+    for (int i = 0; i < tiles; i++) {
+      const int stage = i % NS, tile = t0 + i;
+      const bool more = i + NS < tiles;
+      if (i + NS <= tiles)
+        wait_but<kBehindK>();
+      else
+        wait_but<0>();
+      const uint32_t there = (uint32_t)__builtin_amdgcn_readfirstlane((int)*at<uint32_t>(Lds::kMask + 4 * stage));
+      const lds_cptr kt = at<uint16_t>(stage * Lds::kStage), vt = at<uint16_t>(stage * Lds::kStage + Lds::kTile);
+      f32x4 s[2][NR];
+      mfma16_rows<T, W, 2, NR, 4>(oa, kt, q, s);
+      WaveTileLoader<64>::reads_done();
+      if (more) {
+        fetch_table(tile + 2 * NS, (i + 2 * NS) % (2 * NS));
+        find_rows(tile + NS, (i + NS) % (2 * NS), stage);
+        fetch_tile(0, stage);
+      }
+      const bool depth = tile >= seq->seq_tiles;
+      const int first = (depth ? tile - seq->seq_tiles : tile) * kTileKeys;
+      const bool all_seen = there == ~0u && (depth ? one_token : first + kTileKeys - 1 <= seq->past + first_t);
+      float p[NR][8];
+#pragma unroll
+      for (int nr = 0; nr < NR; nr++) {
+        const Window win = depth ? depth_win[nr] : seq_win[nr];
+#pragma unroll
+        for (int i8 = 0; i8 < 8; i8++) {
+          const int key = 16 * (i8 >> 2) + slot_base(g) + (i8 & 3);
+          const float x = s[i8 >> 2][nr][i8 & 3] * a.scale;
+          p[nr][i8] = all_seen || ((there >> key & 1) && first + key >= win.lo && first + key < win.hi) ? x : kNegInf;
+        }
+        softmax_step<8>(p[nr], m[nr], l[nr], o, nr);
+      }
+      if (more)
+        wait_but<kBehindV>();
+      else
+        wait_but<0>();
+      bool odd = false;
+      if (!all_seen && !one_token) {
+        const int top = __is_same(T, BF16) ? 0x7f80 : 0x7c00;
+        for (int c = lane; c < kTileKeys * CH; c += 64) {
+          const i32x4 v = *(MODA_LDS const i32x4*)(vt + 8 * c);
+#pragma unroll
+          for (int i4 = 0; i4 < 4; i4++) odd = odd || (v[i4] & top) == top || (v[i4] >> 16 & top) == top;
+        }
+      }
+      if (__any(odd)) {
+#pragma unroll
+        for (int nr = 0; nr < NR; nr++) add_key_by_key(p[nr], nr, depth ? depth_win[nr] : seq_win[nr], first, there, vt);
+      } else {
+        // Probabilities go to the matrix instruction in two pieces, rounded and what the rounding left: its time does not
+        // matter here, and o is then as good as its 32-bit sums.
+        i32x4 hi[NR], lo[NR];
+#pragma unroll
+        for (int nr = 0; nr < NR; nr++) {
+          float r[8];
+#pragma unroll
+          for (int i4 = 0; i4 < 4; i4++) {
+            hi[nr][i4] = pack2<T>(p[nr][2 * i4], p[nr][2 * i4 + 1]);
+            float x0, x1;
+            unpack2<T>(hi[nr][i4], x0, x1);
+            r[2 * i4] = p[nr][2 * i4] - x0;
+            r[2 * i4 + 1] = p[nr][2 * i4 + 1] - x1;
+          }
+#pragma unroll
+          for (int i4 = 0; i4 < 4; i4++) lo[nr][i4] = pack2<T>(r[2 * i4], r[2 * i4 + 1]);
+        }
+        constexpr int DEPTH = 4;
+        i32x4 ops[MB];
+#pragma unroll
+        for (int c = 0; c < DEPTH && c < MB; c++) ops[c] = oa.tr_operand(vt, 0, c);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < MB; c++) {
+          if (c + DEPTH < MB) ops[c + DEPTH] = oa.tr_operand(vt, 0, c + DEPTH);
+#pragma unroll
+          for (int nr = 0; nr < NR; nr++) o[c][nr] = mfma16<T>(ops[c], hi[nr], o[c][nr]);
+#pragma unroll
+          for (int nr = 0; nr < NR; nr++) o[c][nr] = mfma16<T>(ops[c], lo[nr], o[c][nr]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      WaveTileLoader<64>::reads_done();
+      if (more) fetch_tile(1, stage);
+    }
+  }
+};
+
+// Walks a wave's run of the axis: part(seq, b, h, rt, t0, t1, whole, slot) for each segment in it.
+template <typename F>
+__device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, F&& part) {
+  const Plan plan(a, lane);
+  const int64_t wave = blockIdx.x, s = wave * plan.per, e = min(s + plan.per, plan.total);
+  if (s >= e) return;
+  const int heads = a.cache.H * a.row_tiles;
+  int b = 0;
+  int64_t start = 0;  // of sequence b, in tiles
+  for (int b0 = 0; b0 < a.cache.B; b0 += 64) {
+    const int64_t own = b0 + lane < a.cache.B ? (int64_t)Seq(a, b0 + lane).tiles * heads : 0;
+    int64_t upto = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t x = __shfl_up((long long)upto, d, 64);
+      if (lane >= d) upto += x;
+    }
+    const uint64_t behind = __ballot(start + upto > s);
+    if (behind) {
+      const int first = __builtin_ctzll(behind);
+      b = b0 + first;
+      start += __shfl((long long)(upto - own), first, 64);
+      break;
+    }
+    start += __shfl((long long)upto, 63, 64);
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  Seq seq(a, b);
+  int64_t rest = s - start;
+  int hr = __builtin_amdgcn_readfirstlane((int)(rest / seq.tiles)), tile = __builtin_amdgcn_readfirstlane((int)(rest - (int64_t)hr * seq.tiles));
+  for (int64_t at = s; at < e;) {
+    const int upto = (int)min((int64_t)seq.tiles, tile + (e - at));
+    part(seq, b, hr / a.row_tiles, hr % a.row_tiles, tile, upto, tile == 0 && upto == seq.tiles, 2 * wave + (at == s ? 0 : 1));
+    at += upto - tile;
+    tile = 0;
+    if (++hr == heads && at < e) {
+      hr = 0;
+      do seq = Seq(a, ++b);
+      while (seq.tiles == 0);
+    }
+  }
+}
+
+template <typename T, int W, int NR, int NS>
+__global__ __launch_bounds__(64, 1) void paged_kernel(const PagedAttendArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  const int lane = threadIdx.x;
+  PagedWave<T, W, NR, NS> w(a, lane, (uint32_t)(uintptr_t)(MODA_LDS char*)lds_raw);
+  walk(a, lane, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int64_t slot) {
+    w.seq = &seq;
+    w.b = b;
+    w.h = h;
+    w.rt = rt;
+    w.run(t0, t1);
+    store_part<T, W, NR, false>(a, seq, b, h, rt, whole, slot, w.o, w.m, w.l, lane);
+  });
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// fp32: operands from global memory into the registers of v_mfma_f32_16x16x4_f32 (see fp32_kernels.hip for the layout)
+// ------------------------------------------------------------------------------------------------------------------
+
+template <int W>
+__global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs a) {
+  constexpr int MB = W / 16;
+  const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, T = a.cache.T;
+  walk(a, lane, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int64_t slot) {
+    const RowOf row(a, rt, 16, n);
+    const float* qp = (const float*)a.q + b * a.sq[0] + row.t * a.sq[1] + row.g * a.sq[2] + h * a.sq[3];
+    f32x4 q[MB], o[MB][1];
+    float m[1] = {kNegInf}, l[1] = {0.f};
+#pragma unroll
+    for (int s = 0; s < MB; s++) {
+      q[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (row.real && 16 * s + 4 * g < a.D) q[s] = *(const f32x4*)(qp + 16 * s + 4 * g);
+      o[s][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int first_t = rt * 16 / a.G;
+    for (int half = 2 * t0; half < 2 * t1; half++) {  // 16 keys at a time
+      const bool depth = half >= 2 * seq.seq_tiles;
+      const int first = (depth ? half - 2 * seq.seq_tiles : half) * 16, key = first + n;
+      const float *kp = nullptr, *vp = nullptr;
+      if (!depth) {
+        const int page = key < seq.len ? a.cache.page_of(b, key) : -1;
+        if (page >= 0) {
+          kp = (const float*)a.cache.k + a.cache.offset(a.cache.sk, page, key, h);
+          vp = (const float*)a.cache.v + a.cache.offset(a.cache.sv, page, key, h);
+        }
+      } else {
+        const int t = key / a.Lv;
+        if (t < seq.fresh) {
+          const int64_t r = (int64_t)t * a.L + (key - t * a.Lv);
+          kp = (const float*)a.kd + b * a.skd[0] + r * a.skd[1] + h * a.skd[2];
+          vp = (const float*)a.vd + b * a.svd[0] + r * a.svd[1] + h * a.svd[2];
+        }
+      }
+      const uint32_t there = (uint32_t)__ballot(kp != nullptr) & 0xffffu;
+      f32x4 k[MB], v[4][MB / 4];
+#pragma unroll
+      for (int s = 0; s < MB; s++) {
+        k[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (kp && 16 * s + 4 * g < a.D) k[s] = *(const f32x4*)(kp + 16 * s + 4 * g);
+      }
+      const float* vrow[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        vrow[r] = (const float*)__shfl((unsigned long long)vp, 4 * g + r, 64);
+#pragma unroll
+        for (int c = 0; c < MB / 4; c++) {
+          v[r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (vrow[r] && 64 * c + 4 * n < a.Dv) v[r][c] = *(const f32x4*)(vrow[r] + 64 * c + 4 * n);
+        }
+      }
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < MB; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c][i], q[c][i], s, 0, 0, 0);
+      const Window win = depth ? Window{row.t * a.Lv, row.t * a.Lv + a.Lv} : Window{0, seq.past + row.t + 1};
+      const bool all_seen = there == 0xffffu && (depth ? T == 1 : first + 15 <= seq.past + first_t);
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int j = 4 * g + i;
+        p[i] = all_seen || ((there >> j & 1) && first + j >= win.lo && first + j < win.hi) ? s[i] * a.scale : kNegInf;
+      }
+      softmax_step<4>(p, m[0], l[0], o, 0);
+      bool odd = false;
+      if (!all_seen && T > 1) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int c = 0; c < MB / 4; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) odd = odd || !(__builtin_fabsf(v[r][c][i]) < __builtin_huge_valf());
+      }
+      if (__any(odd)) {  // see PagedWave::add_key_by_key
+        for (int j = 0; j < 16; j++) {
+          const int i = j & 3;
+          const float x = __shfl(i == 0 ? p[0] : i == 1 ? p[1] : i == 2 ? p[2] : p[3], n + 16 * (j >> 2), 64);
+          const float* from = (const float*)__shfl((unsigned long long)vp, j, 64);
+          if (!((there >> j & 1) && first + j >= win.lo && first + j < win.hi)) continue;
+#pragma unroll
+          for (int c = 0; c < MB; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int at = 64 * (c / 4) + 16 * g + 4 * e + c % 4;
+              if (at < a.Dv) o[c][0][e] += x * from[at];
+            }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < MB; c++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[c][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][c / 4][c % 4], p[r], o[c][0], 0, 0, 0);
+      }
+    }
+    store_part<FP32, W, 1, true>(a, seq, b, h, rt, whole, slot, o, m, l, lane);
+  });
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// joining
+// ------------------------------------------------------------------------------------------------------------------
+
+// A workgroup per query row and head: the parts of its segment, in the order of the axis.  W / 4 threads have four elements
+// each of every (NT * 4 / W)-th part.
+template <typename E, int W, int NT>
+__global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a, int rows_per_tile) {
+  constexpr int LANES = W / 4, GROUPS = NT / LANES;
+  __shared__ f32x4 sums[NT];
+  __shared__ float lsum[GROUPS], tops[NT / 64];
+  const int tid = threadIdx.x, lane = tid & 63, x = tid % LANES, group = tid / LANES;
+  int64_t at = blockIdx.x;
+  const int h = (int)(at % a.cache.H);
+  at /= a.cache.H;
+  const int rows = a.cache.T * a.G, row = (int)(at % rows), b = (int)(at / rows);
+  const int rt = row / rows_per_tile, r = row - rt * rows_per_tile, t = row / a.G, g = row - t * a.G;
+  const Plan plan(a, lane);
+  int64_t start = 0;
+  for (int i = lane; i < b; i += 64) start += Seq(a, i).tiles;
+  start = wave_sum(start) * (a.cache.H * a.row_tiles);
+  const int tiles = Seq(a, b).tiles;
+  start += (int64_t)(h * a.row_tiles + rt) * tiles;
+  int64_t w0 = start / plan.per, w1 = tiles ? (start + tiles - 1) / plan.per : w0;
+  if (tiles && w0 == w1) return;  // one wave had all of it and has stored the row
+  const int parts = tiles ? (int)(w1 - w0 + 1) : 0;
+  auto slot = [&](int p) { return 2 * (w0 + p) + (p == 0 && start != w0 * plan.per ? 1 : 0); };
+  float top = kNegInf;
+  for (int p = tid; p < parts; p += NT) top = fmaxf(top, PartAt(a, slot(p)).ml[2 * r]);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+  if (lane == 0) tops[tid >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NT / 64; i++) top = fmaxf(top, tops[i]);
+  const float from = top == kNegInf ? 0.f : top;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+#pragma unroll 4
+  for (int p = group; p < parts; p += GROUPS) {
+    const PartAt part(a, slot(p));
+    const float w = fast_exp2(part.ml[2 * r] - from);
+    const f32x4 v = *(const f32x4*)(part.o + (int64_t)r * W + 4 * x);
+    l += w * part.ml[2 * r + 1];
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] += w * v[i];
+  }
+  sums[tid] = o;
+  if (x == 0) lsum[group] = l;
+  __syncthreads();
+  if (group > 0) return;
+  l = 0.f;
+  o = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < GROUPS; i++) {
+    l += lsum[i];
+    const f32x4 v = sums[i * LANES + x];
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] += v[e];
+  }
+  const bool empty = l == 0.f;
+  const float inv = empty ? 0.f : 1.f / l;
+  const int64_t to = b * a.so[0] + t * a.so[1] + g * a.so[2] + h * a.so[3];
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (4 * x + e < a.Dv) store_element<E>(a.o, to + 4 * x + e, empty ? 0.f : o[e] * inv);
+  if (x == 0) a.lse[b * a.slse[0] + t * a.slse[1] + g * a.slse[2] + h * a.slse[3]] = empty ? kNegInf : top + __builtin_amdgcn_logf(l);
+}
+
+int tile_width(const PagedAttendArgs& a) {
+  const int d = a.D > a.Dv ? a.D : a.Dv;
+  return d <= 64 ? 64 : d <= 128 ? 128 : 256;
+}
+
+// rows of a row tile, in sixteens: as many as a wave's registers hold without spilling
+int row_blocks(const PagedAttendArgs& a, int dtype) {
+  const int rows = a.cache.T * a.G, width = tile_width(a);
+  return dtype == MODA_HIP_FP32 || rows <= 16 || width == 256 ? 1 : rows <= 32 || width == 128 ? 2 : 4;
+}
+
+template <typename T, int W, int NR, int NS>
+hipError_t launch_waves(const PagedAttendArgs& a, hipStream_t stream) {
+  static LdsAttrState state;
+  constexpr int bytes = WaveLds<W, NS>::kBytes;
+  const hipError_t e = allow_dynamic_lds(state, (const void*)paged_kernel<T, W, NR, NS>, bytes);
+  if (e != hipSuccess) return e;
+  paged_kernel<T, W, NR, NS><<<a.waves, 64, bytes, stream>>>(a);
+  return hipGetLastError();
+}
+template <typename T>
+hipError_t launch_waves_as(const PagedAttendArgs& a, int width, int blocks, hipStream_t stream) {
+  if (width == 256) return launch_waves<T, 256, 1, 2>(a, stream);
+  if (width == 128) return blocks == 1 ? launch_waves<T, 128, 1, 2>(a, stream) : launch_waves<T, 128, 2, 2>(a, stream);
+  return blocks == 1 ? launch_waves<T, 64, 1, 4>(a, stream) : blocks == 2 ? launch_waves<T, 64, 2, 4>(a, stream) : launch_waves<T, 64, 4, 4>(a, stream);
+}
+template <typename E>
+hipError_t launch_join(const PagedAttendArgs& a, int width, int blocks, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.cache.B * a.cache.T * a.G * a.cache.H;
+  const unsigned grid = (unsigned)rows;
+  const int per_tile = 16 * blocks;
+  if (width == 64)
+    paged_join_kernel<E, 64, 256><<<grid, 256, 0, stream>>>(a, per_tile);
+  else if (width == 128)
+    paged_join_kernel<E, 128, 256><<<grid, 256, 0, stream>>>(a, per_tile);
+  else
+    paged_join_kernel<E, 256, 256><<<grid, 256, 0, stream>>>(a, per_tile);
+  return hipGetLastError();
 }
 
 }  // namespace
 
+// How the work is cut: waves on the axis, row tiles, the workspace's rows.  Nothing here depends on what the device arrays hold.
+size_t plan_paged_attend(PagedAttendArgs& a, int dtype) {
+  const int width = tile_width(a), blocks = row_blocks(a, dtype), rows = a.cache.T * a.G;
+  a.row_tiles = (rows + 16 * blocks - 1) / (16 * blocks);
+  a.part_rows = rows < 16 * blocks ? rows : 16 * blocks;
+  a.part_width = width;
+  a.least_tiles = 2;
+  // waves of the whole card: as many as hold their rings in the 160 KB of a compute unit
+  const int per_unit = dtype == MODA_HIP_FP32 ? 8 : width == 256 ? 2 : 4;
+  const int64_t capacity = (int64_t)a.cache.max_pages << a.cache.page_shift;
+  const int64_t most = (int64_t)a.cache.B * a.cache.H * a.row_tiles *
+                       ((capacity + kTileKeys - 1) / kTileKeys + ((int64_t)a.cache.T * a.Lv + kTileKeys - 1) / kTileKeys);
+  a.waves = (int)(most < 256 * per_unit ? (most > 0 ? most : 1) : 256 * per_unit);
+  return (size_t)2 * a.waves * a.part_rows * (a.part_width + 2) * sizeof(float);
+}
+
 hipError_t launch_paged_attend(const PagedAttendArgs& a, int dtype, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.cache.B * a.cache.T * a.G * a.cache.H;
-  paged_attend_kernel<<<(unsigned)rows, 64, 0, stream>>>(a, dtype);
-  return hipGetLastError();
+  const int width = tile_width(a), blocks = row_blocks(a, dtype);
+  hipError_t e;
+  if (dtype == MODA_HIP_FP32) {
+    if (width == 64)
+      paged_fp32_kernel<64><<<a.waves, 64, 0, stream>>>(a);
+    else if (width == 128)
+      paged_fp32_kernel<128><<<a.waves, 64, 0, stream>>>(a);
+    else
+      paged_fp32_kernel<256><<<a.waves, 64, 0, stream>>>(a);
+    e = hipGetLastError();
+    if (e == hipSuccess) e = launch_join<FP32>(a, width, blocks, stream);
+  } else if (dtype == MODA_HIP_FP16) {
+    e = launch_waves_as<FP16>(a, width, blocks, stream);
+    if (e == hipSuccess) e = launch_join<FP16>(a, width, blocks, stream);
+  } else {
+    e = launch_waves_as<BF16>(a, width, blocks, stream);
+    if (e == hipSuccess) e = launch_join<BF16>(a, width, blocks, stream);
+  }
+  return e;
 }
 
 }  // namespace moda
