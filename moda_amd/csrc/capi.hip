@@ -908,7 +908,9 @@ int moda_hip_paged_attend(const moda_hip_paged_cache* cache, const moda_hip_page
   const int es = elem_size(cache->dtype);
   if (!aligned(t->q, t->sq, es, true) || !aligned(t->o, t->so, es, true) || (uintptr_t)t->lse % 4 != 0) return MODA_HIP_EALIGN;
   if (t->L > 0 && (!aligned(t->kd, t->skd, es, true) || !aligned(t->vd, t->svd, es, true))) return MODA_HIP_EALIGN;
-  if (!workspace || workspace_bytes < moda::plan_paged_attend(a, cache->dtype)) return MODA_HIP_EWORKSPACE;
+  const size_t need = moda::plan_paged_attend(a, cache->dtype);
+  if (need == 0) return MODA_HIP_EUNSUPPORTED;
+  if (!workspace || workspace_bytes < need) return MODA_HIP_EWORKSPACE;
   if ((uintptr_t)workspace % 16 != 0) return MODA_HIP_EALIGN;
   if ((rc = check_device())) return rc;
   a.work = (float*)workspace;

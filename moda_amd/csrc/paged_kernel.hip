@@ -26,9 +26,9 @@ constexpr int kTileKeys = 32;
 // what invalid rows and chunks past a head dim read
 __device__ __align__(64) uint32_t zero_line[16];
 
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+__device__ __forceinline__ int wave_sum(int x) {
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor((long long)x, d, 64);
+  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
   return x;
 }
 
@@ -44,14 +44,12 @@ struct Seq {
   }
 };
 
-// Tiles on the whole axis, and how many of them a wave takes.
+// Tiles on the whole axis, and how many of them a wave takes.  The host has made sure that they fit 32 bits.
 struct Plan {
-  int64_t total, per;
-  __device__ __forceinline__ Plan(const PagedAttendArgs& a, int lane) {
-    int64_t sum = 0;
-    for (int b = lane; b < a.cache.B; b += 64) sum += Seq(a, b).tiles;
-    total = wave_sum(sum) * (a.cache.H * a.row_tiles);
-    per = max((total + a.waves - 1) / a.waves, (int64_t)a.least_tiles);
+  int total, per;
+  __device__ __forceinline__ Plan(const PagedAttendArgs& a, int tiles_of_one_head) {
+    total = tiles_of_one_head * (a.cache.H * a.row_tiles);
+    per = max((int)(((unsigned)total + a.waves - 1) / (unsigned)a.waves), a.least_tiles);
   }
 };
 
@@ -71,13 +69,20 @@ __device__ __forceinline__ void wait_but() {
   WaveTileLoader<64>::wait_but<K>();
 }
 
+// The workspace: for each segment the slot of its first part and how many there are (written by the wave that has its first tile;
+// a segment without tiles has none), then statistics and sums by slot.
+__device__ __forceinline__ int64_t segments(const PagedAttendArgs& a) {
+  return ((int64_t)a.cache.B * a.cache.H * a.row_tiles + 1) & ~1ll;  // even: what follows stays on 16 bytes
+}
+
 // A part of a segment that a wave has: its row statistics and sums, row n of 16 (NR times) on lane n = lane & 15, elements
 // 16 c + 4 q + i of o[c] on lane group q = lane >> 4 (MAP: 64 (c / 4) + 16 q + 4 i + c % 4, the order of the fp32 kernel).
 struct PartAt {
   float *ml, *o;
   __device__ __forceinline__ PartAt(const PagedAttendArgs& a, int64_t slot) {
-    ml = a.work + slot * a.part_rows * 2;
-    o = a.work + (int64_t)2 * a.waves * a.part_rows * 2 + slot * a.part_rows * a.part_width;
+    float* first = a.work + segments(a) * 2;
+    ml = first + slot * a.part_rows * 2;
+    o = first + (int64_t)2 * a.waves * a.part_rows * 2 + slot * a.part_rows * a.part_width;
   }
 };
 
@@ -102,7 +107,7 @@ struct RowOf {
 };
 
 template <typename E, int W, int NR, bool MAP>
-__device__ void store_part(const PagedAttendArgs& a, const Seq& seq, int b, int h, int rt, bool whole, int64_t slot, const f32x4 (&o)[W / 16][NR],
+__device__ void store_part(const PagedAttendArgs& a, const Seq& seq, int b, int h, int rt, bool whole, int slot, const f32x4 (&o)[W / 16][NR],
                            const float (&m)[NR], const float (&l_lane)[NR], int lane) {
   const int n = lane & 15, q = lane >> 4;
 #pragma unroll
@@ -145,9 +150,27 @@ __device__ void store_part(const PagedAttendArgs& a, const Seq& seq, int b, int 
   }
 }
 
+// Logits from the sums of a matrix product, in the product's own basic block: the compiler's hazard pass leaves out the wait
+// states that a result needs where its first reader comes behind a branch (seen as element 3 of some logits holding an
+// earlier sum, where a skipped branch led straight from the last product to v_accvgpr_read).
+template <int N>
+__device__ __forceinline__ void scaled(float* x, const f32x4 (&s)[N], float scale) {
+#pragma unroll
+  for (int i = 0; i < 4 * N; i++) {
+    x[i] = s[i >> 2][i & 3] * scale;
+    asm volatile("" : "+v"(x[i]));
+  }
+}
+// ... and before the results of the last products are read behind a loop or a branch: 32 wait states
+__device__ __forceinline__ void products_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
 // Which keys row `nr` of a lane sees in a tile: indices [lo, hi) of the sequence's positions, or of its depth columns.
 struct Window {
   int lo, hi;
+  // key `key` of a tile that begins at index `first` and holds the keys `there`
+  __device__ __forceinline__ bool sees(bool all, uint32_t there, int first, int key) const {
+    return all | ((there >> key & 1) & (first + key >= lo) & (first + key < hi));
+  }
 };
 
 // The running softmax of one tile: x = logits in base 2 (what is not seen: -inf) -> probabilities against the new maximum; the
@@ -255,18 +278,25 @@ struct PagedWave {
     }
   }
 
+  // the K tile of step i + NS, the tile's rows, and the table entries of the tile NS steps further
+  __device__ __forceinline__ void send(int tile, int i, int stage) const {
+    fetch_table(tile + 2 * NS, (i + 2 * NS) % (2 * NS));
+    find_rows(tile + NS, (i + NS) % (2 * NS), stage);
+    fetch_tile(0, stage);
+  }
+
   // Values of a tile that not every row sees, one of them not finite: 0 x inf would reach rows that do not see it, so each row adds up
   // what it sees, key by key.  p: the lane's probabilities (zero where unseen, and where they underflow).
   __device__ void add_key_by_key(const float (&p)[8], int nr, Window win, int first, uint32_t there, lds_cptr tile) {
     const int n = lane & 15, g = lane >> 4;
+#pragma unroll 1
     for (int key = 0; key < kTileKeys; key++) {
       const int low = key & 15, from = (low >> 2) == 0 ? 0 : (low >> 2) == 1 ? 3 : (low >> 2) == 2 ? 1 : 2;  // slot_base(from) = low & 12
       float x = p[0];
 #pragma unroll
       for (int i = 1; i < 8; i++) x = i == (key >> 4) * 4 + (key & 3) ? p[i] : x;
       x = __shfl(x, n + 16 * from, 64);
-      const bool seen = (there >> key & 1) && first + key >= win.lo && first + key < win.hi;
-      if (!seen) continue;
+      if (!win.sees(false, there, first, key)) continue;
 #pragma unroll
       for (int c = 0; c < MB; c++) {
         const int e = 16 * c + 4 * g;
@@ -305,29 +335,30 @@ struct PagedWave {
 #pragma unroll
       for (int c = 0; c < MB; c++) o[c][nr] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // the rows have to be here before the tiles are sent for: the compiler would wait for everything behind them as well
+    // the table's entries and the rows have to be here before the tiles are sent for: the compiler would wait for everything
+    // behind the rows as well
+#pragma unroll
+    for (int j = 0; j < NS; j++) fetch_table(t0 + j, j);
 #pragma unroll
     for (int nr = 0; nr < NR; nr++)
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(q[nr][ks]));
-    const int first_t = rt * 16 * NR / a.G;  // of the row tile's tokens
-
-#pragma unroll
-    for (int j = 0; j < NS; j++) fetch_table(t0 + j, j);
     wait_but<0>();
-#pragma unroll
-    for (int j = 0; j < NS; j++)
-      if (j < tiles) {
-        fetch_table(t0 + j + NS, NS + j);
-        find_rows(t0 + j, j, j);
-        fetch_tile(0, j);
-        fetch_tile(1, j);
-      }
+    const int first_t = rt * 16 * NR / a.G;  // of the row tile's tokens
     // loads behind a tile's K when NS - 1 more tiles are on their way, and behind its V when the next K is as well
     constexpr int kBehindK = NL + (NS - 1) * (2 * NL + 1), kBehindV = (NS - 1) * (2 * NL + 1) + NL + 1;
-    for (int i = 0; i < tiles; i++) {
-      const int stage = i % NS, tile = t0 + i;
+    // step i sends for tile i + NS and works on tile i (the first NS steps only send: one copy of the code)
+#pragma unroll 1
+    for (int i = -NS; i < tiles; i++) {
+      const int stage = (i + NS) % NS, tile = t0 + i;
       const bool more = i + NS < tiles;
+      if (i < 0) {
+        if (more) {
+          send(tile, i, stage);
+          fetch_tile(1, stage);
+        }
+        continue;
+      }
       if (i + NS <= tiles)
         wait_but<kBehindK>();
       else
@@ -336,24 +367,24 @@ struct PagedWave {
       const lds_cptr kt = at<uint16_t>(stage * Lds::kStage), vt = at<uint16_t>(stage * Lds::kStage + Lds::kTile);
       f32x4 s[2][NR];
       mfma16_rows<T, W, 2, NR, 4>(oa, kt, q, s);
-      WaveTileLoader<64>::reads_done();
-      if (more) {
-        fetch_table(tile + 2 * NS, (i + 2 * NS) % (2 * NS));
-        find_rows(tile + NS, (i + NS) % (2 * NS), stage);
-        fetch_tile(0, stage);
+      float p[NR][8];
+#pragma unroll
+      for (int nr = 0; nr < NR; nr++) {
+        const f32x4 both[2] = {s[0][nr], s[1][nr]};
+        scaled(p[nr], both, a.scale);
       }
+      WaveTileLoader<64>::reads_done();
+      if (more) send(tile, i, stage);
       const bool depth = tile >= seq->seq_tiles;
       const int first = (depth ? tile - seq->seq_tiles : tile) * kTileKeys;
       const bool all_seen = there == ~0u && (depth ? one_token : first + kTileKeys - 1 <= seq->past + first_t);
-      float p[NR][8];
 #pragma unroll
       for (int nr = 0; nr < NR; nr++) {
         const Window win = depth ? depth_win[nr] : seq_win[nr];
 #pragma unroll
         for (int i8 = 0; i8 < 8; i8++) {
           const int key = 16 * (i8 >> 2) + slot_base(g) + (i8 & 3);
-          const float x = s[i8 >> 2][nr][i8 & 3] * a.scale;
-          p[nr][i8] = all_seen || ((there >> key & 1) && first + key >= win.lo && first + key < win.hi) ? x : kNegInf;
+          p[nr][i8] = win.sees(all_seen, there, first, key) ? p[nr][i8] : kNegInf;
         }
         softmax_step<8>(p[nr], m[nr], l[nr], o, nr);
       }
@@ -364,6 +395,7 @@ struct PagedWave {
       bool odd = false;
       if (!all_seen && !one_token) {
         const int top = __is_same(T, BF16) ? 0x7f80 : 0x7c00;
+#pragma unroll 2
         for (int c = lane; c < kTileKeys * CH; c += 64) {
           const i32x4 v = *(MODA_LDS const i32x4*)(vt + 8 * c);
 #pragma unroll
@@ -409,42 +441,50 @@ struct PagedWave {
       WaveTileLoader<64>::reads_done();
       if (more) fetch_tile(1, stage);
     }
+    products_done();
   }
 };
 
 // Walks a wave's run of the axis: part(seq, b, h, rt, t0, t1, whole, slot) for each segment in it.
 template <typename F>
 __device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, F&& part) {
-  const Plan plan(a, lane);
-  const int64_t wave = blockIdx.x, s = wave * plan.per, e = min(s + plan.per, plan.total);
-  if (s >= e) return;
   const int heads = a.cache.H * a.row_tiles;
-  int b = 0;
-  int64_t start = 0;  // of sequence b, in tiles
+  // up to 64 sequences are read once; of more the first pass is for the total alone
+  int own = lane < a.cache.B ? Seq(a, lane).tiles : 0, sum = own;
+  for (int b = lane + 64; b < a.cache.B; b += 64) sum += Seq(a, b).tiles;
+  const Plan plan(a, wave_sum(sum));
+  const int wave = blockIdx.x;
+  if ((int64_t)wave * plan.per >= plan.total) return;
+  const int s = wave * plan.per, e = min(s + plan.per, plan.total);  // (per <= total / waves + 1 or least_tiles: s + per fits)
+  int b = 0, start = 0;  // start of sequence b, in tiles
   for (int b0 = 0; b0 < a.cache.B; b0 += 64) {
-    const int64_t own = b0 + lane < a.cache.B ? (int64_t)Seq(a, b0 + lane).tiles * heads : 0;
-    int64_t upto = own;
+    if (b0 > 0) own = b0 + lane < a.cache.B ? Seq(a, b0 + lane).tiles : 0;
+    int upto = own;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t x = __shfl_up((long long)upto, d, 64);
+      const int x = __shfl_up(upto, d, 64);
       if (lane >= d) upto += x;
     }
-    const uint64_t behind = __ballot(start + upto > s);
+    const uint64_t behind = __ballot(start + upto * heads > s);
+    const int first = behind ? __builtin_ctzll(behind) : 63;
+    start += __shfl(behind ? upto - own : upto, first, 64) * heads;
     if (behind) {
-      const int first = __builtin_ctzll(behind);
       b = b0 + first;
-      start += __shfl((long long)(upto - own), first, 64);
       break;
     }
-    start += __shfl((long long)upto, 63, 64);
   }
   b = __builtin_amdgcn_readfirstlane(b);
   Seq seq(a, b);
-  int64_t rest = s - start;
-  int hr = __builtin_amdgcn_readfirstlane((int)(rest / seq.tiles)), tile = __builtin_amdgcn_readfirstlane((int)(rest - (int64_t)hr * seq.tiles));
-  for (int64_t at = s; at < e;) {
-    const int upto = (int)min((int64_t)seq.tiles, tile + (e - at));
-    part(seq, b, hr / a.row_tiles, hr % a.row_tiles, tile, upto, tile == 0 && upto == seq.tiles, 2 * wave + (at == s ? 0 : 1));
+  const int rest = __builtin_amdgcn_readfirstlane(s - start);
+  int hr = __builtin_amdgcn_readfirstlane(rest / seq.tiles), tile = rest - hr * seq.tiles;
+  for (int at = s; at < e;) {
+    const int upto = min(seq.tiles, tile + (e - at)), slot = 2 * wave + (at == s ? 0 : 1);
+    if (tile == 0 && lane == 0) {
+      int* info = (int*)a.work + 2 * ((int64_t)b * heads + hr);
+      info[0] = slot;
+      info[1] = (at + seq.tiles - 1) / plan.per - wave + 1;
+    }
+    part(seq, b, hr / a.row_tiles, hr % a.row_tiles, tile, upto, tile == 0 && upto == seq.tiles, slot);
     at += upto - tile;
     tile = 0;
     if (++hr == heads && at < e) {
@@ -460,7 +500,7 @@ __global__ __launch_bounds__(64, 1) void paged_kernel(const PagedAttendArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   const int lane = threadIdx.x;
   PagedWave<T, W, NR, NS> w(a, lane, (uint32_t)(uintptr_t)(MODA_LDS char*)lds_raw);
-  walk(a, lane, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int64_t slot) {
+  walk(a, lane, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int slot) {
     w.seq = &seq;
     w.b = b;
     w.h = h;
@@ -477,8 +517,9 @@ __global__ __launch_bounds__(64, 1) void paged_kernel(const PagedAttendArgs a) {
 template <int W>
 __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs a) {
   constexpr int MB = W / 16;
-  const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, T = a.cache.T;
-  walk(a, lane, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int64_t slot) {
+  const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
+  const bool one_token = a.cache.T == 1;
+  walk(a, lane, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int slot) {
     const RowOf row(a, rt, 16, n);
     const float* qp = (const float*)a.q + b * a.sq[0] + row.t * a.sq[1] + row.g * a.sq[2] + h * a.sq[3];
     f32x4 q[MB], o[MB][1];
@@ -490,9 +531,15 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
       o[s][0] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const int first_t = rt * 16 / a.G;
-    for (int half = 2 * t0; half < 2 * t1; half++) {  // 16 keys at a time
+    // 16 keys at a time, the next ones on their way while these are worked on
+    struct Keys {
+      f32x4 k[MB], v[4][MB / 4];
+      uint64_t vp;  // of key n
+      uint32_t there;
+    };
+    auto fetch = [&](int half, Keys& x) {
       const bool depth = half >= 2 * seq.seq_tiles;
-      const int first = (depth ? half - 2 * seq.seq_tiles : half) * 16, key = first + n;
+      const int key = (depth ? half - 2 * seq.seq_tiles : half) * 16 + n;
       const float *kp = nullptr, *vp = nullptr;
       if (!depth) {
         const int page = key < seq.len ? a.cache.page_of(b, key) : -1;
@@ -508,39 +555,42 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
           vp = (const float*)a.vd + b * a.svd[0] + r * a.svd[1] + h * a.svd[2];
         }
       }
-      const uint32_t there = (uint32_t)__ballot(kp != nullptr) & 0xffffu;
-      f32x4 k[MB], v[4][MB / 4];
+      x.vp = (uint64_t)vp;
+      x.there = (uint32_t)__ballot(kp != nullptr) & 0xffffu;
+      // a row that is not there, and pieces past the head dim: zeros
 #pragma unroll
       for (int s = 0; s < MB; s++) {
-        k[s] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (kp && 16 * s + 4 * g < a.D) k[s] = *(const f32x4*)(kp + 16 * s + 4 * g);
+        const bool in = kp && 16 * s + 4 * g < a.D;
+        x.k[s] = *(const f32x4*)(in ? kp + 16 * s + 4 * g : (const float*)zero_line);
       }
-      const float* vrow[4];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        vrow[r] = (const float*)__shfl((unsigned long long)vp, 4 * g + r, 64);
+        const float* row_v = (const float*)__shfl((unsigned long long)x.vp, 4 * g + r, 64);
 #pragma unroll
-        for (int c = 0; c < MB / 4; c++) {
-          v[r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if (vrow[r] && 64 * c + 4 * n < a.Dv) v[r][c] = *(const f32x4*)(vrow[r] + 64 * c + 4 * n);
-        }
+        for (int c = 0; c < MB / 4; c++) x.v[r][c] = *(const f32x4*)(row_v && 64 * c + 4 * n < a.Dv ? row_v + 64 * c + 4 * n : (const float*)zero_line);
       }
+    };
+    auto work = [&](int half, const Keys& x) {
+      const bool depth = half >= 2 * seq.seq_tiles;
+      const int first = (depth ? half - 2 * seq.seq_tiles : half) * 16;
+      const uint32_t there = x.there;
+      const auto& k = x.k;
+      const auto& v = x.v;
       f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < MB; c++)
 #pragma unroll
         for (int i = 0; i < 4; i++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c][i], q[c][i], s, 0, 0, 0);
-      const Window win = depth ? Window{row.t * a.Lv, row.t * a.Lv + a.Lv} : Window{0, seq.past + row.t + 1};
-      const bool all_seen = there == 0xffffu && (depth ? T == 1 : first + 15 <= seq.past + first_t);
       float p[4];
+      const f32x4 sums[1] = {s};
+      scaled(p, sums, a.scale);
+      const Window win = depth ? Window{row.t * a.Lv, row.t * a.Lv + a.Lv} : Window{0, seq.past + row.t + 1};
+      const bool all_seen = there == 0xffffu && (depth ? one_token : first + 15 <= seq.past + first_t);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int j = 4 * g + i;
-        p[i] = all_seen || ((there >> j & 1) && first + j >= win.lo && first + j < win.hi) ? s[i] * a.scale : kNegInf;
-      }
+      for (int i = 0; i < 4; i++) p[i] = win.sees(all_seen, there, first, 4 * g + i) ? p[i] : kNegInf;
       softmax_step<4>(p, m[0], l[0], o, 0);
       bool odd = false;
-      if (!all_seen && T > 1) {
+      if (!all_seen && !one_token) {
 #pragma unroll
         for (int r = 0; r < 4; r++)
 #pragma unroll
@@ -549,17 +599,18 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
             for (int i = 0; i < 4; i++) odd = odd || !(__builtin_fabsf(v[r][c][i]) < __builtin_huge_valf());
       }
       if (__any(odd)) {  // see PagedWave::add_key_by_key
+#pragma unroll 1
         for (int j = 0; j < 16; j++) {
           const int i = j & 3;
-          const float x = __shfl(i == 0 ? p[0] : i == 1 ? p[1] : i == 2 ? p[2] : p[3], n + 16 * (j >> 2), 64);
-          const float* from = (const float*)__shfl((unsigned long long)vp, j, 64);
-          if (!((there >> j & 1) && first + j >= win.lo && first + j < win.hi)) continue;
+          const float w = __shfl(i == 0 ? p[0] : i == 1 ? p[1] : i == 2 ? p[2] : p[3], n + 16 * (j >> 2), 64);
+          const float* from = (const float*)__shfl((unsigned long long)x.vp, j, 64);
+          if (!win.sees(false, there, first, j)) continue;
 #pragma unroll
           for (int c = 0; c < MB; c++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               const int at = 64 * (c / 4) + 16 * g + 4 * e + c % 4;
-              if (at < a.Dv) o[c][0][e] += x * from[at];
+              if (at < a.Dv) o[c][0][e] += w * from[at];
             }
         }
       } else {
@@ -568,7 +619,16 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
 #pragma unroll
           for (int r = 0; r < 4; r++) o[c][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][c / 4][c % 4], p[r], o[c][0], 0, 0, 0);
       }
+    };
+    Keys x[2];
+    fetch(2 * t0, x[0]);
+    for (int half = 2 * t0; half < 2 * t1; half += 2) {
+      fetch(half + 1, x[1]);
+      work(half, x[0]);
+      if (half + 2 < 2 * t1) fetch(half + 2, x[0]);
+      work(half + 1, x[1]);
     }
+    products_done();
     store_part<FP32, W, 1, true>(a, seq, b, h, rt, whole, slot, o, m, l, lane);
   });
 }
@@ -581,33 +641,30 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
 // each of every (NT * 4 / W)-th part.
 template <typename E, int W, int NT>
 __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a, int rows_per_tile) {
-  constexpr int LANES = W / 4, GROUPS = NT / LANES;
-  __shared__ f32x4 sums[NT];
-  __shared__ float lsum[GROUPS], tops[NT / 64];
-  const int tid = threadIdx.x, lane = tid & 63, x = tid % LANES, group = tid / LANES;
+  constexpr int LANES = W / 4, GROUPS = NT / LANES, WAVES = NT / 64;
+  __shared__ f32x4 sums[WAVES][LANES];
+  __shared__ float lsum[WAVES], tops[WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, x = tid % LANES, group = tid / LANES;
   int64_t at = blockIdx.x;
   const int h = (int)(at % a.cache.H);
   at /= a.cache.H;
   const int rows = a.cache.T * a.G, row = (int)(at % rows), b = (int)(at / rows);
   const int rt = row / rows_per_tile, r = row - rt * rows_per_tile, t = row / a.G, g = row - t * a.G;
-  const Plan plan(a, lane);
-  int64_t start = 0;
-  for (int i = lane; i < b; i += 64) start += Seq(a, i).tiles;
-  start = wave_sum(start) * (a.cache.H * a.row_tiles);
-  const int tiles = Seq(a, b).tiles;
-  start += (int64_t)(h * a.row_tiles + rt) * tiles;
-  int64_t w0 = start / plan.per, w1 = tiles ? (start + tiles - 1) / plan.per : w0;
-  if (tiles && w0 == w1) return;  // one wave had all of it and has stored the row
-  const int parts = tiles ? (int)(w1 - w0 + 1) : 0;
-  auto slot = [&](int p) { return 2 * (w0 + p) + (p == 0 && start != w0 * plan.per ? 1 : 0); };
+  const int64_t seg = ((int64_t)b * a.cache.H + h) * a.row_tiles + rt;
+  const int first = ((const int*)a.work)[2 * seg], count = ((const int*)a.work)[2 * seg + 1];
+  const int parts = Seq(a, b).tiles ? count : 0;
+  if (parts == 1) return;  // one wave had all of it and has stored the row
+  auto slot = [&](int p) { return p == 0 ? first : (first & ~1) + 2 * p; };
   float top = kNegInf;
   for (int p = tid; p < parts; p += NT) top = fmaxf(top, PartAt(a, slot(p)).ml[2 * r]);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-  if (lane == 0) tops[tid >> 6] = top;
-  __syncthreads();
+  if (WAVES > 1) {
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < NT / 64; i++) top = fmaxf(top, tops[i]);
+    for (int i = 0; i < WAVES; i++) top = fmaxf(top, tops[i]);
+  }
   const float from = top == kNegInf ? 0.f : top;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float l = 0.f;
@@ -620,18 +677,28 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a,
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] += w * v[i];
   }
-  sums[tid] = o;
-  if (x == 0) lsum[group] = l;
-  __syncthreads();
-  if (group > 0) return;
-  l = 0.f;
-  o = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < GROUPS; i++) {
-    l += lsum[i];
-    const f32x4 v = sums[i * LANES + x];
 #pragma unroll
-    for (int e = 0; e < 4; e++) o[e] += v[e];
+  for (int d = LANES; d < 64; d <<= 1) {  // groups of one wave, then waves
+    l += __shfl_xor(l, d, 64);
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] += __shfl_xor(o[i], d, 64);
   }
+  if (WAVES > 1) {
+    if (lane < LANES) sums[wave][x] = o;
+    if (lane == 0) lsum[wave] = l;
+    __syncthreads();
+    if (wave > 0) return;
+    l = lsum[0];
+    o = sums[0][x];
+#pragma unroll
+    for (int i = 1; i < WAVES; i++) {
+      l += lsum[i];
+      const f32x4 v = sums[i][x];
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] += v[e];
+    }
+  }
+  if (lane >= LANES) return;
   const bool empty = l == 0.f;
   const float inv = empty ? 0.f : 1.f / l;
   const int64_t to = b * a.so[0] + t * a.so[1] + g * a.so[2] + h * a.so[3];
@@ -667,18 +734,22 @@ hipError_t launch_waves_as(const PagedAttendArgs& a, int width, int blocks, hipS
   if (width == 128) return blocks == 1 ? launch_waves<T, 128, 1, 2>(a, stream) : launch_waves<T, 128, 2, 2>(a, stream);
   return blocks == 1 ? launch_waves<T, 64, 1, 4>(a, stream) : blocks == 2 ? launch_waves<T, 64, 2, 4>(a, stream) : launch_waves<T, 64, 4, 4>(a, stream);
 }
+// Threads of a row's workgroup: parts of one row are read side by side, and many rows keep the card busy by themselves.
+template <typename E, int W>
+hipError_t launch_join_of(const PagedAttendArgs& a, int per_tile, hipStream_t stream) {
+  const unsigned rows = (unsigned)((int64_t)a.cache.B * a.cache.T * a.G * a.cache.H);
+  if (rows >= 2048)
+    paged_join_kernel<E, W, 64><<<rows, 64, 0, stream>>>(a, per_tile);
+  else if (rows >= 256)
+    paged_join_kernel<E, W, 256><<<rows, 256, 0, stream>>>(a, per_tile);
+  else
+    paged_join_kernel<E, W, 1024><<<rows, 1024, 0, stream>>>(a, per_tile);
+  return hipGetLastError();
+}
 template <typename E>
 hipError_t launch_join(const PagedAttendArgs& a, int width, int blocks, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.cache.B * a.cache.T * a.G * a.cache.H;
-  const unsigned grid = (unsigned)rows;
-  const int per_tile = 16 * blocks;
-  if (width == 64)
-    paged_join_kernel<E, 64, 256><<<grid, 256, 0, stream>>>(a, per_tile);
-  else if (width == 128)
-    paged_join_kernel<E, 128, 256><<<grid, 256, 0, stream>>>(a, per_tile);
-  else
-    paged_join_kernel<E, 256, 256><<<grid, 256, 0, stream>>>(a, per_tile);
-  return hipGetLastError();
+  if (width == 64) return launch_join_of<E, 64>(a, 16 * blocks, stream);
+  return width == 128 ? launch_join_of<E, 128>(a, 16 * blocks, stream) : launch_join_of<E, 256>(a, 16 * blocks, stream);
 }
 
 }  // namespace
@@ -695,8 +766,10 @@ size_t plan_paged_attend(PagedAttendArgs& a, int dtype) {
   const int64_t capacity = (int64_t)a.cache.max_pages << a.cache.page_shift;
   const int64_t most = (int64_t)a.cache.B * a.cache.H * a.row_tiles *
                        ((capacity + kTileKeys - 1) / kTileKeys + ((int64_t)a.cache.T * a.Lv + kTileKeys - 1) / kTileKeys);
+  if (most >= 1ll << 30) return 0;  // the axis is counted in 32 bits
   a.waves = (int)(most < 256 * per_unit ? (most > 0 ? most : 1) : 256 * per_unit);
-  return (size_t)2 * a.waves * a.part_rows * (a.part_width + 2) * sizeof(float);
+  const size_t segments = ((size_t)a.cache.B * a.cache.H * a.row_tiles + 1) / 2 * 2;
+  return (segments * 2 + (size_t)2 * a.waves * a.part_rows * (a.part_width + 2)) * sizeof(float);
 }
 
 hipError_t launch_paged_attend(const PagedAttendArgs& a, int dtype, hipStream_t stream) {
