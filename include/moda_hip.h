@@ -366,7 +366,7 @@ int moda_hip_rotary_rows(int32_t dtype, int64_t B, int64_t T, int64_t D, const m
 /*
  * A paged key/value cache: k_pages [n_pages, page_size, H, D], v_pages [n_pages, page_size, H, Dv] with element strides
  * {page, token in the page, head} and unit inner stride, rows on 16-byte boundaries (base and strides; MODA_HIP_EALIGN
- * otherwise), page_size a power of two, n_pages * page_size and max_pages * page_size below 2^31.  DEVICE arrays: position p of
+ * otherwise), page_size a power of two, n_pages * page_size and max_pages * page_size below 2^31, max_pages below 2^28.  DEVICE arrays: position p of
  * sequence b lies in page table[b * table_stride + p / page_size], max_pages entries a sequence; past[b] tokens of it were there
  * before the call; of its T new tokens new_lens[b] are real (NULL: T).  Counts are taken as at least 0 and past + new tokens as at
  * most max_pages * page_size; a table entry outside [0, n_pages) names no page: its tokens are not stored and not seen.
@@ -381,7 +381,7 @@ int moda_hip_rotary_rows(int32_t dtype, int64_t B, int64_t T, int64_t D, const m
  * and over the L_valid first slots (0: all L) of its own token in kd, vd [B, T * L, H, *].  q, o: [B, T * G, H, *], rows t * G + g,
  * lse [B, T * G, H] fp32 base 2; with `plain` [B, T, H * G, *], heads h * G + g, lse [B, T, H * G].  Rows that see nothing, padded
  * ones among them, have o = 0 and lse = -inf.  cu_seqlens NULL.  All rows on 16-byte boundaries.
- * Head dims up to 256, multiples of 8 (fp32: of 4); B * H * (max_pages * page_size + T * L) / 32 below 2^30 (times T * G / 16 where that
+ * Head dims up to 256, multiples of 8 (fp32: of 4); T * G up to 2^16; B * H * (max_pages * page_size + T * L) / 32 below 2^30 (times T * G / 16 where that
  * is more than 1); MODA_HIP_EUNSUPPORTED otherwise.
  */
 typedef struct moda_hip_paged_cache {

@@ -737,7 +737,7 @@ int fill_cache(const moda_hip_paged_cache* c, moda::PagedKV& to) {
     return MODA_HIP_EINVAL;
   const int64_t step = c->dtype == MODA_HIP_FP32 ? 4 : 8, most = 1ll << 31;
   if (c->D > 256 || c->Dv > 256 || c->D % step != 0 || c->Dv % step != 0 || !is_power_of_two(c->page_size)) return MODA_HIP_EUNSUPPORTED;
-  if (c->n_pages >= most || c->max_pages >= most || c->page_size >= most || c->n_pages * c->page_size >= most ||
+  if (c->n_pages >= most || c->max_pages >= (1 << 28) || c->page_size >= most || c->n_pages * c->page_size >= most ||
       c->max_pages * c->page_size >= most || c->B >= (1 << 20) || c->T >= (1 << 24) || c->H >= (1 << 16) || c->B * c->T >= most ||
       c->total_tokens >= most)
     return MODA_HIP_EUNSUPPORTED;
@@ -862,7 +862,7 @@ int fill_attend(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_a
   if (!t || t->struct_size != (int32_t)sizeof(*t) || cache->cu_seqlens || t->G <= 0 || t->L < 0 || t->L_valid < 0 || t->L_valid > t->L ||
       (t->plain && t->L > 0))
     return MODA_HIP_EINVAL;
-  if (t->G >= (1 << 15) || cache->T * t->G >= (1 << 24) || t->L >= (1 << 20) || cache->T * t->L >= (1 << 30) ||
+  if (t->G >= (1 << 15) || cache->T * t->G > (1 << 16) || t->L >= (1 << 20) || cache->T * t->L >= (1 << 30) ||
       cache->B * cache->T * t->G * cache->H >= (1ll << 31))
     return MODA_HIP_EUNSUPPORTED;
   a.G = (int)t->G;

@@ -77,7 +77,8 @@ struct PagedAttendArgs {
   float scale;  // of logits in base 2
   float* work;
   // how the work is cut (plan_paged_attend)
-  int waves, least_tiles, row_tiles, part_rows, part_width;
+  int waves, least_tiles, row_tiles, part_rows, part_width, even_pages, even_slots;
+  unsigned group_magic;
 };
 
 }  // namespace moda

@@ -26,23 +26,34 @@ constexpr int kTileKeys = 32;
 // what invalid rows and chunks past a head dim read
 __device__ __align__(64) uint32_t zero_line[16];
 
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
+// Sum over lanes 0 .. l in lane l.
+__device__ __forceinline__ int wave_scan(int x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8: within 16 lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
+#endif
   return x;
 }
 
 // Sequence b on the axis: positions that its last new token sees, tiles of them and of its new tokens' depth slots.
 struct Seq {
   int past, fresh, len, seq_tiles, tiles;
-  __device__ __forceinline__ Seq(const PagedAttendArgs& a, int b) {
-    fresh = a.cache.new_of(b);
-    past = a.cache.past_of(b);
+  __device__ __forceinline__ Seq(const PagedAttendArgs& a, int b) : Seq(a, a.cache.past_of(b), a.cache.new_of(b)) {}
+  __device__ __forceinline__ Seq(const PagedAttendArgs& a, int past_, int fresh_) : past(past_), fresh(fresh_) {
     len = fresh > 0 ? min(past + fresh, a.cache.capacity()) : 0;
     seq_tiles = (len + kTileKeys - 1) / kTileKeys;
     tiles = seq_tiles + (fresh * a.Lv + kTileKeys - 1) / kTileKeys;
   }
 };
+
+// of one sequence for the whole wave, in scalar registers
+__device__ __forceinline__ Seq uniform_seq(const PagedAttendArgs& a, int b) {
+  return Seq(a, __builtin_amdgcn_readfirstlane(a.cache.past_of(b)), __builtin_amdgcn_readfirstlane(a.cache.new_of(b)));
+}
 
 // Tiles on the whole axis, and how many of them a wave takes.  The host has made sure that they fit 32 bits.
 struct Plan {
@@ -53,16 +64,11 @@ struct Plan {
   }
 };
 
-// One 16-byte (or 4-byte) piece a lane, global -> LDS, lane l to lds + l * BYTES.  Inline assembly as in tile.h (lds_dma): the
-// compiler does not see these loads and so puts no waits between them and later LDS reads; whoever reads the tile
-// waits by count.  Addresses of its own for every lane: pages lie anywhere in memory.
-template <int BYTES>
+// One 16-byte piece a lane, global -> LDS, lane l to lds + l * 16, from an address of its own; inline assembly for the reason
+// lds_dma (tile.h) gives: the compiler puts no waits between these loads and later LDS reads, whoever reads the tile waits by count.
 __device__ __forceinline__ void global_to_lds(uint32_t lds, uint64_t address) {
   const uint32_t m0v = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
-  if (BYTES == 16)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0v), "v"(address) : "memory", "m0");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, off" : : "s"(m0v), "v"(address) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0v), "v"(address) : "memory", "m0");
 }
 template <int K>
 __device__ __forceinline__ void wait_but() {
@@ -101,7 +107,7 @@ struct RowOf {
   __device__ __forceinline__ RowOf(const PagedAttendArgs& a, int rt, int rows, int r) {
     const int row = rt * rows + r;
     real = row < a.cache.T * a.G;
-    t = row / a.G;
+    t = a.group_magic ? (int)__umulhi((unsigned)row, a.group_magic) : row;
     g = row - t * a.G;
   }
 };
@@ -168,8 +174,8 @@ __device__ __forceinline__ void products_done() { asm volatile("s_nop 15\n\ts_no
 struct Window {
   int lo, hi;
   // key `key` of a tile that begins at index `first` and holds the keys `there`
-  __device__ __forceinline__ bool sees(bool all, uint32_t there, int first, int key) const {
-    return all | ((there >> key & 1) & (first + key >= lo) & (first + key < hi));
+  __device__ __forceinline__ bool sees(uint32_t there, int first, int key) const {
+    return (there >> key & 1) & (first + key >= lo) & (first + key < hi);
   }
 };
 
@@ -223,10 +229,10 @@ struct PagedWave {
   float m[NR], l[NR];
   // the segment
   int b, h, rt;
-  const Seq* seq;
+  Seq seq;
   uint64_t zero;
 
-  __device__ __forceinline__ PagedWave(const PagedAttendArgs& args, int lane_, uint32_t lds_) : a(args), lane(lane_), lds(lds_) {
+  __device__ __forceinline__ PagedWave(const PagedAttendArgs& args, int lane_, uint32_t lds_) : a(args), lane(lane_), lds(lds_), seq(args, 0, 0) {
     oa.init(lane);
     zero = (uint64_t)&zero_line[0];
   }
@@ -235,51 +241,90 @@ struct PagedWave {
     return (MODA_LDS P*)(uintptr_t)(lds + byte);
   }
 
-  // table entries of a tile's positions (lanes r and r + 32: row r)
+  // table entries of a tile's positions (lanes r and r + 32: row r); past the sequence's pages: zeros
   __device__ __forceinline__ void fetch_table(int tile, int ring) const {
-    const int j = tile * kTileKeys + (lane & 31);
-    const bool in = tile < seq->seq_tiles && j < seq->len;
-    const uint64_t p = (uint64_t)(a.cache.table + b * a.cache.table_stride + (j >> a.cache.page_shift));
-    global_to_lds<4>(lds + Lds::kTable + ring * 256, in ? p : zero);
+    const int pages = (seq.len + (1 << a.cache.page_shift) - 1) >> a.cache.page_shift;
+    const i32x4 rs = rsrc_words(a.cache.table + b * a.cache.table_stride, (uint32_t)pages * 4);
+    const unsigned page = ((unsigned)tile * kTileKeys + (lane & 31)) >> a.cache.page_shift;
+    lds_dma<4>(rs, lds + Lds::kTable + ring * 256, tile < seq.seq_tiles ? (int)(page * 4) : kPadOffset, 0);
   }
-  // where the rows of a tile lie, from its table entries; an address of zero: nowhere
-  __device__ __forceinline__ void find_rows(int tile, int ring, int stage) const {
+  // Where the rows of a tile lie.  In sixteens of evenly spaced rows where pages and strides allow (even: pages of 16 tokens and more,
+  // or the depth slots of a single token): two base addresses of K, two of V and how many rows there are, in scalar registers.
+  // Else the address of every row, in LDS; zero: nowhere.
+  bool even;
+  uint64_t base[2][2];
+  int rows[2], stride[2];
+  __device__ __forceinline__ void find_rows(int tile, int ring, int stage) {
     const int r = lane & 31;
-    uint64_t kp = 0, vp = 0;
-    if (tile < seq->seq_tiles) {
-      const int j = tile * kTileKeys + r, page = *at<int>(Lds::kTable + ring * 256 + 4 * lane);
-      if (j < seq->len && (unsigned)page < (unsigned)a.cache.n_pages) {
-        kp = (uint64_t)(a.cache.k + 2 * a.cache.offset(a.cache.sk, page, j, h));
-        vp = (uint64_t)(a.cache.v + 2 * a.cache.offset(a.cache.sv, page, j, h));
+    const bool depth = tile >= seq.seq_tiles;
+    even = depth ? a.even_slots : a.even_pages;
+    uint32_t there;
+    if (even) {
+      const int entry = *at<int>(Lds::kTable + ring * 256 + 4 * lane);
+      const int first = (depth ? tile - seq.seq_tiles : tile) * kTileKeys, count = depth ? a.Lv : seq.len;
+      there = 0;
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        const int j = first + 16 * hf, page = depth ? 0 : __builtin_amdgcn_readlane(entry, 16 * hf);
+        rows[hf] = (unsigned)page < (unsigned)a.cache.n_pages ? max(0, min(16, count - j)) : 0;
+        const int64_t ko = depth ? b * a.skd[0] + j * a.skd[1] + h * a.skd[2] : a.cache.offset(a.cache.sk, page, j, h);
+        const int64_t vo = depth ? b * a.svd[0] + j * a.svd[1] + h * a.svd[2] : a.cache.offset(a.cache.sv, page, j, h);
+        base[hf][0] = (uint64_t)((depth ? a.kd : a.cache.k) + 2 * ko);
+        base[hf][1] = (uint64_t)((depth ? a.vd : a.cache.v) + 2 * vo);
+        there |= ((1u << rows[hf]) - 1) << (16 * hf);
       }
+      stride[0] = (int)(2 * (depth ? a.skd[1] : a.cache.sk[1]));
+      stride[1] = (int)(2 * (depth ? a.svd[1] : a.cache.sv[1]));
     } else {
-      const int col = (tile - seq->seq_tiles) * kTileKeys + r, t = col / a.Lv;
-      if (t < seq->fresh) {
-        const int64_t row = (int64_t)t * a.L + (col - t * a.Lv);
-        kp = (uint64_t)(a.kd + 2 * (b * a.skd[0] + row * a.skd[1] + h * a.skd[2]));
-        vp = (uint64_t)(a.vd + 2 * (b * a.svd[0] + row * a.svd[1] + h * a.svd[2]));
+      uint64_t kp = 0, vp = 0;
+      if (!depth) {
+        const int j = tile * kTileKeys + r, page = *at<int>(Lds::kTable + ring * 256 + 4 * lane);
+        if (j < seq.len && (unsigned)page < (unsigned)a.cache.n_pages) {
+          kp = (uint64_t)(a.cache.k + 2 * a.cache.offset(a.cache.sk, page, j, h));
+          vp = (uint64_t)(a.cache.v + 2 * a.cache.offset(a.cache.sv, page, j, h));
+        }
+      } else {
+        const int col = (tile - seq.seq_tiles) * kTileKeys + r, t = col / a.Lv;
+        if (t < seq.fresh) {
+          const int64_t row = (int64_t)t * a.L + (col - t * a.Lv);
+          kp = (uint64_t)(a.kd + 2 * (b * a.skd[0] + row * a.skd[1] + h * a.skd[2]));
+          vp = (uint64_t)(a.vd + 2 * (b * a.svd[0] + row * a.svd[1] + h * a.svd[2]));
+        }
       }
-    }
-    const uint32_t there = (uint32_t)__ballot(kp != 0);
-    if (lane < 32) {
-      *at<uint64_t>(Lds::kRows + 16 * r) = kp;
-      *at<uint64_t>(Lds::kRows + 16 * r + 8) = vp;
+      there = (uint32_t)__ballot(kp != 0);
+      if (lane < 32) {
+        *at<uint64_t>(Lds::kRows + 16 * r) = kp;
+        *at<uint64_t>(Lds::kRows + 16 * r + 8) = vp;
+      }
     }
     if (lane == 0) *at<uint32_t>(Lds::kMask + 4 * stage) = there;
   }
   // a K (0) or V (1) tile, from the rows found last
   __device__ __forceinline__ void fetch_tile(int which, int stage) const {
     const int prow = lane / CH, pch = lane % CH, dim = which ? a.Dv : a.D;
+    const uint32_t to = lds + stage * Lds::kStage + which * Lds::kTile;
+    if (even) {
+#pragma unroll
+      for (int i = 0; i < NL; i++) {
+        const int row = (i * RPW + prow) & 15, hf = i * RPW / 16, chunk = pch ^ Tile<W>::swz(row);
+        // the range check fills with zeros what lies past the last row and past the head dim
+        const i32x4 rs = rsrc_words((const void*)base[hf][which], (uint32_t)(rows[hf] * stride[which]));
+        lds_dma<16>(rs, to + i * 1024, chunk * 8 < dim ? row * stride[which] + chunk * 16 : kPadOffset, 0);
+      }
+      return;
+    }
+    uint64_t from[NL];
+#pragma unroll
+    for (int i = 0; i < NL; i++) from[i] = *at<uint64_t>(Lds::kRows + 16 * (i * RPW + prow) + 8 * which);
 #pragma unroll
     for (int i = 0; i < NL; i++) {
-      const int row = i * RPW + prow, chunk = pch ^ Tile<W>::swz(row);
-      const uint64_t p = *at<uint64_t>(Lds::kRows + 16 * row + 8 * which);
-      global_to_lds<16>(lds + stage * Lds::kStage + which * Lds::kTile + i * 1024, p != 0 && chunk * 8 < dim ? p + chunk * 16 : zero);
+      const int chunk = pch ^ Tile<W>::swz(i * RPW + prow);
+      global_to_lds(to + i * 1024, from[i] != 0 && chunk * 8 < dim ? from[i] + chunk * 16 : zero);
     }
   }
 
   // the K tile of step i + NS, the tile's rows, and the table entries of the tile NS steps further
-  __device__ __forceinline__ void send(int tile, int i, int stage) const {
+  __device__ __forceinline__ void send(int tile, int i, int stage) {
     fetch_table(tile + 2 * NS, (i + 2 * NS) % (2 * NS));
     find_rows(tile + NS, (i + NS) % (2 * NS), stage);
     fetch_tile(0, stage);
@@ -296,7 +341,7 @@ struct PagedWave {
 #pragma unroll
       for (int i = 1; i < 8; i++) x = i == (key >> 4) * 4 + (key & 3) ? p[i] : x;
       x = __shfl(x, n + 16 * from, 64);
-      if (!win.sees(false, there, first, key)) continue;
+      if (!win.sees(there, first, key)) continue;
 #pragma unroll
       for (int c = 0; c < MB; c++) {
         const int e = 16 * c + 4 * g;
@@ -328,7 +373,7 @@ struct PagedWave {
         if (row.real && e < a.D) x = *(const i32x4*)(a.q + 2 * (from + e));
         q[nr][ks] = x;
       }
-      seq_win[nr] = {0, seq->past + row.t + 1};
+      seq_win[nr] = {0, seq.past + row.t + 1};
       depth_win[nr] = {row.t * a.Lv, row.t * a.Lv + a.Lv};
       m[nr] = kNegInf;
       l[nr] = 0.f;
@@ -375,19 +420,22 @@ struct PagedWave {
       }
       WaveTileLoader<64>::reads_done();
       if (more) send(tile, i, stage);
-      const bool depth = tile >= seq->seq_tiles;
-      const int first = (depth ? tile - seq->seq_tiles : tile) * kTileKeys;
-      const bool all_seen = there == ~0u && (depth ? one_token : first + kTileKeys - 1 <= seq->past + first_t);
+      const bool depth = tile >= seq.seq_tiles;
+      const int first = (depth ? tile - seq.seq_tiles : tile) * kTileKeys;
+      const bool all_seen = there == ~0u && (depth ? one_token : first + kTileKeys - 1 <= seq.past + first_t);
+      if (!all_seen) {
 #pragma unroll
-      for (int nr = 0; nr < NR; nr++) {
-        const Window win = depth ? depth_win[nr] : seq_win[nr];
+        for (int nr = 0; nr < NR; nr++) {
+          const Window win = depth ? depth_win[nr] : seq_win[nr];
 #pragma unroll
-        for (int i8 = 0; i8 < 8; i8++) {
-          const int key = 16 * (i8 >> 2) + slot_base(g) + (i8 & 3);
-          p[nr][i8] = win.sees(all_seen, there, first, key) ? p[nr][i8] : kNegInf;
+          for (int i8 = 0; i8 < 8; i8++) {
+            const int key = 16 * (i8 >> 2) + slot_base(g) + (i8 & 3);
+            p[nr][i8] = win.sees(there, first, key) ? p[nr][i8] : kNegInf;
+          }
         }
-        softmax_step<8>(p[nr], m[nr], l[nr], o, nr);
       }
+#pragma unroll
+      for (int nr = 0; nr < NR; nr++) softmax_step<8>(p[nr], m[nr], l[nr], o, nr);
       if (more)
         wait_but<kBehindV>();
       else
@@ -449,32 +497,27 @@ struct PagedWave {
 template <typename F>
 __device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, F&& part) {
   const int heads = a.cache.H * a.row_tiles;
-  // up to 64 sequences are read once; of more the first pass is for the total alone
+  // Up to 64 sequences are read once; of more the first pass over the others is for the total alone.
   int own = lane < a.cache.B ? Seq(a, lane).tiles : 0, sum = own;
   for (int b = lane + 64; b < a.cache.B; b += 64) sum += Seq(a, b).tiles;
-  const Plan plan(a, wave_sum(sum));
+  const Plan plan(a, __builtin_amdgcn_readlane(wave_scan(sum), 63));
   const int wave = blockIdx.x;
   if ((int64_t)wave * plan.per >= plan.total) return;
-  const int s = wave * plan.per, e = min(s + plan.per, plan.total);  // (per <= total / waves + 1 or least_tiles: s + per fits)
+  const int s = wave * plan.per, e = min(s + plan.per, plan.total);
   int b = 0, start = 0;  // start of sequence b, in tiles
   for (int b0 = 0; b0 < a.cache.B; b0 += 64) {
     if (b0 > 0) own = b0 + lane < a.cache.B ? Seq(a, b0 + lane).tiles : 0;
-    int upto = own;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int x = __shfl_up(upto, d, 64);
-      if (lane >= d) upto += x;
-    }
+    const int upto = wave_scan(own);
     const uint64_t behind = __ballot(start + upto * heads > s);
     const int first = behind ? __builtin_ctzll(behind) : 63;
-    start += __shfl(behind ? upto - own : upto, first, 64) * heads;
+    start += __builtin_amdgcn_readlane(behind ? upto - own : upto, first) * heads;
     if (behind) {
       b = b0 + first;
       break;
     }
   }
   b = __builtin_amdgcn_readfirstlane(b);
-  Seq seq(a, b);
+  Seq seq = uniform_seq(a, b);
   const int rest = __builtin_amdgcn_readfirstlane(s - start);
   int hr = __builtin_amdgcn_readfirstlane(rest / seq.tiles), tile = rest - hr * seq.tiles;
   for (int at = s; at < e;) {
@@ -489,7 +532,7 @@ __device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, F&& par
     tile = 0;
     if (++hr == heads && at < e) {
       hr = 0;
-      do seq = Seq(a, ++b);
+      do seq = uniform_seq(a, ++b);
       while (seq.tiles == 0);
     }
   }
@@ -501,7 +544,7 @@ __global__ __launch_bounds__(64, 1) void paged_kernel(const PagedAttendArgs a) {
   const int lane = threadIdx.x;
   PagedWave<T, W, NR, NS> w(a, lane, (uint32_t)(uintptr_t)(MODA_LDS char*)lds_raw);
   walk(a, lane, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int slot) {
-    w.seq = &seq;
+    w.seq = seq;
     w.b = b;
     w.h = h;
     w.rt = rt;
@@ -587,7 +630,7 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
       const Window win = depth ? Window{row.t * a.Lv, row.t * a.Lv + a.Lv} : Window{0, seq.past + row.t + 1};
       const bool all_seen = there == 0xffffu && (depth ? one_token : first + 15 <= seq.past + first_t);
 #pragma unroll
-      for (int i = 0; i < 4; i++) p[i] = win.sees(all_seen, there, first, 4 * g + i) ? p[i] : kNegInf;
+      for (int i = 0; i < 4; i++) p[i] = all_seen | win.sees(there, first, 4 * g + i) ? p[i] : kNegInf;
       softmax_step<4>(p, m[0], l[0], o, 0);
       bool odd = false;
       if (!all_seen && !one_token) {
@@ -604,7 +647,7 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
           const int i = j & 3;
           const float w = __shfl(i == 0 ? p[0] : i == 1 ? p[1] : i == 2 ? p[2] : p[3], n + 16 * (j >> 2), 64);
           const float* from = (const float*)__shfl((unsigned long long)x.vp, j, 64);
-          if (!win.sees(false, there, first, j)) continue;
+          if (!win.sees(there, first, j)) continue;
 #pragma unroll
           for (int c = 0; c < MB; c++)
 #pragma unroll
@@ -767,6 +810,11 @@ size_t plan_paged_attend(PagedAttendArgs& a, int dtype) {
   const int64_t most = (int64_t)a.cache.B * a.cache.H * a.row_tiles *
                        ((capacity + kTileKeys - 1) / kTileKeys + ((int64_t)a.cache.T * a.Lv + kTileKeys - 1) / kTileKeys);
   if (most >= 1ll << 30) return 0;  // the axis is counted in 32 bits
+  a.group_magic = a.G == 1 ? 0 : (unsigned)((1ull << 32) / a.G) + 1;  // row / G = umulhi(row, magic): rows are below 2^16
+  // sixteen rows through one buffer descriptor: 31-bit offsets, rows that do not reach into the next one
+  const auto even = [&](const int64_t(&s)[3], int dim) { return s[1] >= dim && s[1] < 1 << 25; };
+  a.even_pages = a.cache.page_shift >= 4 && even(a.cache.sk, a.D) && even(a.cache.sv, a.Dv);
+  a.even_slots = a.cache.T == 1 && even(a.skd, a.D) && even(a.svd, a.Dv);
   a.waves = (int)(most < 256 * per_unit ? (most > 0 ? most : 1) : 256 * per_unit);
   const size_t segments = ((size_t)a.cache.B * a.cache.H * a.row_tiles + 1) / 2 * 2;
   return (segments * 2 + (size_t)2 * a.waves * a.part_rows * (a.part_width + 2)) * sizeof(float);
