@@ -55,12 +55,21 @@ __device__ __forceinline__ Seq uniform_seq(const PagedAttendArgs& a, int b) {
   return Seq(a, __builtin_amdgcn_readfirstlane(a.cache.past_of(b)), __builtin_amdgcn_readfirstlane(a.cache.new_of(b)));
 }
 
+// x / d for whole numbers of a wave, d > 0: an estimate in 32-bit floating point, put right (a division of integers is forty
+// instructions one after the other, which a wave by itself waits for).
+__device__ __forceinline__ int uniform_div(int x, int d) {
+  int q = __builtin_amdgcn_readfirstlane((int)((float)x * __builtin_amdgcn_rcpf((float)d)));
+  while ((int64_t)q * d > x) q--;
+  while ((int64_t)(q + 1) * d <= x) q++;
+  return q;
+}
+
 // Tiles on the whole axis, and how many of them a wave takes.  The host has made sure that they fit 32 bits.
 struct Plan {
   int total, per;
   __device__ __forceinline__ Plan(const PagedAttendArgs& a, int tiles_of_one_head) {
     total = tiles_of_one_head * (a.cache.H * a.row_tiles);
-    per = max((int)(((unsigned)total + a.waves - 1) / (unsigned)a.waves), a.least_tiles);
+    per = max(uniform_div(total + a.waves - 1, a.waves), a.least_tiles);
   }
 };
 
@@ -75,8 +84,8 @@ __device__ __forceinline__ void wait_but() {
   WaveTileLoader<64>::wait_but<K>();
 }
 
-// The workspace: for each segment the slot of its first part and how many there are (written by the wave that has its first tile;
-// a segment without tiles has none), then statistics and sums by slot.
+// The workspace: for each segment the slot of its first part and the wave of its last (written by the waves that have its first and
+// its last tile; a segment without tiles has none), then statistics and sums by slot.
 __device__ __forceinline__ int64_t segments(const PagedAttendArgs& a) {
   return ((int64_t)a.cache.B * a.cache.H * a.row_tiles + 1) & ~1ll;  // even: what follows stays on 16 bytes
 }
@@ -170,6 +179,16 @@ __device__ __forceinline__ void scaled(float* x, const f32x4 (&s)[N], float scal
 // ... and before the results of the last products are read behind a loop or a branch: 32 wait states
 __device__ __forceinline__ void products_done() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
+// Maximum over the four lanes of a row.
+__device__ __forceinline__ float row_max(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int xi = __builtin_bit_cast(int, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(xi, xi, false, false);
+  x = fmaxf(__builtin_bit_cast(float, (int)r[0]), __builtin_bit_cast(float, (int)r[1]));
+#endif
+  return pair_max(x);
+}
+
 // Which keys row `nr` of a lane sees in a tile: indices [lo, hi) of the sequence's positions, or of its depth columns.
 struct Window {
   int lo, hi;
@@ -186,7 +205,7 @@ __device__ __forceinline__ void softmax_step(float (&x)[N], float& m, float& l, 
   float top = x[0];
 #pragma unroll
   for (int i = 1; i < N; i++) top = fmaxf(top, x[i]);
-  top = fmaxf(m, quad_max(top));
+  top = fmaxf(m, row_max(top));
   const float from = top == kNegInf ? 0.f : top;
   if (__any(top != m)) {  // (a NaN never equals itself: the sums become NaN with it)
     const float shrink = fast_exp2(m - from);
@@ -230,11 +249,25 @@ struct PagedWave {
   // the segment
   int b, h, rt;
   Seq seq;
-  uint64_t zero;
+  const char *k_head, *v_head;
+  // byte offsets of the lane's piece of a tile, loads i and i + kPeriod (16 rows apart) alike
+  static constexpr int kPeriod = 16 / RPW;
+  int piece[2][kPeriod];
 
-  __device__ __forceinline__ PagedWave(const PagedAttendArgs& args, int lane_, uint32_t lds_) : a(args), lane(lane_), lds(lds_), seq(args, 0, 0) {
+  __device__ __forceinline__ PagedWave(const PagedAttendArgs& args, int lane_, uint32_t lds_) : a(args), lane(lane_), lds(lds_), seq(args, 0, 0) {}
+  __device__ __forceinline__ void init() {
     oa.init(lane);
-    zero = (uint64_t)&zero_line[0];
+    const int prow = lane / CH, pch = lane % CH;
+#pragma unroll
+    for (int i = 0; i < kPeriod; i++) {
+      const int row = i * RPW + prow, chunk = pch ^ Tile<W>::swz(row);
+#pragma unroll
+      for (int which = 0; which < 2; which++) {
+        const int step = (int)(2 * (which ? a.cache.sv[1] : a.cache.sk[1]));
+        piece[which][i] = chunk * 8 < (which ? a.Dv : a.D) ? row * step + chunk * 16 : kPadOffset;
+        asm volatile("" : "+v"(piece[which][i]));
+      }
+    }
   }
   template <typename P>
   __device__ __forceinline__ MODA_LDS P* at(int byte) const {
@@ -249,32 +282,39 @@ struct PagedWave {
     lds_dma<4>(rs, lds + Lds::kTable + ring * 256, tile < seq.seq_tiles ? (int)(page * 4) : kPadOffset, 0);
   }
   // Where the rows of a tile lie.  In sixteens of evenly spaced rows where pages and strides allow (even: pages of 16 tokens and more,
-  // or the depth slots of a single token): two base addresses of K, two of V and how many rows there are, in scalar registers.
-  // Else the address of every row, in LDS; zero: nowhere.
+  // or the depth slots of a single token at the pages' spacing): base addresses and how many rows there are, in scalar
+  // registers.  Else the address of every row, in LDS; zero: nowhere.
   bool even;
   uint64_t base[2][2];
-  int rows[2], stride[2];
+  int rows[2];
   __device__ __forceinline__ void find_rows(int tile, int ring, int stage) {
     const int r = lane & 31;
     const bool depth = tile >= seq.seq_tiles;
     even = depth ? a.even_slots : a.even_pages;
     uint32_t there;
     if (even) {
-      const int entry = *at<int>(Lds::kTable + ring * 256 + 4 * lane);
-      const int first = (depth ? tile - seq.seq_tiles : tile) * kTileKeys, count = depth ? a.Lv : seq.len;
-      there = 0;
+      if (!depth) {
+        const int entry = *at<int>(Lds::kTable + ring * 256 + 4 * lane), first = tile * kTileKeys;
 #pragma unroll
-      for (int hf = 0; hf < 2; hf++) {
-        const int j = first + 16 * hf, page = depth ? 0 : __builtin_amdgcn_readlane(entry, 16 * hf);
-        rows[hf] = (unsigned)page < (unsigned)a.cache.n_pages ? max(0, min(16, count - j)) : 0;
-        const int64_t ko = depth ? b * a.skd[0] + j * a.skd[1] + h * a.skd[2] : a.cache.offset(a.cache.sk, page, j, h);
-        const int64_t vo = depth ? b * a.svd[0] + j * a.svd[1] + h * a.svd[2] : a.cache.offset(a.cache.sv, page, j, h);
-        base[hf][0] = (uint64_t)((depth ? a.kd : a.cache.k) + 2 * ko);
-        base[hf][1] = (uint64_t)((depth ? a.vd : a.cache.v) + 2 * vo);
-        there |= ((1u << rows[hf]) - 1) << (16 * hf);
+        for (int hf = 0; hf < 2; hf++) {
+          const int j = first + 16 * hf, page = __builtin_amdgcn_readlane(entry, 16 * hf), in = j & ((1 << a.cache.page_shift) - 1);
+          rows[hf] = (unsigned)page < (unsigned)a.cache.n_pages ? max(0, min(16, seq.len - j)) : 0;
+          base[hf][0] = (uint64_t)(k_head + 2 * (page * a.cache.sk[0]) + (int64_t)in * (int)(2 * a.cache.sk[1]));
+          base[hf][1] = (uint64_t)(v_head + 2 * (page * a.cache.sv[0]) + (int64_t)in * (int)(2 * a.cache.sv[1]));
+        }
+      } else {
+        const int first = (tile - seq.seq_tiles) * kTileKeys;
+        const char* kd = a.kd + 2 * (b * a.skd[0] + h * a.skd[2]);
+        const char* vd = a.vd + 2 * (b * a.svd[0] + h * a.svd[2]);
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+          const int j = first + 16 * hf;
+          rows[hf] = max(0, min(16, a.Lv - j));
+          base[hf][0] = (uint64_t)(kd + 2 * (j * a.skd[1]));
+          base[hf][1] = (uint64_t)(vd + 2 * (j * a.svd[1]));
+        }
       }
-      stride[0] = (int)(2 * (depth ? a.skd[1] : a.cache.sk[1]));
-      stride[1] = (int)(2 * (depth ? a.svd[1] : a.cache.sv[1]));
+      there = ((1u << rows[0]) - 1) | ((1u << rows[1]) - 1) << 16;
     } else {
       uint64_t kp = 0, vp = 0;
       if (!depth) {
@@ -301,18 +341,20 @@ struct PagedWave {
   }
   // a K (0) or V (1) tile, from the rows found last
   __device__ __forceinline__ void fetch_tile(int which, int stage) const {
-    const int prow = lane / CH, pch = lane % CH, dim = which ? a.Dv : a.D;
     const uint32_t to = lds + stage * Lds::kStage + which * Lds::kTile;
     if (even) {
+      // the range check fills with zeros what lies past the last row and past the head dim
+      const int step = (int)(2 * (which ? a.cache.sv[1] : a.cache.sk[1]));
 #pragma unroll
-      for (int i = 0; i < NL; i++) {
-        const int row = (i * RPW + prow) & 15, hf = i * RPW / 16, chunk = pch ^ Tile<W>::swz(row);
-        // the range check fills with zeros what lies past the last row and past the head dim
-        const i32x4 rs = rsrc_words((const void*)base[hf][which], (uint32_t)(rows[hf] * stride[which]));
-        lds_dma<16>(rs, to + i * 1024, chunk * 8 < dim ? row * stride[which] + chunk * 16 : kPadOffset, 0);
+      for (int hf = 0; hf < 2; hf++) {
+        const i32x4 rs = rsrc_words((const void*)base[hf][which], (uint32_t)(rows[hf] * step));
+#pragma unroll
+        for (int i = 0; i < kPeriod; i++) lds_dma<16>(rs, to + (hf * kPeriod + i) * 1024, piece[which][i], 0);
       }
       return;
     }
+    const int prow = lane / CH, pch = lane % CH, dim = which ? a.Dv : a.D;
+    const uint64_t zero = (uint64_t)&zero_line[0];
     uint64_t from[NL];
 #pragma unroll
     for (int i = 0; i < NL; i++) from[i] = *at<uint64_t>(Lds::kRows + 16 * (i * RPW + prow) + 8 * which);
@@ -360,6 +402,8 @@ struct PagedWave {
   // tiles [t0, t1) of the segment
   __device__ void run(int t0, int t1) {
     const int n = lane & 15, g = lane >> 4, tiles = t1 - t0;
+    k_head = a.cache.k + 2 * (h * a.cache.sk[2]);
+    v_head = a.cache.v + 2 * (h * a.cache.sv[2]);
     const bool one_token = a.cache.T == 1;
     Window seq_win[NR], depth_win[NR];
 #pragma unroll
@@ -494,12 +538,14 @@ struct PagedWave {
 };
 
 // Walks a wave's run of the axis: part(seq, b, h, rt, t0, t1, whole, slot) for each segment in it.
-template <typename F>
-__device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, F&& part) {
+// `meanwhile` runs while the counts are on their way.
+template <typename G, typename F>
+__device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, G&& meanwhile, F&& part) {
   const int heads = a.cache.H * a.row_tiles;
   // Up to 64 sequences are read once; of more the first pass over the others is for the total alone.
   int own = lane < a.cache.B ? Seq(a, lane).tiles : 0, sum = own;
   for (int b = lane + 64; b < a.cache.B; b += 64) sum += Seq(a, b).tiles;
+  meanwhile();
   const Plan plan(a, __builtin_amdgcn_readlane(wave_scan(sum), 63));
   const int wave = blockIdx.x;
   if ((int64_t)wave * plan.per >= plan.total) return;
@@ -519,22 +565,25 @@ __device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, F&& par
   b = __builtin_amdgcn_readfirstlane(b);
   Seq seq = uniform_seq(a, b);
   const int rest = __builtin_amdgcn_readfirstlane(s - start);
-  int hr = __builtin_amdgcn_readfirstlane(rest / seq.tiles), tile = rest - hr * seq.tiles;
+  int hr = uniform_div(rest, seq.tiles), tile = rest - hr * seq.tiles;
+  int h = a.row_tiles == 1 ? hr : uniform_div(hr, a.row_tiles), rt = hr - h * a.row_tiles;
   for (int at = s; at < e;) {
     const int upto = min(seq.tiles, tile + (e - at)), slot = 2 * wave + (at == s ? 0 : 1);
-    if (tile == 0 && lane == 0) {
-      int* info = (int*)a.work + 2 * ((int64_t)b * heads + hr);
-      info[0] = slot;
-      info[1] = (at + seq.tiles - 1) / plan.per - wave + 1;
+    const bool first = tile == 0, last = upto == seq.tiles;
+    if (lane == 0) {
+      int* info = (int*)a.work + 2 * ((int64_t)b * heads + h * a.row_tiles + rt);
+      if (first) info[0] = slot;
+      if (last) info[1] = wave;
     }
-    part(seq, b, hr / a.row_tiles, hr % a.row_tiles, tile, upto, tile == 0 && upto == seq.tiles, slot);
+    part(seq, b, h, rt, tile, upto, first && last, slot);
     at += upto - tile;
     tile = 0;
-    if (++hr == heads && at < e) {
-      hr = 0;
-      do seq = uniform_seq(a, ++b);
-      while (seq.tiles == 0);
-    }
+    if (++rt < a.row_tiles) continue;
+    rt = 0;
+    if (++h < a.cache.H || at >= e) continue;
+    h = 0;
+    do seq = uniform_seq(a, ++b);
+    while (seq.tiles == 0);
   }
 }
 
@@ -543,7 +592,7 @@ __global__ __launch_bounds__(64, 1) void paged_kernel(const PagedAttendArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   const int lane = threadIdx.x;
   PagedWave<T, W, NR, NS> w(a, lane, (uint32_t)(uintptr_t)(MODA_LDS char*)lds_raw);
-  walk(a, lane, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int slot) {
+  walk(a, lane, [&] { w.init(); }, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int slot) {
     w.seq = seq;
     w.b = b;
     w.h = h;
@@ -562,7 +611,7 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
   constexpr int MB = W / 16;
   const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
   const bool one_token = a.cache.T == 1;
-  walk(a, lane, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int slot) {
+  walk(a, lane, [] {}, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int slot) {
     const RowOf row(a, rt, 16, n);
     const float* qp = (const float*)a.q + b * a.sq[0] + row.t * a.sq[1] + row.g * a.sq[2] + h * a.sq[3];
     f32x4 q[MB], o[MB][1];
@@ -694,8 +743,8 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a,
   const int rows = a.cache.T * a.G, row = (int)(at % rows), b = (int)(at / rows);
   const int rt = row / rows_per_tile, r = row - rt * rows_per_tile, t = row / a.G, g = row - t * a.G;
   const int64_t seg = ((int64_t)b * a.cache.H + h) * a.row_tiles + rt;
-  const int first = ((const int*)a.work)[2 * seg], count = ((const int*)a.work)[2 * seg + 1];
-  const int parts = Seq(a, b).tiles ? count : 0;
+  const int first = ((const int*)a.work)[2 * seg], last = ((const int*)a.work)[2 * seg + 1];
+  const int parts = Seq(a, b).tiles ? last - (first >> 1) + 1 : 0;
   if (parts == 1) return;  // one wave had all of it and has stored the row
   auto slot = [&](int p) { return p == 0 ? first : (first & ~1) + 2 * p; };
   float top = kNegInf;
@@ -814,7 +863,7 @@ size_t plan_paged_attend(PagedAttendArgs& a, int dtype) {
   // sixteen rows through one buffer descriptor: 31-bit offsets, rows that do not reach into the next one
   const auto even = [&](const int64_t(&s)[3], int dim) { return s[1] >= dim && s[1] < 1 << 25; };
   a.even_pages = a.cache.page_shift >= 4 && even(a.cache.sk, a.D) && even(a.cache.sv, a.Dv);
-  a.even_slots = a.cache.T == 1 && even(a.skd, a.D) && even(a.svd, a.Dv);
+  a.even_slots = a.cache.T == 1 && even(a.skd, a.D) && even(a.svd, a.Dv) && a.skd[1] == a.cache.sk[1] && a.svd[1] == a.cache.sv[1];
   a.waves = (int)(most < 256 * per_unit ? (most > 0 ? most : 1) : 256 * per_unit);
   const size_t segments = ((size_t)a.cache.B * a.cache.H * a.row_tiles + 1) / 2 * 2;
   return (segments * 2 + (size_t)2 * a.waves * a.part_rows * (a.part_width + 2)) * sizeof(float);
