@@ -381,7 +381,7 @@ int moda_hip_rotary_rows(int32_t dtype, int64_t B, int64_t T, int64_t D, const m
  * and over the L_valid first slots (0: all L) of its own token in kd, vd [B, T * L, H, *].  q, o: [B, T * G, H, *], rows t * G + g,
  * lse [B, T * G, H] fp32 base 2; with `plain` [B, T, H * G, *], heads h * G + g, lse [B, T, H * G].  Rows that see nothing, padded
  * ones among them, have o = 0 and lse = -inf.  cu_seqlens NULL.  All rows on 16-byte boundaries.
- * Head dims up to 256, multiples of 8 (fp32: of 4); T * G up to 2^16; B * H * (max_pages * page_size + T * L) / 32 below 2^30 (times T * G / 16 where that
+ * Head dims up to 256, multiples of 8 (fp32: of 4); T * G up to 2^16, T * L to 2^22; B * H * (max_pages * page_size + T * (L_valid + 15)) / 32 below 2^30 (times T * G / 16 where that
  * is more than 1); MODA_HIP_EUNSUPPORTED otherwise.
  */
 typedef struct moda_hip_paged_cache {

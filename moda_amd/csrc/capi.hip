@@ -862,7 +862,7 @@ int fill_attend(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_a
   if (!t || t->struct_size != (int32_t)sizeof(*t) || cache->cu_seqlens || t->G <= 0 || t->L < 0 || t->L_valid < 0 || t->L_valid > t->L ||
       (t->plain && t->L > 0))
     return MODA_HIP_EINVAL;
-  if (t->G >= (1 << 15) || cache->T * t->G > (1 << 16) || t->L >= (1 << 20) || cache->T * t->L >= (1 << 30) ||
+  if (t->G >= (1 << 15) || cache->T * t->G > (1 << 16) || t->L >= (1 << 20) || cache->T * t->L > (1 << 22) ||
       cache->B * cache->T * t->G * cache->H >= (1ll << 31))
     return MODA_HIP_EUNSUPPORTED;
   a.G = (int)t->G;

@@ -78,6 +78,8 @@ struct PagedAttendArgs {
   float* work;
   // how the work is cut (plan_paged_attend)
   int waves, least_tiles, row_tiles, part_rows, part_width, even_pages, even_slots;
+  int slot_blocks;  // sixteens of a token's depth slots
+  float blocks_inverse;
   unsigned group_magic;
 };
 

@@ -26,6 +26,18 @@ constexpr int kTileKeys = 32;
 // what invalid rows and chunks past a head dim read
 __device__ __align__(64) uint32_t zero_line[16];
 
+// The kernel's arguments, read again where they are used: kept from the start they take every scalar register there is, and the main
+// loop's own move to vector lanes and back.  (They begin the kernel's argument segment.)
+__device__ __forceinline__ PagedAttendArgs reload() {
+  PagedAttendArgs a;
+#if defined(__HIP_DEVICE_COMPILE__)
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  __builtin_memcpy(&a, (const void*)p, sizeof(a));
+#endif
+  return a;
+}
+
 // Sum over lanes 0 .. l in lane l.
 __device__ __forceinline__ int wave_scan(int x) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -39,14 +51,25 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// Sequence b on the axis: positions that its last new token sees, tiles of them and of its new tokens' depth slots.
+// Pointers out of the argument block are global memory; read from a copy of it the compiler does not know.
+template <typename V>
+__device__ __forceinline__ const __attribute__((address_space(1))) V* in_global(const void* p) {
+  return (const __attribute__((address_space(1))) V*)(uint64_t)p;
+}
+template <typename V>
+__device__ __forceinline__ __attribute__((address_space(1))) V* out_global(void* p) {
+  return (__attribute__((address_space(1))) V*)(uint64_t)p;
+}
+
+// Sequence b on the axis: positions that its last new token sees, tiles of them and of its new tokens' depth slots.  The slots of
+// a token begin a sixteen of their own: slot l of token t has index 16 blocks t + l.
 struct Seq {
   int past, fresh, len, seq_tiles, tiles;
   __device__ __forceinline__ Seq(const PagedAttendArgs& a, int b) : Seq(a, a.cache.past_of(b), a.cache.new_of(b)) {}
   __device__ __forceinline__ Seq(const PagedAttendArgs& a, int past_, int fresh_) : past(past_), fresh(fresh_) {
     len = fresh > 0 ? min(past + fresh, a.cache.capacity()) : 0;
     seq_tiles = (len + kTileKeys - 1) / kTileKeys;
-    tiles = seq_tiles + (fresh * a.Lv + kTileKeys - 1) / kTileKeys;
+    tiles = seq_tiles + (fresh * a.slot_blocks + 1) / 2;
   }
 };
 
@@ -103,8 +126,10 @@ struct PartAt {
 
 template <typename E>
 __device__ __forceinline__ void store_element(char* p, int64_t i, float x) {
-  ((typename E::elem*)p)[i] = (typename E::elem)x;
+  out_global<typename E::elem>(p)[i] = (typename E::elem)x;
 }
+// token that a sixteen of depth slots belongs to (at most 2^22 slots: off by less than 1 / 16 blocks, the estimate is exact)
+__device__ __forceinline__ int token_of_block(const PagedAttendArgs& a, int block) { return (int)(((float)block + 0.5f) * a.blocks_inverse); }
 struct FP32 {
   typedef float elem;
 };
@@ -122,8 +147,9 @@ struct RowOf {
 };
 
 template <typename E, int W, int NR, bool MAP>
-__device__ void store_part(const PagedAttendArgs& a, const Seq& seq, int b, int h, int rt, bool whole, int slot, const f32x4 (&o)[W / 16][NR],
+__device__ __forceinline__ void store_part(const Seq& seq, int b, int h, int rt, bool whole, int slot, const f32x4 (&o)[W / 16][NR],
                            const float (&m)[NR], const float (&l_lane)[NR], int lane) {
+  const PagedAttendArgs a = reload();
   const int n = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int nr = 0; nr < NR; nr++) {
@@ -135,17 +161,17 @@ __device__ void store_part(const PagedAttendArgs& a, const Seq& seq, int b, int 
       const PartAt part(a, slot);
       const int r = 16 * nr + n;
       if (q == 0) {
-        part.ml[2 * r] = padded ? kNegInf : m[nr];
-        part.ml[2 * r + 1] = padded ? 0.f : l;
+        out_global<float>(part.ml)[2 * r] = padded ? kNegInf : m[nr];
+        out_global<float>(part.ml)[2 * r + 1] = padded ? 0.f : l;
       }
 #pragma unroll
       for (int c = 0; c < W / 16; c++) {
         float* to = part.o + (int64_t)r * W;
         if (!MAP) {
-          *(f32x4*)(to + 16 * c + 4 * q) = o[c][nr];
+          *out_global<f32x4>(to + 16 * c + 4 * q) = o[c][nr];
         } else if (c % 4 == 0) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) *(f32x4*)(to + 16 * c + 16 * q + 4 * i) = f32x4{o[c][nr][i], o[c + 1][nr][i], o[c + 2][nr][i], o[c + 3][nr][i]};
+          for (int i = 0; i < 4; i++) *out_global<f32x4>(to + 16 * c + 16 * q + 4 * i) = f32x4{o[c][nr][i], o[c + 1][nr][i], o[c + 2][nr][i], o[c + 3][nr][i]};
         }
       }
       continue;
@@ -161,7 +187,8 @@ __device__ void store_part(const PagedAttendArgs& a, const Seq& seq, int b, int 
         if (e < a.Dv) store_element<E>(a.o, to + e, empty ? 0.f : o[c][nr][i] * inv);
       }
     if (q == 0)
-      a.lse[b * a.slse[0] + row.t * a.slse[1] + row.g * a.slse[2] + h * a.slse[3]] = empty ? kNegInf : m[nr] + __builtin_amdgcn_logf(l);
+      out_global<float>(a.lse)[b * a.slse[0] + row.t * a.slse[1] + row.g * a.slse[2] + h * a.slse[3]] =
+          empty ? kNegInf : m[nr] + __builtin_amdgcn_logf(l);
   }
 }
 
@@ -282,7 +309,7 @@ struct PagedWave {
     lds_dma<4>(rs, lds + Lds::kTable + ring * 256, tile < seq.seq_tiles ? (int)(page * 4) : kPadOffset, 0);
   }
   // Where the rows of a tile lie.  In sixteens of evenly spaced rows where pages and strides allow (even: pages of 16 tokens and more,
-  // or the depth slots of a single token at the pages' spacing): base addresses and how many rows there are, in scalar
+  // or depth slots at the pages' spacing): base addresses and how many rows there are, in scalar
   // registers.  Else the address of every row, in LDS; zero: nowhere.
   bool even;
   uint64_t base[2][2];
@@ -303,19 +330,21 @@ struct PagedWave {
           base[hf][1] = (uint64_t)(v_head + 2 * (page * a.cache.sv[0]) + (int64_t)in * (int)(2 * a.cache.sv[1]));
         }
       } else {
-        const int first = (tile - seq.seq_tiles) * kTileKeys;
+        const PagedAttendArgs a = reload();
         const char* kd = a.kd + 2 * (b * a.skd[0] + h * a.skd[2]);
         const char* vd = a.vd + 2 * (b * a.svd[0] + h * a.svd[2]);
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {
-          const int j = first + 16 * hf;
-          rows[hf] = max(0, min(16, a.Lv - j));
-          base[hf][0] = (uint64_t)(kd + 2 * (j * a.skd[1]));
-          base[hf][1] = (uint64_t)(vd + 2 * (j * a.svd[1]));
+          const int block = 2 * (tile - seq.seq_tiles) + hf, t = __builtin_amdgcn_readfirstlane(token_of_block(a, block));
+          const int slot = 16 * (block - t * a.slot_blocks);
+          rows[hf] = t < seq.fresh ? min(16, a.Lv - slot) : 0;
+          base[hf][0] = (uint64_t)(kd + 2 * (((int64_t)t * a.L + slot) * a.skd[1]));
+          base[hf][1] = (uint64_t)(vd + 2 * (((int64_t)t * a.L + slot) * a.svd[1]));
         }
       }
       there = ((1u << rows[0]) - 1) | ((1u << rows[1]) - 1) << 16;
     } else {
+      const PagedAttendArgs a = reload();
       uint64_t kp = 0, vp = 0;
       if (!depth) {
         const int j = tile * kTileKeys + r, page = *at<int>(Lds::kTable + ring * 256 + 4 * lane);
@@ -324,9 +353,9 @@ struct PagedWave {
           vp = (uint64_t)(a.cache.v + 2 * a.cache.offset(a.cache.sv, page, j, h));
         }
       } else {
-        const int col = (tile - seq.seq_tiles) * kTileKeys + r, t = col / a.Lv;
-        if (t < seq.fresh) {
-          const int64_t row = (int64_t)t * a.L + (col - t * a.Lv);
+        const int block = 2 * (tile - seq.seq_tiles) + (r >> 4), t = token_of_block(a, block), slot = 16 * (block - t * a.slot_blocks) + (r & 15);
+        if (t < seq.fresh && slot < a.Lv) {
+          const int64_t row = (int64_t)t * a.L + slot;
           kp = (uint64_t)(a.kd + 2 * (b * a.skd[0] + row * a.skd[1] + h * a.skd[2]));
           vp = (uint64_t)(a.vd + 2 * (b * a.svd[0] + row * a.svd[1] + h * a.svd[2]));
         }
@@ -406,6 +435,10 @@ struct PagedWave {
     v_head = a.cache.v + 2 * (h * a.cache.sv[2]);
     const bool one_token = a.cache.T == 1;
     Window seq_win[NR], depth_win[NR];
+    int first_t;  // of the row tile's tokens
+    {
+    const PagedAttendArgs a = reload();
+    first_t = RowOf(a, rt, 16 * NR, 0).t;
 #pragma unroll
     for (int nr = 0; nr < NR; nr++) {
       const RowOf row(a, rt, 16 * NR, 16 * nr + n);
@@ -414,15 +447,16 @@ struct PagedWave {
       for (int ks = 0; ks < KS; ks++) {
         const int e = 32 * ks + 8 * g;
         i32x4 x = {0, 0, 0, 0};
-        if (row.real && e < a.D) x = *(const i32x4*)(a.q + 2 * (from + e));
+        if (row.real && e < a.D) x = *in_global<i32x4>(a.q + 2 * (from + e));
         q[nr][ks] = x;
       }
       seq_win[nr] = {0, seq.past + row.t + 1};
-      depth_win[nr] = {row.t * a.Lv, row.t * a.Lv + a.Lv};
+      depth_win[nr] = {row.t * a.slot_blocks * 16, row.t * a.slot_blocks * 16 + a.Lv};
       m[nr] = kNegInf;
       l[nr] = 0.f;
 #pragma unroll
       for (int c = 0; c < MB; c++) o[c][nr] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     }
     // the table's entries and the rows have to be here before the tiles are sent for: the compiler would wait for everything
     // behind the rows as well
@@ -433,7 +467,6 @@ struct PagedWave {
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(q[nr][ks]));
     wait_but<0>();
-    const int first_t = rt * 16 * NR / a.G;  // of the row tile's tokens
     // loads behind a tile's K when NS - 1 more tiles are on their way, and behind its V when the next K is as well
     constexpr int kBehindK = NL + (NS - 1) * (2 * NL + 1), kBehindV = (NS - 1) * (2 * NL + 1) + NL + 1;
     // step i sends for tile i + NS and works on tile i (the first NS steps only send: one copy of the code)
@@ -587,18 +620,25 @@ __device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, G&& mea
   }
 }
 
-template <typename T, int W, int NR, int NS>
-__global__ __launch_bounds__(64, 1) void paged_kernel(const PagedAttendArgs a) {
+// Stages of a wave's ring and waves of a compute unit (four at one a SIMD).
+template <int W, int NR>
+struct Shape {
+  static constexpr int kStages = W == 64 ? (NR <= 2 ? 2 : 4) : W == 128 && NR == 2 ? 2 : 1;
+  static constexpr int kWaves = W == 64 ? (NR <= 2 ? 8 : 4) : W == 128 && NR == 1 ? (8) : 4;
+};
+
+template <typename T, int W, int NR>
+__global__ __launch_bounds__(64, (Shape<W, NR>::kWaves + 3) / 4) void paged_kernel(const PagedAttendArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   const int lane = threadIdx.x;
-  PagedWave<T, W, NR, NS> w(a, lane, (uint32_t)(uintptr_t)(MODA_LDS char*)lds_raw);
+  PagedWave<T, W, NR, Shape<W, NR>::kStages> w(a, lane, (uint32_t)(uintptr_t)(MODA_LDS char*)lds_raw);
   walk(a, lane, [&] { w.init(); }, [&](const Seq& seq, int b, int h, int rt, int t0, int t1, bool whole, int slot) {
     w.seq = seq;
     w.b = b;
     w.h = h;
     w.rt = rt;
     w.run(t0, t1);
-    store_part<T, W, NR, false>(a, seq, b, h, rt, whole, slot, w.o, w.m, w.l, lane);
+    store_part<T, W, NR, false>(seq, b, h, rt, whole, slot, w.o, w.m, w.l, lane);
   });
 }
 
@@ -622,7 +662,7 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
       if (row.real && 16 * s + 4 * g < a.D) q[s] = *(const f32x4*)(qp + 16 * s + 4 * g);
       o[s][0] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const int first_t = rt * 16 / a.G;
+    const int first_t = RowOf(a, rt, 16, 0).t;
     // 16 keys at a time, the next ones on their way while these are worked on
     struct Keys {
       f32x4 k[MB], v[4][MB / 4];
@@ -632,7 +672,7 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
     auto fetch = [&](int half, Keys& x) {
       const bool depth = half >= 2 * seq.seq_tiles;
       const int key = (depth ? half - 2 * seq.seq_tiles : half) * 16 + n;
-      const float *kp = nullptr, *vp = nullptr;
+      const float *kp = nullptr, *vp = nullptr;  // (read as global memory below: a choice between them and zeros would make flat loads)
       if (!depth) {
         const int page = key < seq.len ? a.cache.page_of(b, key) : -1;
         if (page >= 0) {
@@ -640,9 +680,9 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
           vp = (const float*)a.cache.v + a.cache.offset(a.cache.sv, page, key, h);
         }
       } else {
-        const int t = key / a.Lv;
-        if (t < seq.fresh) {
-          const int64_t r = (int64_t)t * a.L + (key - t * a.Lv);
+        const int t = token_of_block(a, key >> 4), slot = key - 16 * t * a.slot_blocks;
+        if (t < seq.fresh && slot < a.Lv) {
+          const int64_t r = (int64_t)t * a.L + slot;
           kp = (const float*)a.kd + b * a.skd[0] + r * a.skd[1] + h * a.skd[2];
           vp = (const float*)a.vd + b * a.svd[0] + r * a.svd[1] + h * a.svd[2];
         }
@@ -650,16 +690,18 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
       x.vp = (uint64_t)vp;
       x.there = (uint32_t)__ballot(kp != nullptr) & 0xffffu;
       // a row that is not there, and pieces past the head dim: zeros
+      typedef const __attribute__((address_space(1))) f32x4* global_f32x4;
+      const float* zeros = (const float*)zero_line;
 #pragma unroll
       for (int s = 0; s < MB; s++) {
         const bool in = kp && 16 * s + 4 * g < a.D;
-        x.k[s] = *(const f32x4*)(in ? kp + 16 * s + 4 * g : (const float*)zero_line);
+        x.k[s] = *(global_f32x4)(uint64_t)(in ? kp + 16 * s + 4 * g : zeros);
       }
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const float* row_v = (const float*)__shfl((unsigned long long)x.vp, 4 * g + r, 64);
 #pragma unroll
-        for (int c = 0; c < MB / 4; c++) x.v[r][c] = *(const f32x4*)(row_v && 64 * c + 4 * n < a.Dv ? row_v + 64 * c + 4 * n : (const float*)zero_line);
+        for (int c = 0; c < MB / 4; c++) x.v[r][c] = *(global_f32x4)(uint64_t)(row_v && 64 * c + 4 * n < a.Dv ? row_v + 64 * c + 4 * n : zeros);
       }
     };
     auto work = [&](int half, const Keys& x) {
@@ -676,7 +718,7 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
       float p[4];
       const f32x4 sums[1] = {s};
       scaled(p, sums, a.scale);
-      const Window win = depth ? Window{row.t * a.Lv, row.t * a.Lv + a.Lv} : Window{0, seq.past + row.t + 1};
+      const Window win = depth ? Window{row.t * a.slot_blocks * 16, row.t * a.slot_blocks * 16 + a.Lv} : Window{0, seq.past + row.t + 1};
       const bool all_seen = there == 0xffffu && (depth ? one_token : first + 15 <= seq.past + first_t);
 #pragma unroll
       for (int i = 0; i < 4; i++) p[i] = all_seen | win.sees(there, first, 4 * g + i) ? p[i] : kNegInf;
@@ -721,7 +763,7 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
       work(half + 1, x[1]);
     }
     products_done();
-    store_part<FP32, W, 1, true>(a, seq, b, h, rt, whole, slot, o, m, l, lane);
+    store_part<FP32, W, 1, true>(seq, b, h, rt, whole, slot, o, m, l, lane);
   });
 }
 
@@ -729,15 +771,17 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
 // joining
 // ------------------------------------------------------------------------------------------------------------------
 
-// A workgroup per query row and head: the parts of its segment, in the order of the axis.  W / 4 threads have four elements
-// each of every (NT * 4 / W)-th part.
-template <typename E, int W, int NT>
+// A workgroup per query row, head and WC of its W elements: the parts of its segment, in the order of the axis.  WC / 4 threads have four
+// elements each of every (NT * 4 / WC)-th part.
+template <typename E, int W, int WC, int NT>
 __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a, int rows_per_tile) {
-  constexpr int LANES = W / 4, GROUPS = NT / LANES, WAVES = NT / 64;
+  constexpr int LANES = WC / 4, GROUPS = NT / LANES, WAVES = NT / 64;
   __shared__ f32x4 sums[WAVES][LANES];
   __shared__ float lsum[WAVES], tops[WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, x = tid % LANES, group = tid / LANES;
   int64_t at = blockIdx.x;
+  const int e0 = W == WC ? 0 : (int)(at % (W / WC)) * WC;  // the workgroup's first element
+  at /= W / WC;
   const int h = (int)(at % a.cache.H);
   at /= a.cache.H;
   const int rows = a.cache.T * a.G, row = (int)(at % rows), b = (int)(at / rows);
@@ -764,7 +808,7 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a,
   for (int p = group; p < parts; p += GROUPS) {
     const PartAt part(a, slot(p));
     const float w = fast_exp2(part.ml[2 * r] - from);
-    const f32x4 v = *(const f32x4*)(part.o + (int64_t)r * W + 4 * x);
+    const f32x4 v = *(const f32x4*)(part.o + (int64_t)r * W + e0 + 4 * x);
     l += w * part.ml[2 * r + 1];
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] += w * v[i];
@@ -795,9 +839,11 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a,
   const float inv = empty ? 0.f : 1.f / l;
   const int64_t to = b * a.so[0] + t * a.so[1] + g * a.so[2] + h * a.so[3];
 #pragma unroll
-  for (int e = 0; e < 4; e++)
-    if (4 * x + e < a.Dv) store_element<E>(a.o, to + 4 * x + e, empty ? 0.f : o[e] * inv);
-  if (x == 0) a.lse[b * a.slse[0] + t * a.slse[1] + g * a.slse[2] + h * a.slse[3]] = empty ? kNegInf : top + __builtin_amdgcn_logf(l);
+  for (int e = 0; e < 4; e++) {
+    const int at_e = e0 + 4 * x + e;
+    if (at_e < a.Dv) store_element<E>(a.o, to + at_e, empty ? 0.f : o[e] * inv);
+  }
+  if (e0 + x == 0) a.lse[b * a.slse[0] + t * a.slse[1] + g * a.slse[2] + h * a.slse[3]] = empty ? kNegInf : top + __builtin_amdgcn_logf(l);
 }
 
 int tile_width(const PagedAttendArgs& a) {
@@ -808,34 +854,43 @@ int tile_width(const PagedAttendArgs& a) {
 // rows of a row tile, in sixteens: as many as a wave's registers hold without spilling
 int row_blocks(const PagedAttendArgs& a, int dtype) {
   const int rows = a.cache.T * a.G, width = tile_width(a);
-  return dtype == MODA_HIP_FP32 || rows <= 16 || width == 256 ? 1 : rows <= 32 || width == 128 ? 2 : 4;
+  return dtype == MODA_HIP_FP32 || rows <= 16 || width == 256 ? 1 : rows <= 32 || width == 128 ? 2 : rows <= 48 ? 3 : 4;
 }
 
-template <typename T, int W, int NR, int NS>
+template <typename T, int W, int NR>
 hipError_t launch_waves(const PagedAttendArgs& a, hipStream_t stream) {
-  static LdsAttrState state;
-  constexpr int bytes = WaveLds<W, NS>::kBytes;
-  const hipError_t e = allow_dynamic_lds(state, (const void*)paged_kernel<T, W, NR, NS>, bytes);
-  if (e != hipSuccess) return e;
-  paged_kernel<T, W, NR, NS><<<a.waves, 64, bytes, stream>>>(a);
+  constexpr int bytes = WaveLds<W, Shape<W, NR>::kStages>::kBytes;
+  static_assert(bytes * Shape<W, NR>::kWaves <= 160 << 10 && bytes <= 64 << 10, "the rings of a compute unit");
+  paged_kernel<T, W, NR><<<a.waves, 64, bytes, stream>>>(a);
   return hipGetLastError();
 }
 template <typename T>
 hipError_t launch_waves_as(const PagedAttendArgs& a, int width, int blocks, hipStream_t stream) {
-  if (width == 256) return launch_waves<T, 256, 1, 2>(a, stream);
-  if (width == 128) return blocks == 1 ? launch_waves<T, 128, 1, 2>(a, stream) : launch_waves<T, 128, 2, 2>(a, stream);
-  return blocks == 1 ? launch_waves<T, 64, 1, 4>(a, stream) : blocks == 2 ? launch_waves<T, 64, 2, 4>(a, stream) : launch_waves<T, 64, 4, 4>(a, stream);
+  if (width == 256) return launch_waves<T, 256, 1>(a, stream);
+  if (width == 128) return blocks == 1 ? launch_waves<T, 128, 1>(a, stream) : launch_waves<T, 128, 2>(a, stream);
+  return blocks == 1   ? launch_waves<T, 64, 1>(a, stream)
+         : blocks == 2 ? launch_waves<T, 64, 2>(a, stream)
+         : blocks == 3 ? launch_waves<T, 64, 3>(a, stream)
+                       : launch_waves<T, 64, 4>(a, stream);
 }
+int waves_of_a_unit(int width, int blocks) {
+  if (width == 256) return Shape<256, 1>::kWaves;
+  if (width == 128) return blocks == 1 ? Shape<128, 1>::kWaves : Shape<128, 2>::kWaves;
+  return blocks == 1 ? Shape<64, 1>::kWaves : blocks == 2 ? Shape<64, 2>::kWaves : blocks == 3 ? Shape<64, 3>::kWaves : Shape<64, 4>::kWaves;
+}
+
 // Threads of a row's workgroup: parts of one row are read side by side, and many rows keep the card busy by themselves.
 template <typename E, int W>
 hipError_t launch_join_of(const PagedAttendArgs& a, int per_tile, hipStream_t stream) {
   const unsigned rows = (unsigned)((int64_t)a.cache.B * a.cache.T * a.G * a.cache.H);
   if (rows >= 2048)
-    paged_join_kernel<E, W, 64><<<rows, 64, 0, stream>>>(a, per_tile);
+    paged_join_kernel<E, W, W, 64><<<rows, 64, 0, stream>>>(a, per_tile);
   else if (rows >= 256)
-    paged_join_kernel<E, W, 256><<<rows, 256, 0, stream>>>(a, per_tile);
+    paged_join_kernel<E, W, W, 256><<<rows, 256, 0, stream>>>(a, per_tile);
+  else if (rows >= 64)
+    paged_join_kernel<E, W, W, 1024><<<rows, 1024, 0, stream>>>(a, per_tile);
   else
-    paged_join_kernel<E, W, 1024><<<rows, 1024, 0, stream>>>(a, per_tile);
+    paged_join_kernel<E, W, 32, 1024><<<rows * (W / 32), 1024, 0, stream>>>(a, per_tile);
   return hipGetLastError();
 }
 template <typename E>
@@ -852,18 +907,20 @@ size_t plan_paged_attend(PagedAttendArgs& a, int dtype) {
   a.row_tiles = (rows + 16 * blocks - 1) / (16 * blocks);
   a.part_rows = rows < 16 * blocks ? rows : 16 * blocks;
   a.part_width = width;
-  a.least_tiles = 2;
+  a.least_tiles = 1;
   // waves of the whole card: as many as hold their rings in the 160 KB of a compute unit
-  const int per_unit = dtype == MODA_HIP_FP32 ? 8 : width == 256 ? 2 : 4;
+  const int per_unit = dtype == MODA_HIP_FP32 ? (width == 64 ? 8 : 4) : waves_of_a_unit(width, blocks);
+  a.slot_blocks = (a.Lv + 15) / 16;
+  a.blocks_inverse = 1.f / (float)(a.slot_blocks > 0 ? a.slot_blocks : 1);
   const int64_t capacity = (int64_t)a.cache.max_pages << a.cache.page_shift;
   const int64_t most = (int64_t)a.cache.B * a.cache.H * a.row_tiles *
-                       ((capacity + kTileKeys - 1) / kTileKeys + ((int64_t)a.cache.T * a.Lv + kTileKeys - 1) / kTileKeys);
+                       ((capacity + kTileKeys - 1) / kTileKeys + ((int64_t)a.cache.T * a.slot_blocks + 1) / 2);
   if (most >= 1ll << 30) return 0;  // the axis is counted in 32 bits
   a.group_magic = a.G == 1 ? 0 : (unsigned)((1ull << 32) / a.G) + 1;  // row / G = umulhi(row, magic): rows are below 2^16
   // sixteen rows through one buffer descriptor: 31-bit offsets, rows that do not reach into the next one
   const auto even = [&](const int64_t(&s)[3], int dim) { return s[1] >= dim && s[1] < 1 << 25; };
   a.even_pages = a.cache.page_shift >= 4 && even(a.cache.sk, a.D) && even(a.cache.sv, a.Dv);
-  a.even_slots = a.cache.T == 1 && even(a.skd, a.D) && even(a.svd, a.Dv) && a.skd[1] == a.cache.sk[1] && a.svd[1] == a.cache.sv[1];
+  a.even_slots = even(a.skd, a.D) && even(a.svd, a.Dv) && a.skd[1] == a.cache.sk[1] && a.svd[1] == a.cache.sv[1];
   a.waves = (int)(most < 256 * per_unit ? (most > 0 ? most : 1) : 256 * per_unit);
   const size_t segments = ((size_t)a.cache.B * a.cache.H * a.row_tiles + 1) / 2 * 2;
   return (segments * 2 + (size_t)2 * a.waves * a.part_rows * (a.part_width + 2)) * sizeof(float);
