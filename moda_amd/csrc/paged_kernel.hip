@@ -623,8 +623,8 @@ __device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, G&& mea
 // Stages of a wave's ring and waves of a compute unit (four at one a SIMD).
 template <int W, int NR>
 struct Shape {
-  static constexpr int kStages = W == 64 ? (NR <= 2 ? 2 : 4) : W == 128 && NR == 2 ? 2 : 1;
-  static constexpr int kWaves = W == 64 ? (NR <= 2 ? 8 : 4) : W == 128 && NR == 1 ? (8) : 4;
+  static constexpr int kStages = W == 64 || (W == 128 && NR == 2) ? 2 : 1;
+  static constexpr int kWaves = W == 64 || (W == 128 && NR == 1) ? 8 : 4;
 };
 
 template <typename T, int W, int NR>
@@ -854,7 +854,7 @@ int tile_width(const PagedAttendArgs& a) {
 // rows of a row tile, in sixteens: as many as a wave's registers hold without spilling
 int row_blocks(const PagedAttendArgs& a, int dtype) {
   const int rows = a.cache.T * a.G, width = tile_width(a);
-  return dtype == MODA_HIP_FP32 || rows <= 16 || width == 256 ? 1 : rows <= 32 || width == 128 ? 2 : rows <= 48 ? 3 : 4;
+  return dtype == MODA_HIP_FP32 || rows <= 16 || width == 256 ? 1 : 2;
 }
 
 template <typename T, int W, int NR>
@@ -868,15 +868,12 @@ template <typename T>
 hipError_t launch_waves_as(const PagedAttendArgs& a, int width, int blocks, hipStream_t stream) {
   if (width == 256) return launch_waves<T, 256, 1>(a, stream);
   if (width == 128) return blocks == 1 ? launch_waves<T, 128, 1>(a, stream) : launch_waves<T, 128, 2>(a, stream);
-  return blocks == 1   ? launch_waves<T, 64, 1>(a, stream)
-         : blocks == 2 ? launch_waves<T, 64, 2>(a, stream)
-         : blocks == 3 ? launch_waves<T, 64, 3>(a, stream)
-                       : launch_waves<T, 64, 4>(a, stream);
+  return blocks == 1 ? launch_waves<T, 64, 1>(a, stream) : launch_waves<T, 64, 2>(a, stream);
 }
 int waves_of_a_unit(int width, int blocks) {
   if (width == 256) return Shape<256, 1>::kWaves;
   if (width == 128) return blocks == 1 ? Shape<128, 1>::kWaves : Shape<128, 2>::kWaves;
-  return blocks == 1 ? Shape<64, 1>::kWaves : blocks == 2 ? Shape<64, 2>::kWaves : blocks == 3 ? Shape<64, 3>::kWaves : Shape<64, 4>::kWaves;
+  return blocks == 1 ? Shape<64, 1>::kWaves : Shape<64, 2>::kWaves;
 }
 
 // Threads of a row's workgroup: parts of one row are read side by side, and many rows keep the card busy by themselves.
