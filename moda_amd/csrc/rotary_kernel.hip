@@ -42,11 +42,21 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int B, int64_t n) 
 }
 
 // A thread has chunk c of VEC pairs (or, past the rotated elements, of VEC elements) of every `groups`-th (row, head) item of
-// one token.  VEC elements are 16 bytes, or one where rows do not lie on that grid.
-template <typename E, int VEC, bool INTER, bool PAGED>
+// one token.  VEC elements are 16 bytes, or one where rows do not lie on that grid.  STREAM: nontemporal accesses.
+//
+// Bound by the bytes: 64 K tokens of 16 + 4 heads of 128 (671 MB in and out) take 114 us, 5.9 TB/s, where a copy of 4 GiB
+// reaches 4.7.  Small calls by the chain counts -> page -> rows: 4 us for one token, 6 into a cache.
+template <typename E, int VEC, bool INTER, bool PAGED, bool STREAM>
 __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
   typedef typename E::bits bits;
   typedef bits vec __attribute__((ext_vector_type(VEC)));
+  auto get = [](const bits* p) { return STREAM ? __builtin_nontemporal_load((const vec*)p) : *(const vec*)p; };
+  auto put = [](vec x, bits* p) {
+    if (STREAM)
+      __builtin_nontemporal_store(x, (vec*)p);
+    else
+      *(vec*)p = x;
+  };
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, unit = id >> a.lane_shift;
   const int c0 = (int)(id & ((1 << a.lane_shift) - 1));
   const int64_t n = unit / a.groups;
@@ -115,7 +125,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
       for (int c = c0; c < chunks; c += 1 << a.lane_shift) {
         if (c < rot) {
           const int e0 = INTER ? 2 * c * VEC : c * VEC, e1 = INTER ? e0 + VEC : a.rot / 2 + e0;
-          const vec u = *(const vec*)(xr + e0), v = *(const vec*)(xr + e1);
+          const vec u = get(xr + e0), v = get(xr + e1);
           vec yu, yv;
 #pragma unroll
           for (int i = 0; i < VEC; i++) {
@@ -132,18 +142,18 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
             }
           }
           if (y) {
-            *(vec*)(yr + e0) = yu;
-            *(vec*)(yr + e1) = yv;
+            put(yu, yr + e0);
+            put(yv, yr + e1);
           }
           if (PAGED && depth) {
-            *(vec*)(dr + e0) = yu;
-            *(vec*)(dr + e1) = yv;
+            put(yu, dr + e0);
+            put(yv, dr + e1);
           }
         } else {
           const int e = rot_elems + (c - rot) * VEC;
-          const vec u = *(const vec*)(xr + e);
-          if (y) *(vec*)(yr + e) = u;
-          if (PAGED && depth) *(vec*)(dr + e) = u;
+          const vec u = get(xr + e);
+          if (y) put(u, yr + e);
+          if (PAGED && depth) put(u, dr + e);
         }
       }
     }
@@ -151,17 +161,20 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
 }
 
 template <typename E, int VEC, bool PAGED>
-static void launch_rows_as(const RowArgs& a, bool inter, int64_t blocks, hipStream_t stream) {
-  if (inter)
-    rows_kernel<E, VEC, true, PAGED><<<(unsigned)blocks, 256, 0, stream>>>(a);
-  else
-    rows_kernel<E, VEC, false, PAGED><<<(unsigned)blocks, 256, 0, stream>>>(a);
+static void launch_rows_as(const RowArgs& a, bool inter, bool stream_through, int64_t blocks, hipStream_t stream) {
+  const unsigned grid = (unsigned)blocks;
+  if (VEC > 1 && stream_through) {
+    inter ? rows_kernel<E, VEC, true, PAGED, VEC != 1><<<grid, 256, 0, stream>>>(a) : rows_kernel<E, VEC, false, PAGED, VEC != 1><<<grid, 256, 0, stream>>>(a);
+    return;
+  }
+  inter ? rows_kernel<E, VEC, true, PAGED, false><<<grid, 256, 0, stream>>>(a) : rows_kernel<E, VEC, false, PAGED, false><<<grid, 256, 0, stream>>>(a);
 }
 
 // `vec`: all rows lie on the 16-byte grid and the rotated elements are whole vectors of pairs
 hipError_t launch_rows(RowArgs& a, int dtype, bool vec, bool inter, bool paged, hipStream_t stream) {
   const int v = !vec ? 1 : dtype == MODA_HIP_FP32 ? 4 : 8;
   int most = 1;
+  int64_t bytes = 0;  // in and out, of a token
   a.items = 0;
   for (int p = 0; p < a.n_parts; p++) {
     RowPart& part = a.part[p];
@@ -169,15 +182,19 @@ hipError_t launch_rows(RowArgs& a, int dtype, bool vec, bool inter, bool paged, 
     most = max(most, part.rotated ? chunks : (chunks + 1) / 2);  // copies: two chunks a thread, as many bytes as a rotated one
     part.heads_magic = part.heads == 1 ? 0 : (unsigned)((1ull << 32) / part.heads) + 1;
     a.items += part.rows * part.heads;
+    bytes += 2ll * part.rows * part.heads * part.dim * (dtype == MODA_HIP_FP32 ? 4 : 2);
   }
   a.lane_shift = 0;
   while ((1 << a.lane_shift) < most && a.lane_shift < 8) a.lane_shift++;
-  // one item a thread until the machine is full (256 compute units of 2048 threads), more after that: the angles are then shared
+  // One item a thread until the machine is full (256 compute units of 2048 threads), then up to five, which share the angles: 64 K
+  // tokens of 20 items with 20, 10, 5 and 3 items a thread 153, 136, 126 and 161 us.
   const int64_t full = 256 * 2048, lanes = a.tokens << a.lane_shift;
-  a.groups = (int)max((int64_t)1, min((int64_t)a.items, full / max(lanes, (int64_t)1)));
+  a.groups = (int)max((int64_t)(a.items + 4) / 5, min((int64_t)a.items, full / max(lanes, (int64_t)1)));
+  // What does not fit the 256 MB memory-side cache passes it by (115 us instead of 126); what does is found there by whoever reads it next.
+  const bool stream_through = a.tokens * bytes > 256ll << 20;
   const int64_t blocks = (lanes * a.groups + 255) / 256;
   if (blocks >= (1ll << 31)) return hipErrorInvalidValue;
-#define MODA_ROWS(E, V) paged ? launch_rows_as<E, V, true>(a, inter, blocks, stream) : launch_rows_as<E, V, false>(a, inter, blocks, stream)
+#define MODA_ROWS(E, V) paged ? launch_rows_as<E, V, true>(a, inter, stream_through, blocks, stream) : launch_rows_as<E, V, false>(a, inter, stream_through, blocks, stream)
   if (dtype == MODA_HIP_FP32)
     vec ? (MODA_ROWS(Fp32, 4)) : (MODA_ROWS(Fp32, 1));
   else if (dtype == MODA_HIP_FP16)
