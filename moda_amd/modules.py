@@ -28,6 +28,8 @@ from torch import nn
 from . import _lib
 from .depth_cache import DepthCache, stack_depth
 from .ops import _chunk_tokens, _tracing, parallel_moda, parallel_moda_chunk_visible
+from .paged import PagedKVCache
+from .rotary import Rotary, apply_rotary
 
 
 class DepthStream:
@@ -143,11 +145,18 @@ class MoDAAttention(nn.Module):
 
     ``ffn_kv=True`` adds a second projection ``kv_ffn`` and the method ``project_depth_kv`` that maps
     another hidden state (e.g. the block's FFN output) to depth K/V, for callers that also feed the
-    depth stream from their feed-forward layers."""
+    depth stream from their feed-forward layers.
+
+    ``rotary`` (a ``Rotary``; the reference's model has none) rotates queries and keys by their tokens' ``positions`` (int ``[N]``
+    or ``[B, N]``, by default 0, 1, ..); the keys that are returned and pushed are the rotated ones, a depth slot standing at its own
+    token's position.  ``step`` is the call for new tokens of sequences in a ``PagedKVCache``."""
+
+    rotary: Optional[Rotary] = None  # (of modules pickled before there was one)
 
     def __init__(self, dim, num_heads=8, num_kv_heads=1, qkv_bias=False, attn_drop=0., proj_drop=0.,
-                 is_causal=False, ffn_kv=False, chunk_rows=None):
+                 is_causal=False, ffn_kv=False, chunk_rows=None, rotary: Optional[Rotary] = None):
         super().__init__()
+        self.rotary = rotary
         self.chunk_rows = chunk_rows  # not None: chunk-visible attention with chunks of that many query rows
         if dim % num_heads != 0:
             raise ValueError(f"dim ({dim}) must be divisible by num_heads ({num_heads})")
@@ -170,16 +179,38 @@ class MoDAAttention(nn.Module):
         kv = kv.reshape(B, N, 2, self.num_kv_heads, self.head_dim)
         return kv[:, :, 0], kv[:, :, 1]
 
-    def project_depth_kv(self, h: torch.Tensor):
+    def project_depth_kv(self, h: torch.Tensor, positions: Optional[torch.Tensor] = None):
         """Depth K/V ``[B, N, num_kv_heads, head_dim]`` of a hidden state other than the attention input."""
         assert self.kv_ffn is not None, "constructed without ffn_kv=True"
-        return self._split_kv(self.kv_ffn(h))
+        k, v = self._split_kv(self.kv_ffn(h))
+        return (k if self.rotary is None else apply_rotary(None, k, self.rotary, positions)[1]), v
 
-    def forward(self, x, depth_k=None, depth_v=None, depth_valid=None, stream: Optional[DepthStream] = None):
+    def step(self, x, cache: PagedKVCache, layer: int, depth: Optional[DepthCache] = None, new_lens: Optional[torch.Tensor] = None):
+        """``forward`` for the ``N`` newest tokens ``x [B, N, dim]`` of the sequences in ``cache`` (of which ``new_lens [B]`` are real),
+        whose keys and values go there: attention over all their positions so far and over the slots of ``depth``, to which this
+        layer's keys and values are added.  Returns the output alone.  No gradients."""
+        assert self.is_causal and self.chunk_rows is None, "a cache serves causal attention without chunks"
         B, N, C = x.shape
         G = self.moda_group_num
         q = self.q(x).reshape(B, N * G, self.num_kv_heads, self.head_dim)
         k, v = self._split_kv(self.kv(x))
+        n = 0 if depth is None else depth.n
+        rotated = cache.append(layer, k, v, new_lens=new_lens, q=None if self.rotary is None else q, rotary=self.rotary, moda_group_num=G,
+                               depth=depth)
+        seen = {} if n == 0 else {"cached_k": depth.k, "cached_v": depth.v, "depth_valid": n}
+        o = cache.attend(layer, q if rotated is None else rotated, new_lens=new_lens, scale=self.scale, moda_group_num=G, **seen)
+        return self.proj_drop(self.proj(o.reshape(B, N, C)))
+
+    def forward(self, x, depth_k=None, depth_v=None, depth_valid=None, stream: Optional[DepthStream] = None,
+                positions: Optional[torch.Tensor] = None):
+        B, N, C = x.shape
+        G = self.moda_group_num
+        q = self.q(x).reshape(B, N * G, self.num_kv_heads, self.head_dim)
+        k, v = self._split_kv(self.kv(x))
+        if self.rotary is not None:
+            q, k = apply_rotary(q, k, self.rotary, positions, moda_group_num=G)
+        else:
+            assert positions is None, "positions are for a rotation: construct with rotary"
         if stream is not None:
             assert depth_k is None and depth_v is None, "pass either a stream or explicit depth tensors"
             o = stream.attend(q, k, v, scale=self.scale, moda_group_num=G, is_causal=self.is_causal,
@@ -205,10 +236,14 @@ class MoDAStack(nn.Module):
     embedding and the classifier, for timing and testing whole-model steps.  Pre-norm blocks as in the
     reference (``x + f(norm(x))``, deit/models.py:288-292) or, with ``post_norm=True``, ``norm(x + f(x))``;
     ``ffn_kv=True`` also pushes K/V projected from every block's output into the stream (two slots per
-    block)."""
+    block).  ``rotary``: as ``MoDAAttention``'s, one for all blocks.
+
+    A causal stack also generates: ``prefill`` runs prompts and leaves their keys and values in a ``PagedKVCache``, ``decode`` the
+    tokens that follow, each over its sequence's pages and, as in ``forward``, over the depth slots of its own earlier layers.  A captured
+    ``decode`` follows the cache's counts as they grow (pages are reserved between replays)."""
 
     def __init__(self, dim, depth, num_heads, num_kv_heads, mlp_ratio=4., qkv_bias=True, is_causal=False,
-                 post_norm=False, ffn_kv=False, chunk_rows=None):
+                 post_norm=False, ffn_kv=False, chunk_rows=None, rotary: Optional[Rotary] = None):
         super().__init__()
         self.post_norm, self.ffn_kv = post_norm, ffn_kv
         self.blocks = nn.ModuleList()
@@ -216,7 +251,7 @@ class MoDAStack(nn.Module):
             blk = nn.Module()
             blk.norm1 = nn.LayerNorm(dim, eps=1e-6)
             blk.attn = MoDAAttention(dim, num_heads, num_kv_heads, qkv_bias=qkv_bias, is_causal=is_causal,
-                                     ffn_kv=ffn_kv, chunk_rows=chunk_rows)
+                                     ffn_kv=ffn_kv, chunk_rows=chunk_rows, rotary=rotary)
             blk.norm2 = nn.LayerNorm(dim, eps=1e-6)
             hidden = int(dim * mlp_ratio)
             blk.mlp = nn.Sequential(nn.Linear(dim, hidden), nn.GELU(), nn.Linear(hidden, dim))
@@ -236,7 +271,7 @@ class MoDAStack(nn.Module):
             if not (all(type(m) is nn.Linear for m in linears) and type(norm1) is nn.LayerNorm and type(norm2) is nn.LayerNorm
                     and type(act) is nn.GELU and act.approximate == "none" and type(drop) is nn.Dropout):
                 return None
-            if (drop.training and drop.p > 0) or (self.ffn_kv and kv_ffn is None):
+            if (drop.training and drop.p > 0) or (self.ffn_kv and kv_ffn is None) or attn.rotary is not None:
                 return None
             for m in (attn, mlp, norm1, norm2, act, drop, *linears):
                 if m._forward_hooks or m._forward_pre_hooks or "forward" in m.__dict__:
@@ -275,22 +310,72 @@ class MoDAStack(nn.Module):
         cb = 0 if attn.chunk_rows is None else _chunk_tokens(attn.moda_group_num, attn.chunk_rows)
         return _lib.host().stack_forward(x, plain[0], plain[1], attn.num_heads, attn.num_kv_heads, bool(attn.is_causal), cb, self.post_norm)
 
-    def forward(self, x, inplace_cache: Optional[bool] = None):
-        if inplace_cache is not False:
+    def forward(self, x, inplace_cache: Optional[bool] = None, positions: Optional[torch.Tensor] = None):
+        if inplace_cache is not False and positions is None:
             y = self._forward_native(x)
             if y is not None:
                 return y
-        stream = DepthStream(len(self.blocks) * (2 if self.ffn_kv else 1), inplace=inplace_cache)
+        stream = DepthStream(self._slots(), inplace=inplace_cache)
+        at = {} if positions is None else {"positions": positions}
         for blk in self.blocks:
-            if self.post_norm:
-                a, k, v = blk.attn(x, stream=stream)
-                x = blk.norm1(x + a)
-                x = blk.norm2(x + blk.mlp(x))
-            else:
-                a, k, v = blk.attn(blk.norm1(x), stream=stream)
-                x = x + a
-                x = x + blk.mlp(blk.norm2(x))
+            x, k, v = self._block(blk, x, lambda h: blk.attn(h, stream=stream, **at))
+            stream.push(k, v)
+            if self.ffn_kv:
+                stream.push(*blk.attn.project_depth_kv(x, **at))
+        return x
+
+    def _slots(self):
+        return len(self.blocks) * (2 if self.ffn_kv else 1)
+
+    def _block(self, blk, x, attend):
+        """One block around ``attend(h) -> (output, ...)``: the residual stream, then whatever else ``attend`` returned."""
+        if self.post_norm:
+            a, *rest = attend(x)
+            x = blk.norm1(x + a)
+            return (blk.norm2(x + blk.mlp(x)), *rest)
+        a, *rest = attend(blk.norm1(x))
+        x = x + a
+        return (x + blk.mlp(blk.norm2(x)), *rest)
+
+    @torch.no_grad()
+    def prefill(self, x, cache: PagedKVCache, lens: Optional[torch.Tensor] = None):
+        """Prompts ``x [batch, N, dim]``, of which the first ``lens [batch]`` (int32; none given: all ``N``) tokens are real, for the
+        empty sequences of ``cache`` (pages reserved): ``forward``'s result, keys and values of all layers in the cache, its
+        counts advanced.  Rows behind a prompt's end hold nothing of use."""
+        self._check_cache(x, cache)
+        stream = DepthStream(self._slots())
+        for i, blk in enumerate(self.blocks):
+            x, k, v = self._block(blk, x, lambda h: blk.attn(h, stream=stream))
+            cache.append(i, k, v, new_lens=lens)
             stream.push(k, v)
             if self.ffn_kv:
                 stream.push(*blk.attn.project_depth_kv(x))
+        cache.advance(x.shape[1] if lens is None else lens)
         return x
+
+    @torch.no_grad()
+    def decode(self, x, cache: PagedKVCache, lens: Optional[torch.Tensor] = None):
+        """The next tokens ``x [batch, N, dim]`` of the cache's sequences -- one each, or a few (drafted ones, pieces of a prompt),
+        of which the first ``lens [batch]`` (int32) are real: their rows of ``forward`` over the whole sequence.  Keys and values
+        go to the cache, its counts advance."""
+        self._check_cache(x, cache)
+        B, N, _ = x.shape
+        if N == 0:
+            return x
+        attn = self.blocks[0].attn
+        depth = DepthCache(B, N, self._slots(), attn.num_kv_heads, attn.head_dim, cache.k.dtype, cache.k.device)
+        positions = None
+        if self.ffn_kv and attn.rotary is not None:
+            positions = cache.past[:, None] + torch.arange(N, dtype=torch.int32, device=cache.past.device)
+        for i, blk in enumerate(self.blocks):
+            (x,) = self._block(blk, x, lambda h: (blk.attn.step(h, cache, i, depth, lens),))
+            if self.ffn_kv:
+                depth.append(*blk.attn.project_depth_kv(x, positions))
+        cache.advance(N if lens is None else lens)
+        return x
+
+    def _check_cache(self, x, cache):
+        assert len(self.blocks) > 0 and all(blk.attn.is_causal and blk.attn.chunk_rows is None for blk in self.blocks), \
+            "a cache serves causal stacks without chunks"
+        assert cache.k.shape[0] == len(self.blocks), f"the cache has {cache.k.shape[0]} layers, the stack {len(self.blocks)}"
+        assert x.dim() == 3 and x.shape[0] == cache.batch, f"x must be [{cache.batch}, tokens, dim]"
