@@ -340,7 +340,7 @@ int moda_hip_attend_block_tail(const moda_hip_desc* desc, const void* q, const v
  * interleaved, else (i, i + dim / 2) -- by the angle 2 pi * position * rates[i]:
  *   y0 = amplitude * (x0 cos - x1 sin), y1 = amplitude * (x0 sin + x1 cos).
  * rates: DEVICE array of dim / 2 values in 64 bits, in turns per position (product and fraction are taken in 64 bits).  dim
- * even, at most the head dim.  inverse: by the opposite angle, which makes the gradient of x from that of y.
+ * even, at most the head dim, which is at most 512.  inverse: by the opposite angle, which makes the gradient of x from that of y.
  *
  * moda_hip_rotary_rows: up to three tensors [B, T * rows_per_token, heads, D] -> the same shape, for one set of positions: row r
  * is at position positions[b * position_stride + r / rows_per_token] (int32, or int64 where positions64; position_stride 0:
@@ -366,7 +366,7 @@ int moda_hip_rotary_rows(int32_t dtype, int64_t B, int64_t T, int64_t D, const m
 /*
  * A paged key/value cache: k_pages [n_pages, page_size, H, D], v_pages [n_pages, page_size, H, Dv] with element strides
  * {page, token in the page, head} and unit inner stride, rows on 16-byte boundaries (base and strides; MODA_HIP_EALIGN
- * otherwise), page_size a power of two, n_pages * page_size and max_pages * page_size below 2^31, max_pages below 2^28.  DEVICE arrays: position p of
+ * otherwise), page_size a power of two, n_pages * page_size below 2^31, max_pages * page_size up to 2^30, max_pages below 2^28.  DEVICE arrays: position p of
  * sequence b lies in page table[b * table_stride + p / page_size], max_pages entries a sequence; past[b] tokens of it were there
  * before the call; of its T new tokens new_lens[b] are real (NULL: T).  Counts are taken as at least 0 and past + new tokens as at
  * most max_pages * page_size; a table entry outside [0, n_pages) names no page: its tokens are not stored and not seen.

@@ -738,7 +738,7 @@ int fill_cache(const moda_hip_paged_cache* c, moda::PagedKV& to) {
   const int64_t step = c->dtype == MODA_HIP_FP32 ? 4 : 8, most = 1ll << 31;
   if (c->D > 256 || c->Dv > 256 || c->D % step != 0 || c->Dv % step != 0 || !is_power_of_two(c->page_size)) return MODA_HIP_EUNSUPPORTED;
   if (c->n_pages >= most || c->max_pages >= (1 << 28) || c->page_size >= most || c->n_pages * c->page_size >= most ||
-      c->max_pages * c->page_size >= most || c->B >= (1 << 20) || c->T >= (1 << 24) || c->H >= (1 << 16) || c->B * c->T >= most ||
+      c->max_pages * c->page_size > most / 2 || c->B >= (1 << 20) || c->T >= (1 << 24) || c->H >= (1 << 16) || c->B * c->T >= most ||
       c->total_tokens >= most)
     return MODA_HIP_EUNSUPPORTED;
   if (!c->k_pages || !c->v_pages || !c->table || !c->past) return MODA_HIP_EINVAL;
@@ -770,7 +770,7 @@ int moda_hip_rotary_rows(int32_t dtype, int64_t B, int64_t T, int64_t D, const m
     return MODA_HIP_EINVAL;
   int rc = check_rotary(rotary, D);
   if (rc) return rc;
-  if (B >= (1ll << 31) || T >= (1ll << 31) || B * T >= (1ll << 31) || D > 4096) return MODA_HIP_EUNSUPPORTED;
+  if (B >= (1ll << 31) || T >= (1ll << 31) || B * T >= (1ll << 31) || D > 512) return MODA_HIP_EUNSUPPORTED;
   const int es = elem_size(dtype), step = 16 / es;
   bool vec = rotary->dim % (2 * step) == 0 && D % step == 0;
   moda::RowArgs a = {};

@@ -1081,7 +1081,7 @@ OptTensor paged_append(const Tensor& k_in, const Tensor& v_in, const Tensor& ck,
   CONTRACT(k_in.dim() == 4 && v_in.dim() == 4, "k, v must be [B, T, H, D]");
   const int64_t tb = k_in.size(0), T = k_in.size(1), H = k_in.size(2), D = k_in.size(3), Dv = v_in.size(3);
   CONTRACT(has_shape(v_in, {tb, T, H, Dv}), "k and v must agree in batch size, tokens and heads");
-  no_gradients({&k_in, &v_in, &q_in, &kd, &vd}, "paged_append");
+  no_gradients({&k_in, &v_in, &q_in, &ck, &cv, &kd, &vd}, "paged_append");
   CONTRACT(!cu.defined() || (tb == 1 && cu.dim() == 1 && cu.size(0) >= 1), "with cu_seqlens all new tokens share one packed axis: batch size must be 1, offsets [n+1]");
   CONTRACT(!cu.defined() || !new_lens.has_value(), "new tokens are counted by cu_seqlens or by new_lens, not both");
   const int64_t B = cu.defined() ? cu.size(0) - 1 : tb;

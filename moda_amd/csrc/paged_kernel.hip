@@ -124,9 +124,14 @@ struct PartAt {
   }
 };
 
+// four elements from a multiple of four on (rows lie on 16-byte boundaries)
 template <typename E>
-__device__ __forceinline__ void store_element(char* p, int64_t i, float x) {
-  out_global<typename E::elem>(p)[i] = (typename E::elem)x;
+__device__ __forceinline__ void store_four(char* p, int64_t i, const f32x4& x) {
+  typedef typename E::elem elem4 __attribute__((ext_vector_type(4)));
+  elem4 y;
+#pragma unroll
+  for (int e = 0; e < 4; e++) y[e] = (typename E::elem)x[e];
+  *out_global<elem4>((typename E::elem*)p + i) = y;
 }
 // token that a sixteen of depth slots belongs to (at most 2^22 slots: off by less than 1 / 16 blocks, the estimate is exact)
 __device__ __forceinline__ int token_of_block(const PagedAttendArgs& a, int block) { return (int)(((float)block + 0.5f) * a.blocks_inverse); }
@@ -180,12 +185,16 @@ __device__ __forceinline__ void store_part(const Seq& seq, int b, int h, int rt,
     const float inv = empty ? 0.f : 1.f / l;
     const int64_t to = b * a.so[0] + row.t * a.so[1] + row.g * a.so[2] + h * a.so[3];
 #pragma unroll
-    for (int c = 0; c < W / 16; c++)
+    for (int c = 0; c < W / 16; c++) {
+      const int e = MAP ? 64 * (c / 4) + 16 * q + 4 * (c % 4) : 16 * c + 4 * q;
+      f32x4 x;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int e = MAP ? 64 * (c / 4) + 16 * q + 4 * i + c % 4 : 16 * c + 4 * q + i;
-        if (e < a.Dv) store_element<E>(a.o, to + e, empty ? 0.f : o[c][nr][i] * inv);
+        const float v = MAP ? o[c / 4 * 4 + i][nr][c % 4] : o[c][nr][i];
+        x[i] = empty ? 0.f : v * inv;
       }
+      if (e < a.Dv) store_four<E>(a.o, to + e, x);
+    }
     if (q == 0)
       out_global<float>(a.lse)[b * a.slse[0] + row.t * a.slse[1] + row.g * a.slse[2] + h * a.slse[3]] =
           empty ? kNegInf : m[nr] + __builtin_amdgcn_logf(l);
@@ -575,28 +584,31 @@ struct PagedWave {
 template <typename G, typename F>
 __device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, G&& meanwhile, F&& part) {
   const int heads = a.cache.H * a.row_tiles;
-  // Up to 64 sequences are read once; of more the first pass over the others is for the total alone.
-  int own = lane < a.cache.B ? Seq(a, lane).tiles : 0, sum = own;
+  // Up to 64 sequences are read once; of more the first pass over the others is for the total alone.  Counts that somebody
+  // changes meanwhile make wrong results; places stay within the arrays and loops end all the same.
+  Seq own(a, 0, 0);
+  if (lane < a.cache.B) own = Seq(a, lane);
+  int sum = own.tiles;
   for (int b = lane + 64; b < a.cache.B; b += 64) sum += Seq(a, b).tiles;
   meanwhile();
   const Plan plan(a, __builtin_amdgcn_readlane(wave_scan(sum), 63));
   const int wave = blockIdx.x;
   if ((int64_t)wave * plan.per >= plan.total) return;
   const int s = wave * plan.per, e = min(s + plan.per, plan.total);
-  int b = 0, start = 0;  // start of sequence b, in tiles
-  for (int b0 = 0; b0 < a.cache.B; b0 += 64) {
-    if (b0 > 0) own = b0 + lane < a.cache.B ? Seq(a, b0 + lane).tiles : 0;
-    const int upto = wave_scan(own);
+  int b = 0, start = 0, first_lane = 0;  // start of sequence b, in tiles
+  for (int b0 = 0;;) {
+    const int upto = wave_scan(own.tiles);
     const uint64_t behind = __ballot(start + upto * heads > s);
-    const int first = behind ? __builtin_ctzll(behind) : 63;
-    start += __builtin_amdgcn_readlane(behind ? upto - own : upto, first) * heads;
+    first_lane = behind ? __builtin_ctzll(behind) : 63;
+    start += __builtin_amdgcn_readlane(behind ? upto - own.tiles : upto, first_lane) * heads;
     if (behind) {
-      b = b0 + first;
+      b = b0 + first_lane;
       break;
     }
+    if ((b0 += 64) >= a.cache.B) return;
+    own = b0 + lane < a.cache.B ? Seq(a, b0 + lane) : Seq(a, 0, 0);
   }
-  b = __builtin_amdgcn_readfirstlane(b);
-  Seq seq = uniform_seq(a, b);
+  Seq seq(a, __builtin_amdgcn_readlane(own.past, first_lane), __builtin_amdgcn_readlane(own.fresh, first_lane));
   const int rest = __builtin_amdgcn_readfirstlane(s - start);
   int hr = uniform_div(rest, seq.tiles), tile = rest - hr * seq.tiles;
   int h = a.row_tiles == 1 ? hr : uniform_div(hr, a.row_tiles), rt = hr - h * a.row_tiles;
@@ -615,8 +627,10 @@ __device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, G&& mea
     rt = 0;
     if (++h < a.cache.H || at >= e) continue;
     h = 0;
-    do seq = uniform_seq(a, ++b);
-    while (seq.tiles == 0);
+    do {
+      if (++b >= a.cache.B) return;
+      seq = uniform_seq(a, b);
+    } while (seq.tiles == 0);
   }
 }
 
@@ -788,7 +802,7 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a,
   const int rt = row / rows_per_tile, r = row - rt * rows_per_tile, t = row / a.G, g = row - t * a.G;
   const int64_t seg = ((int64_t)b * a.cache.H + h) * a.row_tiles + rt;
   const int first = ((const int*)a.work)[2 * seg], last = ((const int*)a.work)[2 * seg + 1];
-  const int parts = Seq(a, b).tiles ? last - (first >> 1) + 1 : 0;
+  const int parts = Seq(a, b).tiles && (unsigned)first < 2u * a.waves && (unsigned)last < (unsigned)a.waves ? last - (first >> 1) + 1 : 0;
   if (parts == 1) return;  // one wave had all of it and has stored the row
   auto slot = [&](int p) { return p == 0 ? first : (first & ~1) + 2 * p; };
   float top = kNegInf;
@@ -839,10 +853,8 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a,
   const float inv = empty ? 0.f : 1.f / l;
   const int64_t to = b * a.so[0] + t * a.so[1] + g * a.so[2] + h * a.so[3];
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const int at_e = e0 + 4 * x + e;
-    if (at_e < a.Dv) store_element<E>(a.o, to + at_e, empty ? 0.f : o[e] * inv);
-  }
+  for (int e = 0; e < 4; e++) o[e] = empty ? 0.f : o[e] * inv;
+  if (e0 + 4 * x < a.Dv) store_four<E>(a.o, to + e0 + 4 * x, o);
   if (e0 + x == 0) a.lse[b * a.slse[0] + t * a.slse[1] + g * a.slse[2] + h * a.slse[3]] = empty ? kNegInf : top + __builtin_amdgcn_logf(l);
 }
 

@@ -28,7 +28,7 @@ struct Fp32 {
   __device__ static bits narrow(float x) { return __float_as_uint(x); }
 };
 
-// sequence of token n of a packed axis (B: behind the last one)
+// sequence of token n of a packed axis (B: behind the last one); any offsets at all leave it within 0 .. B
 __device__ __forceinline__ int sequence_of(const int32_t* cu, int B, int64_t n) {
   int lo = 0, hi = B;  // cu[lo] <= n < cu[hi], hi = B standing for any
   while (lo < hi) {
@@ -70,8 +70,8 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
   if (PAGED) {
     if (a.cache.cu) {
       b = sequence_of(a.cache.cu, a.cache.B, n);
-      turn = b < a.cache.B;
-      pos = turn ? n - a.cache.cu[b] : 0;
+      pos = b < a.cache.B ? n - a.cache.cu[b] : -1;
+      turn = pos >= 0;  // (below zero: before the first sequence, or offsets out of order)
       stored = turn;
     } else {
       stored = tt < a.cache.new_of(b);

@@ -156,7 +156,7 @@ def test_c_entries_refuse_rotations():
                dict(rot=dict(dim=7)), dict(rot=dict(dim=66)), dict(part=dict(x=None)), dict(part=dict(y=None)), dict(part=dict(rows=0)),
                dict(part=dict(heads=0))):
         assert call(**kw) == EINVAL, kw
-    for kw in (dict(T=1 << 31), dict(B=1 << 20, T=1 << 20), dict(D=8192, rot=dict(dim=64)), dict(part=dict(rows=1 << 15)), dict(part=dict(heads=1 << 20))):
+    for kw in (dict(T=1 << 31), dict(B=1 << 20, T=1 << 20), dict(D=516, rot=dict(dim=64)), dict(part=dict(rows=1 << 15)), dict(part=dict(heads=1 << 20))):
         assert call(**kw) == EUNSUPPORTED, kw
     for kw in (dict(part=dict(x=AT + 1)), dict(part=dict(y=AT + 1)), dict(rot=dict(rates=AT + 4)), dict(pos=AT + 2), dict(pos=AT + 4, pos64=1)):
         assert call(**kw) == EALIGN, kw
@@ -168,7 +168,7 @@ BAD_PAGES = [
     (EINVAL, dict(k_pages=None)), (EINVAL, dict(v_pages=None)), (EINVAL, dict(table=None)), (EINVAL, dict(past=None)),
     (EINVAL, dict(new_lens=AT, cu_seqlens=AT)),
     (EUNSUPPORTED, dict(D=264)), (EUNSUPPORTED, dict(Dv=264)), (EUNSUPPORTED, dict(D=12)), (EUNSUPPORTED, dict(Dv=60)),
-    (EUNSUPPORTED, dict(page_size=24)), (EUNSUPPORTED, dict(n_pages=1 << 27)), (EUNSUPPORTED, dict(max_pages=1 << 27)),
+    (EUNSUPPORTED, dict(page_size=24)), (EUNSUPPORTED, dict(n_pages=1 << 27)), (EUNSUPPORTED, dict(max_pages=1 << 27)), (EUNSUPPORTED, dict(max_pages=(1 << 26) + 1)), (EUNSUPPORTED, dict(page_size=1, max_pages=1 << 28)),
     (EUNSUPPORTED, dict(n_pages=1 << 62)), (EUNSUPPORTED, dict(T=1 << 24)), (EUNSUPPORTED, dict(B=1 << 20)),
     (EALIGN, dict(k_pages=AT + 8)), (EALIGN, dict(v_pages=AT + 2)), (EALIGN, dict(k=strides(2048, 128, 60))), (EALIGN, dict(v=strides(2049, 128, 64))),
     (EALIGN, dict(table=AT + 1)), (EALIGN, dict(past=AT + 2)), (EALIGN, dict(new_lens=AT + 3)),

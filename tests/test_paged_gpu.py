@@ -80,6 +80,9 @@ ROTATIONS = [
     (FP32, 1, 5, 1, 1, 1, 6, 2, False, "far"),
     (BF16, 1, 3000, 4, 4, 4, 64, 64, False, None),
     (BF16, 1, 7, 16, 8, 1, 256, 128, True, "far"),
+    (FP32, 1, 3, 1, 1, 1, 512, 512, False, None),      # as many pairs as there are lanes
+    (BF16, 1, 2, 1, 1, 1, 510, 510, True, "int32"),    # the same element by element
+    (BF16, 1, 70000, 4, 4, 4, 128, 128, False, None),  # more than the memory-side cache holds
 ]
 
 
@@ -487,6 +490,27 @@ def test_append(case, packed, gpu_device):
         close(depth["cached_v"], dv, torch.zeros_like(dv), "depth v")
 
 
+def test_append_takes_offsets_as_they_are(gpu_device):
+    """Rows before the first packed sequence, and an offset below the one before it: nowhere, and nothing out of place."""
+    torch.manual_seed(19)
+    ck, cv = torch.zeros(3, 16, 1, 64, device=gpu_device), torch.zeros(3, 16, 1, 64, device=gpu_device)
+    table = torch.tensor([[0], [1], [2]], dtype=torch.int32, device=gpu_device)
+    past = torch.zeros(3, dtype=torch.int32, device=gpu_device)
+    k, v, q = (torch.randn(1, 9, 1, 64, device=gpu_device) for _ in range(3))
+    rot = moda_amd.Rotary(64)
+    cu = torch.tensor([2, 4, 4, 7], dtype=torch.int32, device=gpu_device)
+    q1 = moda_amd.paged_append(k, v, ck, cv, table, past, cu_seqlens=cu, q=q, rotary=rot)
+    want = torch.zeros_like(cv)
+    want[0, :2], want[2, :3] = v[0, 2:4], v[0, 4:7]
+    assert torch.equal(cv, want)
+    assert torch.equal(q1[:, :2], q[:, :2]) and torch.equal(q1[:, 7:], q[:, 7:])
+    for offsets in ([0, 5, 2, 9], [9, 0, -4, 2 ** 31 - 1], [-7, -5, -3, -1]):
+        cv.zero_()
+        moda_amd.paged_append(k, v, ck, cv, table, past, cu_seqlens=torch.tensor(offsets, dtype=torch.int32, device=gpu_device))
+        rows = {tuple(r) for r in v[0, :, 0].tolist()} | {(0.0,) * 64}
+        assert {tuple(r) for r in cv.view(-1, 64).tolist()} <= rows
+
+
 def test_append_drops_what_has_no_place(gpu_device):
     torch.manual_seed(13)
     ck, cv = torch.zeros(4, 16, 1, 64, dtype=BF16, device=gpu_device), torch.zeros(4, 16, 1, 64, dtype=BF16, device=gpu_device)
@@ -714,7 +738,7 @@ def test_refusals(gpu_device):
     cu = torch.tensor([0, 3], dtype=torch.int32, device=dev)
     moda_amd.paged_append(**good, cu_seqlens=cu)
     for kw in (dict(k=z(1, 3, 1, 64)), dict(v=z(1, 2, 2, 64)), dict(k=z(1, 3, 2, 32)), dict(k=z(3, 2, 64)), dict(k=z(1, 3, 2, 64, dtype=FP16)),
-               dict(k=z(1, 3, 2, 64).requires_grad_()), dict(q=z(1, 3, 2, 64)), dict(q=z(1, 5, 2, 64), rotary=rot, moda_group_num=2),
+               dict(k=z(1, 3, 2, 64).requires_grad_()), dict(cache_k=z(4, 16, 2, 64).requires_grad_()), dict(q=z(1, 3, 2, 64)), dict(q=z(1, 5, 2, 64), rotary=rot, moda_group_num=2),
                dict(rotary=moda_amd.Rotary(66)), dict(cu_seqlens=cu, new_lens=past), dict(cu_seqlens=cu.long()), dict(cu_seqlens=cu.cpu()),
                dict(cached_k=z(1, 6, 2, 64)), dict(cached_k=z(1, 6, 2, 64), cached_v=z(1, 6, 2, 64), depth_slot=2),
                dict(cached_k=z(1, 7, 2, 64), cached_v=z(1, 7, 2, 64)), dict(cache_k=z(1, 16, 2, 64).expand(4, 16, 2, 64)),
