@@ -77,7 +77,7 @@ struct PagedAttendArgs {
   float scale;  // of logits in base 2
   float* work;
   // how the work is cut (plan_paged_attend)
-  int waves, least_tiles, row_tiles, part_rows, part_width, even_pages, even_slots;
+  int waves, row_tiles, part_rows, part_width;
   int slot_blocks;  // sixteens of a token's depth slots
   float blocks_inverse;
   unsigned group_magic;

@@ -92,7 +92,7 @@ struct Plan {
   int total, per;
   __device__ __forceinline__ Plan(const PagedAttendArgs& a, int tiles_of_one_head) {
     total = tiles_of_one_head * (a.cache.H * a.row_tiles);
-    per = max(uniform_div(total + a.waves - 1, a.waves), a.least_tiles);
+    per = uniform_div(total + a.waves - 1, a.waves);
   }
 };
 
@@ -285,26 +285,8 @@ struct PagedWave {
   // the segment
   int b, h, rt;
   Seq seq;
-  const char *k_head, *v_head;
-  // byte offsets of the lane's piece of a tile, loads i and i + kPeriod (16 rows apart) alike
-  static constexpr int kPeriod = 16 / RPW;
-  int piece[2][kPeriod];
-
   __device__ __forceinline__ PagedWave(const PagedAttendArgs& args, int lane_, uint32_t lds_) : a(args), lane(lane_), lds(lds_), seq(args, 0, 0) {}
-  __device__ __forceinline__ void init() {
-    oa.init(lane);
-    const int prow = lane / CH, pch = lane % CH;
-#pragma unroll
-    for (int i = 0; i < kPeriod; i++) {
-      const int row = i * RPW + prow, chunk = pch ^ Tile<W>::swz(row);
-#pragma unroll
-      for (int which = 0; which < 2; which++) {
-        const int step = (int)(2 * (which ? a.cache.sv[1] : a.cache.sk[1]));
-        piece[which][i] = chunk * 8 < (which ? a.Dv : a.D) ? row * step + chunk * 16 : kPadOffset;
-        asm volatile("" : "+v"(piece[which][i]));
-      }
-    }
-  }
+  __device__ __forceinline__ void init() { oa.init(lane); }
   template <typename P>
   __device__ __forceinline__ MODA_LDS P* at(int byte) const {
     return (MODA_LDS P*)(uintptr_t)(lds + byte);
@@ -317,80 +299,36 @@ struct PagedWave {
     const unsigned page = ((unsigned)tile * kTileKeys + (lane & 31)) >> a.cache.page_shift;
     lds_dma<4>(rs, lds + Lds::kTable + ring * 256, tile < seq.seq_tiles ? (int)(page * 4) : kPadOffset, 0);
   }
-  // Where the rows of a tile lie.  In sixteens of evenly spaced rows where pages and strides allow (even: pages of 16 tokens and more,
-  // or depth slots at the pages' spacing): base addresses and how many rows there are, in scalar
-  // registers.  Else the address of every row, in LDS; zero: nowhere.
-  bool even;
-  uint64_t base[2][2];
-  int rows[2];
-  __device__ __forceinline__ void find_rows(int tile, int ring, int stage) {
+  // Where the rows of a tile lie, every row for itself (two base addresses a tile for pages of 16 tokens and more, in scalar
+  // registers, made no case faster by more than 1 % and the largest slower by 2): lane r's address of row r; zero: nowhere.
+  __device__ __forceinline__ void find_rows(int tile, int ring, int stage) const {
+    const PagedAttendArgs a = reload();
     const int r = lane & 31;
-    const bool depth = tile >= seq.seq_tiles;
-    even = depth ? a.even_slots : a.even_pages;
-    uint32_t there;
-    if (even) {
-      if (!depth) {
-        const int entry = *at<int>(Lds::kTable + ring * 256 + 4 * lane), first = tile * kTileKeys;
-#pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-          const int j = first + 16 * hf, page = __builtin_amdgcn_readlane(entry, 16 * hf), in = j & ((1 << a.cache.page_shift) - 1);
-          rows[hf] = (unsigned)page < (unsigned)a.cache.n_pages ? max(0, min(16, seq.len - j)) : 0;
-          base[hf][0] = (uint64_t)(k_head + 2 * (page * a.cache.sk[0]) + (int64_t)in * (int)(2 * a.cache.sk[1]));
-          base[hf][1] = (uint64_t)(v_head + 2 * (page * a.cache.sv[0]) + (int64_t)in * (int)(2 * a.cache.sv[1]));
-        }
-      } else {
-        const PagedAttendArgs a = reload();
-        const char* kd = a.kd + 2 * (b * a.skd[0] + h * a.skd[2]);
-        const char* vd = a.vd + 2 * (b * a.svd[0] + h * a.svd[2]);
-#pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-          const int block = 2 * (tile - seq.seq_tiles) + hf, t = __builtin_amdgcn_readfirstlane(token_of_block(a, block));
-          const int slot = 16 * (block - t * a.slot_blocks);
-          rows[hf] = t < seq.fresh ? min(16, a.Lv - slot) : 0;
-          base[hf][0] = (uint64_t)(kd + 2 * (((int64_t)t * a.L + slot) * a.skd[1]));
-          base[hf][1] = (uint64_t)(vd + 2 * (((int64_t)t * a.L + slot) * a.svd[1]));
-        }
+    uint64_t kp = 0, vp = 0;
+    if (tile < seq.seq_tiles) {
+      const int j = tile * kTileKeys + r, page = *at<int>(Lds::kTable + ring * 256 + 4 * lane);
+      if (j < seq.len && (unsigned)page < (unsigned)a.cache.n_pages) {
+        kp = (uint64_t)(a.cache.k + 2 * a.cache.offset(a.cache.sk, page, j, h));
+        vp = (uint64_t)(a.cache.v + 2 * a.cache.offset(a.cache.sv, page, j, h));
       }
-      there = ((1u << rows[0]) - 1) | ((1u << rows[1]) - 1) << 16;
     } else {
-      const PagedAttendArgs a = reload();
-      uint64_t kp = 0, vp = 0;
-      if (!depth) {
-        const int j = tile * kTileKeys + r, page = *at<int>(Lds::kTable + ring * 256 + 4 * lane);
-        if (j < seq.len && (unsigned)page < (unsigned)a.cache.n_pages) {
-          kp = (uint64_t)(a.cache.k + 2 * a.cache.offset(a.cache.sk, page, j, h));
-          vp = (uint64_t)(a.cache.v + 2 * a.cache.offset(a.cache.sv, page, j, h));
-        }
-      } else {
-        const int block = 2 * (tile - seq.seq_tiles) + (r >> 4), t = token_of_block(a, block), slot = 16 * (block - t * a.slot_blocks) + (r & 15);
-        if (t < seq.fresh && slot < a.Lv) {
-          const int64_t row = (int64_t)t * a.L + slot;
-          kp = (uint64_t)(a.kd + 2 * (b * a.skd[0] + row * a.skd[1] + h * a.skd[2]));
-          vp = (uint64_t)(a.vd + 2 * (b * a.svd[0] + row * a.svd[1] + h * a.svd[2]));
-        }
+      const int block = 2 * (tile - seq.seq_tiles) + (r >> 4), t = token_of_block(a, block), slot = 16 * (block - t * a.slot_blocks) + (r & 15);
+      if (t < seq.fresh && slot < a.Lv) {
+        const int64_t row = (int64_t)t * a.L + slot;
+        kp = (uint64_t)(a.kd + 2 * (b * a.skd[0] + row * a.skd[1] + h * a.skd[2]));
+        vp = (uint64_t)(a.vd + 2 * (b * a.svd[0] + row * a.svd[1] + h * a.svd[2]));
       }
-      there = (uint32_t)__ballot(kp != 0);
-      if (lane < 32) {
-        *at<uint64_t>(Lds::kRows + 16 * r) = kp;
-        *at<uint64_t>(Lds::kRows + 16 * r + 8) = vp;
-      }
+    }
+    const uint32_t there = (uint32_t)__ballot(kp != 0);
+    if (lane < 32) {
+      *at<uint64_t>(Lds::kRows + 16 * r) = kp;
+      *at<uint64_t>(Lds::kRows + 16 * r + 8) = vp;
     }
     if (lane == 0) *at<uint32_t>(Lds::kMask + 4 * stage) = there;
   }
-  // a K (0) or V (1) tile, from the rows found last
+  // a K (0) or V (1) tile, from the rows found last (all addresses first: a load's assembly block is a barrier to the reads behind it)
   __device__ __forceinline__ void fetch_tile(int which, int stage) const {
     const uint32_t to = lds + stage * Lds::kStage + which * Lds::kTile;
-    if (even) {
-      // the range check fills with zeros what lies past the last row and past the head dim
-      const int step = (int)(2 * (which ? a.cache.sv[1] : a.cache.sk[1]));
-#pragma unroll
-      for (int hf = 0; hf < 2; hf++) {
-        const i32x4 rs = rsrc_words((const void*)base[hf][which], (uint32_t)(rows[hf] * step));
-#pragma unroll
-        for (int i = 0; i < kPeriod; i++) lds_dma<16>(rs, to + (hf * kPeriod + i) * 1024, piece[which][i], 0);
-      }
-      return;
-    }
     const int prow = lane / CH, pch = lane % CH, dim = which ? a.Dv : a.D;
     const uint64_t zero = (uint64_t)&zero_line[0];
     uint64_t from[NL];
@@ -404,7 +342,7 @@ struct PagedWave {
   }
 
   // the K tile of step i + NS, the tile's rows, and the table entries of the tile NS steps further
-  __device__ __forceinline__ void send(int tile, int i, int stage) {
+  __device__ __forceinline__ void send(int tile, int i, int stage) const {
     fetch_table(tile + 2 * NS, (i + 2 * NS) % (2 * NS));
     find_rows(tile + NS, (i + NS) % (2 * NS), stage);
     fetch_tile(0, stage);
@@ -440,8 +378,6 @@ struct PagedWave {
   // tiles [t0, t1) of the segment
   __device__ void run(int t0, int t1) {
     const int n = lane & 15, g = lane >> 4, tiles = t1 - t0;
-    k_head = a.cache.k + 2 * (h * a.cache.sk[2]);
-    v_head = a.cache.v + 2 * (h * a.cache.sv[2]);
     const bool one_token = a.cache.T == 1;
     Window seq_win[NR], depth_win[NR];
     int first_t;  // of the row tile's tokens
@@ -735,7 +671,7 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
       const Window win = depth ? Window{row.t * a.slot_blocks * 16, row.t * a.slot_blocks * 16 + a.Lv} : Window{0, seq.past + row.t + 1};
       const bool all_seen = there == 0xffffu && (depth ? one_token : first + 15 <= seq.past + first_t);
 #pragma unroll
-      for (int i = 0; i < 4; i++) p[i] = all_seen | win.sees(there, first, 4 * g + i) ? p[i] : kNegInf;
+      for (int i = 0; i < 4; i++) p[i] = (all_seen | win.sees(there, first, 4 * g + i)) ? p[i] : kNegInf;
       softmax_step<4>(p, m[0], l[0], o, 0);
       bool odd = false;
       if (!all_seen && !one_token) {
@@ -916,7 +852,6 @@ size_t plan_paged_attend(PagedAttendArgs& a, int dtype) {
   a.row_tiles = (rows + 16 * blocks - 1) / (16 * blocks);
   a.part_rows = rows < 16 * blocks ? rows : 16 * blocks;
   a.part_width = width;
-  a.least_tiles = 1;
   // waves of the whole card: as many as hold their rings in the 160 KB of a compute unit
   const int per_unit = dtype == MODA_HIP_FP32 ? (width == 64 ? 8 : 4) : waves_of_a_unit(width, blocks);
   a.slot_blocks = (a.Lv + 15) / 16;
@@ -926,10 +861,6 @@ size_t plan_paged_attend(PagedAttendArgs& a, int dtype) {
                        ((capacity + kTileKeys - 1) / kTileKeys + ((int64_t)a.cache.T * a.slot_blocks + 1) / 2);
   if (most >= 1ll << 30) return 0;  // the axis is counted in 32 bits
   a.group_magic = a.G == 1 ? 0 : (unsigned)((1ull << 32) / a.G) + 1;  // row / G = umulhi(row, magic): rows are below 2^16
-  // sixteen rows through one buffer descriptor: 31-bit offsets, rows that do not reach into the next one
-  const auto even = [&](const int64_t(&s)[3], int dim) { return s[1] >= dim && s[1] < 1 << 25; };
-  a.even_pages = a.cache.page_shift >= 4 && even(a.cache.sk, a.D) && even(a.cache.sv, a.Dv);
-  a.even_slots = even(a.skd, a.D) && even(a.svd, a.Dv) && a.skd[1] == a.cache.sk[1] && a.svd[1] == a.cache.sv[1];
   a.waves = (int)(most < 256 * per_unit ? (most > 0 ? most : 1) : 256 * per_unit);
   const size_t segments = ((size_t)a.cache.B * a.cache.H * a.row_tiles + 1) / 2 * 2;
   return (segments * 2 + (size_t)2 * a.waves * a.part_rows * (a.part_width + 2)) * sizeof(float);
