@@ -984,6 +984,10 @@ struct Rotate : torch::autograd::Function<Rotate> {
       back->inverse = !back->inverse;
       const auto g = pair(ctx->saved_data["q"].toBool(), ctx->saved_data["k"].toBool(), grads);
       if (!g.first.defined() && !g.second.defined()) return variable_list(5);
+      if (!at::GradMode::is_enabled()) {  // no second derivative asked for
+        const auto r = rotate(*back, s[0], g.first, g.second, s[1]);
+        return variable_list{r.first, r.second, Tensor(), Tensor(), Tensor()};
+      }
       const auto r = pair(g.first.defined(), g.second.defined(), apply(optional(g.first), optional(g.second), s[0], optional(s[1]), back));
       return variable_list{r.first, r.second, Tensor(), Tensor(), Tensor()};
     });

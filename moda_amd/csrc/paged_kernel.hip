@@ -7,12 +7,17 @@
 //
 // What bounds it is the stream of keys and values from HBM: each is read once for all rows of its key/value head, four rows
 // make 4 FLOP of a byte, the matrix instruction does a hundred times that.  So the work is cut for the stream alone.  All
-// tiles of 32 keys -- of every sequence, key/value head and 16 (32, 64) rows -- stand on one axis, sequences with
+// tiles of 32 keys -- of every sequence, key/value head and 16 (32) rows -- stand on one axis, sequences with
 // their lengths as they are on the device; each of a fixed number of waves, as many as keep the card's loads in flight, takes an equal
 // run of it, whatever the lengths are, and the host needs to know none of them (a captured launch follows them as they grow).
 // A wave is a workgroup by itself: it fetches its tiles into a ring of its own and waits for nobody.  Runs that begin or end
 // inside a segment (one sequence, head and row tile) leave maximum, sum and o in the workspace, at most two of them a
 // wave; a second launch joins them in the order of the axis, so that results do not depend on who came first.
+//
+// Measured (bf16, head dim 128, four rows a head; a copy of 4 GiB reaches 4.7 TB/s in and out, reading alone more): 256 sequences
+// of 12 - 24 K tokens, 4 heads (9.4 GB) 1.58 ms, 6.0 TB/s; one sequence of 1 M tokens 361 us + 9 for joining, 5.8 TB/s; 64 of 1 - 8 K
+// 117 + 6 us, 5.2 TB/s; one of 101 tokens 6.4 + 4.6 us, the chain counts -> table -> rows -> keys -> products and a second
+// launch.  Four and more rows of eight drafted tokens are bound by the vector instructions of a wave's tile (some 500 a tile).
 #include "paged.h"
 #include "tile16.h"
 #include "../../include/moda_hip.h"
@@ -570,11 +575,15 @@ __device__ __forceinline__ void walk(const PagedAttendArgs& a, int lane, G&& mea
   }
 }
 
-// Stages of a wave's ring and waves of a compute unit (four at one a SIMD).
+// Stages of a wave's ring and waves of a compute unit (four at one a SIMD).  With several waves a SIMD one stage does: K of the next
+// tile is sent for once the scores are formed, V once it is used, and while a wave waits the others work.  Measured: 128 sequences of
+// 4 - 8 K tokens, 64 query heads of 64 on 8, with 2 stages and 8 waves 304 us, 1 and 12: 286, 1 and 16: 299 (registers for
+// four waves a SIMD leave none over); head dim 128, 2 stages and 4 waves against 1 and 8: 2048 short sequences 145 -> 121
+// us, 8 of 2 K tokens 15.3 -> 13.2, a million tokens 356 -> 361.
 template <int W, int NR>
 struct Shape {
-  static constexpr int kStages = W == 64 || (W == 128 && NR == 2) ? 2 : 1;
-  static constexpr int kWaves = W == 64 || (W == 128 && NR == 1) ? 8 : 4;
+  static constexpr int kStages = NR == 2 ? 2 : 1;
+  static constexpr int kWaves = NR == 2 ? (W == 64 ? 8 : 4) : W == 64 ? 12 : W == 128 ? 8 : 4;
 };
 
 template <typename T, int W, int NR>
@@ -613,7 +622,7 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
       o[s][0] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const int first_t = RowOf(a, rt, 16, 0).t;
-    // 16 keys at a time, the next ones on their way while these are worked on
+    // 16 keys at a time, up to head dim 128 with the next ones on their way while these are worked on
     struct Keys {
       f32x4 k[MB], v[4][MB / 4];
       uint64_t vp;  // of key n
@@ -704,13 +713,22 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
           for (int r = 0; r < 4; r++) o[c][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][c / 4][c % 4], p[r], o[c][0], 0, 0, 0);
       }
     };
-    Keys x[2];
-    fetch(2 * t0, x[0]);
-    for (int half = 2 * t0; half < 2 * t1; half += 2) {
-      fetch(half + 1, x[1]);
-      work(half, x[0]);
-      if (half + 2 < 2 * t1) fetch(half + 2, x[0]);
-      work(half + 1, x[1]);
+    if constexpr (W == 256) {  // two sets of keys and values do not fit beside q and o: 451 us spilled, 388 one after the other (32 x 1 - 8 K tokens)
+      Keys x;
+#pragma unroll 1
+      for (int half = 2 * t0; half < 2 * t1; half++) {
+        fetch(half, x);
+        work(half, x);
+      }
+    } else {
+      Keys x[2];
+      fetch(2 * t0, x[0]);
+      for (int half = 2 * t0; half < 2 * t1; half += 2) {
+        fetch(half + 1, x[1]);
+        work(half, x[0]);
+        if (half + 2 < 2 * t1) fetch(half + 2, x[0]);
+        work(half + 1, x[1]);
+      }
     }
     products_done();
     store_part<FP32, W, 1, true>(seq, b, h, rt, whole, slot, o, m, l, lane);
