@@ -186,9 +186,9 @@ hipError_t launch_rows(RowArgs& a, int dtype, bool vec, bool inter, bool paged, 
   }
   a.lane_shift = 0;
   while ((1 << a.lane_shift) < most && a.lane_shift < 8) a.lane_shift++;
-  // One item a thread until the machine is full (256 compute units of 2048 threads), then up to five, which share the angles: 64 K
-  // tokens of 20 items with 20, 10, 5 and 3 items a thread 153, 136, 126 and 161 us.
-  const int64_t full = 256 * 2048, lanes = a.tokens << a.lane_shift;
+  // One item a thread until there are two waves a SIMD, then up to five, which share the angles.  64 K tokens of 20 items with 20, 10, 5
+  // and 3 items a thread: 153, 136, 126 and 161 us; 4 K tokens with 5, 10 and 20 threads a token's chunk 11.2, 11.5 and 12.7 us.
+  const int64_t full = 256 * 512, lanes = a.tokens << a.lane_shift;
   a.groups = (int)max((int64_t)(a.items + 4) / 5, min((int64_t)a.items, full / max(lanes, (int64_t)1)));
   // What does not fit the 256 MB memory-side cache passes it by (115 us instead of 126); what does is found there by whoever reads it next.
   const bool stream_through = a.tokens * bytes > 256ll << 20;
