@@ -1099,8 +1099,8 @@ OptTensor paged_append(const Tensor& k_in, const Tensor& v_in, const Tensor& ck,
   CONTRACT(kd.defined() == vd.defined(), "depth k and v must be given together");
   moda_hip_paged_append_args a = {};
   a.struct_size = sizeof(a);
-  if (kd.defined()) {
-    CONTRACT(kd.dim() == 4 && T > 0 && kd.size(1) % T == 0 && kd.size(1) > 0, "depth k/v must be [B, T*L, H, D]");
+  if (kd.defined() && tb * T > 0) {
+    CONTRACT(kd.dim() == 4 && kd.size(1) % T == 0 && kd.size(1) > 0, "depth k/v must be [B, T*L, H, D]");
     a.L = kd.size(1) / T;
     a.slot = slot;
     CONTRACT(has_shape(kd, {tb, T * a.L, H, D}) && has_shape(vd, {tb, T * a.L, H, Dv}), "depth k/v must be [B, T*L, H, D]");

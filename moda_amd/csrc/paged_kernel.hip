@@ -842,7 +842,8 @@ int waves_of_a_unit(int width, int blocks) {
   return blocks == 1 ? Shape<64, 1>::kWaves : Shape<64, 2>::kWaves;
 }
 
-// Threads of a row's workgroup: parts of one row are read side by side, and many rows keep the card busy by themselves.
+// Threads of a row's workgroup: parts of one row are read side by side, and many rows keep the card busy by themselves.  Few rows of many
+// parts are spread by elements as well (16 rows of 512 parts 12.5 -> 8.6 us; 128 rows of 130 parts: 6.8 spread, 4.5 not).
 template <typename E, int W>
 hipError_t launch_join_of(const PagedAttendArgs& a, int per_tile, hipStream_t stream) {
   const unsigned rows = (unsigned)((int64_t)a.cache.B * a.cache.T * a.G * a.cache.H);
@@ -870,7 +871,7 @@ size_t plan_paged_attend(PagedAttendArgs& a, int dtype) {
   a.row_tiles = (rows + 16 * blocks - 1) / (16 * blocks);
   a.part_rows = rows < 16 * blocks ? rows : 16 * blocks;
   a.part_width = width;
-  // waves of the whole card: as many as hold their rings in the 160 KB of a compute unit
+  // waves of the whole card: what holds its rings in the 160 KB of a compute unit, fp32 by its registers
   const int per_unit = dtype == MODA_HIP_FP32 ? (width == 64 ? 8 : 4) : waves_of_a_unit(width, blocks);
   a.slot_blocks = (a.Lv + 15) / 16;
   a.blocks_inverse = 1.f / (float)(a.slot_blocks > 0 ? a.slot_blocks : 1);

@@ -746,5 +746,6 @@ def test_refusals(gpu_device):
         with pytest.raises((AssertionError, TypeError)):
             moda_amd.paged_append(**{**good, **kw})
     assert moda_amd.paged_append(z(1, 0, 2, 64), z(1, 0, 2, 64), ck, cv, table, past) is None
+    assert moda_amd.paged_append(z(1, 0, 2, 64), z(1, 0, 2, 64), ck, cv, table, past, cached_k=z(1, 0, 2, 64), cached_v=z(1, 0, 2, 64)) is None
     assert moda_amd.paged_moda(z(1, 0, 2, 64), ck, cv, table, past).shape == (1, 0, 2, 64)
     assert moda_amd.paged_moda(z(0, 4, 2, 64), ck, cv, z(0, 3, dtype=torch.int32), z(0, dtype=torch.int32), moda_group_num=4).shape == (0, 4, 2, 64)
