@@ -353,6 +353,44 @@ struct PagedWave {
     fetch_tile(0, stage);
   }
 
+  // Probabilities w times a tile's values.  They go to the matrix instruction in pieces, each the rounding of what those before it left:
+  // three of bf16 hold all 24 bits, two of fp16 hold 22.  Half the bits less (two pieces of bf16: 16) and 0.2 % of the bf16 results were
+  // rounded the other way than the exact ones, with all of them 0.01 %, as many as where everything is in 32 bits.
+  static constexpr int kPieces = __is_same(T, BF16) ? 3 : 2;
+  __device__ __forceinline__ void add_products(float (&w)[NR][8], lds_cptr tile) {
+    i32x4 piece[kPieces][NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+#pragma unroll
+      for (int k = 0; k < kPieces; k++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) piece[k][nr][i] = pack2<T>(w[nr][2 * i], w[nr][2 * i + 1]);
+        if (k + 1 == kPieces) continue;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float x0, x1;
+          unpack2<T>(piece[k][nr][i], x0, x1);
+          w[nr][2 * i] -= x0;
+          w[nr][2 * i + 1] -= x1;
+        }
+      }
+    }
+    constexpr int DEPTH = 4;
+    i32x4 ops[MB];
+#pragma unroll
+    for (int c = 0; c < DEPTH && c < MB; c++) ops[c] = oa.tr_operand(tile, 0, c);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < MB; c++) {
+      if (c + DEPTH < MB) ops[c + DEPTH] = oa.tr_operand(tile, 0, c + DEPTH);
+#pragma unroll
+      for (int k = 0; k < kPieces; k++)
+#pragma unroll
+        for (int nr = 0; nr < NR; nr++) o[c][nr] = mfma16<T>(ops[c], piece[k][nr], o[c][nr]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
   // Values of a tile that not every row sees, one of them not finite: 0 x inf would reach rows that do not see it, so each row adds up
   // what it sees, key by key.  p: the lane's probabilities (zero where unseen, and where they underflow).
   __device__ void add_key_by_key(const float (&p)[8], int nr, Window win, int first, uint32_t there, lds_cptr tile) {
@@ -481,37 +519,7 @@ struct PagedWave {
 #pragma unroll
         for (int nr = 0; nr < NR; nr++) add_key_by_key(p[nr], nr, depth ? depth_win[nr] : seq_win[nr], first, there, vt);
       } else {
-        // Probabilities go to the matrix instruction in two pieces, rounded and what the rounding left: its time does not
-        // matter here, and o is then as good as its 32-bit sums.
-        i32x4 hi[NR], lo[NR];
-#pragma unroll
-        for (int nr = 0; nr < NR; nr++) {
-          float r[8];
-#pragma unroll
-          for (int i4 = 0; i4 < 4; i4++) {
-            hi[nr][i4] = pack2<T>(p[nr][2 * i4], p[nr][2 * i4 + 1]);
-            float x0, x1;
-            unpack2<T>(hi[nr][i4], x0, x1);
-            r[2 * i4] = p[nr][2 * i4] - x0;
-            r[2 * i4 + 1] = p[nr][2 * i4 + 1] - x1;
-          }
-#pragma unroll
-          for (int i4 = 0; i4 < 4; i4++) lo[nr][i4] = pack2<T>(r[2 * i4], r[2 * i4 + 1]);
-        }
-        constexpr int DEPTH = 4;
-        i32x4 ops[MB];
-#pragma unroll
-        for (int c = 0; c < DEPTH && c < MB; c++) ops[c] = oa.tr_operand(vt, 0, c);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int c = 0; c < MB; c++) {
-          if (c + DEPTH < MB) ops[c + DEPTH] = oa.tr_operand(vt, 0, c + DEPTH);
-#pragma unroll
-          for (int nr = 0; nr < NR; nr++) o[c][nr] = mfma16<T>(ops[c], hi[nr], o[c][nr]);
-#pragma unroll
-          for (int nr = 0; nr < NR; nr++) o[c][nr] = mfma16<T>(ops[c], lo[nr], o[c][nr]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        add_products(p, vt);
       }
       WaveTileLoader<64>::reads_done();
       if (more) fetch_tile(1, stage);
