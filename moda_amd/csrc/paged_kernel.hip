@@ -118,7 +118,7 @@ __device__ __forceinline__ int64_t segments(const PagedAttendArgs& a) {
   return ((int64_t)a.cache.B * a.cache.H * a.row_tiles + 1) & ~1ll;  // even: what follows stays on 16 bytes
 }
 
-// A part of a segment that a wave has: its row statistics and sums, row n of 16 (NR times) on lane n = lane & 15, elements
+// A part of a segment that a wave has: its row statistics (m, sum) and sums, row n of 16 (NR times) on lane n = lane & 15, elements
 // 16 c + 4 q + i of o[c] on lane group q = lane >> 4 (MAP: 64 (c / 4) + 16 q + 4 i + c % 4, the order of the fp32 kernel).
 struct PartAt {
   float *ml, *o;
@@ -143,6 +143,23 @@ __device__ __forceinline__ int token_of_block(const PagedAttendArgs& a, int bloc
 struct FP32 {
   typedef float elem;
 };
+
+// What a row's exponents are taken against is its running maximum `top`, for fp16 less 15: probabilities up to 2^15 leave the type
+// 2^-39 of the largest one as its last bit, not 2^-24.  (Maxima of 2^24 and more, whose neighbours are further apart, stay as they are: no
+// probability may pass 2^16.)
+template <typename E>
+constexpr float kLead = __is_same(E, FP16) ? 15.f : 0.f;
+template <typename E>
+__device__ __forceinline__ float base_of(float top) {
+  if (kLead<E> == 0.f) return top;
+  const float y = top - kLead<E>;
+  return top - y > kLead<E> + 0.5f ? top : y;
+}
+// log2 of a row's sum l of probabilities against m
+template <typename E>
+__device__ __forceinline__ float log_sum(float m, float l) {
+  return kLead<E> == 0.f ? m + __builtin_amdgcn_logf(l) : (m + kLead<E>) + __builtin_amdgcn_logf(l * (1.f / (float)(1 << (int)kLead<E>)));
+}
 
 // the row of the call that row r of a row tile is
 struct RowOf {
@@ -202,7 +219,7 @@ __device__ __forceinline__ void store_part(const Seq& seq, int b, int h, int rt,
     }
     if (q == 0)
       out_global<float>(a.lse)[b * a.slse[0] + row.t * a.slse[1] + row.g * a.slse[2] + h * a.slse[3]] =
-          empty ? kNegInf : m[nr] + __builtin_amdgcn_logf(l);
+          empty ? kNegInf : log_sum<E>(m[nr], l);
   }
 }
 
@@ -239,16 +256,27 @@ struct Window {
   }
 };
 
-// The running softmax of one tile: x = logits in base 2 (what is not seen: -inf) -> probabilities against the new maximum; the
-// sums so far are brought to it.  In lanes of one row (four) the maximum agrees, the sum is the lane's own.
-template <int N, int MB, int NR>
-__device__ __forceinline__ void softmax_step(float (&x)[N], float& m, float& l, f32x4 (&o)[MB][NR], int nr) {
-  float top = x[0];
+// The running softmax of one tile: x = logits in base 2 (what is not seen: -inf) -> probabilities against m (base_of the new maximum);
+// the sums so far are brought to it.  In lanes of one row (four) m agrees, the sum is the lane's own.  Returns, for the wave, whether one of them is
+// small (PagedWave::add_small).
+template <typename E, int N, int MB, int NR>
+__device__ __forceinline__ bool softmax_step(float (&x)[N], float& m, float& l, f32x4 (&o)[MB][NR], int nr) {
+  float top = x[0], least = x[0];
 #pragma unroll
-  for (int i = 1; i < N; i++) top = fmaxf(top, x[i]);
-  top = fmaxf(m, row_max(top));
-  const float from = top == kNegInf ? 0.f : top;
-  if (__any(top != m)) {  // (a NaN never equals itself: the sums become NaN with it)
+  for (int i = 1; i < N; i++) {
+    top = fmaxf(top, x[i]);
+    if (kLead<E> != 0.f) least = fminf(least, x[i]);
+  }
+  top = fmaxf(m, base_of<E>(row_max(top)));
+  const float from = top == kNegInf ? 0.f : top, small_below = from - 10.f;
+  bool small = false;
+  if (__any((top != m) | (kLead<E> != 0.f && least < small_below))) {  // (a NaN never equals itself: the sums become NaN with it)
+    if (kLead<E> != 0.f) {
+      bool here = false;
+#pragma unroll
+      for (int i = 0; i < N; i++) here |= (x[i] < small_below) & (x[i] > kNegInf);
+      small = __any(here);
+    }
     const float shrink = fast_exp2(m - from);
     l *= shrink;
 #pragma unroll
@@ -262,6 +290,7 @@ __device__ __forceinline__ void softmax_step(float (&x)[N], float& m, float& l, 
     x[i] = fast_exp2(x[i] - from);
     l += x[i];
   }
+  return small;
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -354,7 +383,7 @@ struct PagedWave {
   }
 
   // Probabilities w times a tile's values.  They go to the matrix instruction in pieces, each the rounding of what those before it left:
-  // three of bf16 hold all 24 bits, two of fp16 hold 22.  Half the bits less (two pieces of bf16: 16) and 0.2 % of the bf16 results were
+  // three of bf16 hold all 24 bits, two of fp16 hold 22 where the second still has them (see add_small).  Half the bits less (two pieces of bf16: 16) and 0.2 % of the bf16 results were
   // rounded the other way than the exact ones, with all of them 0.01 %, as many as where everything is in 32 bits.
   static constexpr int kPieces = __is_same(T, BF16) ? 3 : 2;
   __device__ __forceinline__ void add_products(float (&w)[NR][8], lds_cptr tile) {
@@ -389,6 +418,34 @@ struct PagedWave {
         for (int nr = 0; nr < NR; nr++) o[c][nr] = mfma16<T>(ops[c], piece[k][nr], o[c][nr]);
       __builtin_amdgcn_sched_barrier(0);
     }
+  }
+
+  // fp16: probabilities below 2^-10 -- 2^-25 of the row's largest -- would be left fewer than 14 bits above the type's last one, 2^-24, and
+  // in the end none, while the sum under them counts them.  They take a product of their own, 2^25 times as large, o with them; what they
+  // lose then is 2^-64 of the largest.  (Asking for them and the code for them cost drafted tokens 6 % at head dim 64, 12 at 128, one token
+  // nothing; a second pass over the runs that have them, instead, twice the time where there are some.)
+  static constexpr float kUp = 0x1p25f;
+  __device__ __forceinline__ void scale_sums(float by) {
+#pragma unroll
+    for (int c = 0; c < MB; c++)
+#pragma unroll
+      for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[c][nr][i] *= by;
+  }
+  __device__ __forceinline__ void add_small(float (&p)[NR][8], lds_cptr tile) {
+    float w[NR][8];
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const bool small = p[nr][i] < 0x1p-10f;
+        w[nr][i] = small ? p[nr][i] * kUp : 0.f;
+        p[nr][i] = small ? 0.f : p[nr][i];
+      }
+    scale_sums(kUp);
+    add_products(w, tile);
+    scale_sums(1.f / kUp);
   }
 
   // Values of a tile that not every row sees, one of them not finite: 0 x inf would reach rows that do not see it, so each row adds up
@@ -499,8 +556,9 @@ struct PagedWave {
           }
         }
       }
+      bool small = false;
 #pragma unroll
-      for (int nr = 0; nr < NR; nr++) softmax_step<8>(p[nr], m[nr], l[nr], o, nr);
+      for (int nr = 0; nr < NR; nr++) small |= softmax_step<T, 8>(p[nr], m[nr], l[nr], o, nr);
       if (more)
         wait_but<kBehindV>();
       else
@@ -515,10 +573,11 @@ struct PagedWave {
           for (int i4 = 0; i4 < 4; i4++) odd = odd || (v[i4] & top) == top || (v[i4] >> 16 & top) == top;
         }
       }
-      if (__any(odd)) {
+      if (__builtin_expect(__any(odd), false)) {
 #pragma unroll
         for (int nr = 0; nr < NR; nr++) add_key_by_key(p[nr], nr, depth ? depth_win[nr] : seq_win[nr], first, there, vt);
       } else {
+        if (__builtin_expect(small, false)) add_small(p, vt);
         add_products(p, vt);
       }
       WaveTileLoader<64>::reads_done();
@@ -689,7 +748,7 @@ __global__ __launch_bounds__(64, 1) void paged_fp32_kernel(const PagedAttendArgs
       const bool all_seen = there == 0xffffu && (depth ? one_token : first + 15 <= seq.past + first_t);
 #pragma unroll
       for (int i = 0; i < 4; i++) p[i] = (all_seen | win.sees(there, first, 4 * g + i)) ? p[i] : kNegInf;
-      softmax_step<4>(p, m[0], l[0], o, 0);
+      softmax_step<FP32, 4>(p, m[0], l[0], o, 0);
       bool odd = false;
       if (!all_seen && !one_token) {
 #pragma unroll
@@ -817,7 +876,7 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a,
 #pragma unroll
   for (int e = 0; e < 4; e++) o[e] = empty ? 0.f : o[e] * inv;
   if (e0 + 4 * x < a.Dv) store_four<E>(a.o, to + e0 + 4 * x, o);
-  if (e0 + x == 0) a.lse[b * a.slse[0] + t * a.slse[1] + g * a.slse[2] + h * a.slse[3]] = empty ? kNegInf : top + __builtin_amdgcn_logf(l);
+  if (e0 + x == 0) a.lse[b * a.slse[0] + t * a.slse[1] + g * a.slse[2] + h * a.slse[3]] = empty ? kNegInf : log_sum<E>(top, l);
 }
 
 int tile_width(const PagedAttendArgs& a) {

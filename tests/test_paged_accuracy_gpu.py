@@ -62,3 +62,41 @@ def test_probabilities_keep_their_bits(dtype, gpu_device):
     # 4 keys in at most 3 pieces, the division, the exponential and the pieces of the sum under it
     tol = U[dtype] * want.abs() + (math.log(2) * e + 2 * 2.0 ** -23 + (12 + 2) * 2.0 ** -24) * magnitude + TINY[dtype]
     within(o, want, tol, str(dtype))
+
+
+@pytest.mark.parametrize("gap", [12, 18, 22, 26, 33, 40])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=str)
+def test_small_probabilities_count_in_the_sums_and_in_the_result(dtype, gap, gpu_device):
+    """A first key `gap` bits ahead of 4000 others and without a value, as of a model that parks its attention there: the result is made
+    of the others alone.  So many sequences (of the same pages) that a wave has all keys of one in its run; and the same in many runs."""
+    g = torch.Generator().manual_seed(32)
+    H, D, Dv, n = 8, 8, 8, 4001
+    keys, values = torch.zeros(1, n, H, D, dtype=dtype), torch.zeros(1, n, H, Dv, dtype=dtype)
+    keys[:, 1:, :, 0] = (-(gap + torch.rand(1, n - 1, H, generator=g)) * math.log(2)).to(dtype)
+    values[:, 1:] = ((1 + torch.rand(1, n - 1, H, Dv, generator=g)) * 2.0 ** min(gap - 12, 14)).to(dtype)
+    p = torch.exp(keys[..., :1].double())
+    want, lse = (p * values.double()).sum(1) / p.sum(1), torch.log2(p.sum(1))[..., 0]
+    # logits of at most gap + 1; off by e and, against what they are taken, by 2^-24 of their size and 15; the sums: 32 keys of a tile
+    # in three pieces, the tiles and their changes of scale, parts
+    e = 2.0 ** -23 * (gap + 1.1) + 2.0 ** -24 * (gap + 17)
+    depth = (96 + 2 * 126 + 16) * 2.0 ** -24
+    tol = U[dtype] * want.abs() + (2 * math.log(2) * e + 3 * 2.0 ** -23 + 2 * depth) * want.abs() + n * 2.0 ** (15 - 64) + TINY[dtype]
+    ck, cv, table, past = pages_of(keys, values, gpu_device)
+    for B in (384, 1):
+        q = torch.zeros(B, 1, H, D, dtype=dtype)
+        q[..., 0] = 1
+        o, l = moda_amd.paged_moda_fwd(q.to(gpu_device), ck, cv, table.expand(B, -1), past.expand(B).contiguous(), scale=1.0)
+        within(o[:, 0].double().cpu(), want.expand(B, -1, -1), tol.expand(B, -1, -1), f"o of {B}")
+        within(l[:, 0].double().cpu(), lse.expand(B, -1), torch.full((B, H), math.log(2) * e + depth + 2.0 ** -21), f"lse of {B}")
+
+
+def test_fp16_logits_too_large_to_count_in_ones(gpu_device):
+    """Logits of 2^24 and more, where numbers are further apart than one: the largest probability stays what the type can hold."""
+    for size in (2.0 ** 11, 2.0 ** 12, 2.0 ** 12 + 4, 30000.0, 60000.0):
+        keys, values = torch.full((1, 40, 1, 8), size / 2, dtype=FP16), torch.zeros(1, 40, 1, 8, dtype=FP16)
+        keys[0, 17], values[0, 17] = size, 3.0
+        q = torch.full((1, 1, 1, 8), size, dtype=FP16)
+        o, lse = moda_amd.paged_moda_fwd(q.to(gpu_device), *pages_of(keys, values, gpu_device), scale=1.0)
+        assert (o == 3).all(), (size, o)
+        exact = 8 * size * size * math.log2(math.e)
+        assert abs(float(lse) - exact) <= exact * 12 * 2.0 ** -24, size
