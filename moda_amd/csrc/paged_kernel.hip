@@ -32,7 +32,8 @@ constexpr int kTileKeys = 32;
 __device__ __align__(64) uint32_t zero_line[16];
 
 // The kernel's arguments, read again where they are used: kept from the start they take every scalar register there is, and the main
-// loop's own move to vector lanes and back.  (They begin the kernel's argument segment.)
+// loop's own move to vector lanes and back.  (They begin the kernel's argument segment, which only a kernel knows: in a function that is
+// called, not inlined, its address is zero.  Whoever calls this is forced inline.)
 __device__ __forceinline__ PagedAttendArgs reload() {
   PagedAttendArgs a;
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -448,9 +449,10 @@ struct PagedWave {
     scale_sums(1.f / kUp);
   }
 
-  // Values of a tile that not every row sees, one of them not finite: 0 x inf would reach rows that do not see it, so each row adds up
-  // what it sees, key by key.  p: the lane's probabilities (zero where unseen, and where they underflow).
-  __device__ void add_key_by_key(const float (&p)[8], int nr, Window win, int first, uint32_t there, lds_cptr tile) {
+  // Values of a tile, one of them not finite: each row adds up what it sees, key by key.  0 x inf would reach rows that do not see it, and of
+  // an infinite value that a row sees the pieces of its probability would make inf and, the second being zero or negative, NaN.  p: the
+  // lane's probabilities (zero where unseen, and where they underflow 32 bits: NaN then, as in any 32-bit sum).
+  __device__ __forceinline__ void add_key_by_key(const float (&p)[8], int nr, Window win, int first, uint32_t there, lds_cptr tile) {
     const int n = lane & 15, g = lane >> 4;
 #pragma unroll 1
     for (int key = 0; key < kTileKeys; key++) {
@@ -475,8 +477,8 @@ struct PagedWave {
     }
   }
 
-  // tiles [t0, t1) of the segment
-  __device__ void run(int t0, int t1) {
+  // Tiles [t0, t1) of the segment.  `careful`: every tile's values are looked at, not only those that some row does not see.
+  __device__ __forceinline__ void run(int t0, int t1, bool careful) {
     const int n = lane & 15, g = lane >> 4, tiles = t1 - t0;
     const bool one_token = a.cache.T == 1;
     Window seq_win[NR], depth_win[NR];
@@ -564,7 +566,7 @@ struct PagedWave {
       else
         wait_but<0>();
       bool odd = false;
-      if (!all_seen && !one_token) {
+      if (careful || (!all_seen && !one_token)) {
         const int top = __is_same(T, BF16) ? 0x7f80 : 0x7c00;
 #pragma unroll 2
         for (int c = lane; c < kTileKeys * CH; c += 64) {
@@ -584,6 +586,17 @@ struct PagedWave {
       if (more) fetch_tile(1, stage);
     }
     products_done();
+  }
+  // whether a result is NaN and its row's sum is not: from a value that is not finite
+  __device__ __forceinline__ bool spoiled() const {
+    bool bad = false;
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+      for (int c = 0; c < MB; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) bad |= (o[c][nr][i] != o[c][nr][i]) & (l[nr] == l[nr]);
+    return __any(bad);
   }
 };
 
@@ -663,7 +676,10 @@ __global__ __launch_bounds__(64, (Shape<W, NR>::kWaves + 3) / 4) void paged_kern
     w.b = b;
     w.h = h;
     w.rt = rt;
-    w.run(t0, t1);
+    for (bool careful = false;; careful = true) {
+      w.run(t0, t1, careful);
+      if (careful || __builtin_expect(!w.spoiled(), true)) break;
+    }
     store_part<T, W, NR, false>(seq, b, h, rt, whole, slot, w.o, w.m, w.l, lane);
   });
 }

@@ -100,3 +100,62 @@ def test_fp16_logits_too_large_to_count_in_ones(gpu_device):
         assert (o == 3).all(), (size, o)
         exact = 8 * size * size * math.log2(math.e)
         assert abs(float(lse) - exact) <= exact * 12 * 2.0 ** -24, size
+
+
+def attention64(q, keys, values, scale):
+    """q [rows, D], keys [n, D], values [n, Dv] in 64 bits -> o, lse (base 2), and what they may be off by before o is rounded: logits of D
+    products and a scale (e); a probability of the last unit of its exponential; sums of n terms in any order."""
+    s = q @ keys.T * (scale / math.log(2))
+    lse = torch.logsumexp(s * math.log(2), -1) / math.log(2)
+    p = torch.exp2(s - lse[:, None])
+    e = (q.abs() @ keys.abs().T).amax(-1) * (scale / math.log(2)) * (q.shape[1] + 4) * 2.0 ** -24
+    n = keys.shape[0]
+    finite = values.masked_fill(~values.isfinite(), 0)
+    tol = (2 * math.log(2) * e[:, None] + (2 * n + 100) * 2.0 ** -24) * (p @ finite.abs())
+    return p @ values, lse, tol, e + (n + 20) * 2.0 ** -24 + 2.0 ** -22 * lse.abs().clamp(min=1)
+
+
+def same(got, want, tol, what):
+    """Equal where the reference is not finite (NaN with NaN, infinities by their sign), else within tol."""
+    got, want = got.double().cpu(), want.double()
+    odd = ~want.isfinite()
+    assert torch.equal(got[odd].isnan(), want[odd].isnan()) and bool((got[odd] == want[odd])[~want[odd].isnan()].all()), \
+        f"{what}: {got[odd][:8].tolist()} for {want[odd][:8].tolist()}"
+    within(got.masked_fill(odd, 0), want.masked_fill(odd, 0), tol.masked_fill(odd, 1), what)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=str)
+@pytest.mark.parametrize("T,G,D", [(1, 4, 64), (1, 1, 128), (1, 8, 256), (1, 40, 64), (4, 4, 64), (3, 8, 64), (5, 8, 64), (3, 8, 128), (9, 8, 128), (5, 8, 256),
+                                   (5, 3, 80)], ids=str)
+def test_values_and_keys_that_are_not_finite(dtype, T, G, D, gpu_device):
+    """Infinities and NaN in values, early, in the middle and at the end, seen by all rows, by some, and by one token's alone; NaN in a
+    key.  What a row sees of them is in its result -- inf as inf, inf and -inf as NaN -- and nothing else is; rows of 16 and fewer, of a tile of
+    32 and of several tiles."""
+    g = torch.Generator().manual_seed(33)
+    B, H, L, Lv, n = 3, 2, 6, 5, 231
+    keys, values = torch.randn(B, n, H, D, generator=g).to(dtype), torch.randn(B, n, H, D, generator=g).to(dtype)
+    kd, vd = torch.randn(B, T * L, H, D, generator=g).to(dtype), torch.randn(B, T * L, H, D, generator=g).to(dtype)
+    q = torch.randn(B, T * G, H, D, generator=g).to(dtype)
+    inf, nan = math.inf, math.nan
+    values[0, 3, 0, 1], values[0, 100, 0, 2], values[0, 50, 0, 4], values[0, n - 1, 0, 5] = inf, -inf, nan, inf
+    values[0, 3, 0, 3], values[0, 180, 0, 3] = inf, -inf
+    values[1, n - 1, 1, D - 1], values[1, n - 2, 1, D - 2], vd[1, (T - 1) * L + 2, 0, 6], vd[1, 0, 1, 7] = -inf, inf, -inf, nan
+    vd[:, Lv::L], kd[:, Lv::L] = nan, nan  # slots that are not valid
+    keys[2, n - 1, 0, 0], kd[2, 1, 1, 2] = nan, nan
+    past = torch.full((B,), n - T, dtype=torch.int32, device=gpu_device)
+    ck, cv, table, _ = pages_of(keys, values, gpu_device)
+    o, lse = moda_amd.paged_moda_fwd(q.to(gpu_device), ck, cv, table, past, cached_k=kd.to(gpu_device), cached_v=vd.to(gpu_device), depth_valid=Lv,
+                                     moda_group_num=G)
+    for b in range(B):
+        for t in range(T):
+            for h in range(H):
+                seen = n - T + t + 1
+                slots = slice(t * L, t * L + Lv)
+                k, v = (torch.cat([x[b, :seen, h], y[b, slots, h]]).double() for x, y in ((keys, kd), (values, vd)))
+                rows = (b, slice(t * G, t * G + G), h)
+                if k.isnan().any():
+                    assert o[rows].isnan().all() and lse[rows].isnan().all(), (b, t, h)
+                    continue
+                x, l, tol, tl = attention64(q[rows].double(), k, v, D ** -0.5)
+                same(o[rows], x, tol + U[dtype] * x.abs() + TINY[dtype], f"o {b} {t} {h}")
+                same(lse[rows], l, tl, f"lse {b} {t} {h}")
