@@ -1016,9 +1016,12 @@ std::pair<OptTensor, OptTensor> apply_rotary(const OptTensor& q, const OptTensor
 // ------------------------------------------------------------------------------------------------------------------
 
 void no_gradients(std::initializer_list<const Tensor*> xs, const char* what) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* x : xs)
-    CONTRACT(!x->defined() || !x->requires_grad(), what, " has no backward pass: call it under torch.no_grad()");
+  const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* x : xs) {
+    if (!x->defined()) continue;
+    CONTRACT(!backward || !x->requires_grad(), what, " has no backward pass: call it under torch.no_grad()");
+    CONTRACT(!forward || !x->_fw_grad(0).defined(), what, " has no forward-mode derivative: it would drop the tangent it is given");
+  }
 }
 
 const int32_t* counts(const Tensor& x, const char* name, std::initializer_list<int64_t> shape, const Tensor& cache) {
