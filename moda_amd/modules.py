@@ -341,8 +341,11 @@ class MoDAStack(nn.Module):
     def prefill(self, x, cache: PagedKVCache, lens: Optional[torch.Tensor] = None):
         """Prompts ``x [batch, N, dim]``, of which the first ``lens [batch]`` (int32; none given: all ``N``) tokens are real, for the
         empty sequences of ``cache`` (pages reserved): ``forward``'s result, keys and values of all layers in the cache, its
-        counts advanced.  Rows behind a prompt's end hold nothing of use."""
+        counts advanced.  Rows behind a prompt's end hold nothing of use.  Sequences with tokens of their own (``decode`` goes on with those)
+        or without pages for the prompt are an error, for which the call waits for the device (not in a captured one, which does not look)."""
         self._check_cache(x, cache)
+        if not torch.cuda.is_current_stream_capturing():
+            cache.check_prompts(x.shape[1], lens)
         stream = DepthStream(self._slots())
         for i, blk in enumerate(self.blocks):
             x, k, v = self._block(blk, x, lambda h: blk.attn(h, stream=stream))

@@ -126,6 +126,21 @@ class PagedKVCache:
         self._free.extend(reversed(self._pages[b]))
         self._pages[b] = []
 
+    def check_prompts(self, tokens: int, lens: Optional[torch.Tensor] = None):
+        """An error unless each sequence that a prompt of ``tokens`` (``lens [batch]``: of at most that many) goes to is empty and has pages
+        for it.  Waits for the device."""
+        assert lens is None or (lens.shape == self.past.shape and lens.device == self.past.device), "lens must be [batch], on the cache's device"
+        new = torch.full_like(self.past, tokens) if lens is None else lens.clamp(0, tokens)
+        need = (new + (self.page_size - 1)) // self.page_size
+        missing = (self.page_table < 0) | (self.page_table >= self.n_pages)
+        at = torch.arange(self.page_table.shape[1], device=self.past.device)
+        short = (missing & (at < need[:, None])).any() | (need > at.numel()).any()
+        started, short = torch.stack([((self.past > 0) & (new > 0)).any(), short]).tolist()
+        if started:
+            raise RuntimeError("a prompt is for an empty sequence, and one of these has tokens: release it, or go on with decode")
+        if short:
+            raise RuntimeError("a prompt's tokens have no pages: reserve them")
+
     def append(self, layer: int, k, v, new_lens=None, cu_seqlens=None, q=None, rotary: Optional[Rotary] = None, moda_group_num: int = 1,
                depth: Optional[DepthCache] = None):
         """``paged_append`` on a layer's pages; ``depth``: and as the next slot of a depth cache of the same tokens."""

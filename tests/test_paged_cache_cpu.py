@@ -1,0 +1,32 @@
+"""What a cache of pages counts and refuses, without a GPU."""
+import pytest
+import torch
+
+import moda_amd
+
+
+def cache(**kw):
+    args = dict(layers=1, n_pages=6, page_size=16, H=1, D=8, dtype=torch.float32, device="cpu", batch=3, max_tokens=64)
+    return moda_amd.PagedKVCache(**{**args, **kw})
+
+
+def test_prompts_need_empty_sequences_and_pages():
+    c = cache()
+    for b, n in enumerate((33, 16, 0)):
+        c.reserve(b, n)
+    lens = lambda *n: torch.tensor(n, dtype=torch.int32)  # noqa: E731
+    c.check_prompts(33, lens(33, 16, 0))
+    c.check_prompts(40, lens(40, 9, -5))  # three pages; counts below zero are none
+    c.check_prompts(0)
+    for n, l in ((33, None), (33, lens(33, 17, 0)), (49, lens(49, 0, 0)), (33, lens(1, 1, 1)), (65, lens(99, 0, 0))):
+        with pytest.raises(RuntimeError, match="pages"):
+            c.check_prompts(n, l)
+    c.past.copy_(lens(0, 1, -3))
+    c.check_prompts(33, lens(33, 0, 0))
+    with pytest.raises(RuntimeError, match="empty"):
+        c.check_prompts(33, lens(33, 1, 0))
+    c.release(1)
+    c.reserve(1, 16)
+    c.check_prompts(33, lens(33, 1, 0))
+    with pytest.raises(AssertionError):
+        c.check_prompts(33, lens(33, 1))

@@ -47,3 +47,37 @@ def test_forward_mode_derivatives_are_refused(gpu_device):
             attend(), append(), plain()
     with fw.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
         moda_amd.apply_rotary(fw.make_dual(k, torch.ones_like(k)), None, moda_amd.Rotary(64))
+
+
+def stack(dev, depth=2, rotary=True):
+    torch.manual_seed(41)
+    return moda_amd.MoDAStack(64, depth, 4, 2, mlp_ratio=2.0, is_causal=True, rotary=moda_amd.Rotary(16) if rotary else None).to(dev).eval()
+
+
+def stack_cache(dev, batch=2, n_pages=8, max_tokens=64):
+    return moda_amd.PagedKVCache(2, n_pages, 16, 2, 16, torch.float32, dev, batch=batch, max_tokens=max_tokens)
+
+
+def test_prefill_refuses_sequences_that_have_tokens_or_no_pages(gpu_device):
+    """Keys rotated from position zero would lie behind those that are there; tokens without pages would be gone."""
+    dev = gpu_device
+    m, c = stack(dev), stack_cache(dev)
+    x = torch.randn(2, 20, 64, device=dev)
+    with pytest.raises(RuntimeError, match="pages"):
+        m.prefill(x, c)
+    c.reserve(0, 20)
+    with pytest.raises(RuntimeError, match="pages"):
+        m.prefill(x, c)
+    first = torch.tensor([20, 0], dtype=torch.int32, device=dev)
+    m.prefill(x, c, lens=first)
+    assert c.past.tolist() == [20, 0]
+    c.reserve(0, 64), c.reserve(1, 20)
+    with pytest.raises(RuntimeError, match="empty"):
+        m.prefill(x, c)
+    m.prefill(x, c, lens=20 - first)  # the other one, beside a sequence that goes on
+    assert c.past.tolist() == [20, 20]
+    c.release(0)
+    c.reserve(0, 20)
+    m.prefill(x, c, lens=first)
+    with pytest.raises(AssertionError):
+        m.prefill(x, c, lens=first[:1])
