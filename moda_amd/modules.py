@@ -353,7 +353,7 @@ class MoDAStack(nn.Module):
             stream.push(k, v)
             if self.ffn_kv:
                 stream.push(*blk.attn.project_depth_kv(x))
-        cache.advance(x.shape[1] if lens is None else lens)
+        cache.advance(x.shape[1] if lens is None else lens.clamp(0, x.shape[1]))
         return x
 
     @torch.no_grad()
@@ -374,7 +374,7 @@ class MoDAStack(nn.Module):
             (x,) = self._block(blk, x, lambda h: (blk.attn.step(h, cache, i, depth, lens),))
             if self.ffn_kv:
                 depth.append(*blk.attn.project_depth_kv(x, positions))
-        cache.advance(N if lens is None else lens)
+        cache.advance(N if lens is None else lens.clamp(0, N))  # what append and attend took it as
         return x
 
     def _check_cache(self, x, cache):

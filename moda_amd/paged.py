@@ -158,5 +158,6 @@ class PagedKVCache:
                           moda_group_num)
 
     def advance(self, n):
-        """The step's tokens count from now on: an int for all sequences, or int32 ``[batch]`` (``new_lens``)."""
+        """The step's tokens count from now on: an int for all sequences, or int32 ``[batch]``, as they are (``new_lens`` that may be out of
+        the call's range are bounded by it there: pass ``new_lens.clamp(0, T)``; negative ones take tokens back)."""
         self.past.add_(n)

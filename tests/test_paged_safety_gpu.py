@@ -81,3 +81,47 @@ def test_prefill_refuses_sequences_that_have_tokens_or_no_pages(gpu_device):
     m.prefill(x, c, lens=first)
     with pytest.raises(AssertionError):
         m.prefill(x, c, lens=first[:1])
+
+
+def test_counts_of_new_tokens_are_bounded_everywhere(gpu_device):
+    """More real tokens than the call has, or fewer than none, count as all and none: in what is stored, seen and counted, also captured."""
+    dev = gpu_device
+    m = stack(dev)
+    x, y = torch.randn(2, 20, 64, device=dev), torch.randn(2, 3, 64, device=dev)
+    out = []
+    for lens in ([50, 20], [20, 20]):
+        c = stack_cache(dev)
+        c.k.fill_(math.nan), c.v.fill_(math.nan)
+        for b in range(2):
+            c.reserve(b, 64)
+        r = [m.prefill(x, c, lens=torch.tensor(lens, dtype=torch.int32, device=dev))]
+        r.append(m.decode(y, c, lens=torch.tensor([9, -4], dtype=torch.int32, device=dev))[:1])
+        assert c.past.tolist() == [23, 20]
+        r.append(m.decode(y, c))
+        out.append(r)
+    for a, b in zip(*out):
+        assert torch.equal(a, b) and a.isfinite().all()
+
+
+def test_captured_prefill(gpu_device):
+    """Nothing waits for the device while a graph is captured; counts of new tokens are bounded there too."""
+    dev = gpu_device
+    m, c = stack(dev), stack_cache(dev)
+    for b in range(2):
+        c.reserve(b, 40)
+    x, lens = torch.randn(2, 20, 64, device=dev), torch.tensor([20, 7], dtype=torch.int32, device=dev)
+    m.prefill(x, c, lens=lens)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = m.prefill(x, c, lens=lens)
+    for n in ([33, 5], [1, 0], [-2, 20]):
+        x.normal_()
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        c.past.zero_()
+        graph.replay()
+        kept = got.clone()
+        assert c.past.tolist() == [min(max(i, 0), 20) for i in n]
+        c.past.zero_()
+        want = m.prefill(x, c, lens=lens)
+        assert torch.equal(kept, want)
