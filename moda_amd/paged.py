@@ -106,7 +106,8 @@ class PagedKVCache:
         self._pages: List[List[int]] = [[] for _ in range(self.batch)]
 
     def reserve(self, b: int, tokens: int):
-        """Pages for the first ``tokens`` positions of sequence ``b`` (those it has stay where they are)."""
+        """Pages for the first ``tokens`` positions of sequence ``b`` (those it has stay where they are).  Reserve before the step that needs
+        them: tokens that had no page were not stored, and no longer count once there are pages behind the last one."""
         own, need = self._pages[b], -(-int(tokens) // self.page_size)
         if need > self.page_table.shape[1]:
             raise ValueError(f"{tokens} tokens are more than a sequence may have ({self.page_table.shape[1] * self.page_size})")
@@ -117,6 +118,7 @@ class PagedKVCache:
             raise RuntimeError(f"the cache is full: {more} pages needed, {len(self._free)} free")
         new = [self._free.pop() for _ in range(more)]
         self.page_table[b, len(own):need] = torch.tensor(new, dtype=torch.int32).to(self.page_table.device)
+        self.past[b].clamp_(max=len(own) * self.page_size)  # the new pages hold nothing yet
         own.extend(new)
 
     def release(self, b: int):

@@ -30,3 +30,18 @@ def test_prompts_need_empty_sequences_and_pages():
     c.check_prompts(33, lens(33, 1, 0))
     with pytest.raises(AssertionError):
         c.check_prompts(33, lens(33, 1))
+
+
+def test_pages_that_come_late_hold_no_tokens():
+    """Positions that were counted without a page were dropped: the page that would hold them now has not been written."""
+    c = cache()
+    c.reserve(0, 20), c.reserve(1, 16), c.reserve(2, 1)
+    c.past.copy_(torch.tensor([35, 9, 17], dtype=torch.int32))
+    c.reserve(0, 32)  # has them already
+    assert c.past.tolist() == [35, 9, 17]
+    c.reserve(0, 40)
+    c.reserve(1, 17)
+    assert c.past.tolist() == [32, 9, 17]
+    c.release(1)
+    c.reserve(2, 30)
+    assert c.past.tolist() == [32, 0, 16]

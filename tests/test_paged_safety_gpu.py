@@ -125,3 +125,22 @@ def test_captured_prefill(gpu_device):
         c.past.zero_()
         want = m.prefill(x, c, lens=lens)
         assert torch.equal(kept, want)
+
+
+def test_tokens_without_a_page_are_never_read(gpu_device):
+    """A sequence that ran past its pages goes on behind what is stored once it has more: nothing of the pages' former contents is seen."""
+    dev = gpu_device
+    m, c = stack(dev, rotary=False), stack_cache(dev, batch=1)
+    c.k.fill_(math.nan), c.v.fill_(math.nan)
+    x = torch.randn(1, 24, 64, device=dev)
+    c.reserve(0, 16)
+    m.prefill(x[:, :14], c)
+    for i in range(14, 20):  # the last four have no page
+        assert m.decode(x[:, i:i + 1], c).isfinite().all()
+    c.reserve(0, 40)
+    assert c.past.tolist() == [16]
+    out = m.decode(x[:, 20:], c)
+    with torch.no_grad():
+        want = m(torch.cat([x[:, :16], x[:, 20:]], 1))[:, 16:]
+    # fp32 on both sides, sums of at most 128 terms in other orders through two blocks of five
+    assert (out - want).abs().max() <= 2 * 5 * 128 * 2.0 ** -24 * want.abs().max()
