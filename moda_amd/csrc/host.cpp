@@ -4,6 +4,7 @@
 // backward enters the kernels straight from the autograd engine.  Python module moda_amd._host.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -917,6 +918,14 @@ void check_rates(const Tensor& rates, int64_t dim, const Tensor& x) {
   CONTRACT(rates.device() == x.device(), "rates and tensors must be on one device");
 }
 
+// The table of rates was made on the stream of its first call and goes with its Rotary, whenever the caller drops that: its memory
+// is not given away before the work that is on this stream now is done.
+const double* rates_of(const Tensor& rates) {
+  const c10::impl::VirtualGuardImpl device(rates.device().type());
+  device.recordDataPtrOnStream(rates.storage().data_ptr(), device.getStream(rates.device()));
+  return rates.const_data_ptr<double>();
+}
+
 // one launch for both tensors (either may be undefined): q [B, T * G, Hq, D], k [B, T, H, D]
 std::pair<Tensor, Tensor> rotate(const Rotation& r, const Tensor& rates, const Tensor& q_in, const Tensor& k_in, const Tensor& positions_in) {
   const Tensor& any = q_in.defined() ? q_in : k_in;
@@ -949,7 +958,7 @@ std::pair<Tensor, Tensor> rotate(const Rotation& r, const Tensor& rates, const T
     parts[n++] = {in_ptr(in[i]), out_ptr(out[i]), strides_of(in[i]), strides_of(out[i]), i == 0 ? r.G : 1, in[i].size(2)};
   }
   if (n == 0) return {out[0], out[1]};
-  const moda_hip_rotary how = {rates.const_data_ptr<double>(), r.dim, (float)r.amplitude, r.interleaved, r.inverse, 0};
+  const moda_hip_rotary how = {rates_of(rates), r.dim, (float)r.amplitude, r.interleaved, r.inverse, 0};
   c10::OptionalDeviceGuard guard(any.device());
   check_rc(moda_hip_rotary_rows(dt, B, T, D, parts, n, in_ptr(positions), positions.defined() && positions.scalar_type() == at::kLong,
                                 positions.defined() && positions.dim() == 2 ? positions.stride(0) : 0, &how, stream_of(any)),
@@ -1132,7 +1141,7 @@ OptTensor paged_append(const Tensor& k_in, const Tensor& v_in, const Tensor& ck,
   if (rates.has_value()) {
     check_rates(*rates, dim, ck);
     CONTRACT(dim <= D, "the rotation turns ", dim, " elements of a head, which has ", D);
-    how = {rates->const_data_ptr<double>(), dim, (float)amplitude, interleaved, 0, 0};
+    how = {rates_of(*rates), dim, (float)amplitude, interleaved, 0, 0};
   }
   if (tb * T == 0) return optional(q_out);
   const Tensor k = usable(k_in, false), v = usable(v_in, false);

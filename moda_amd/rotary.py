@@ -29,7 +29,8 @@ class Rotary:
     ``amplitude`` (on the rotated elements) and ``rates`` replace what the rules above give.
 
     The rates stay on the host in 64 bits; each device gets a copy at its first call (before a graph capture make one
-    ordinary call, as for every operator of this package)."""
+    ordinary call, as for every operator of this package; a captured call reads that copy at every replay: keep the ``Rotary`` as long
+    as the graph).  A ``Rotary`` may be dropped while calls on any stream are still under way."""
 
     def __init__(self, dim: int, base: float = 10000.0, interleaved: bool = False, scaling: Optional[str] = None, factor: float = 1.0,
                  original_length: Optional[int] = None, slow: float = 1.0, fast: float = 32.0, amplitude: Optional[float] = None,

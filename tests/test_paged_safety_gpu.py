@@ -144,3 +144,34 @@ def test_tokens_without_a_page_are_never_read(gpu_device):
         want = m(torch.cat([x[:, :16], x[:, 20:]], 1))[:, 16:]
     # fp32 on both sides, sums of at most 128 terms in other orders through two blocks of five
     assert (out - want).abs().max() <= 2 * 5 * 128 * 2.0 ** -24 * want.abs().max()
+
+
+@pytest.mark.parametrize("call", ["rotate", "append"])
+def test_a_rotary_dropped_while_another_stream_uses_it(call, gpu_device):
+    """The rates' memory belongs to the stream that made them: it stays theirs until the calls of other streams are done."""
+    dev = gpu_device
+    rot = moda_amd.Rotary(64)
+    x = torch.randn(1, 3, 2, 64, device=dev).to(BF16)
+    ck, cv, table, past = pages(dev)
+
+    def run(rot):
+        if call == "rotate":
+            return moda_amd.apply_rotary(x, None, rot)[0]
+        return moda_amd.paged_append(x, x, ck, cv, table, past, q=x, rotary=rot)
+
+    want = run(rot)
+    busy = torch.randn(8192, 8192, device=dev).to(BF16)
+    out = torch.empty_like(busy)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(30):
+            torch.mm(busy, busy, out=out)
+        got = run(rot)
+    at = rot.rates(x.device).data_ptr()
+    del rot
+    taken = [torch.full((32,), math.nan, dtype=torch.float64, device=dev) for _ in range(200)]
+    assert not side.query(), "the other stream was done too early for this test to say anything"
+    assert all(t.data_ptr() != at for t in taken)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
