@@ -830,12 +830,13 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a,
   __shared__ f32x4 sums[WAVES][LANES];
   __shared__ float lsum[WAVES], tops[WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, x = tid % LANES, group = tid / LANES;
-  int64_t at = blockIdx.x;
+  unsigned at = blockIdx.y * gridDim.x + blockIdx.x;  // (rows are below 2^31)
   const int e0 = W == WC ? 0 : (int)(at % (W / WC)) * WC;  // the workgroup's first element
   at /= W / WC;
-  const int h = (int)(at % a.cache.H);
-  at /= a.cache.H;
-  const int rows = a.cache.T * a.G, row = (int)(at % rows), b = (int)(at / rows);
+  const int h = (int)(at % (unsigned)a.cache.H);
+  at /= (unsigned)a.cache.H;
+  const int rows = a.cache.T * a.G, row = (int)(at % (unsigned)rows), b = (int)(at / (unsigned)rows);
+  if (b >= a.cache.B) return;
   const int rt = row / rows_per_tile, r = row - rt * rows_per_tile, t = row / a.G, g = row - t * a.G;
   const int64_t seg = ((int64_t)b * a.cache.H + h) * a.row_tiles + rt;
   const int first = ((const int*)a.work)[2 * seg], last = ((const int*)a.work)[2 * seg + 1];
@@ -929,15 +930,19 @@ int waves_of_a_unit(int width, int blocks) {
 // parts are spread by elements as well (16 rows of 512 parts 12.5 -> 8.6 us; 128 rows of 130 parts: 6.8 spread, 4.5 not).
 template <typename E, int W>
 hipError_t launch_join_of(const PagedAttendArgs& a, int per_tile, hipStream_t stream) {
-  const unsigned rows = (unsigned)((int64_t)a.cache.B * a.cache.T * a.G * a.cache.H);
+  const int64_t rows = (int64_t)a.cache.B * a.cache.T * a.G * a.cache.H;
+  const auto grid = [](int64_t n) {  // an axis of a launch has less than 2^32 threads
+    const unsigned x = (unsigned)(n < 1 << 20 ? n : 1 << 20);
+    return dim3(x, (unsigned)((n + x - 1) / x));
+  };
   if (rows >= 2048)
-    paged_join_kernel<E, W, W, 64><<<rows, 64, 0, stream>>>(a, per_tile);
+    paged_join_kernel<E, W, W, 64><<<grid(rows), 64, 0, stream>>>(a, per_tile);
   else if (rows >= 256)
-    paged_join_kernel<E, W, W, 256><<<rows, 256, 0, stream>>>(a, per_tile);
+    paged_join_kernel<E, W, W, 256><<<grid(rows), 256, 0, stream>>>(a, per_tile);
   else if (rows >= 64)
-    paged_join_kernel<E, W, W, 1024><<<rows, 1024, 0, stream>>>(a, per_tile);
+    paged_join_kernel<E, W, W, 1024><<<grid(rows), 1024, 0, stream>>>(a, per_tile);
   else
-    paged_join_kernel<E, W, 32, 1024><<<rows * (W / 32), 1024, 0, stream>>>(a, per_tile);
+    paged_join_kernel<E, W, 32, 1024><<<grid(rows * (W / 32)), 1024, 0, stream>>>(a, per_tile);
   return hipGetLastError();
 }
 template <typename E>

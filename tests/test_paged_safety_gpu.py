@@ -175,3 +175,19 @@ def test_a_rotary_dropped_while_another_stream_uses_it(call, gpu_device):
     assert all(t.data_ptr() != at for t in taken)
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+def test_attention_of_2_to_the_26_rows(gpu_device):
+    """As many rows as an axis of one launch has no threads for: each sequence sees its first key."""
+    dev = gpu_device
+    B, H, G, D = 1 << 14, 256, 16, 8
+    ck, cv, _, _ = pages(dev, n=1, H=H, D=D)
+    torch.manual_seed(42)
+    ck[0, 0], cv[0, 0] = torch.randn(H, D, device=dev), torch.randn(H, D, device=dev)
+    table, past = torch.zeros(1, 1, dtype=torch.int32, device=dev).expand(B, 1), torch.zeros(B, dtype=torch.int32, device=dev)
+    q = torch.zeros(B, 1, H * G, D, dtype=BF16, device=dev)
+    q[..., 0] = 1
+    o, lse = moda_amd.paged_attn_fwd(q, ck, cv, table, past, scale=1.0)
+    assert torch.equal(o.view(B, H, G, D), cv[0, 0][:, None].expand(B, H, G, D))
+    want = ck[0, 0, :, 0].float()[:, None] * math.log2(math.e)
+    assert ((lse.view(B, H, G) - want).abs() <= 2.0 ** -22 * want.abs()).all()
