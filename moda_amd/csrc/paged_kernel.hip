@@ -587,15 +587,18 @@ struct PagedWave {
     }
     products_done();
   }
-  // whether a result is NaN and its row's sum is not: from a value that is not finite
+  // Whether a result is NaN and its row's sum is not: from a value that is not finite.  (Asked of all elements of a row together: infinities of
+  // both signs among them run once more for nothing.)
   __device__ __forceinline__ bool spoiled() const {
     bool bad = false;
 #pragma unroll
-    for (int nr = 0; nr < NR; nr++)
+    for (int nr = 0; nr < NR; nr++) {
+      f32x4 all = o[0][nr];
 #pragma unroll
-      for (int c = 0; c < MB; c++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) bad |= (o[c][nr][i] != o[c][nr][i]) & (l[nr] == l[nr]);
+      for (int c = 1; c < MB; c++) all += o[c][nr];
+      const float sum = (all[0] + all[1]) + (all[2] + all[3]);
+      bad |= (sum != sum) & (l[nr] == l[nr]);
+    }
     return __any(bad);
   }
 };
