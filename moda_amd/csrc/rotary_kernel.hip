@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
     else
       *(vec*)p = x;
   };
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, unit = id >> a.lane_shift;
+  const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x, unit = id >> a.lane_shift;
   const int c0 = (int)(id & ((1 << a.lane_shift) - 1));
   const int64_t n = unit / a.groups;
   if (n >= a.tokens) return;
@@ -162,7 +162,9 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
 
 template <typename E, int VEC, bool PAGED>
 static void launch_rows_as(const RowArgs& a, bool inter, bool stream_through, int64_t blocks, hipStream_t stream) {
-  const unsigned grid = (unsigned)blocks;
+  // an axis of a launch has less than 2^32 threads
+  const unsigned x = (unsigned)(blocks < 1 << 20 ? blocks : 1 << 20);
+  const dim3 grid(x, (unsigned)((blocks + x - 1) / x));
   if (VEC > 1 && stream_through) {
     inter ? rows_kernel<E, VEC, true, PAGED, VEC != 1><<<grid, 256, 0, stream>>>(a) : rows_kernel<E, VEC, false, PAGED, VEC != 1><<<grid, 256, 0, stream>>>(a);
     return;

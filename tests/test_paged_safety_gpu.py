@@ -191,3 +191,14 @@ def test_attention_of_2_to_the_26_rows(gpu_device):
     assert torch.equal(o.view(B, H, G, D), cv[0, 0][:, None].expand(B, H, G, D))
     want = ck[0, 0, :, 0].float()[:, None] * math.log2(math.e)
     assert ((lse.view(B, H, G) - want).abs() <= 2.0 ** -22 * want.abs()).all()
+
+
+def test_rotation_of_2_to_the_30_tokens(gpu_device):
+    """As many threads as an axis of one launch does not have."""
+    T, rot = 1 << 30, moda_amd.Rotary(8)
+    x = torch.randn(1, 1, 1, 8, device=gpu_device).to(BF16)
+    y = moda_amd.apply_rotary(None, x.expand(1, T, 1, 8), rot)[1]
+    at = torch.tensor([0, 1, 12345, (1 << 28) - 1, 1 << 28, (1 << 29) + 7, T - 2, T - 1], device=gpu_device)
+    want = moda_amd.apply_rotary(None, x.expand(1, 8, 1, 8), rot, positions=at)[1]
+    assert torch.equal(y[0, at], want[0])
+    assert bool((y.view(torch.int16)[:, ::4096] != 0).any(-1).all())
