@@ -741,7 +741,7 @@ int fill_cache(const moda_hip_paged_cache* c, moda::PagedKV& to) {
       c->max_pages * c->page_size > most / 2 || c->B >= (1 << 20) || c->T >= (1 << 24) || c->H >= (1 << 16) || c->B * c->T >= most ||
       c->total_tokens >= most)
     return MODA_HIP_EUNSUPPORTED;
-  if (!c->k_pages || !c->v_pages || !c->table || !c->past) return MODA_HIP_EINVAL;
+  if (!c->k_pages || !c->v_pages || (c->B > 0 && (!c->table || !c->past))) return MODA_HIP_EINVAL;  // (arrays of no sequences may be NULL)
   if (!aligned(c->k_pages, c->k, elem_size(c->dtype), true) || !aligned(c->v_pages, c->v, elem_size(c->dtype), true)) return MODA_HIP_EALIGN;
   for (const void* p : {c->table, c->past, c->new_lens, c->cu_seqlens})
     if ((uintptr_t)p % sizeof(int32_t) != 0) return MODA_HIP_EALIGN;

@@ -1,8 +1,13 @@
 """What a cache of pages counts and refuses, without a GPU."""
+import ctypes
+
 import pytest
 import torch
 
 import moda_amd
+from moda_amd import _lib
+
+from test_paged_cpu import AT, EINVAL, AppendC, pages, strides
 
 
 def cache(**kw):
@@ -45,3 +50,11 @@ def test_pages_that_come_late_hold_no_tokens():
     c.release(1)
     c.reserve(2, 30)
     assert c.past.tolist() == [32, 0, 16]
+
+
+def test_arrays_of_no_sequences_may_be_null():
+    lib, s = _lib.load(), strides(128, 128, 64)
+    a = AppendC(struct_size=ctypes.sizeof(AppendC), k=AT, v=AT, sk=s, sv=s)
+    for kw, code in ((dict(B=0, table=None, past=None), 0), (dict(B=0, table=None, past=None, cu_seqlens=AT, total_tokens=0), 0),
+                     (dict(table=None), EINVAL), (dict(past=None), EINVAL), (dict(B=0, k_pages=None), EINVAL)):
+        assert lib.moda_hip_paged_append(ctypes.byref(pages(**kw)), ctypes.byref(a), None, None) == code, kw

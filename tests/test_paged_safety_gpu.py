@@ -202,3 +202,14 @@ def test_rotation_of_2_to_the_30_tokens(gpu_device):
     want = moda_amd.apply_rotary(None, x.expand(1, 8, 1, 8), rot, positions=at)[1]
     assert torch.equal(y[0, at], want[0])
     assert bool((y.view(torch.int16)[:, ::4096] != 0).any(-1).all())
+
+
+def test_packed_tokens_of_no_sequence(gpu_device):
+    """Offsets of no sequences: all rows are behind the last one, stored nowhere and returned as they are."""
+    dev = gpu_device
+    ck, cv, _, _ = pages(dev)
+    table, past = (torch.empty(*s, dtype=torch.int32, device=dev) for s in ((0, 3), (0,)))
+    x, q, kd = torch.randn(1, 5, 2, 64, device=dev).to(BF16), torch.randn(1, 10, 2, 64, device=dev).to(BF16), torch.zeros(1, 15, 2, 64, dtype=BF16, device=dev)
+    q1 = moda_amd.paged_append(x, x, ck, cv, table, past, cu_seqlens=torch.zeros(1, dtype=torch.int32, device=dev), q=q, rotary=moda_amd.Rotary(64),
+                               moda_group_num=2, cached_k=kd, cached_v=kd.clone(), depth_slot=1)
+    assert torch.equal(q1, q) and not ck.any() and not cv.any() and not kd.any()
