@@ -1059,6 +1059,7 @@ moda_hip_paged_cache describe_cache(const Tensor& ck, const Tensor& cv, const Te
   const int64_t P = ck.size(1);
   CONTRACT(P > 0 && (P & (P - 1)) == 0, "the page size must be a power of two, got ", P);
   CONTRACT(ck.size(0) > 0, "the cache has no pages");
+  CONTRACT(ck.size(3) > 0 && cv.size(3) > 0, "the cache's head dims must be positive");
   CONTRACT(table.dim() == 2 && table.scalar_type() == at::kInt && table.device() == ck.device() && table.size(0) == B && table.size(1) > 0 &&
                (table.stride(1) == 1 || table.size(1) == 1) && table.stride(0) >= 0,
            "page_table must be an int32 tensor [", B, ", pages of a sequence] with unit inner stride on the cache's device");

@@ -213,3 +213,15 @@ def test_packed_tokens_of_no_sequence(gpu_device):
     q1 = moda_amd.paged_append(x, x, ck, cv, table, past, cu_seqlens=torch.zeros(1, dtype=torch.int32, device=dev), q=q, rotary=moda_amd.Rotary(64),
                                moda_group_num=2, cached_k=kd, cached_v=kd.clone(), depth_slot=1)
     assert torch.equal(q1, q) and not ck.any() and not cv.any() and not kd.any()
+
+
+def test_caches_without_a_head_dim_are_refused(gpu_device):
+    """Values of no elements: the row sums would be left as their memory was."""
+    dev = gpu_device
+    ck, cv, table, past = pages(dev)
+    q = torch.zeros(1, 1, 2, 64, dtype=BF16, device=dev)
+    for k, v, x in ((ck, cv[..., :0], q), (ck[..., :0], cv, q[..., :0]), (ck[..., :0], cv[..., :0], q[..., :0])):
+        with pytest.raises(AssertionError, match="head dims"):
+            moda_amd.paged_moda_fwd(x, k, v, table, past)
+        with pytest.raises(AssertionError, match="head dims"):
+            moda_amd.paged_append(x, q[..., :v.shape[3]], k, v, table, past)
