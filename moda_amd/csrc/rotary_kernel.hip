@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
   int64_t tb = n / a.T, tt = n - tb * a.T;  // batch and token of the tensors
   int64_t pos = tt;
   int page = -1, b = (int)tb;
-  bool turn = true, stored = false;  // whether q, k are rotated; whether the token goes to the cache
+  bool turn = true, stored = false;  // whether the token is of a sequence; whether it goes to the cache
   if (PAGED) {
     if (a.cache.cu) {
       b = sequence_of(a.cache.cu, a.cache.B, n);
@@ -76,7 +76,20 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
     } else {
       stored = tt < a.cache.new_of(b);
     }
-    if (turn) pos += a.cache.past_of(b);
+    if (!turn) {  // a token of no sequence: q as it is, infinities and signs of zero with it
+      for (int p = 0; p < a.n_parts; p++) {
+        const RowPart& part = a.part[p];
+        if (!part.y) continue;
+        for (int item = group; item < part.rows * part.heads; item += a.groups) {
+          const int r = part.heads_magic ? (int)__umulhi((unsigned)item, part.heads_magic) : item, h = item - r * part.heads;
+          const bits* x = (const bits*)part.x + tb * part.sx[0] + (tt * part.rows + r) * part.sx[1] + h * part.sx[2];
+          bits* y = (bits*)part.y + tb * part.sy[0] + (tt * part.rows + r) * part.sy[1] + h * part.sy[2];
+          for (int e = c0 * VEC; e < part.dim; e += VEC << a.lane_shift) put(get(x + e), y + e);
+        }
+      }
+      return;
+    }
+    pos += a.cache.past_of(b);
     if (stored && pos < a.cache.capacity()) page = a.cache.page_of(b, (int)pos);
   } else if (a.positions) {
     const int64_t at = tb * a.position_stride + tt;
@@ -91,8 +104,8 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
       const double t = (double)pos * a.rates[c0 * VEC + i];
       float s, c;
       sincospif(2.f * (float)(t - rint(t)), &s, &c);
-      cs[i] = turn ? c * a.amplitude : 1.f;
-      sn[i] = turn ? s * a.amplitude * a.sign : 0.f;
+      cs[i] = c * a.amplitude;
+      sn[i] = s * a.amplitude * a.sign;
     }
   }
 

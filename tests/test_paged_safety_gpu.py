@@ -225,3 +225,21 @@ def test_caches_without_a_head_dim_are_refused(gpu_device):
             moda_amd.paged_moda_fwd(x, k, v, table, past)
         with pytest.raises(AssertionError, match="head dims"):
             moda_amd.paged_append(x, q[..., :v.shape[3]], k, v, table, past)
+
+
+@pytest.mark.parametrize("D", [64, 20])
+@pytest.mark.parametrize("dtype", [BF16, torch.float16, torch.float32], ids=str)
+def test_rows_of_no_sequence_stay_as_they_are(dtype, D, gpu_device):
+    """To the bit: infinities, NaN and signs of zero, too."""
+    dev = gpu_device
+    ck, cv, table, past = pages(dev, D=64, dtype=dtype)
+    R = 64 if D == 64 else 20
+    q = torch.randn(1, 7, 2, 64, device=dev).to(dtype)
+    q[:, 3:, 0, ::3], q[:, 3:, 1, 1::5], q[:, 3:, 1, 2::7], q[:, 0] = math.inf, -0.0, math.nan, -0.0
+    cu = torch.tensor([1, 3], dtype=torch.int32, device=dev)
+    for inter in (False, True):
+        q1 = moda_amd.paged_append(q, q, ck, cv, table, past, cu_seqlens=cu, q=q, rotary=moda_amd.Rotary(R, interleaved=inter))
+        bits = torch.int32 if dtype == torch.float32 else torch.int16
+        for rows in (slice(0, 1), slice(3, 7)):
+            assert torch.equal(q1[:, rows].view(bits), q[:, rows].view(bits))
+        assert not torch.equal(q1[:, 2], q[:, 2])
