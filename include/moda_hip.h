@@ -375,7 +375,7 @@ int moda_hip_rotary_rows(int32_t dtype, int64_t B, int64_t T, int64_t D, const m
  * (DEVICE, B + 1 offsets) the new tokens are packed, [1, total_tokens, H, *], sequence b owning cu[b] .. cu[b + 1] - 1; T is then not
  * read and new_lens NULL; rows behind the last sequence go nowhere (q: as they are).  k (with `rotary`) is rotated by its position
  * on the way, and so is q [B, T * G, Hq, D] (or NULL) to q_out, padded rows included.  kd, vd (or NULL): the token's k and
- * v, as stored, also go to slot `slot` of the depth caches [B, T * L, H, *].  A page that is written belongs to one sequence: two tokens
+ * v, as stored (whether or not there is a page for it), also go to slot `slot` of the depth caches [B, T * L, H, *].  A page that is written belongs to one sequence: two tokens
  * for the same place leave either of them, piece by piece.
  * moda_hip_paged_attend: row (t, g) of sequence b attends over positions <= past[b] + t, that is, the new tokens are in the cache already,
  * and over the L_valid first slots (0: all L) of its own token in kd, vd [B, T * L, H, *].  q, o: [B, T * G, H, *], rows t * G + g,

@@ -31,12 +31,12 @@ def paged_append(k, v, cache_k, cache_v, page_table, past, new_lens=None, cu_seq
                  moda_group_num: int = 1, cached_k=None, cached_v=None, depth_slot: int = 0) -> Optional[torch.Tensor]:
     """New token ``i`` of sequence ``b`` -- rows ``k [B, T, H, D]``, ``v [B, T, H, Dv]`` -- to position ``past[b] + i`` of the cache, in
     place.  ``new_lens [B]`` (int32): how many of the ``T`` tokens of a padded batch are real; or ``cu_seqlens [B + 1]`` (int32, on the
-    device): the new tokens are packed, ``k [1, total, H, D]``.  Padded rows, rows behind the last sequence and positions past
-    the table's end go nowhere.
+    device): the new tokens are packed, ``k [1, total, H, D]``.  Padded rows and rows behind the last sequence go nowhere, positions
+    without a page (past the table's end, or an entry that names none) to no page.
 
     ``rotary``: ``k`` is rotated by its position on the way, and so is ``q [B, T*moda_group_num, HQ, D]``, which is returned (padded rows
-    rotated as well, rows behind the last packed sequence as they are).  ``cached_k, cached_v [B, T*L, H, *]``: the stored ``k, v`` also
-    go to slot ``depth_slot`` of each token.  No backward pass."""
+    rotated as well, rows behind the last packed sequence as they are).  ``cached_k, cached_v [B, T*L, H, *]``: ``k, v``, as stored, also
+    go to slot ``depth_slot`` of each real token, with or without a page.  No backward pass."""
     _refuse_tracing("paged_append")
     _check_device(cache_k)
     rates, dim, amplitude, interleaved = None, 0, 1.0, False

@@ -227,6 +227,22 @@ def test_caches_without_a_head_dim_are_refused(gpu_device):
             moda_amd.paged_append(x, q[..., :v.shape[3]], k, v, table, past)
 
 
+def test_tokens_without_a_page_have_their_depth_slot(gpu_device):
+    """The attention of such a token still reads its own depth slots: they are written, of padded tokens they are not."""
+    dev = gpu_device
+    ck, cv, _, _ = pages(dev)
+    table = torch.tensor([[0, -1], [9, 2]], dtype=torch.int32, device=dev)  # two pages of 16; each sequence has a hole
+    past, new = torch.tensor([14, 14], dtype=torch.int32, device=dev), torch.tensor([20, 6], dtype=torch.int32, device=dev)
+    k, v = (torch.randn(2, 20, 2, 64, device=dev).to(BF16) for _ in range(2))
+    kd, vd = (torch.zeros(2, 20, 3, 2, 64, dtype=BF16, device=dev) for _ in range(2))
+    moda_amd.paged_append(k, v, ck, cv, table, past, new_lens=new, cached_k=kd.view(2, 60, 2, 64), cached_v=vd.view(2, 60, 2, 64), depth_slot=1)
+    for x, c, d in ((k, ck, kd), (v, cv, vd)):
+        pages_, slots = torch.zeros_like(c), torch.zeros_like(d)
+        pages_[0, 14:], pages_[2, :4] = x[0, :2], x[1, 2:6]
+        slots[0, :, 1], slots[1, :6, 1] = x[0], x[1, :6]
+        assert torch.equal(c, pages_) and torch.equal(d, slots)
+
+
 @pytest.mark.parametrize("D", [64, 20])
 @pytest.mark.parametrize("dtype", [BF16, torch.float16, torch.float32], ids=str)
 def test_rows_of_no_sequence_stay_as_they_are(dtype, D, gpu_device):
