@@ -12,6 +12,8 @@ import torch
 
 import moda_amd
 
+from test_paged_gpu import ATTEND, Cache
+
 pytestmark = pytest.mark.gpu
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -159,3 +161,73 @@ def test_values_and_keys_that_are_not_finite(dtype, T, G, D, gpu_device):
                 x, l, tol, tl = attention64(q[rows].double(), k, v, D ** -0.5)
                 same(o[rows], x, tol + U[dtype] * x.abs() + TINY[dtype], f"o {b} {t} {h}")
                 same(lse[rows], l, tl, f"lse {b} {t} {h}")
+
+
+def rounded_attention64(q, keys, values, scale, dtype, tiles):
+    """q [rows, D] in 64 bits -> o, lse and how far a call in `dtype` may be from them where its probabilities meet the values with all their
+    bits.  `tiles`: of 32 keys in the whole call, of which a wave of a thousand or more has an equal run, in order: each key is added in
+    at most three pieces (96 additions a tile), the tiles bring sums to a new scale, and the runs of a row are joined."""
+    s = q @ keys.T * (scale / math.log(2))
+    lse = torch.logsumexp(s * math.log(2), -1) / math.log(2)
+    p = torch.exp2(s - lse[:, None])
+    o, magnitude = p @ values, p @ values.abs()
+    e = (q.abs() @ keys.abs().T).amax(-1) * (scale / math.log(2)) * (q.shape[1] + 4) * 2.0 ** -24
+    sums = (98 * -(-tiles // 1024) + -(-keys.shape[0] // 32) + 20) * 2.0 ** -24
+    return o, lse, U[dtype] * o.abs() + (2 * math.log(2) * e[:, None] + 2 * sums + 2.0 ** -21) * magnitude + TINY[dtype], \
+        e + sums + 2.0 ** -21 + 2.0 ** -23 * lse.abs()
+
+
+def check_rounded(c, q, o, lse, T, G, H, new, scale, plain, depth=None, L=0, Lv=0):
+    """`c`: K, V of each sequence and past, on the CPU (test_paged_gpu.Cache)."""
+    lengths = [c.past[b] + new[b] if new[b] else 0 for b in range(q.shape[0])]
+    tiles = H * -(-T * G // 16) * sum(-(-n // 32) + (T * -(-Lv // 16) + 1) // 2 + 1 for n in lengths)
+    for b in range(q.shape[0]):
+        for t in range(T):
+            for h in range(H):
+                at = (b, t, slice(h * G, h * G + G)) if plain else (b, slice(t * G, t * G + G), h)
+                if t >= new[b]:
+                    assert (o[at] == 0).all() and (lse[at] == -math.inf).all(), (b, t, h)
+                    continue
+                keys, values = c.K[b][:c.past[b] + t + 1, h].double(), c.V[b][:c.past[b] + t + 1, h].double()
+                if depth:
+                    r = slice(t * L, t * L + Lv)
+                    keys, values = torch.cat([keys, depth[0][b, r, h].double()]), torch.cat([values, depth[1][b, r, h].double()])
+                x, l, tol, tl = rounded_attention64(q[at].double().cpu(), keys, values, scale, q.dtype, tiles)
+                within(o[at].double().cpu(), x, tol, f"o {b} {t} {h}")
+                within(lse[at].double().cpu(), l, tl, f"lse {b} {t} {h}")
+
+
+@pytest.mark.parametrize("case", ATTEND, ids=str)
+@pytest.mark.parametrize("plain", [False, True], ids=["folded", "plain"])
+def test_attention_is_at_its_rounding(case, plain, gpu_device):
+    """The cases of the test of attention over pages, without an allowance for probabilities in 16 bits."""
+    dtype, H, G, D, Dv, P, T, L, Lv, past, new, layout = case
+    if plain:
+        L = Lv = 0
+    torch.manual_seed(51)
+    B = len(past)
+    new = new or [T] * B
+    c = Cache(gpu_device, dtype, B, H, D, Dv, P, past, new, layout)
+    q = torch.randn((B, T, H * G, D) if plain else (B, T * G, H, D)).to(dtype).to(gpu_device)
+    lens = torch.tensor(new, dtype=torch.int32, device=gpu_device)
+    depth = None
+    if plain:
+        o, lse = moda_amd.paged_attn_fwd(q, c.k, c.v, c.table_dev, c.past_dev, new_lens=lens)
+    else:
+        if L:
+            depth = torch.randn(B, T * L, H, D).to(dtype), torch.randn(B, T * L, H, Dv).to(dtype)
+        dev = [x.to(gpu_device) for x in depth] if depth else [None, None]
+        o, lse = moda_amd.paged_moda_fwd(q, c.k, c.v, c.table_dev, c.past_dev, new_lens=lens, cached_k=dev[0], cached_v=dev[1], depth_valid=Lv or None,
+                                         moda_group_num=G)
+    check_rounded(c, q, o, lse, T, G, H, new, D ** -0.5, plain, depth, L, Lv)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 128), (FP16, 64), (FP32, 64), (BF16, 256)], ids=str)
+def test_a_long_split_cache_is_at_its_rounding(dtype, D, gpu_device):
+    """What one tile of values too few or in a wrong place would change is more than this allows (tests/test_paged_tolerance_cpu.py)."""
+    torch.manual_seed(52)
+    past = [20000, 3, 9999]
+    c = Cache(gpu_device, dtype, 3, 1, D, D, 64, past, [1] * 3)
+    q = torch.randn(3, 4, 1, D).to(dtype).to(gpu_device)
+    o, lse = moda_amd.paged_moda_fwd(q, c.k, c.v, c.table_dev, c.past_dev, moda_group_num=4)
+    check_rounded(c, q, o, lse, 1, 4, 1, [1] * 3, D ** -0.5, False)
