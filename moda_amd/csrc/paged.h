@@ -83,4 +83,10 @@ struct PagedAttendArgs {
   unsigned group_magic;
 };
 
+// A launch of n workgroups: an axis has less than 2^32 threads, so the second one counts runs of 2^20 (a constant, so that kernels need not load
+// the launch's shape).  The last run may reach past n.
+constexpr unsigned kGridRun = 1 << 20;
+inline dim3 grid_of(int64_t n) { return dim3((unsigned)(n < kGridRun ? n : kGridRun), (unsigned)((n + kGridRun - 1) / kGridRun)); }
+__device__ __forceinline__ unsigned workgroup() { return blockIdx.y * kGridRun + blockIdx.x; }
+
 }  // namespace moda

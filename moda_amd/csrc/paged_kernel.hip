@@ -5,9 +5,10 @@
 // in one pass over keys and values with the running maximum m, the sum and o in 32 bits.  A row that sees nothing has
 // o = 0 and lse = -inf.
 //
-// What bounds it is the stream of keys and values from HBM: each is read once for all rows of its key/value head, four rows
+// What bounds it is the stream of keys and values from HBM: each is read once for 16 (32) rows of its key/value head, four rows
 // make 4 FLOP of a byte, the matrix instruction does a hundred times that.  So the work is cut for the stream alone.  All
-// tiles of 32 keys -- of every sequence, key/value head and 16 (32) rows -- stand on one axis, sequences with
+// tiles of 32 keys -- of every sequence, key/value head and 16 (32) rows of the call, whether or not the sequence has new tokens
+// in them -- stand on one axis, sequences with
 // their lengths as they are on the device; each of a fixed number of waves, as many as keep the card's loads in flight, takes an equal
 // run of it, whatever the lengths are, and the host needs to know none of them (a captured launch follows them as they grow).
 // A wave is a workgroup by itself: it fetches its tiles into a ring of its own and waits for nobody.  Runs that begin or end
@@ -15,9 +16,11 @@
 // wave; a second launch joins them in the order of the axis, so that results do not depend on who came first.
 //
 // Measured (bf16, head dim 128, four rows a head; a copy of 4 GiB reaches 4.7 TB/s in and out, reading alone more): 256 sequences
-// of 12 - 24 K tokens, 4 heads (9.4 GB) 1.58 ms, 6.0 TB/s; one sequence of 1 M tokens 361 us + 9 for joining, 5.8 TB/s; 64 of 1 - 8 K
-// 117 + 6 us, 5.2 TB/s; one of 101 tokens 6.4 + 4.6 us, the chain counts -> table -> rows -> keys -> products and a second
-// launch.  Four and more rows of eight drafted tokens are bound by the vector instructions of a wave's tile (some 500 a tile).
+// of 12 - 24 K tokens, 4 heads (9.4 GB) 1.57 ms, 6.0 TB/s; one sequence of 1 M tokens 361 us + 8 for joining, 5.9 TB/s; 64 of 1 - 8 K
+// 117 + 5.5 us, 5.2 TB/s; one of 101 tokens 6.7 + 4.7 us, the chain counts -> table -> rows -> keys -> products and a second
+// launch.  More than 16 rows a head are bound by the vector instructions of a wave's tile (some 500), and by the tiles of rows that are
+// not there: five drafted tokens of eight rows, two row tiles, of sequences that have up to five, 34 + 6 us, 36 % of the tiles for
+// padded tokens alone.
 #include "paged.h"
 #include "tile16.h"
 #include "../../include/moda_hip.h"
@@ -384,8 +387,9 @@ struct PagedWave {
   }
 
   // Probabilities w times a tile's values.  They go to the matrix instruction in pieces, each the rounding of what those before it left:
-  // three of bf16 hold all 24 bits, two of fp16 hold 22 where the second still has them (see add_small).  Half the bits less (two pieces of bf16: 16) and 0.2 % of the bf16 results were
-  // rounded the other way than the exact ones, with all of them 0.01 %, as many as where everything is in 32 bits.
+  // three of bf16 hold all 24 bits, two of fp16 hold 22 (but see add_small).  With two of bf16, 16 bits, 0.2 % of the results were rounded the
+  // other way than the exact ones, with three 0.01 %, as many as where everything is in 32 bits; the third costs drafted tokens 4 % and one token
+  // nothing.
   static constexpr int kPieces = __is_same(T, BF16) ? 3 : 2;
   __device__ __forceinline__ void add_products(float (&w)[NR][8], lds_cptr tile) {
     i32x4 piece[kPieces][NR];
@@ -833,7 +837,7 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedAttendArgs a,
   __shared__ f32x4 sums[WAVES][LANES];
   __shared__ float lsum[WAVES], tops[WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, x = tid % LANES, group = tid / LANES;
-  unsigned at = blockIdx.y * gridDim.x + blockIdx.x;  // (rows are below 2^31)
+  unsigned at = workgroup();  // (rows are below 2^31)
   const int e0 = W == WC ? 0 : (int)(at % (W / WC)) * WC;  // the workgroup's first element
   at /= W / WC;
   const int h = (int)(at % (unsigned)a.cache.H);
@@ -934,18 +938,14 @@ int waves_of_a_unit(int width, int blocks) {
 template <typename E, int W>
 hipError_t launch_join_of(const PagedAttendArgs& a, int per_tile, hipStream_t stream) {
   const int64_t rows = (int64_t)a.cache.B * a.cache.T * a.G * a.cache.H;
-  const auto grid = [](int64_t n) {  // an axis of a launch has less than 2^32 threads
-    const unsigned x = (unsigned)(n < 1 << 20 ? n : 1 << 20);
-    return dim3(x, (unsigned)((n + x - 1) / x));
-  };
   if (rows >= 2048)
-    paged_join_kernel<E, W, W, 64><<<grid(rows), 64, 0, stream>>>(a, per_tile);
+    paged_join_kernel<E, W, W, 64><<<grid_of(rows), 64, 0, stream>>>(a, per_tile);
   else if (rows >= 256)
-    paged_join_kernel<E, W, W, 256><<<grid(rows), 256, 0, stream>>>(a, per_tile);
+    paged_join_kernel<E, W, W, 256><<<grid_of(rows), 256, 0, stream>>>(a, per_tile);
   else if (rows >= 64)
-    paged_join_kernel<E, W, W, 1024><<<grid(rows), 1024, 0, stream>>>(a, per_tile);
+    paged_join_kernel<E, W, W, 1024><<<grid_of(rows), 1024, 0, stream>>>(a, per_tile);
   else
-    paged_join_kernel<E, W, 32, 1024><<<grid(rows * (W / 32)), 1024, 0, stream>>>(a, per_tile);
+    paged_join_kernel<E, W, 32, 1024><<<grid_of(rows * (W / 32)), 1024, 0, stream>>>(a, per_tile);
   return hipGetLastError();
 }
 template <typename E>

@@ -45,7 +45,8 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int B, int64_t n) 
 // one token.  VEC elements are 16 bytes, or one where rows do not lie on that grid.  STREAM: nontemporal accesses.
 //
 // Bound by the bytes: 64 K tokens of 16 + 4 heads of 128 (671 MB in and out) take 114 us, 5.9 TB/s, where a copy of 4 GiB
-// reaches 4.7.  Small calls by the chain counts -> page -> rows: 4 us for one token, 6 into a cache.
+// reaches 4.7.  Small calls by loads that are sent one after the other, counts, page, rates and last the rows, which need none of
+// them: 4.4 us for one token, 5.5 into a cache.
 template <typename E, int VEC, bool INTER, bool PAGED, bool STREAM>
 __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
   typedef typename E::bits bits;
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
     else
       *(vec*)p = x;
   };
-  const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x, unit = id >> a.lane_shift;
+  const int64_t id = (int64_t)workgroup() * 256 + threadIdx.x, unit = id >> a.lane_shift;
   const int c0 = (int)(id & ((1 << a.lane_shift) - 1));
   const int64_t n = unit / a.groups;
   if (n >= a.tokens) return;
@@ -175,9 +176,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowArgs a) {
 
 template <typename E, int VEC, bool PAGED>
 static void launch_rows_as(const RowArgs& a, bool inter, bool stream_through, int64_t blocks, hipStream_t stream) {
-  // an axis of a launch has less than 2^32 threads
-  const unsigned x = (unsigned)(blocks < 1 << 20 ? blocks : 1 << 20);
-  const dim3 grid(x, (unsigned)((blocks + x - 1) / x));
+  const dim3 grid = grid_of(blocks);
   if (VEC > 1 && stream_through) {
     inter ? rows_kernel<E, VEC, true, PAGED, VEC != 1><<<grid, 256, 0, stream>>>(a) : rows_kernel<E, VEC, false, PAGED, VEC != 1><<<grid, 256, 0, stream>>>(a);
     return;
@@ -201,8 +200,10 @@ hipError_t launch_rows(RowArgs& a, int dtype, bool vec, bool inter, bool paged, 
   }
   a.lane_shift = 0;
   while ((1 << a.lane_shift) < most && a.lane_shift < 8) a.lane_shift++;
-  // One item a thread until there are two waves a SIMD, then up to five, which share the angles.  64 K tokens of 20 items with 20, 10, 5
-  // and 3 items a thread: 153, 136, 126 and 161 us; 4 K tokens with 5, 10 and 20 threads a token's chunk 11.2, 11.5 and 12.7 us.
+  // One item a thread until there are two waves a SIMD, then up to five, which share the angles.  With up to 3, 4, 5, 8 and 10 items a thread,
+  // 64 K tokens, bf16: 16 items of 128 elements 89, 92, 92, 98, 98 us; 20: 111, 112, 112, 118, 125; 40: 220, 218, 219, 226, 232; 72 of 64
+  // elements 238, 241, 246, 248, 244; fp32: 40 items 443, 455, 465, 471, 482.  4 K tokens, bf16: 20 items 10.8, 10.5, 10.4, 10.4, 10.5; 40: 16.9,
+  // 16.5, 16.2, 17.0, 18.4.  Below nine items it makes no difference.
   const int64_t full = 256 * 512, lanes = a.tokens << a.lane_shift;
   a.groups = (int)max((int64_t)(a.items + 4) / 5, min((int64_t)a.items, full / max(lanes, (int64_t)1)));
   // What does not fit the 256 MB memory-side cache passes it by (115 us instead of 126); what does is found there by whoever reads it next.
