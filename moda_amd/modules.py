@@ -344,7 +344,9 @@ class MoDAStack(nn.Module):
         counts advanced.  Rows behind a prompt's end hold nothing of use.  Sequences with tokens of their own (``decode`` goes on with those)
         or without pages for the prompt are an error, for which the call waits for the device (not in a captured one, which does not look)."""
         self._check_cache(x, cache)
-        if not torch.cuda.is_current_stream_capturing():
+        with torch.cuda.device_of(cache.past):
+            captured = torch.cuda.is_current_stream_capturing()
+        if not captured:
             cache.check_prompts(x.shape[1], lens)
         stream = DepthStream(self._slots())
         for i, blk in enumerate(self.blocks):
