@@ -16,8 +16,8 @@
 // wave; a second launch joins them in the order of the axis, so that results do not depend on who came first.
 //
 // Measured (bf16, head dim 128, four rows a head; a copy of 4 GiB reaches 4.7 TB/s in and out, reading alone more): 256 sequences
-// of 12 - 24 K tokens, 4 heads (9.4 GB) 1.57 ms, 6.0 TB/s; one sequence of 1 M tokens 361 us + 8 for joining, 5.9 TB/s; 64 of 1 - 8 K
-// 117 + 5.5 us, 5.2 TB/s; one of 101 tokens 6.7 + 4.7 us, the chain counts -> table -> rows -> keys -> products and a second
+// of 12 - 24 K tokens, 4 heads (9.4 GB) 1.59 ms, 5.9 TB/s; one sequence of 1 M tokens 359 us + 8 for joining, 6.0 TB/s; 64 of 1 - 8 K
+// 117 + 5.4 us, 5.2 TB/s; one of 101 tokens 6.6 + 4.4 us, the chain counts -> table -> rows -> keys -> products and a second
 // launch.  More than 16 rows a head are bound by the vector instructions of a wave's tile (some 500), and by the tiles of rows that are
 // not there: five drafted tokens of eight rows, two row tiles, of sequences that have up to five, 34 + 6 us, 36 % of the tiles for
 // padded tokens alone.
