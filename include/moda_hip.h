@@ -2,7 +2,8 @@
  * moda_hip.h -- C ABI of libmoda_hip.so: fused sequence+depth attention
  * (MoDA) for AMD MI355X (gfx950), forward and backward, plus the depth-KV
  * cache reorganisation; rotary positions, a paged key/value cache and the
- * attention of new tokens over it.
+ * attention of new tokens over it; token embedding and the cross entropy over
+ * a vocabulary.
  *
  * Every pointer that names tensor data is a DEVICE pointer.  Strides are in
  * elements; the innermost (head-dim) stride is always 1.  For the matrix-core
@@ -417,6 +418,58 @@ typedef struct moda_hip_paged_attend_args {
 size_t moda_hip_paged_attend_workspace_bytes(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_args* args);
 int moda_hip_paged_attend(const moda_hip_paged_cache* cache, const moda_hip_paged_attend_args* args, void* workspace,
                           size_t workspace_bytes, void* stream);
+
+/*
+ * The two ends of a language model.  Tokens and targets: DEVICE arrays of n numbers, int32 or (tokens64, targets64) int64; one outside
+ * 0 .. vocab - 1 is no word.  Row strides ld_* in elements, unit inner stride; rows that lie on 16-byte boundaries move by 16 bytes, others
+ * element by element.
+ *
+ * moda_hip_embed_rows: y[i] = scale * weight[tokens[i]] (fp32, rounded once), zeros for what is no word.
+ * moda_hip_embed_grad: d_weight[v] = scale * the sum of dy[i] over the i with tokens[i] = v, all vocab rows written (zeros where there is none).
+ * fp32 sums in the order of i, cut every 32 places of the sorted tokens: the same bits every time.  Workspace of
+ * moda_hip_embed_grad_workspace_bytes, 16-byte boundary, not initialised.
+ * n below 2^30, vocab below 2^31 - 256, width below 2^24.
+ */
+int moda_hip_embed_rows(int32_t dtype, const void* tokens, int32_t tokens64, int64_t n, const void* weight, int64_t ld_weight, int64_t vocab,
+                        int64_t width, float scale, void* y, int64_t ld_y, void* stream);
+size_t moda_hip_embed_grad_workspace_bytes(int64_t n, int64_t vocab, int64_t width);
+int moda_hip_embed_grad(int32_t dtype, const void* tokens, int32_t tokens64, int64_t n, const void* dy, int64_t ld_dy, int64_t vocab,
+                        int64_t width, float scale, void* d_weight, int64_t ld_d_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Cross entropy of rows x [rows, width] over the vocabulary weight [vocab, width]: logits z = scale * x weight^T (fp32, never stored),
+ *   lse = log sum_v exp z[v],  loss = lse - z[target];  a row whose target is ignore_index or no word has loss 0 and lse 0, is not read
+ *   and has no gradient.
+ * moda_hip_vocab_loss_fwd: lse [rows] fp32 in base 2 (log2 of the sum), loss fp32: [rows] (MODA_HIP_LOSS_ROWS), or one value, the sum
+ * (MODA_HIP_LOSS_SUM) or the mean over the rows that have a target (MODA_HIP_LOSS_MEAN; 0 where none has).
+ * moda_hip_vocab_loss_bwd: from the same arguments, lse as the forward pass left it and d_loss (fp32, [rows] or one value):
+ *   dz[v] = d_loss * (exp(z[v] - lse) - [v = target]) (mean: over the number of rows that count), rounded to the tensors' type (fp32: not),
+ *   dx = scale * dz weight, d_weight = scale * dz^T x (either may be NULL: not wanted).
+ * fp16: dz is kept larger by a power of two that follows the largest |d_loss|.  The vocabulary is taken in pieces such that a piece of dz, and
+ * where it has to be laid out anew (fp32, rows off the 16-byte grid or 4 MiB and more apart) of the weight, keeps within 1 GiB (256 words at least).
+ * Workspace of ..._workspace_bytes (which reads the sizes, strides and pointers of its arguments), 256-byte boundary, not initialised; one for
+ * each call that may overlap another.  rows below 2^24, vocab below 2^31 - 256, width up to 2^16; MODA_HIP_EUNSUPPORTED otherwise.
+ */
+#define MODA_HIP_LOSS_ROWS 0
+#define MODA_HIP_LOSS_SUM 1
+#define MODA_HIP_LOSS_MEAN 2
+typedef struct moda_hip_vocab_loss_args {
+  int32_t struct_size, dtype;
+  int64_t rows, vocab, width;
+  const void *x, *weight, *targets;
+  int64_t ld_x, ld_weight, ignore_index;
+  int32_t targets64, reduction;
+  float scale;
+  int32_t reserved;
+  float *loss, *lse;
+  const float* d_loss;
+  void *dx, *d_weight;
+  int64_t ld_dx, ld_d_weight;
+} moda_hip_vocab_loss_args;
+size_t moda_hip_vocab_loss_fwd_workspace_bytes(const moda_hip_vocab_loss_args* args);
+int moda_hip_vocab_loss_fwd(const moda_hip_vocab_loss_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t moda_hip_vocab_loss_bwd_workspace_bytes(const moda_hip_vocab_loss_args* args);
+int moda_hip_vocab_loss_bwd(const moda_hip_vocab_loss_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Which kernels a descriptor runs on: 1 = the matrix-core kernels (tensor rows must then be 16-byte aligned, see

@@ -28,6 +28,15 @@ from .ops import (  # noqa: F401
 from .depth_cache import build_depth_cache, stack_depth, DepthCache  # noqa: F401
 from .rotary import Rotary, RotaryFunction, apply_rotary  # noqa: F401
 from .paged import paged_append, paged_attn, paged_attn_fwd, paged_moda, paged_moda_fwd, PagedKVCache  # noqa: F401
+from .vocab import (  # noqa: F401
+    EmbedTokensFunction,
+    LinearCrossEntropyFunction,
+    embed_tokens,
+    embed_tokens_bwd,
+    linear_cross_entropy,
+    linear_cross_entropy_bwd,
+    linear_cross_entropy_fwd,
+)
 from .modules import DepthStream, MoDAAttention, MoDAStack  # noqa: F401
 
 __all__ = [
@@ -57,6 +66,11 @@ __all__ = [
     "paged_moda",
     "paged_moda_fwd",
     "PagedKVCache",
+    "embed_tokens",
+    "embed_tokens_bwd",
+    "linear_cross_entropy",
+    "linear_cross_entropy_fwd",
+    "linear_cross_entropy_bwd",
     "DepthStream",
     "MoDAAttention",
     "MoDAStack",

@@ -40,6 +40,13 @@ EXPORTS = (
     "moda_hip_paged_append",
     "moda_hip_paged_attend_workspace_bytes",
     "moda_hip_paged_attend",
+    "moda_hip_embed_rows",
+    "moda_hip_embed_grad_workspace_bytes",
+    "moda_hip_embed_grad",
+    "moda_hip_vocab_loss_fwd_workspace_bytes",
+    "moda_hip_vocab_loss_fwd",
+    "moda_hip_vocab_loss_bwd_workspace_bytes",
+    "moda_hip_vocab_loss_bwd",
     "moda_hip_uses_matrix_cores",
     "moda_hip_strerror",
     "moda_hip_version",

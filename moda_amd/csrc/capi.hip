@@ -11,6 +11,7 @@
 #include "kargs.h"
 #include "paged.h"
 #include "tuning.h"
+#include "vocab.h"
 
 namespace moda {
 hipError_t launch_fwd(const KArgs& a, int dtype, int hd, hipStream_t stream);
@@ -34,6 +35,17 @@ hipError_t launch_attend_tail(const moda_hip_block_tail_args* args, const KArgs&
 hipError_t launch_rows(RowArgs& a, int dtype, bool vec, bool inter, bool paged, hipStream_t stream);
 size_t plan_paged_attend(PagedAttendArgs& a, int dtype);
 hipError_t launch_paged_attend(const PagedAttendArgs& a, int dtype, hipStream_t stream);
+hipError_t launch_embed_rows(EmbedArgs& a, int dtype, bool vec, hipStream_t stream);
+hipError_t launch_embed_grad(EmbedArgs& a, int dtype, bool vec, char* work, hipStream_t stream);
+hipError_t launch_gather_rows(const GatherArgs& a, int dtype, hipStream_t stream);
+hipError_t launch_lay_rows(const LayArgs& a, int dtype, hipStream_t stream);
+hipError_t launch_stats(const ProductArgs& a, int dtype, ProductTile tile, hipStream_t stream);
+hipError_t launch_grad_logits(const ProductArgs& a, int dtype, ProductTile tile, hipStream_t stream);
+hipError_t launch_grad_rows(const ProductArgs& a, int dtype, ProductTile tile, hipStream_t stream);
+hipError_t launch_grad_weight(const ProductArgs& a, int dtype, ProductTile tile, hipStream_t stream);
+hipError_t launch_join_stats(const JoinStatsArgs& a, hipStream_t stream);
+hipError_t launch_loss_total(const LossTotalArgs& a, hipStream_t stream);
+hipError_t launch_join_sums(const JoinSumsArgs& a, int dtype, hipStream_t stream);
 }  // namespace moda
 
 using moda::KArgs;
@@ -916,6 +928,309 @@ int moda_hip_paged_attend(const moda_hip_paged_cache* cache, const moda_hip_page
   a.work = (float*)workspace;
   return moda::launch_paged_attend(a, cache->dtype, (hipStream_t)stream) == hipSuccess ? MODA_HIP_OK : MODA_HIP_ELAUNCH;
 }
+
+namespace {
+// rows of `width` elements, `ld` apart: whether they lie on the 16-byte grid
+bool on_grid(const void* p, int64_t ld, int es) { return (uintptr_t)p % 16 == 0 && ld % (16 / es) == 0; }
+
+int check_tokens(int32_t dtype, const void* tokens, int32_t tokens64, int64_t n, int64_t vocab, int64_t width, float scale) {
+  if (!known_dtype(dtype) || n < 0 || vocab <= 0 || width <= 0 || (n > 0 && !tokens) || !(scale - scale == 0.f)) return MODA_HIP_EINVAL;
+  if ((uintptr_t)tokens % (tokens64 ? 8 : 4) != 0) return MODA_HIP_EALIGN;
+  if (n >= (1ll << 30) || vocab >= (1ll << 31) - 256 || width >= (1ll << 24)) return MODA_HIP_EUNSUPPORTED;
+  return MODA_HIP_OK;
+}
+moda::EmbedArgs embed_args(const void* tokens, int32_t tokens64, int64_t n, const void* in, int64_t ld_in, int64_t vocab, int64_t width, float scale,
+                           void* out, int64_t ld_out) {
+  moda::EmbedArgs a = {};
+  a.words = {tokens, n, vocab, -1, tokens64 != 0};
+  a.weight = (const char*)in;
+  a.y = (char*)out;
+  a.ld_in = ld_in;
+  a.ld_out = ld_out;
+  a.width = width;
+  a.scale = scale;
+  return a;
+}
+}  // namespace
+
+int moda_hip_embed_rows(int32_t dtype, const void* tokens, int32_t tokens64, int64_t n, const void* weight, int64_t ld_weight, int64_t vocab,
+                        int64_t width, float scale, void* y, int64_t ld_y, void* stream) {
+  int rc = check_tokens(dtype, tokens, tokens64, n, vocab, width, scale);
+  if (rc) return rc;
+  if (n == 0) return MODA_HIP_OK;
+  if (!weight || !y || ld_weight < 0 || ld_y < width) return MODA_HIP_EINVAL;
+  const int es = elem_size(dtype);
+  if ((uintptr_t)weight % es != 0 || (uintptr_t)y % es != 0) return MODA_HIP_EALIGN;
+  if ((rc = check_device())) return rc;
+  moda::EmbedArgs a = embed_args(tokens, tokens64, n, weight, ld_weight, vocab, width, scale, y, ld_y);
+  const bool vec = width % (16 / es) == 0 && on_grid(weight, ld_weight, es) && on_grid(y, ld_y, es);
+  return moda::launch_embed_rows(a, dtype, vec, (hipStream_t)stream) == hipSuccess ? MODA_HIP_OK : MODA_HIP_ELAUNCH;
+}
+
+size_t moda_hip_embed_grad_workspace_bytes(int64_t n, int64_t vocab, int64_t width) {
+  return n <= 0 || n >= (1ll << 30) || vocab <= 0 || width <= 0 || width >= (1ll << 24) ? 0 : moda::plan_embed_grad(n, vocab, width).bytes;
+}
+
+int moda_hip_embed_grad(int32_t dtype, const void* tokens, int32_t tokens64, int64_t n, const void* dy, int64_t ld_dy, int64_t vocab, int64_t width,
+                        float scale, void* d_weight, int64_t ld_d_weight, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_tokens(dtype, tokens, tokens64, n, vocab, width, scale);
+  if (rc) return rc;
+  if (!d_weight || ld_d_weight < width || (n > 0 && (!dy || ld_dy < 0))) return MODA_HIP_EINVAL;
+  const int es = elem_size(dtype);
+  if ((uintptr_t)dy % es != 0 || (uintptr_t)d_weight % es != 0) return MODA_HIP_EALIGN;
+  if (n > 0 && (!workspace || workspace_bytes < moda::plan_embed_grad(n, vocab, width).bytes)) return MODA_HIP_EWORKSPACE;
+  if ((uintptr_t)workspace % 16 != 0) return MODA_HIP_EALIGN;
+  if ((rc = check_device())) return rc;
+  moda::EmbedArgs a = embed_args(tokens, tokens64, n, dy, ld_dy, vocab, width, scale, d_weight, ld_d_weight);
+  const bool vec = width % (16 / es) == 0 && on_grid(dy, ld_dy, es) && on_grid(d_weight, ld_d_weight, es);
+  return moda::launch_embed_grad(a, dtype, vec, (char*)workspace, (hipStream_t)stream) == hipSuccess ? MODA_HIP_OK : MODA_HIP_ELAUNCH;
+}
+
+namespace {
+int plan_vocab_loss(const moda_hip_vocab_loss_args* t, bool backward, moda::LossPlan& p) {
+  if (!t || t->struct_size != (int32_t)sizeof(*t)) return MODA_HIP_EINVAL;
+  int rc = check_tokens(t->dtype, t->targets, t->targets64, t->rows, t->vocab, t->width, t->scale);
+  if (rc) return rc;
+  if (t->reduction < MODA_HIP_LOSS_ROWS || t->reduction > MODA_HIP_LOSS_MEAN || t->ld_x < 0 || t->ld_weight < 0) return MODA_HIP_EINVAL;
+  if (t->rows >= (1ll << 24) || t->vocab >= (1ll << 31) - 256 || t->width > (1ll << 16)) return MODA_HIP_EUNSUPPORTED;
+  const int es = elem_size(t->dtype);
+  // in place: on the grid, in whole pieces of it, no row reaching into the next, and rows near enough for a tile's 32-bit offsets
+  const auto in_place = [&](const void* at, int64_t ld) { return on_grid(at, ld, es) && t->width % 8 == 0 && ld >= t->width && ld * es < (4ll << 20); };
+  p = moda::plan_loss(t->rows, t->vocab, t->width, t->dtype == MODA_HIP_FP32, in_place(t->x, t->ld_x), in_place(t->weight, t->ld_weight), backward,
+                      t->dx != nullptr, t->d_weight != nullptr, t->reduction != MODA_HIP_LOSS_ROWS);
+  return MODA_HIP_OK;
+}
+
+}  // namespace
+}  // extern "C"
+
+namespace {
+// What both passes do with a piece of the vocabulary.
+struct VocabLoss {
+  const moda_hip_vocab_loss_args* t;
+  moda::LossPlan p;
+  char* work;
+  hipStream_t stream;
+  bool backward;
+  int es() const { return elem_size(t->dtype); }
+  moda::LossHead* head() const { return p.direct ? nullptr : (moda::LossHead*)(work + p.head); }
+  moda::Words words() const { return {t->targets, t->rows, t->vocab, t->ignore_index, t->targets64 != 0}; }
+  template <typename T>
+  T* at(size_t offset) const {
+    return (T*)(work + offset);
+  }
+  int64_t piece_words(int64_t i) const { return t->vocab - i * p.piece < p.piece ? t->vocab - i * p.piece : p.piece; }
+
+  hipError_t gather() const {
+    moda::GatherArgs a = {};
+    a.words = words();
+    a.x = (const char*)t->x;
+    a.ld_x = t->ld_x;
+    a.width = t->width;
+    a.head = head();
+    a.row_of = at<int>(p.row_of);
+    a.target = at<int>(p.target);
+    a.rows = at<uint16_t>(p.rows);
+    a.rows_ld = p.rows_ld;
+    a.rows_plane = t->rows * p.rows_ld;
+    if (t->rows > moda::kScanMost) {
+      a.counts = at<int>(p.counts);
+      a.exponents = at<int>(p.exponents);
+    }
+    a.vec_x = on_grid(t->x, t->ld_x, es());
+    if (!backward) {
+      a.loss = t->reduction == MODA_HIP_LOSS_ROWS ? t->loss : at<float>(p.losses);
+      a.lse_out = t->lse;
+    } else {
+      a.d_loss = t->d_loss;
+      a.d_loss_stride = t->reduction == MODA_HIP_LOSS_ROWS;
+      a.lse_in = t->lse;
+      a.factor = at<float>(p.factor);
+      a.lse = at<float>(p.lse);
+      a.dx = (char*)t->dx;
+      a.ld_dx = t->ld_dx;
+      a.vec_dx = on_grid(t->dx, t->ld_dx, es());
+      a.mean = t->reduction == MODA_HIP_LOSS_MEAN;
+      a.fp16 = t->dtype == MODA_HIP_FP16;
+    }
+    return moda::launch_gather_rows(a, t->dtype, stream);
+  }
+  // the weights of piece i as the products read them
+  hipError_t weights(int64_t i, moda::ProductArgs& a) const {
+    const char* from = (const char*)t->weight + i * p.piece * t->ld_weight * es();
+    if (!p.copy_weight) {
+      a.f = (const uint16_t*)from;
+      a.f_ld = t->ld_weight;
+      return hipSuccess;
+    }
+    moda::LayArgs l = {from, t->ld_weight, t->width, piece_words(i), at<uint16_t>(p.weight), p.rows_ld, p.piece * p.rows_ld, on_grid(t->weight, t->ld_weight, es())};
+    a.f = l.to;
+    a.f_ld = l.to_ld;
+    a.f_plane = l.to_plane;
+    return moda::launch_lay_rows(l, t->dtype, stream);
+  }
+  moda::ProductArgs logits(int64_t i, const moda::ProductArgs& weights) const {
+    moda::ProductArgs a = weights;
+    a.p = p.direct ? (const uint16_t*)t->x : at<uint16_t>(p.rows);
+    a.p_ld = p.direct ? t->ld_x : p.rows_ld;
+    a.p_plane = t->rows * p.rows_ld;
+    a.f_count = (int)piece_words(i);
+    a.p_count = (int)t->rows;
+    a.k_count = (int)p.k;
+    a.head = head();
+    a.splits = 1;
+    a.c = (float)(t->scale * 1.4426950408889634);
+    a.words = words();
+    a.target = at<int>(p.target);
+    a.first_word = (int)(i * p.piece);
+    return a;
+  }
+};
+}  // namespace
+
+extern "C" {
+
+size_t moda_hip_vocab_loss_fwd_workspace_bytes(const moda_hip_vocab_loss_args* t) {
+  moda::LossPlan p;
+  return plan_vocab_loss(t, false, p) ? 0 : p.bytes;
+}
+size_t moda_hip_vocab_loss_bwd_workspace_bytes(const moda_hip_vocab_loss_args* t) {
+  moda::LossPlan p;
+  return plan_vocab_loss(t, true, p) ? 0 : p.bytes;
+}
+
+namespace {
+// what both passes ask of their arguments; the call, if there is anything to do
+int begin_vocab_loss(const moda_hip_vocab_loss_args* t, bool backward, void* workspace, size_t workspace_bytes, void* stream, VocabLoss& v) {
+  int rc = plan_vocab_loss(t, backward, v.p);
+  if (rc) return rc;
+  if (!t->weight || (t->rows > 0 && (!t->x || !t->lse))) return MODA_HIP_EINVAL;
+  const int es = elem_size(t->dtype);
+  if ((uintptr_t)t->x % es != 0 || (uintptr_t)t->weight % es != 0 || (uintptr_t)t->lse % 4 != 0) return MODA_HIP_EALIGN;
+  if (v.p.bytes > 0 && (!workspace || workspace_bytes < v.p.bytes)) return MODA_HIP_EWORKSPACE;
+  if ((uintptr_t)workspace % 256 != 0) return MODA_HIP_EALIGN;
+  v.t = t;
+  v.work = (char*)workspace;
+  v.stream = (hipStream_t)stream;
+  v.backward = backward;
+  return check_device();
+}
+}  // namespace
+
+#define MODA_TRY(call) \
+  if ((call) != hipSuccess) return MODA_HIP_ELAUNCH
+
+int moda_hip_vocab_loss_fwd(const moda_hip_vocab_loss_args* t, void* workspace, size_t workspace_bytes, void* stream) {
+  VocabLoss v;
+  const int rc = begin_vocab_loss(t, false, workspace, workspace_bytes, stream, v);
+  if (rc) return rc;
+  const bool rows_out = t->reduction == MODA_HIP_LOSS_ROWS;
+  if (!t->loss && (t->rows > 0 || !rows_out)) return MODA_HIP_EINVAL;
+  if ((uintptr_t)t->loss % 4 != 0) return MODA_HIP_EALIGN;
+  if (t->rows == 0 && rows_out) return MODA_HIP_OK;
+  float* losses = rows_out ? t->loss : v.at<float>(v.p.losses);
+  if (!v.p.direct) MODA_TRY(v.gather());
+  const int64_t tile = moda::tile_f(v.p.logits.tile);
+  for (int64_t i = 0; i < v.p.pieces; i++) {
+    moda::ProductArgs w = {};
+    MODA_TRY(v.weights(i, w));
+    moda::ProductArgs a = v.logits(i, w);
+    a.stats = v.at<float2>(v.p.stats) + i * ((v.p.piece + tile - 1) / tile) * t->rows;
+    a.stats_ld = t->rows;
+    a.target_logit = v.at<float>(v.p.target_logit);
+    MODA_TRY(moda::launch_stats(a, t->dtype, v.p.logits.tile, v.stream));
+  }
+  const int64_t last = (v.piece_words(v.p.pieces - 1) + tile - 1) / tile;
+  moda::JoinStatsArgs j = {v.at<float2>(v.p.stats), v.at<float>(v.p.target_logit), t->rows, (v.p.pieces - 1) * ((v.p.piece + tile - 1) / tile) + last,
+                           v.head(), v.words(), v.at<int>(v.p.row_of), losses, t->lse};
+  if (t->rows > 0) MODA_TRY(moda::launch_join_stats(j, v.stream));
+  if (!rows_out) MODA_TRY(moda::launch_loss_total({losses, t->loss, v.words(), v.head(), t->reduction == MODA_HIP_LOSS_MEAN}, v.stream));
+  return MODA_HIP_OK;
+}
+
+int moda_hip_vocab_loss_bwd(const moda_hip_vocab_loss_args* t, void* workspace, size_t workspace_bytes, void* stream) {
+  VocabLoss v;
+  const int rc = begin_vocab_loss(t, true, workspace, workspace_bytes, stream, v);
+  if (rc) return rc;
+  const int es = elem_size(t->dtype);
+  if ((t->rows > 0 && !t->d_loss) || (t->dx && t->ld_dx < t->width) || (t->d_weight && t->ld_d_weight < t->width)) return MODA_HIP_EINVAL;
+  if ((uintptr_t)t->d_loss % 4 != 0 || (uintptr_t)t->dx % es != 0 || (uintptr_t)t->d_weight % es != 0) return MODA_HIP_EALIGN;
+  if (!t->dx && !t->d_weight) return MODA_HIP_OK;
+  const moda::LossPlan& p = v.p;
+  // four results of a row are stored as one where they lie on that grid
+  const auto by_four = [&](const void* at, int64_t ld) { return (uintptr_t)at % (4 * es) == 0 && ld % 4 == 0; };
+  MODA_TRY(v.gather());
+  for (int64_t i = 0; i < p.pieces; i++) {
+    moda::ProductArgs w = {};
+    MODA_TRY(v.weights(i, w));
+    moda::ProductArgs a = v.logits(i, w);
+    a.factor = v.at<float>(p.factor);
+    a.lse = v.at<float>(p.lse);
+    a.dz = v.at<uint16_t>(p.dz);
+    a.dz_ld = p.dz_ld;
+    a.dz_plane = t->rows * p.dz_ld;
+    MODA_TRY(moda::launch_grad_logits(a, t->dtype, p.logits.tile, v.stream));
+    if (t->dx) {
+      moda::ProductArgs r = w;
+      r.p = a.dz;
+      r.p_ld = a.dz_ld;
+      r.p_plane = a.dz_plane;
+      r.f_count = (int)(p.copy_weight ? p.rows_ld : t->width);
+      r.p_count = (int)t->rows;
+      r.k_count = (int)v.piece_words(i);
+      r.head = v.head();
+      r.splits = p.grad_rows.splits;
+      r.row_of = v.at<int>(p.row_of);
+      r.scale = t->scale;
+      if (p.acc_rows) {
+        r.acc = v.at<float>(p.dx_acc);
+        r.acc_ld = p.acc_ld;
+        r.acc_split = t->rows * p.acc_ld;
+        r.add = i > 0;
+      } else {
+        r.f_count = (int)t->width;
+        r.out = (char*)t->dx;
+        r.out_ld = t->ld_dx;
+        r.out_vec = by_four(t->dx, t->ld_dx);
+      }
+      MODA_TRY(moda::launch_grad_rows(r, t->dtype, p.grad_rows.tile, v.stream));
+    }
+    if (t->d_weight) {
+      char* out = (char*)t->d_weight + i * p.piece * t->ld_d_weight * es;
+      moda::ProductArgs g = {};
+      g.f = v.at<uint16_t>(p.rows);
+      g.f_ld = p.rows_ld;
+      g.f_plane = t->rows * p.rows_ld;
+      g.p = a.dz;
+      g.p_ld = a.dz_ld;
+      g.p_plane = a.dz_plane;
+      g.f_count = (int)t->width;
+      g.p_count = (int)v.piece_words(i);
+      g.k_count = (int)t->rows;
+      g.head = v.head();
+      g.splits = p.grad_weight.splits;
+      g.scale = t->scale;
+      g.out = out;
+      g.out_ld = t->ld_d_weight;
+      g.out_vec = by_four(out, t->ld_d_weight);
+      if (g.splits > 1) {
+        g.acc = v.at<float>(p.dw_acc);
+        g.acc_ld = p.acc_ld;
+        g.acc_split = p.piece * p.acc_ld;
+      }
+      MODA_TRY(moda::launch_grad_weight(g, t->dtype, p.grad_weight.tile, v.stream));
+      if (g.splits > 1)
+        MODA_TRY(moda::launch_join_sums({g.acc, g.acc_ld, g.acc_split, g.p_count, t->width, g.splits, v.head(), 0, nullptr, out, g.out_ld, g.out_vec, t->scale},
+                                        t->dtype, v.stream));
+    }
+  }
+  if (t->dx && p.acc_rows && t->rows > 0)
+    MODA_TRY(moda::launch_join_sums({v.at<float>(p.dx_acc), p.acc_ld, t->rows * p.acc_ld, t->rows, t->width, p.grad_rows.splits, v.head(), 1,
+                                     v.at<int>(p.row_of), (char*)t->dx, t->ld_dx, by_four(t->dx, t->ld_dx), t->scale},
+                                    t->dtype, v.stream));
+  return MODA_HIP_OK;
+}
+#undef MODA_TRY
 
 int moda_hip_uses_matrix_cores(const moda_hip_desc* d) {
   KArgs a;

@@ -8,6 +8,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -1216,6 +1217,231 @@ std::pair<Tensor, Tensor> paged_attend(const Tensor& q_in, const Tensor& ck, con
   return {o, lse};
 }
 
+// ------------------------------------------------------------------------------------------------------------------
+// the two ends of a language model (moda_amd/vocab.py)
+// ------------------------------------------------------------------------------------------------------------------
+
+// Rows [n, width] as the kernels read them: any distance between rows, unit inner stride.
+struct Rows {
+  Tensor x;
+  int64_t n, width, ld;
+};
+Rows rows_of(const Tensor& in, bool may_copy = true) {
+  const int64_t width = in.size(-1);
+  Tensor x = in.dim() == 2 ? in : in.reshape({width > 0 ? in.numel() / width : 0, width});
+  if (may_copy && x.size(1) > 1 && x.stride(1) != 1) x = x.contiguous();
+  return {x, x.size(0), width, x.stride(0)};
+}
+Tensor words_of(const Tensor& in, const char* name, const Tensor& beside) {
+  CONTRACT(in.scalar_type() == at::kInt || in.scalar_type() == at::kLong, name, " must be int32 or int64");
+  CONTRACT(in.device() == beside.device(), name, " must be on the tensors' device");
+  return in.contiguous();
+}
+void check_weight(const Tensor& weight) {
+  CONTRACT(weight.dim() == 2 && weight.size(0) > 0 && weight.size(1) > 0, "weight must be [vocabulary, width]");
+  check_device(weight);
+  dtype_code(weight);
+}
+void finite_scale(double scale) { CONTRACT(std::isfinite((float)scale), "scale must be finite, got ", scale); }
+
+Tensor embed_rows(const Tensor& tokens_in, const Tensor& weight_in, double scale) {
+  check_weight(weight_in);
+  finite_scale(scale);
+  const Tensor tokens = words_of(tokens_in, "tokens", weight_in);
+  const Rows w = rows_of(weight_in);
+  std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
+  shape.push_back(w.width);
+  Tensor y = at::empty(shape, weight_in.options());
+  if (y.numel() == 0) return y;
+  c10::OptionalDeviceGuard guard(y.device());
+  check_rc(moda_hip_embed_rows(dtype_code(y), in_ptr(tokens), tokens.scalar_type() == at::kLong, tokens.numel(), in_ptr(w.x), w.ld, w.n, w.width,
+                               (float)scale, out_ptr(y), w.width, stream_of(y)),
+           "moda_hip_embed_rows");
+  return y;
+}
+
+Tensor embed_grad(const Tensor& tokens_in, const Tensor& dy_in, int64_t vocab, double scale) {
+  CONTRACT(dy_in.dim() == tokens_in.dim() + 1 && dy_in.sizes().slice(0, tokens_in.dim()) == tokens_in.sizes() && dy_in.size(-1) > 0,
+           "the gradient of the rows must be [tokens .., width]");
+  CONTRACT(vocab > 0, "the vocabulary must have a word");
+  check_device(dy_in);
+  finite_scale(scale);
+  const int dt = dtype_code(dy_in);
+  const Tensor tokens = words_of(tokens_in, "tokens", dy_in);
+  const Rows d = rows_of(dy_in);
+  Tensor dw = at::empty({vocab, d.width}, dy_in.options());
+  c10::OptionalDeviceGuard guard(dw.device());
+  const size_t bytes = moda_hip_embed_grad_workspace_bytes(d.n, vocab, d.width);
+  Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 16)}, dw.options().dtype(at::kByte));
+  check_rc(moda_hip_embed_grad(dt, in_ptr(tokens), tokens.scalar_type() == at::kLong, d.n, in_ptr(d.x), d.ld, vocab, d.width, (float)scale, out_ptr(dw),
+                               d.width, out_ptr(ws), (size_t)ws.nbytes(), stream_of(dw)),
+           "moda_hip_embed_grad");
+  return dw;
+}
+
+// Lookup and gradient are each other's gradient: one node for both.
+struct Embedding : c10::intrusive_ptr_target {
+  int64_t vocab = 0;
+  double scale = 1.0;
+  bool lookup = true;
+};
+struct Embed : torch::autograd::Function<Embed> {
+  static Tensor compute(const Embedding& how, const Tensor& x, const Tensor& tokens) {
+    return how.lookup ? embed_rows(tokens, x, how.scale) : embed_grad(tokens, x, how.vocab, how.scale);
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& tokens, const c10::intrusive_ptr<Embedding>& how) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["state"] = owning(how);
+    ctx->set_materialize_grads(false);
+    return {compute(*how, x, tokens)};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return in_engine([&] {
+      if (!grads[0].defined()) return variable_list(3);
+      const Tensor tokens = ctx->get_saved_variables()[0];
+      auto back = c10::make_intrusive<Embedding>(*owned<Embedding>(ctx));
+      back->lookup = !back->lookup;
+      return variable_list{at::GradMode::is_enabled() ? apply(grads[0], tokens, back)[0] : compute(*back, grads[0], tokens), Tensor(), Tensor()};
+    });
+  }
+};
+
+// Whether a call has to leave a node behind (or, for a tangent, to be refused by it).
+bool watched(std::initializer_list<const Tensor*> xs) {
+  const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* x : xs)
+    if ((backward && x->requires_grad()) || (forward && x->_fw_grad(0).defined())) return true;
+  return false;
+}
+
+Tensor embed_tokens(const Tensor& tokens, const Tensor& weight, double scale, bool differentiable) {
+  py::gil_scoped_release nogil;
+  if (!differentiable || !watched({&weight})) return embed_rows(tokens, weight, scale);
+  auto how = c10::make_intrusive<Embedding>();
+  how->vocab = weight.dim() == 2 ? weight.size(0) : 0;
+  how->scale = scale;
+  return Embed::apply(weight, tokens, how)[0];
+}
+
+// What a cross entropy is besides its tensors.
+struct CrossEntropy : c10::intrusive_ptr_target {
+  double scale = 1.0;
+  int64_t ignore_index = -100;
+  int reduction = MODA_HIP_LOSS_MEAN;
+};
+
+struct LossCall {
+  moda_hip_vocab_loss_args a = {};
+  Rows x, w;
+  Tensor targets;
+};
+LossCall describe_loss(const CrossEntropy& how, const Tensor& x, const Tensor& weight, const Tensor& targets) {
+  check_weight(weight);
+  finite_scale(how.scale);
+  CONTRACT(x.dim() >= 1 && x.size(-1) == weight.size(1), "rows must be [.., ", weight.size(1), "], as wide as the weight's");
+  CONTRACT(x.sizes().slice(0, x.dim() - 1) == targets.sizes(), "targets must be ", x.sizes().slice(0, x.dim() - 1), ", one for each row");
+  same_dtype({&x, &weight});
+  CONTRACT(x.device() == weight.device(), "rows and weight must be on one device");
+  LossCall c;
+  c.targets = words_of(targets, "targets", weight);
+  c.x = rows_of(x);
+  c.w = rows_of(weight);
+  c.a.struct_size = sizeof(c.a);
+  c.a.dtype = dtype_code(x);
+  c.a.rows = c.x.n;
+  c.a.vocab = c.w.n;
+  c.a.width = c.w.width;
+  c.a.x = in_ptr(c.x.x);
+  c.a.weight = in_ptr(c.w.x);
+  c.a.targets = in_ptr(c.targets);
+  c.a.ld_x = c.x.ld;
+  c.a.ld_weight = c.w.ld;
+  c.a.ignore_index = how.ignore_index;
+  c.a.targets64 = targets.scalar_type() == at::kLong;
+  c.a.reduction = how.reduction;
+  c.a.scale = (float)how.scale;
+  return c;
+}
+Tensor loss_workspace(size_t bytes, const Tensor& beside) {
+  return at::empty({(int64_t)std::max<size_t>(bytes, 16)}, beside.options().dtype(at::kByte));
+}
+
+// loss and log sums (base 2) of the rows
+std::pair<Tensor, Tensor> loss_forward(const CrossEntropy& how, const Tensor& x, const Tensor& weight, const Tensor& targets) {
+  LossCall c = describe_loss(how, x, weight, targets);
+  const auto fp32 = weight.options().dtype(at::kFloat);
+  Tensor lse = at::empty(targets.sizes(), fp32), loss = how.reduction == MODA_HIP_LOSS_ROWS ? at::empty(targets.sizes(), fp32) : at::empty({}, fp32);
+  c.a.loss = (float*)out_ptr(loss);
+  c.a.lse = (float*)out_ptr(lse);
+  c10::OptionalDeviceGuard guard(weight.device());
+  Tensor ws = loss_workspace(moda_hip_vocab_loss_fwd_workspace_bytes(&c.a), weight);
+  check_rc(moda_hip_vocab_loss_fwd(&c.a, out_ptr(ws), (size_t)ws.nbytes(), stream_of(weight)), "moda_hip_vocab_loss_fwd");
+  return {loss, lse};
+}
+
+std::pair<Tensor, Tensor> loss_backward(const CrossEntropy& how, const Tensor& x, const Tensor& weight, const Tensor& targets, const Tensor& lse_in,
+                                        const Tensor& d_loss_in, bool want_dx, bool want_dw) {
+  LossCall c = describe_loss(how, x, weight, targets);
+  const bool rows = how.reduction == MODA_HIP_LOSS_ROWS;
+  CONTRACT(lse_in.scalar_type() == at::kFloat && lse_in.sizes() == targets.sizes() && lse_in.device() == weight.device(), "lse must be fp32, one for each row");
+  CONTRACT((rows ? d_loss_in.sizes() == targets.sizes() : d_loss_in.numel() == 1) && d_loss_in.device() == weight.device(),
+           rows ? "d_loss must have a value for each row" : "d_loss must be one value");
+  const Tensor lse = lse_in.contiguous(), d_loss = d_loss_in.to(at::kFloat).contiguous();
+  Tensor dx, dw;
+  if (want_dx) dx = at::empty(x.sizes(), x.options());
+  if (want_dw) dw = at::empty(weight.sizes(), weight.options());
+  c.a.lse = (float*)in_ptr(lse);
+  c.a.d_loss = (const float*)in_ptr(d_loss);
+  c.a.dx = want_dx ? out_ptr(dx) : nullptr;
+  c.a.d_weight = want_dw ? out_ptr(dw) : nullptr;
+  c.a.ld_dx = c.a.ld_d_weight = c.a.width;
+  c10::OptionalDeviceGuard guard(weight.device());
+  Tensor ws = loss_workspace(moda_hip_vocab_loss_bwd_workspace_bytes(&c.a), weight);
+  check_rc(moda_hip_vocab_loss_bwd(&c.a, out_ptr(ws), (size_t)ws.nbytes(), stream_of(weight)), "moda_hip_vocab_loss_bwd");
+  return {dx, dw};
+}
+
+struct VocabLoss : torch::autograd::Function<VocabLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& targets,
+                               const c10::intrusive_ptr<CrossEntropy>& how) {
+    auto r = loss_forward(*how, x, weight, targets);
+    ctx->save_for_backward({x, weight, targets, r.second});
+    ctx->saved_data["state"] = owning(how);
+    ctx->set_materialize_grads(false);
+    return {r.first};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return in_engine([&] {
+      if (!grads[0].defined()) return variable_list(4);
+      const variable_list s = ctx->get_saved_variables();
+      const bool dx = ctx->needs_input_grad(0), dw = ctx->needs_input_grad(1);
+      const auto g = loss_backward(*owned<CrossEntropy>(ctx), s[0], s[1], s[2], s[3], grads[0], dx, dw);
+      variable_list out = {g.first, g.second};
+      if (at::GradMode::is_enabled()) {  // whoever differentiates these again is told
+        for (Tensor& g : out)
+          if (g.defined()) g.set_requires_grad(true);
+        out = (*std::make_shared<torch::autograd::DelayedError>("linear_cross_entropy has no second derivative", 2))(std::move(out));
+      }
+      return variable_list{out[0], out[1], Tensor(), Tensor()};
+    });
+  }
+};
+
+c10::intrusive_ptr<CrossEntropy> make_cross_entropy(double scale, int64_t ignore_index, int reduction) {
+  auto how = c10::make_intrusive<CrossEntropy>();
+  how->scale = scale;
+  how->ignore_index = ignore_index;
+  how->reduction = reduction;
+  return how;
+}
+
+Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& targets, double scale, int64_t ignore_index, int reduction) {
+  py::gil_scoped_release nogil;
+  const auto how = make_cross_entropy(scale, ignore_index, reduction);
+  if (!watched({&x, &weight})) return loss_forward(*how, x, weight, targets).first;
+  return VocabLoss::apply(x, weight, targets, how)[0];
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -1240,6 +1466,23 @@ PYBIND11_MODULE(_host, m) {
   m.def("apply_rotary", &apply_rotary);
   m.def("paged_append", &paged_append);
   m.def("paged_attend", &paged_attend);
+  m.def("embed_tokens", &embed_tokens);
+  m.def("embed_grad", [](const Tensor& tokens, const Tensor& dy, int64_t vocab, double scale) {
+    py::gil_scoped_release nogil;
+    no_gradients({&dy}, "embed_tokens_bwd");
+    return embed_grad(tokens, dy, vocab, scale);
+  });
+  m.def("linear_cross_entropy", &linear_cross_entropy);
+  m.def("linear_cross_entropy_fwd", [](const Tensor& x, const Tensor& weight, const Tensor& targets, double scale, int64_t ignore_index, int reduction) {
+    py::gil_scoped_release nogil;
+    return loss_forward(*make_cross_entropy(scale, ignore_index, reduction), x, weight, targets);
+  });
+  m.def("linear_cross_entropy_bwd", [](const Tensor& x, const Tensor& weight, const Tensor& targets, const Tensor& lse, const Tensor& d_loss, double scale,
+                                       int64_t ignore_index, int reduction, bool want_dx, bool want_dw) {
+    py::gil_scoped_release nogil;
+    const auto r = loss_backward(*make_cross_entropy(scale, ignore_index, reduction), x, weight, targets, lse, d_loss, want_dx, want_dw);
+    return std::make_pair(optional(r.first), optional(r.second));
+  });
   m.def("stack_forward", [](const Tensor& x, const std::vector<std::vector<OptTensor>>& params, const std::vector<std::array<double, 2>>& eps,
                             int64_t heads, int64_t kv_heads, bool is_causal, int64_t chunk_tokens, bool post_norm) {
     std::vector<Block> blocks;
