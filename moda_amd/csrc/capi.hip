@@ -1035,7 +1035,7 @@ struct VocabLoss {
     a.rows_plane = t->rows * p.rows_ld;
     if (t->rows > moda::kScanMost) {
       a.counts = at<int>(p.counts);
-      a.exponents = at<int>(p.exponents);
+      a.largest = at<int>(p.largest);
     }
     a.vec_x = on_grid(t->x, t->ld_x, es());
     if (!backward) {
@@ -1051,7 +1051,7 @@ struct VocabLoss {
       a.ld_dx = t->ld_dx;
       a.vec_dx = on_grid(t->dx, t->ld_dx, es());
       a.mean = t->reduction == MODA_HIP_LOSS_MEAN;
-      a.fp16 = t->dtype == MODA_HIP_FP16;
+      a.up = t->dtype == MODA_HIP_FP16 ? 0x1p14f : 1.f;  // (fp16: probabilities down to 2^-28 have all their bits)
     }
     return moda::launch_gather_rows(a, t->dtype, stream);
   }

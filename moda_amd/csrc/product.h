@@ -156,17 +156,14 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wf = wave % WF, wp = wave / WF;
 
   int p_count = a.p_count, k_count = a.k_count;
-  float up = 1.f, down = 1.f;
+  float down = 1.f;
   if (a.head) {
     const int live = __builtin_amdgcn_readfirstlane(a.head->live);
     if (PROD == kGradWeight)
       k_count = live;
     else
       p_count = live;
-    if (PROD != kStats) {
-      up = a.head->up;
-      down = a.head->down;
-    }
+    if (PROD == kGradRows || PROD == kGradWeight) down = a.head->down;
   }
   // Which tile: the workgroups of one XCD (every eighth) have neighbouring ones, in columns of eight tiles of p through all f.
   const int tiles_f = (a.f_count + BF - 1) / BF, tiles_p = (p_count + BP - 1) / BP;
@@ -303,7 +300,7 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
       const int p = p_of(nb);
       const bool there = p < p_count;
       const int target = there ? a.target[p] - a.first_word : -1;
-      const float factor = there ? a.factor[p] * up : 0.f, lse = there ? a.lse[p] : 0.f;
+      const float factor = there ? a.factor[p] : 0.f, lse = there ? a.lse[p] : 0.f;
 #pragma unroll
       for (int mb = 0; mb < MB; mb++) {
         const int f = f_of(mb);

@@ -85,11 +85,11 @@ inline EmbedGradPlan plan_embed_grad(int64_t n, int64_t vocab, int64_t width) {
 // cross entropy over a vocabulary
 // ---------------------------------------------------------------------------------------------------------------------
 
-// What the device alone knows of a call: how many rows have a target, and by which power of two the gradient of the logits is kept larger
-// than it is (fp16).
+// What the device alone knows of a call: how many rows have a target, and by what the two products that read the gradient of the logits
+// are multiplied.
 struct LossHead {
   int live;
-  float up, down;
+  float down;
 };
 
 // Rows with a target, one behind the other: their numbers, targets, factors and log sums, and the rows themselves as the products read
@@ -102,8 +102,8 @@ struct GatherArgs {
   int *row_of, *target;
   uint16_t* rows;
   int64_t rows_ld, rows_plane;
-  // of 1024 targets each, where there are many: rows with a target, the exponent of the largest upstream gradient among them
-  int *counts, *exponents;
+  // of 1024 targets each, where there are many: rows with a target, the largest upstream gradient among them (bits of a float)
+  int *counts, *largest;
   // forward: zeros for the rows without
   float *loss, *lse_out;
   // backward
@@ -112,7 +112,8 @@ struct GatherArgs {
   float *factor, *lse;
   char* dx;  // zeros for the rows without (or NULL)
   int64_t ld_dx;
-  int mean, fp16, vec_x, vec_dx;
+  float up;  // the gradient of the logits is kept this many times as large
+  int mean, vec_x, vec_dx;
 };
 
 struct LayArgs {  // rows of a matrix as the products read them
@@ -224,7 +225,7 @@ struct LossPlan {
   Tiling logits, grad_rows, grad_weight;
   int64_t stat_tiles, acc_ld;
   bool acc_rows;  // the gradient of the rows is added up in fp32
-  size_t head, row_of, target, factor, lse, target_logit, counts, exponents, stats, rows, weight, dz, dx_acc, dw_acc, losses, bytes;
+  size_t head, row_of, target, factor, lse, target_logit, counts, largest, stats, rows, weight, dz, dx_acc, dw_acc, losses, bytes;
 };
 
 constexpr int64_t kGatherBlock = 32, kCountBlock = 1024, kScanMost = 16384;
@@ -275,7 +276,7 @@ inline LossPlan plan_loss(int64_t n, int64_t vocab, int64_t width, bool fp32, bo
   p.factor = take(backward, n * 4);
   p.lse = take(backward, n * 4);
   p.counts = take(gathers && n > kScanMost, (n + kCountBlock - 1) / kCountBlock * 4);
-  p.exponents = take(gathers && n > kScanMost, (n + kCountBlock - 1) / kCountBlock * 4);
+  p.largest = take(gathers && n > kScanMost, (n + kCountBlock - 1) / kCountBlock * 4);
   p.rows = take(gathers, n * p.rows_ld * 2 * p.planes);
   p.weight = take(p.copy_weight, p.piece * p.rows_ld * 2 * p.planes);
   p.target_logit = take(!backward, n * 4);

@@ -59,12 +59,6 @@ __device__ __forceinline__ void lay_eight(const char* row, int64_t c, int64_t wi
   }
 }
 
-// the exponent e of a finite x, |x| < 2^e; least for zero and what is not finite
-__device__ __forceinline__ int exponent_of(float x) {
-  const int e = (int)(__float_as_uint(x) >> 23 & 255);
-  return e == 255 ? -1000 : e - 126;  // (smaller ones than 2^-126: as that)
-}
-
 // Sums of the workgroup's 256 threads, and their largest.
 __device__ __forceinline__ void over_block(int& a, int& b, int& largest) {
   __shared__ int sums[3][4];
@@ -86,23 +80,25 @@ __device__ __forceinline__ void over_block(int& a, int& b, int& largest) {
   largest = max(max(sums[2][0], sums[2][1]), max(sums[2][2], sums[2][3]));
 }
 
-__device__ __forceinline__ int row_exponent(const GatherArgs& a, int64_t i) {
-  return a.fp16 && a.d_loss ? exponent_of(a.d_loss[i * a.d_loss_stride]) : -1000;
+// the size of a row's upstream gradient as the bits of a float, which order as it does; zero where it is not finite
+__device__ __forceinline__ int size_of(const GatherArgs& a, int64_t i) {
+  const int bits = a.d_loss ? (int)(__float_as_uint(a.d_loss[i * a.d_loss_stride]) & 0x7fffffffu) : 0;
+  return bits < 0x7f800000 ? bits : 0;
 }
 
 // Where every workgroup of the gather would otherwise look at more than kScanMost targets: rows with one of each kCountBlock.
 __global__ __launch_bounds__(256) void count_rows_kernel(const GatherArgs a) {
   const int64_t first = (int64_t)workgroup() * kCountBlock;
-  int live = 0, unused = 0, e = -1000;
+  int live = 0, unused = 0, e = 0;
   for (int64_t i = first + threadIdx.x; i < first + kCountBlock && i < a.words.n; i += 256)
     if (a.words.of(i) >= 0) {
       live++;
-      e = max(e, row_exponent(a, i));
+      e = max(e, size_of(a, i));
     }
   over_block(live, unused, e);
   if (threadIdx.x == 0) {
     a.counts[workgroup()] = live;
-    a.exponents[workgroup()] = e;
+    a.largest[workgroup()] = e;
   }
 }
 
@@ -112,7 +108,7 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
   __shared__ int to[kGatherBlock];  // where a row goes, or -1
   const int tid = threadIdx.x;
   const int64_t n = a.words.n, first = (int64_t)workgroup() * kGatherBlock;
-  int before = 0, all = 0, e = -1000;
+  int before = 0, all = 0, e = 0;
   int64_t from = 0, upto = n;
   if (a.counts) {
     const int64_t own = first / kCountBlock, blocks = (n + kCountBlock - 1) / kCountBlock;
@@ -120,7 +116,7 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
       const int c = a.counts[i];
       all += c;
       before += i < own ? c : 0;
-      e = max(e, a.exponents[i]);
+      e = max(e, a.largest[i]);
     }
     from = own * kCountBlock;
     upto = first;
@@ -130,15 +126,14 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
     before += live && i < first;
     if (!a.counts && live) {
       all++;
-      e = max(e, row_exponent(a, i));
+      e = max(e, size_of(a, i));
     }
   }
   over_block(before, all, e);
-  const float share = a.mean ? 1.f / (float)max(all, 1) : 1.f;
-  // fp16: gradients of logits are kept 2^14 times as large as they would be where the largest upstream one lies between 1/2 and 1, so that
-  // probabilities down to 2^-28 of it have all their bits
-  const int up = a.fp16 && a.d_loss && e > -1000 ? min(max(14 - e + (a.mean ? exponent_of((float)max(all, 1)) - 1 : 0), -100), 120) : 0;
-  if (first == 0 && tid == 0) *a.head = LossHead{all, ldexpf(1.f, up), ldexpf(1.f, -up)};
+  // The gradient of a logit is rounded to 16 bits.  The factor that rows share stays out of that, or its own rounding would be in all of them,
+  // the same way: it is kept relative to the largest upstream gradient, which the products multiply by at their end.
+  const float most = e > 0 ? __uint_as_float((uint32_t)e) : 1.f;
+  if (first == 0 && tid == 0) *a.head = LossHead{all, a.d_loss ? most / (a.mean ? (float)max(all, 1) : 1.f) / a.up : 1.f};
   if (tid < 64) {
     const int64_t i = first + tid;
     const int word = tid < kGatherBlock && i < n ? a.words.of(i) : -1;
@@ -149,7 +144,7 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
       a.row_of[at] = (int)i;
       a.target[at] = word;
       if (a.d_loss) {
-        a.factor[at] = a.d_loss[i * a.d_loss_stride] * share;
+        a.factor[at] = a.d_loss[i * a.d_loss_stride] / most * a.up;
         a.lse[at] = a.lse_in[i];
       }
     } else if (tid < kGatherBlock && i < n && a.loss) {
