@@ -968,7 +968,7 @@ int moda_hip_embed_rows(int32_t dtype, const void* tokens, int32_t tokens64, int
 }
 
 size_t moda_hip_embed_grad_workspace_bytes(int64_t n, int64_t vocab, int64_t width) {
-  return n <= 0 || n >= (1ll << 30) || vocab <= 0 || width <= 0 || width >= (1ll << 24) ? 0 : moda::plan_embed_grad(n, vocab, width).bytes;
+  return n < 0 || n >= (1ll << 30) || vocab <= 0 || vocab >= (1ll << 31) - 256 || width <= 0 || width >= (1ll << 24) ? 0 : moda::plan_embed_grad(n, vocab, width).bytes;
 }
 
 int moda_hip_embed_grad(int32_t dtype, const void* tokens, int32_t tokens64, int64_t n, const void* dy, int64_t ld_dy, int64_t vocab, int64_t width,
@@ -978,7 +978,7 @@ int moda_hip_embed_grad(int32_t dtype, const void* tokens, int32_t tokens64, int
   if (!d_weight || ld_d_weight < width || (n > 0 && (!dy || ld_dy < 0))) return MODA_HIP_EINVAL;
   const int es = elem_size(dtype);
   if ((uintptr_t)dy % es != 0 || (uintptr_t)d_weight % es != 0) return MODA_HIP_EALIGN;
-  if (n > 0 && (!workspace || workspace_bytes < moda::plan_embed_grad(n, vocab, width).bytes)) return MODA_HIP_EWORKSPACE;
+  if (!workspace || workspace_bytes < moda::plan_embed_grad(n, vocab, width).bytes) return MODA_HIP_EWORKSPACE;
   if ((uintptr_t)workspace % 16 != 0) return MODA_HIP_EALIGN;
   if ((rc = check_device())) return rc;
   moda::EmbedArgs a = embed_args(tokens, tokens64, n, dy, ld_dy, vocab, width, scale, d_weight, ld_d_weight);

@@ -90,8 +90,11 @@ __device__ __forceinline__ Entry entry(const SortArgs& a, int64_t i) {
   return {w < 0 ? (uint32_t)a.words.vocab : (uint32_t)w, (uint32_t)i};
 }
 
+// (The first pass clears the words' ranges besides.)
 __global__ __launch_bounds__(kSortThreads) void count_digits_kernel(const SortArgs a) {
   __shared__ uint32_t count[kDigits];
+  if (!a.keys)
+    for (int64_t v = (int64_t)blockIdx.x * kSortThreads + threadIdx.x; v < a.words.vocab; v += (int64_t)a.blocks * kSortThreads) a.range[v] = int2{0, 0};
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) count[d] = 0;
   __syncthreads();
   const int64_t first = (int64_t)blockIdx.x * kSortThreads * a.rounds;
@@ -107,15 +110,30 @@ __global__ __launch_bounds__(kSortThreads) void count_digits_kernel(const SortAr
 // waves and lanes before it in this round.
 __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(const SortArgs a) {
   constexpr int W = kSortThreads / 64;
+  static_assert(kSortThreads == 2 * kDigits, "two threads a digit");
   __shared__ uint32_t base[kDigits], in_wave[W][kDigits], total[kDigits / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t before = 0, all = 0, upto = 0;
-  if (tid < kDigits) {
-    for (int b = 0; b < a.blocks; b++) {
-      const uint32_t c = a.counts[(int64_t)b * kDigits + tid];
+  {
+    uint32_t* other = &in_wave[0][0];  // what the second thread of a digit has counted
+    const int d = tid & (kDigits - 1), half = (a.blocks + 1) / 2, from = tid < kDigits ? 0 : half, to = tid < kDigits ? half : a.blocks;
+#pragma unroll 16
+    for (int b = from; b < to; b++) {
+      const uint32_t c = a.counts[b * kDigits + d];
       all += c;
       before += b < (int)blockIdx.x ? c : 0;
     }
+    if (tid >= kDigits) {
+      other[2 * d] = all;
+      other[2 * d + 1] = before;
+    }
+    __syncthreads();
+    if (tid < kDigits) {
+      all += other[2 * d];
+      before += other[2 * d + 1];
+    }
+  }
+  if (tid < kDigits) {
     upto = all;  // of the digits of this wave up to this one
     for (int s = 1; s < 64; s <<= 1) {
       const uint32_t o = __shfl_up(upto, s, 64);
@@ -168,130 +186,77 @@ __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(const SortAr
 // sums of the rows of a word
 // ---------------------------------------------------------------------------------------------------------------------
 
-// How many of the places lo .. hi - 1 satisfy `holds`, which none does behind one that does not; by a wave, 64 places in one go.  (In 32 bits:
-// a loop of this form over 64-bit uniform values was compiled to selects by a stale condition.)
-template <typename Holds>
-__device__ __forceinline__ int count_while(int lo, int hi, Holds holds) {
-  const int lane = threadIdx.x & 63, first = lo;
-  while (hi > lo) {
-    const int step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step - 1;  // the last place of this lane's piece
-    const int from = lo + __popcll(__ballot(at < hi && holds(at))) * step;  // pieces that hold altogether
-    hi = min(from + step - 1, hi);
-    lo = min(from, hi);
-  }
-  return lo - first;
+__global__ __launch_bounds__(256) void word_ranges_kernel(const SortArgs a) {
+  const int i = (int)(workgroup() * 256 + threadIdx.x), n = (int)a.words.n;
+  if (i >= n) return;
+  const uint32_t k = a.keys[i];
+  if (k >= (uint32_t)a.words.vocab) return;
+  if (i == 0 || a.keys[i - 1] != k) a.range[k].x = i;
+  if (i == n - 1 || a.keys[i + 1] != k) a.range[k].y = i + 1;
 }
 
-// the sum of the rows at places[first .. last), in their order, of a lane's kChunks vectors from c0 on
+// The sum of the rows at places[first .. last), in their order, of a lane's kChunks vectors from c0 on; `lanes` neighbouring lanes share the
+// rows, have a place of theirs each and hand them round.
 template <typename E, int VEC>
 __device__ __forceinline__ void add_rows(const EmbedArgs& a, int first, int last, int64_t c0, int lanes, float (&sum)[kChunks][VEC]) {
   typedef typename Vectors<E, VEC>::vec vec;
   typedef typename E::bits bits;
+  constexpr int ROWS = 4;  // in flight
+  const int lane = threadIdx.x & 63, sub = lane & (lanes - 1), group = lane - sub;
 #pragma unroll
   for (int i = 0; i < kChunks; i++)
 #pragma unroll
     for (int j = 0; j < VEC; j++) sum[i][j] = 0.f;
   const bits* x = (const bits*)a.weight;
-  constexpr int ROWS = 2;  // in flight
-  for (int r = first; r < last; r += ROWS) {
-    vec v[ROWS][kChunks];
+  for (int b = first; b < last; b += lanes) {
+    const int place = b + sub < last ? (int)a.places[b + sub] : 0, count = min(lanes, last - b);
+    for (int r = 0; r < count; r += ROWS) {
+      vec v[ROWS][kChunks];
 #pragma unroll
-    for (int k = 0; k < ROWS; k++) {
-      const bool there = r + k < last;
-      const bits* row = x + (int64_t)(there ? a.places[r + k] : 0) * a.ld_in;
+      for (int k = 0; k < ROWS; k++) {
+        const bits* row = x + (int64_t)__shfl(place, group + r + k, 64) * a.ld_in;
 #pragma unroll
-      for (int i = 0; i < kChunks; i++) {
-        const int64_t c = c0 + i * lanes;
-        v[k][i] = vec{};
-        if (there && c * VEC < a.width) v[k][i] = *(const vec*)(row + c * VEC);
+        for (int i = 0; i < kChunks; i++) {
+          const int64_t c = c0 + i * lanes;
+          v[k][i] = vec{};
+          if (r + k < count && c * VEC < a.width) v[k][i] = *(const vec*)(row + c * VEC);
+        }
       }
+#pragma unroll
+      for (int k = 0; k < ROWS; k++)
+#pragma unroll
+        for (int i = 0; i < kChunks; i++)
+#pragma unroll
+          for (int j = 0; j < VEC; j++) sum[i][j] += E::widen(v[k][i][j]);  // (a row past the end is zeros: nothing is added)
     }
-#pragma unroll
-    for (int k = 0; k < ROWS; k++)
-#pragma unroll
-      for (int i = 0; i < kChunks; i++)
-#pragma unroll
-        for (int j = 0; j < VEC; j++) sum[i][j] += E::widen(v[k][i][j]);  // (a row past the end is zeros: nothing is added)
   }
 }
 
-// Blocks below word_blocks: kWordsOfBlock words each, a word's rows added up where they are at most kRunRows, zeros where there are none.
-// Blocks behind: pieces of kRunRows sorted places, of which those of longer runs (two at most: each is longer than a piece) are added up
-// into parts.
-constexpr int kWordsOfBlock = 32;
+// Blocks below chunk_blocks: pieces of kRunRows sorted places, of which those of longer runs are added up into parts.  Such a run covers
+// the first or the last place of each piece that it reaches into, so that there are two at most.
+// Blocks behind: words, kWordsOfGroup for each group of lanes: a word's rows added up where they are at most kRunRows, zeros where it has none.
+constexpr int kWordsOfGroup = 2;
 constexpr int kLeastShift = 3;  // eight lanes a row at least
 template <typename E, int VEC, bool STREAM>
 __global__ __launch_bounds__(256) void embed_grad_kernel(const EmbedArgs a) {
   typedef typename Vectors<E, VEC>::vec vec;
   typedef typename E::bits bits;
-  const int lanes = 1 << a.lane_shift, lane = threadIdx.x & 63, sub = lane & (lanes - 1), wave = threadIdx.x >> 6;
+  const int lanes = 1 << a.lane_shift, sub = threadIdx.x & (lanes - 1), groups = 256 >> a.lane_shift, group = threadIdx.x >> a.lane_shift;
   const unsigned block = workgroup();
   const int n = (int)a.words.n, vocab = (int)a.words.vocab;
   float sum[kChunks][VEC];
-  if (block < a.word_blocks) {
-    __shared__ int from[kWordsOfBlock], upto[kWordsOfBlock], range[2];
-    const int w0 = (int)block * kWordsOfBlock;
-    if (threadIdx.x < kWordsOfBlock) from[threadIdx.x] = upto[threadIdx.x] = 0;
-    if (wave < 2) {
-      const uint32_t w = (uint32_t)min(wave == 0 ? w0 : w0 + min(kWordsOfBlock, vocab - w0), vocab);
-      const int at = count_while(0, n, [&](int i) { return a.keys[i] < w; });
-      if (lane == 0) range[wave] = at;
-    }
-    __syncthreads();
-    const int lo = range[0], hi = range[1];
-    for (int i = lo + (int)threadIdx.x; i < hi; i += 256) {
-      const uint32_t k = a.keys[i];
-      if (i == lo || a.keys[i - 1] != k) from[k - w0] = i;
-      if (i == hi - 1 || a.keys[i + 1] != k) upto[k - w0] = i + 1;
-    }
-    __syncthreads();
-    const int rows = 256 >> a.lane_shift;  // words at once
-    for (int w = threadIdx.x >> a.lane_shift; w < kWordsOfBlock; w += rows) {
-      if (w >= vocab - w0) break;
-      const int first = from[w], last = upto[w];
-      if (last - first > kRunRows) continue;
-      bits* y = (bits*)a.y + (int64_t)(w0 + w) * a.ld_out;
-      for (int64_t c0 = sub; c0 * VEC < a.width; c0 += lanes * kChunks) {
-        add_rows<E, VEC>(a, first, last, c0, lanes, sum);
+  if (block < a.chunk_blocks) {
+    const int chunk = (int)block * groups + group, p0 = chunk * kRunRows, p1 = min(p0 + kRunRows, n);
+    if (chunk >= a.chunks) return;
+    const uint32_t k[2] = {a.keys[p0], a.keys[p1 - 1]};
 #pragma unroll
-        for (int i = 0; i < kChunks; i++) {
-          const int64_t c = c0 + i * lanes;
-          if (c * VEC >= a.width) break;
-          vec v;
-#pragma unroll
-          for (int j = 0; j < VEC; j++) v[j] = E::narrow(last > first ? sum[i][j] * a.scale : 0.f);
-          if (STREAM)
-            __builtin_nontemporal_store(v, (vec*)(y + c * VEC));
-          else
-            *(vec*)(y + c * VEC) = v;
-        }
-      }
-    }
-    return;
-  }
-  // the keys of this block's pieces, and of kRunRows places on either side
-  __shared__ uint32_t near[(256 >> kLeastShift) * kRunRows + 2 * kRunRows];
-  const int of_block = 256 >> a.lane_shift, group = threadIdx.x >> a.lane_shift;
-  const int chunk0 = (int)(block - a.word_blocks) * of_block, chunk = chunk0 + group;
-  for (int i = threadIdx.x; i < (of_block + 2) * kRunRows; i += 256) {
-    const int at = (chunk0 - 1) * kRunRows + i;
-    near[i] = at >= 0 && at < n ? a.keys[at] : 0xffffffffu;  // (no key is as large)
-  }
-  __syncthreads();
-  const uint32_t* keys = near + (group + 1) * kRunRows;
-  for (int first = 0; first < kRunRows;) {
-    const uint32_t k = keys[first];
-    if (k >= (uint32_t)vocab) return;  // no words from here on
-    int last = first + 1;
-    while (last < kRunRows && keys[last] == k) last++;
-    // longer than kRunRows?  A run that is has more than that many places within that many of this one's ends.
-    int b = first, e = last;
-    while (b > -kRunRows && keys[b - 1] == k) b--;
-    while (e < 2 * kRunRows && keys[e] == k) e++;
-    if (e - b > kRunRows) {
-      float* part = a.parts + (2ll * chunk + (first > 0)) * a.part_ld;
-      for (int64_t c0 = sub; c0 * VEC < a.width; c0 += lanes * kChunks) {
-        add_rows<E, VEC>(a, chunk * kRunRows + first, chunk * kRunRows + last, c0, lanes, sum);
+    for (int s = 0; s < 2; s++) {
+      if (k[s] >= (uint32_t)vocab || (s == 1 && k[1] == k[0])) break;
+      const int2 run = a.range[k[s]];
+      if (run.y - run.x <= kRunRows) continue;
+      float* part = a.parts + (2ll * chunk + s) * a.part_ld;
+      for (int64_t c0 = sub; (c0 - sub) * VEC < a.width; c0 += lanes * kChunks) {  // (by all lanes: they hand places round)
+        add_rows<E, VEC>(a, max(run.x, p0), min(run.y, p1), c0, lanes, sum);
 #pragma unroll
         for (int i = 0; i < kChunks; i++) {
           const int64_t c = c0 + i * lanes;
@@ -301,36 +266,56 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const EmbedArgs a) {
         }
       }
     }
-    first = last;
+    return;
+  }
+  const int64_t w0 = ((int64_t)(block - a.chunk_blocks) * groups + group) * kWordsOfGroup;
+  int2 run[kWordsOfGroup];
+#pragma unroll
+  for (int w = 0; w < kWordsOfGroup; w++) run[w] = w0 + w < vocab ? a.range[w0 + w] : int2{0, 0x7fffffff};
+#pragma unroll
+  for (int w = 0; w < kWordsOfGroup; w++) {
+    if (run[w].y - run[w].x > kRunRows) continue;
+    bits* y = (bits*)a.y + (w0 + w) * a.ld_out;
+    for (int64_t c0 = sub; (c0 - sub) * VEC < a.width; c0 += lanes * kChunks) {  // (by all lanes: they hand places round)
+      add_rows<E, VEC>(a, run[w].x, run[w].y, c0, lanes, sum);
+#pragma unroll
+      for (int i = 0; i < kChunks; i++) {
+        const int64_t c = c0 + i * lanes;
+        if (c * VEC >= a.width) break;
+        vec v;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) v[j] = E::narrow(run[w].y > run[w].x ? sum[i][j] * a.scale : 0.f);
+        if (STREAM)
+          __builtin_nontemporal_store(v, (vec*)(y + c * VEC));
+        else
+          *(vec*)(y + c * VEC) = v;
+      }
+    }
   }
 }
 
-// Runs longer than kRunRows, by the piece that they begin in (one at most): the sum of their parts.
+// Runs longer than kRunRows, by the piece that they begin in (one at most; they reach its last place): the sum of their parts.
 template <typename E>
 __global__ __launch_bounds__(256) void embed_join_kernel(const EmbedArgs a) {
-  const int chunk = (int)workgroup(), n = (int)a.words.n, p0 = chunk * kRunRows, p1 = min(p0 + kRunRows, n);
-  if (p0 >= n) return;
-  // the last run that begins here, if it reaches past kRunRows places
-  int first = p1 - 1;
-  const uint32_t k = a.keys[first];
-  if (k >= (uint32_t)a.words.vocab) return;  // (a run that ends before the piece does is no long one)
-  while (first > p0 && a.keys[first - 1] == k) first--;
-  if (first == p0 && p0 > 0 && a.keys[p0 - 1] == k) return;  // begins earlier
-  if (first + kRunRows >= n || a.keys[first + kRunRows] != k) return;
-  const int last = first + kRunRows + count_while(first + kRunRows, n, [&](int i) { return a.keys[i] == k; });
-  const int end = (last + kRunRows - 1) / kRunRows;  // pieces
+  const int chunk = (int)workgroup(), p0 = chunk * kRunRows, p1 = min(p0 + kRunRows, (int)a.words.n);
+  if (chunk >= a.chunks) return;
+  const uint32_t k = a.keys[p1 - 1];
+  if (k >= (uint32_t)a.words.vocab) return;
+  const int2 run = a.range[k];
+  if (run.x < p0 || run.y - run.x <= kRunRows) return;
+  const int end = (run.y + kRunRows - 1) / kRunRows;  // pieces
   typename E::bits* y = (typename E::bits*)a.y + (int64_t)k * a.ld_out;
   for (int64_t c = threadIdx.x; c < a.width; c += 256) {
-    const float* part = a.parts + (2ll * chunk + (first > p0)) * a.part_ld + c;
+    const float* part = a.parts + (2ll * chunk + (run.x > p0)) * a.part_ld + c;
     float s = *part;
     part = a.parts + 2ll * (chunk + 1) * a.part_ld + c;
     int q = chunk + 1;
-    for (; q + 8 <= end; q += 8, part += 16 * a.part_ld) {
-      float v[8];
+    for (; q + 16 <= end; q += 16, part += 32 * a.part_ld) {
+      float v[16];
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = part[2 * i * a.part_ld];
+      for (int i = 0; i < 16; i++) v[i] = part[2 * i * a.part_ld];
 #pragma unroll
-      for (int i = 0; i < 8; i++) s += v[i];
+      for (int i = 0; i < 16; i++) s += v[i];
     }
     for (; q < end; q++, part += 2 * a.part_ld) s += *part;
     y[c] = E::narrow(s * a.scale);
@@ -343,11 +328,11 @@ hipError_t rows_as(const EmbedArgs& a, bool through, int64_t blocks, hipStream_t
   return hipGetLastError();
 }
 template <typename E, int VEC>
-hipError_t grad_as(const EmbedArgs& a, bool through, int64_t blocks, int64_t chunks, hipStream_t stream) {
+hipError_t grad_as(const EmbedArgs& a, bool through, int64_t blocks, hipStream_t stream) {
   through ? embed_grad_kernel<E, VEC, true><<<grid_of(blocks), 256, 0, stream>>>(a) : embed_grad_kernel<E, VEC, false><<<grid_of(blocks), 256, 0, stream>>>(a);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && chunks > 1) {
-    embed_join_kernel<E><<<grid_of(chunks), 256, 0, stream>>>(a);
+  if (e == hipSuccess && a.chunks > 1) {
+    embed_join_kernel<E><<<grid_of(a.chunks), 256, 0, stream>>>(a);
     e = hipGetLastError();
   }
   return e;
@@ -378,9 +363,10 @@ hipError_t launch_embed_grad(EmbedArgs& a, int dtype, bool vec, char* work, hipS
   SortArgs s = {};
   s.words = a.words;
   s.counts = (uint32_t*)(work + p.counts);
+  s.range = (int2*)(work + p.range);
   s.rounds = p.rounds;
   s.blocks = p.blocks;
-  for (int i = 0; i < p.passes && a.words.n > 0; i++) {
+  for (int i = 0; i < p.passes; i++) {
     s.shift = i * kDigitBits;
     s.keys = i == 0 ? nullptr : (const uint32_t*)(work + p.keys[(i - 1) & 1]);
     s.places = i == 0 ? nullptr : (const uint32_t*)(work + p.places[(i - 1) & 1]);
@@ -392,20 +378,26 @@ hipError_t launch_embed_grad(EmbedArgs& a, int dtype, bool vec, char* work, hipS
     place_digits_kernel<<<p.blocks, kSortThreads, 0, stream>>>(s);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  a.keys = (const uint32_t*)(work + p.keys[(p.passes - 1) & 1]);
+  a.keys = s.keys = (const uint32_t*)(work + p.keys[(p.passes - 1) & 1]);
   a.places = (const uint32_t*)(work + p.places[(p.passes - 1) & 1]);
+  if (a.words.n > 0) word_ranges_kernel<<<grid_of((a.words.n + 255) / 256), 256, 0, stream>>>(s);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  a.range = s.range;
   a.parts = (float*)(work + p.parts);
   a.part_ld = p.part_ld;
+  a.chunks = (int)p.chunks;
   const int es = dtype == MODA_HIP_FP32 ? 4 : 2, v = vec ? 16 / es : 1;
   a.lane_shift = lane_shift_of(a.width, v, kLeastShift);
-  a.word_blocks = (unsigned)((a.words.vocab + kWordsOfBlock - 1) / kWordsOfBlock);
-  const int64_t of_block = 256 >> a.lane_shift, blocks = a.word_blocks + (p.chunks + of_block - 1) / of_block;
+  const int64_t groups = 256 >> a.lane_shift, of_block = groups * kWordsOfGroup;
+  a.chunk_blocks = (unsigned)((p.chunks + groups - 1) / groups);
+  const int64_t blocks = a.chunk_blocks + (a.words.vocab + of_block - 1) / of_block;
   const bool through = (a.words.n + a.words.vocab) * a.width * es > 256ll << 20;
   if (dtype == MODA_HIP_FP32)
-    return vec ? grad_as<Element<MODA_HIP_FP32>, 4>(a, through, blocks, p.chunks, stream) : grad_as<Element<MODA_HIP_FP32>, 1>(a, through, blocks, p.chunks, stream);
+    return vec ? grad_as<Element<MODA_HIP_FP32>, 4>(a, through, blocks, stream) : grad_as<Element<MODA_HIP_FP32>, 1>(a, through, blocks, stream);
   if (dtype == MODA_HIP_FP16)
-    return vec ? grad_as<Element<MODA_HIP_FP16>, 8>(a, through, blocks, p.chunks, stream) : grad_as<Element<MODA_HIP_FP16>, 1>(a, through, blocks, p.chunks, stream);
-  return vec ? grad_as<Element<MODA_HIP_BF16>, 8>(a, through, blocks, p.chunks, stream) : grad_as<Element<MODA_HIP_BF16>, 1>(a, through, blocks, p.chunks, stream);
+    return vec ? grad_as<Element<MODA_HIP_FP16>, 8>(a, through, blocks, stream) : grad_as<Element<MODA_HIP_FP16>, 1>(a, through, blocks, stream);
+  return vec ? grad_as<Element<MODA_HIP_BF16>, 8>(a, through, blocks, stream) : grad_as<Element<MODA_HIP_BF16>, 1>(a, through, blocks, stream);
 }
 
 }  // namespace moda

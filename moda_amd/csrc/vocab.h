@@ -29,11 +29,13 @@ struct EmbedArgs {
   int64_t width;
   float scale;
   int lane_shift;  // 2^lane_shift lanes share a row
-  // backward: words and places in the order of words, the partial sums of long runs
+  // backward: words and places in the order of words, where a word's places are in it, the partial sums of long runs
   const uint32_t *keys, *places;
+  const int2* range;
   float* parts;
   int64_t part_ld;
-  unsigned word_blocks;
+  int chunks;
+  unsigned chunk_blocks;
 };
 
 // The order of words: passes over digits of their number, lowest first, each stable.  A block of kSortThreads * rounds tokens counts its
@@ -44,6 +46,7 @@ struct SortArgs {
   const uint32_t *keys, *places;  // NULL in the first pass: the words themselves
   uint32_t *keys_out, *places_out;
   uint32_t* counts;  // [blocks][kDigits]
+  int2* range;       // [vocab]
   int rounds, blocks, shift;
 };
 
@@ -53,7 +56,7 @@ constexpr int kRunRows = 32;
 struct EmbedGradPlan {
   int passes, rounds, blocks;
   int64_t chunks, part_ld;  // pieces of kRunRows sorted places; floats of a part
-  size_t keys[2], places[2], counts, parts, bytes;
+  size_t keys[2], places[2], counts, range, parts, bytes;
 };
 inline EmbedGradPlan plan_embed_grad(int64_t n, int64_t vocab, int64_t width) {
   EmbedGradPlan p = {};
@@ -63,6 +66,7 @@ inline EmbedGradPlan plan_embed_grad(int64_t n, int64_t vocab, int64_t width) {
   p.rounds = (int)((n + (int64_t)kSortThreads * kMostSortBlocks - 1) / ((int64_t)kSortThreads * kMostSortBlocks));
   if (p.rounds < 1) p.rounds = 1;
   p.blocks = (int)((n + (int64_t)kSortThreads * p.rounds - 1) / ((int64_t)kSortThreads * p.rounds));
+  if (p.blocks < 1) p.blocks = 1;  // (clears the words' ranges where there are no tokens)
   p.chunks = (n + kRunRows - 1) / kRunRows;
   p.part_ld = (width + 3) / 4 * 4;
   size_t at = 0;
@@ -76,6 +80,7 @@ inline EmbedGradPlan plan_embed_grad(int64_t n, int64_t vocab, int64_t width) {
     p.places[i] = take(n * sizeof(uint32_t));
   }
   p.counts = take((size_t)p.blocks * kDigits * sizeof(uint32_t));
+  p.range = take((size_t)vocab * sizeof(int2));
   p.parts = take((size_t)p.chunks * 2 * p.part_ld * sizeof(float));
   p.bytes = at;
   return p;
@@ -228,7 +233,7 @@ struct LossPlan {
   size_t head, row_of, target, factor, lse, target_logit, counts, largest, stats, rows, weight, dz, dx_acc, dw_acc, losses, bytes;
 };
 
-constexpr int64_t kGatherBlock = 32, kCountBlock = 1024, kScanMost = 16384;
+constexpr int64_t kGatherBlock = 8, kCountBlock = 1024, kScanMost = 8192;
 constexpr int64_t kDirectRows = 128;
 
 // grid16: x lies on the 16-byte grid (its rows may be read in place); weight16: the weight does

@@ -18,46 +18,45 @@ namespace {
 
 constexpr float kLn2 = 0.69314718055994531f;
 
-// Eight elements of a row from column c on (zeros behind its end) -> the products' planes.
+// Eight elements of a row from column c on (zeros behind its end), on their way to the products' planes.
 template <int DT>
-__device__ __forceinline__ void lay_eight(const char* row, int64_t c, int64_t width, bool vec, uint16_t* to, int64_t plane) {
-  if constexpr (DT == MODA_HIP_FP32) {
-    float v[8];
-    const float* x = (const float*)row + c;
+struct Eight {
+  static constexpr int SIZE = DT == MODA_HIP_FP32 ? 2 : 1;
+  i32x4 v[SIZE];
+  __device__ __forceinline__ void load(const char* row, int64_t c, int64_t width, bool vec) {
     if (vec && c + 8 <= width) {
-      const f32x4 lo = *(const f32x4*)x, hi = *(const f32x4*)(x + 4);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        v[i] = lo[i];
-        v[4 + i] = hi[i];
+      for (int i = 0; i < SIZE; i++) v[i] = *(const i32x4*)(row + c * 2 * SIZE + 16 * i);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < SIZE; i++) v[i] = i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (c + i >= width) break;
+      if constexpr (SIZE == 2)
+        v[i >> 2][i & 3] = ((const int*)row)[c + i];
+      else
+        v[0][i >> 1] |= (int)((uint32_t)((const uint16_t*)row)[c + i] << (16 * (i & 1)));
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* to, int64_t plane) const {
+    if constexpr (SIZE == 2) {
+      uint16_t piece[8][3];
+#pragma unroll
+      for (int i = 0; i < 8; i++) three_pieces(__int_as_float(v[i >> 2][i & 3]), piece[i]);
+#pragma unroll
+      for (int k = 0; k < 3; k++) {
+        i32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = piece[2 * i][k] | piece[2 * i + 1][k] << 16;
+        *(i32x4*)(to + k * plane) = w;
       }
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = c + i < width ? x[i] : 0.f;
+      *(i32x4*)to = v[0];
     }
-    uint16_t piece[8][3];
-#pragma unroll
-    for (int i = 0; i < 8; i++) three_pieces(v[i], piece[i]);
-#pragma unroll
-    for (int k = 0; k < 3; k++) {
-      i32x4 w;
-#pragma unroll
-      for (int i = 0; i < 4; i++) w[i] = piece[2 * i][k] | piece[2 * i + 1][k] << 16;
-      *(i32x4*)(to + k * plane + c) = w;
-    }
-  } else {
-    const uint16_t* x = (const uint16_t*)row + c;
-    i32x4 w = {0, 0, 0, 0};
-    if (vec && c + 8 <= width) {
-      w = *(const i32x4*)x;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (c + i < width) w[i >> 1] |= (int)((uint32_t)x[i] << (16 * (i & 1)));
-    }
-    *(i32x4*)(to + c) = w;
   }
-}
+};
 
 // Sums of the workgroup's 256 threads, and their largest.
 __device__ __forceinline__ void over_block(int& a, int& b, int& largest) {
@@ -121,14 +120,25 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
     from = own * kCountBlock;
     upto = first;
   }
-  for (int64_t i = from + tid; i < upto; i += 256) {
-    const bool live = a.words.of(i) >= 0;
-    before += live && i < first;
-    if (!a.counts && live) {
-      all++;
-      e = max(e, size_of(a, i));
+  constexpr int AHEAD = 8;  // targets in flight
+  for (int64_t i0 = from + tid; i0 < upto; i0 += 256 * AHEAD) {
+    int word[AHEAD], size[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) {
+      const int64_t i = i0 + 256 * k;
+      word[k] = i < upto ? a.words.of(i) : -1;
+      size[k] = i < upto && a.d_loss_stride ? size_of(a, i) : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) {
+      before += word[k] >= 0 && i0 + 256 * k < first;
+      if (!a.counts && word[k] >= 0) {
+        all++;
+        e = max(e, size[k]);
+      }
     }
   }
+  if (a.d_loss && !a.d_loss_stride) e = size_of(a, 0);
   over_block(before, all, e);
   // The gradient of a logit is rounded to 16 bits.  The factor that rows share stays out of that, or its own rounding would be in all of them,
   // the same way: it is kept relative to the largest upstream gradient, which the products multiply by at their end.
@@ -153,18 +163,26 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
     }
   }
   __syncthreads();
-  const int64_t chunks = a.rows_ld / 8, out_chunks = (a.width + 7) / 8;
-  for (int64_t w = tid; w < kGatherBlock * chunks; w += 256) {
-    const int r = (int)(w / chunks);
-    const int64_t c = w - r * chunks, i = first + r;
-    if (i >= n) break;
+  constexpr int ES = DT == MODA_HIP_FP32 ? 4 : 2, COPIES = 4;  // (in flight)
+  const int chunks = (int)(a.rows_ld / 8), lane = tid & 63;
+  for (int r = tid >> 6; r < kGatherBlock && first + r < n; r += 4) {
+    const int64_t i = first + r;
     if (to[r] >= 0) {
-      lay_eight<DT>(a.x + i * a.ld_x * (DT == MODA_HIP_FP32 ? 4 : 2), c * 8, a.width, a.vec_x, a.rows + to[r] * a.rows_ld, a.rows_plane);
-    } else if (a.dx && c < out_chunks) {
-      char* row = a.dx + i * a.ld_dx * (DT == MODA_HIP_FP32 ? 4 : 2);
-      const float zeros[4] = {0.f, 0.f, 0.f, 0.f};
+      const char* row = a.x + i * a.ld_x * ES;
+      uint16_t* out = a.rows + to[r] * a.rows_ld;
+      for (int c0 = lane; c0 < chunks; c0 += 64 * COPIES) {
+        Eight<DT> x[COPIES];
 #pragma unroll
-      for (int h = 0; h < 2; h++) store_four<BF16, DT == MODA_HIP_FP32>(row, c * 8 + 4 * h, zeros, (int)min(a.width - c * 8 - 4 * h, (int64_t)4), a.vec_dx);
+        for (int k = 0; k < COPIES; k++)
+          if (c0 + 64 * k < chunks) x[k].load(row, (c0 + 64 * k) * 8, a.width, a.vec_x);
+#pragma unroll
+        for (int k = 0; k < COPIES; k++)
+          if (c0 + 64 * k < chunks) x[k].store(out + (c0 + 64 * k) * 8, a.rows_plane);
+      }
+    } else if (a.dx) {
+      const float zeros[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int64_t c = 4 * lane; c < a.width; c += 256)
+        store_four<BF16, DT == MODA_HIP_FP32>(a.dx + i * a.ld_dx * ES, c, zeros, (int)min(a.width - c, (int64_t)4), a.vec_dx);
     }
   }
 }
@@ -172,33 +190,45 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
 template <int DT>
 __global__ __launch_bounds__(256) void lay_rows_kernel(const LayArgs a) {
   const int64_t chunks = a.to_ld / 8, w = (int64_t)workgroup() * 256 + threadIdx.x, r = w / chunks, c = w - r * chunks;
-  if (r < a.rows) lay_eight<DT>(a.x + r * a.ld_x * (DT == MODA_HIP_FP32 ? 4 : 2), c * 8, a.width, a.vec, a.to + r * a.to_ld, a.to_plane);
+  if (r >= a.rows) return;
+  Eight<DT> x;
+  x.load(a.x + r * a.ld_x * (DT == MODA_HIP_FP32 ? 4 : 2), c * 8, a.width, a.vec);
+  x.store(a.to + r * a.to_ld + c * 8, a.to_plane);
 }
 
-// Sixteen lanes a row take every sixteenth tile of words each and meet in LDS, in a fixed order.
+// LANES lanes a row take every LANES-th tile of words each and meet in LDS, in a fixed order.
+template <int LANES>
 __global__ __launch_bounds__(256) void join_stats_kernel(const JoinStatsArgs a) {
-  __shared__ float largest[16][17], sum[16][17];
-  const int r = threadIdx.x & 15, part = threadIdx.x >> 4;
+  constexpr int ROWS = 256 / LANES, AHEAD = 4;
+  __shared__ float largest[LANES][ROWS + 1], sum[LANES][ROWS + 1];
+  const int r = threadIdx.x % ROWS, part = threadIdx.x / ROWS;
   const int rows = a.head ? a.head->live : (int)a.words.n;
-  const int64_t p = (int64_t)workgroup() * 16 + r;
+  const int64_t p = (int64_t)workgroup() * ROWS + r;
   float m = kNegInf, s = 0.f;
-  if (p < rows)
-    for (int64_t t = part; t < a.tiles; t += 16) {
-      const float2 x = a.stats[t * a.stats_ld + p];
-      if (x.x > m) {
-        s = s * fast_exp2(m - x.x) + x.y;
-        m = x.x;
-      } else {
-        s += x.x == kNegInf ? x.y : x.y * fast_exp2(x.x - m);  // (a sum of no logit above minus infinity is zero, or NaN)
-      }
+  const auto add = [](float& m, float& s, float xm, float xs) {  // (a sum of no logit above minus infinity is zero, or NaN)
+    if (xm > m) {
+      s = (m == kNegInf ? s : s * fast_exp2(m - xm)) + xs;
+      m = xm;
+    } else {
+      s += xm == kNegInf ? xs : xs * fast_exp2(xm - m);
     }
-  largest[part][r] = m;
-  sum[part][r] = s;
-  __syncthreads();
+  };
+  if (p < rows)
+    for (int64_t t0 = part; t0 < a.tiles; t0 += LANES * AHEAD) {
+      float2 x[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; k++) x[k] = t0 + LANES * k < a.tiles ? a.stats[(t0 + LANES * k) * a.stats_ld + p] : float2{kNegInf, 0.f};
+#pragma unroll
+      for (int k = 0; k < AHEAD; k++) add(m, s, x[k].x, x[k].y);
+    }
+  for (int half = LANES / 2; half > 0; half >>= 1) {
+    largest[part][r] = m;
+    sum[part][r] = s;
+    __syncthreads();
+    if (part < half) add(m, s, largest[part + half][r], sum[part + half][r]);
+    __syncthreads();
+  }
   if (part != 0 || p >= rows) return;
-  for (int i = 1; i < 16; i++) m = fmaxf(m, largest[i][r]);
-  s = 0.f;
-  for (int i = 0; i < 16; i++) s += largest[i][r] == kNegInf ? sum[i][r] : sum[i][r] * fast_exp2(largest[i][r] - m);
   const float log_sum = log2f(s);
   float lse = m + log_sum;
   const int word = a.head ? 0 : a.words.of(p);
@@ -277,7 +307,13 @@ hipError_t launch_grad_logits(const ProductArgs& a, int dtype, ProductTile tile,
   return launch_product<kGradLogits>(a, dtype, tile, stream);
 }
 hipError_t launch_join_stats(const JoinStatsArgs& a, hipStream_t stream) {
-  join_stats_kernel<<<grid_of((a.words.n + 15) / 16), 256, 0, stream>>>(a);
+  // lanes enough for one round of loads where there are few rows, coalesced loads where there are many
+  if (a.words.n <= 512)
+    join_stats_kernel<256><<<grid_of(a.words.n), 256, 0, stream>>>(a);
+  else if (a.words.n <= 8192)
+    join_stats_kernel<64><<<grid_of((a.words.n + 3) / 4), 256, 0, stream>>>(a);
+  else
+    join_stats_kernel<16><<<grid_of((a.words.n + 15) / 16), 256, 0, stream>>>(a);
   return hipGetLastError();
 }
 hipError_t launch_loss_total(const LossTotalArgs& a, hipStream_t stream) {
