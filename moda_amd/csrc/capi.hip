@@ -39,10 +39,10 @@ hipError_t launch_embed_rows(EmbedArgs& a, int dtype, bool vec, hipStream_t stre
 hipError_t launch_embed_grad(EmbedArgs& a, int dtype, bool vec, char* work, hipStream_t stream);
 hipError_t launch_gather_rows(const GatherArgs& a, int dtype, hipStream_t stream);
 hipError_t launch_lay_rows(const LayArgs& a, int dtype, hipStream_t stream);
-hipError_t launch_stats(const ProductArgs& a, int dtype, ProductTile tile, hipStream_t stream);
-hipError_t launch_grad_logits(const ProductArgs& a, int dtype, ProductTile tile, hipStream_t stream);
-hipError_t launch_grad_rows(const ProductArgs& a, int dtype, ProductTile tile, hipStream_t stream);
-hipError_t launch_grad_weight(const ProductArgs& a, int dtype, ProductTile tile, hipStream_t stream);
+hipError_t launch_stats(const ProductArgs& a, int dtype, ProductTile tile, int compute_units, hipStream_t stream);
+hipError_t launch_grad_logits(const ProductArgs& a, int dtype, ProductTile tile, int compute_units, hipStream_t stream);
+hipError_t launch_grad_rows(const ProductArgs& a, int dtype, ProductTile tile, int compute_units, hipStream_t stream);
+hipError_t launch_grad_weight(const ProductArgs& a, int dtype, ProductTile tile, int compute_units, hipStream_t stream);
 hipError_t launch_join_stats(const JoinStatsArgs& a, hipStream_t stream);
 hipError_t launch_loss_total(const LossTotalArgs& a, hipStream_t stream);
 hipError_t launch_join_sums(const JoinSumsArgs& a, int dtype, hipStream_t stream);
@@ -1012,6 +1012,7 @@ struct VocabLoss {
   char* work;
   hipStream_t stream;
   bool backward;
+  int compute_units;
   int es() const { return elem_size(t->dtype); }
   moda::LossHead* head() const { return p.direct ? nullptr : (moda::LossHead*)(work + p.head); }
   moda::Words words() const { return {t->targets, t->rows, t->vocab, t->ignore_index, t->targets64 != 0}; }
@@ -1113,7 +1114,7 @@ int begin_vocab_loss(const moda_hip_vocab_loss_args* t, bool backward, void* wor
   v.work = (char*)workspace;
   v.stream = (hipStream_t)stream;
   v.backward = backward;
-  return check_device();
+  return check_device(&v.compute_units);
 }
 }  // namespace
 
@@ -1138,7 +1139,7 @@ int moda_hip_vocab_loss_fwd(const moda_hip_vocab_loss_args* t, void* workspace, 
     a.stats = v.at<float2>(v.p.stats) + i * ((v.p.piece + tile - 1) / tile) * t->rows;
     a.stats_ld = t->rows;
     a.target_logit = v.at<float>(v.p.target_logit);
-    MODA_TRY(moda::launch_stats(a, t->dtype, v.p.logits.tile, v.stream));
+    MODA_TRY(moda::launch_stats(a, t->dtype, v.p.logits.tile, v.compute_units, v.stream));
   }
   const int64_t last = (v.piece_words(v.p.pieces - 1) + tile - 1) / tile;
   moda::JoinStatsArgs j = {v.at<float2>(v.p.stats), v.at<float>(v.p.target_logit), t->rows, (v.p.pieces - 1) * ((v.p.piece + tile - 1) / tile) + last,
@@ -1169,7 +1170,7 @@ int moda_hip_vocab_loss_bwd(const moda_hip_vocab_loss_args* t, void* workspace, 
     a.dz = v.at<uint16_t>(p.dz);
     a.dz_ld = p.dz_ld;
     a.dz_plane = t->rows * p.dz_ld;
-    MODA_TRY(moda::launch_grad_logits(a, t->dtype, p.logits.tile, v.stream));
+    MODA_TRY(moda::launch_grad_logits(a, t->dtype, p.logits.tile, v.compute_units, v.stream));
     if (t->dx) {
       moda::ProductArgs r = w;
       r.p = a.dz;
@@ -1193,7 +1194,7 @@ int moda_hip_vocab_loss_bwd(const moda_hip_vocab_loss_args* t, void* workspace, 
         r.out_ld = t->ld_dx;
         r.out_vec = by_four(t->dx, t->ld_dx);
       }
-      MODA_TRY(moda::launch_grad_rows(r, t->dtype, p.grad_rows.tile, v.stream));
+      MODA_TRY(moda::launch_grad_rows(r, t->dtype, p.grad_rows.tile, v.compute_units, v.stream));
     }
     if (t->d_weight) {
       char* out = (char*)t->d_weight + i * p.piece * t->ld_d_weight * es;
@@ -1218,7 +1219,7 @@ int moda_hip_vocab_loss_bwd(const moda_hip_vocab_loss_args* t, void* workspace, 
         g.acc_ld = p.acc_ld;
         g.acc_split = p.piece * p.acc_ld;
       }
-      MODA_TRY(moda::launch_grad_weight(g, t->dtype, p.grad_weight.tile, v.stream));
+      MODA_TRY(moda::launch_grad_weight(g, t->dtype, p.grad_weight.tile, v.compute_units, v.stream));
       if (g.splits > 1)
         MODA_TRY(moda::launch_join_sums({g.acc, g.acc_ld, g.acc_split, g.p_count, t->width, g.splits, v.head(), 0, nullptr, out, g.out_ld, g.out_vec, t->scale},
                                         t->dtype, v.stream));

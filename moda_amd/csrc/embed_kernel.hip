@@ -294,32 +294,37 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const EmbedArgs a) {
   }
 }
 
-// Runs longer than kRunRows, by the piece that they begin in (one at most; they reach its last place): the sum of their parts.
+// Runs longer than kRunRows, by the piece that they begin in (one at most; they reach its last place): the sum of their parts, four columns
+// a thread.
 template <typename E>
 __global__ __launch_bounds__(256) void embed_join_kernel(const EmbedArgs a) {
-  const int chunk = (int)workgroup(), p0 = chunk * kRunRows, p1 = min(p0 + kRunRows, (int)a.words.n);
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  const unsigned of_row = (unsigned)((a.part_ld + 1023) / 1024), block = workgroup();
+  const int chunk = (int)(block / of_row), p0 = chunk * kRunRows, p1 = min(p0 + kRunRows, (int)a.words.n);
   if (chunk >= a.chunks) return;
   const uint32_t k = a.keys[p1 - 1];
   if (k >= (uint32_t)a.words.vocab) return;
   const int2 run = a.range[k];
   if (run.x < p0 || run.y - run.x <= kRunRows) return;
   const int end = (run.y + kRunRows - 1) / kRunRows;  // pieces
-  typename E::bits* y = (typename E::bits*)a.y + (int64_t)k * a.ld_out;
-  for (int64_t c = threadIdx.x; c < a.width; c += 256) {
-    const float* part = a.parts + (2ll * chunk + (run.x > p0)) * a.part_ld + c;
-    float s = *part;
-    part = a.parts + 2ll * (chunk + 1) * a.part_ld + c;
-    int q = chunk + 1;
-    for (; q + 16 <= end; q += 16, part += 32 * a.part_ld) {
-      float v[16];
+  const int64_t c = (int64_t)(block % of_row) * 1024 + threadIdx.x * 4;
+  if (c >= a.width) return;
+  const float* part = a.parts + (2ll * chunk + (run.x > p0)) * a.part_ld + c;
+  f32x4 s = *(const f32x4*)part;
+  part = a.parts + 2ll * (chunk + 1) * a.part_ld + c;
+  int q = chunk + 1;
+  for (; q + 16 <= end; q += 16, part += 32 * a.part_ld) {
+    f32x4 v[16];
 #pragma unroll
-      for (int i = 0; i < 16; i++) v[i] = part[2 * i * a.part_ld];
+    for (int i = 0; i < 16; i++) v[i] = *(const f32x4*)(part + 2 * i * a.part_ld);
 #pragma unroll
-      for (int i = 0; i < 16; i++) s += v[i];
-    }
-    for (; q < end; q++, part += 2 * a.part_ld) s += *part;
-    y[c] = E::narrow(s * a.scale);
+    for (int i = 0; i < 16; i++) s += v[i];
   }
+  for (; q < end; q++, part += 2 * a.part_ld) s += *(const f32x4*)part;
+  typename E::bits* y = (typename E::bits*)a.y + (int64_t)k * a.ld_out;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (c + i < a.width) y[c + i] = E::narrow(s[i] * a.scale);
 }
 
 template <typename E, int VEC>
@@ -332,7 +337,7 @@ hipError_t grad_as(const EmbedArgs& a, bool through, int64_t blocks, hipStream_t
   through ? embed_grad_kernel<E, VEC, true><<<grid_of(blocks), 256, 0, stream>>>(a) : embed_grad_kernel<E, VEC, false><<<grid_of(blocks), 256, 0, stream>>>(a);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && a.chunks > 1) {
-    embed_join_kernel<E><<<grid_of(a.chunks), 256, 0, stream>>>(a);
+    embed_join_kernel<E><<<grid_of(a.chunks * ((a.part_ld + 1023) / 1024)), 256, 0, stream>>>(a);
     e = hipGetLastError();
   }
   return e;

@@ -145,129 +145,45 @@ __device__ __forceinline__ void store_four(char* out, int64_t at, const float (&
   }
 }
 
-// WF x WP waves share a tile of BF x BP, NST stages of LDS hold 64 k of both operands each.
-template <typename T, int BF, int BP, int WF, int WP, int NST, Product PROD, bool PLANES>
-__global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductArgs a) {
-  constexpr int NT = 64 * WF * WP, MB = BF / WF / 16, NB = BP / WP / 16, DIST = NST - 1, STAGE = (BF + BP) * 64;
-  constexpr bool FC = PROD == kGradRows || PROD == kGradWeight, PC = PROD == kGradWeight;  // operands with f or p innermost
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  lds_ptr smem = (lds_ptr)smem_raw;
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wf = wave % WF, wp = wave / WF;
-
-  int p_count = a.p_count, k_count = a.k_count;
-  float down = 1.f;
-  if (a.head) {
-    const int live = __builtin_amdgcn_readfirstlane(a.head->live);
-    if (PROD == kGradWeight)
-      k_count = live;
-    else
-      p_count = live;
-    if (PROD == kGradRows || PROD == kGradWeight) down = a.head->down;
-  }
-  // Which tile: the workgroups of one XCD (every eighth) have neighbouring ones, in columns of eight tiles of p through all f.
-  const int tiles_f = (a.f_count + BF - 1) / BF, tiles_p = (p_count + BP - 1) / BP;
-  const int split = blockIdx.y;
-  const int64_t tiles = (int64_t)tiles_f * tiles_p, of_xcd = (tiles + 7) / 8;
-  const int64_t id = (int64_t)(blockIdx.x & 7) * of_xcd + (blockIdx.x >> 3);
-  if ((int64_t)(blockIdx.x >> 3) >= of_xcd || id >= tiles) return;
-  const int band = (int)(id / (8ll * tiles_f)), in_band = (int)(id - band * 8ll * tiles_f);
-  const int band_p = tiles_p - 8 * band < 8 ? tiles_p - 8 * band : 8;
-  const int f0 = in_band / band_p * BF, p0 = (8 * band + in_band % band_p) * BP;
-
-  const int steps_all = (k_count + 63) / 64;
-  const int first = (int)((int64_t)steps_all * split / a.splits), steps = (int)((int64_t)steps_all * (split + 1) / a.splits) - first;
-  const int n_steps = PLANES ? 6 * steps : steps;
-
-  OperandLoader<FC, BF, NT> lf;
-  OperandLoader<PC, BP, NT> lp;
-  lf.init(tid, (int)a.f_ld * 2, a.f_count - f0);
-  lp.init(tid, (int)a.p_ld * 2, p_count - p0);
-  const uint16_t* fb = a.f + (FC ? (int64_t)f0 : (int64_t)f0 * a.f_ld);
-  const uint16_t* pb = a.p + (PC ? (int64_t)p0 : (int64_t)p0 * a.p_ld);
-
-  int ld_st = 0, ld_pair = 0, ld_step = 0;
-  auto issue = [&]() {
-    lds_ptr fs = smem + ld_st * STAGE;
-    const int k0 = (first + ld_step) * 64;
-    lf.load(fs, fb + (PLANES ? plane_f(ld_pair) * a.f_plane : 0), a.f_ld, k0, k_count);
-    lp.load(fs + BF * 64, pb + (PLANES ? plane_p(ld_pair) * a.p_plane : 0), a.p_ld, k0, k_count);
-    ld_st = (ld_st + 1 == NST) ? 0 : ld_st + 1;
-    if (++ld_step == steps && PLANES) {
-      ld_step = 0;
-      ld_pair++;
-    }
-  };
-  constexpr int LOADS = decltype(lf)::N + decltype(lp)::N;
-  typedef AsyncTileLoader<64, 64, 256> Wait;
-  auto wait_tile = [&](int next) {  // the loads of step `next` have landed
-    const int behind = n_steps - 1 - next;  // of later steps, up to DIST - 1 of which are on their way
-    if (DIST >= 3 && behind >= 2)
-      Wait::template wait_but<2 * LOADS <= 60 ? 2 * LOADS : 0>();
-    else if (DIST >= 2 && behind >= 1)
-      Wait::template wait_but<LOADS <= 60 ? LOADS : 0>();
-    else
-      Wait::wait_all();
-  };
-
-  TileOperand<FC, BF, MB> of;
-  TileOperand<PC, BP, NB> op;
-  of.init(lane, wf * MB);
-  op.init(lane, wp * NB);
-  f32x4 acc[MB][NB];
-#pragma unroll
-  for (int mb = 0; mb < MB; mb++)
-#pragma unroll
-    for (int nb = 0; nb < NB; nb++) acc[mb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-#pragma unroll
-  for (int j = 0; j < DIST; j++)
-    if (j < n_steps) issue();
-  wait_tile(0);
-  __syncthreads();
-  int st = 0;
-  for (int it = 0; it < n_steps; it++) {
-    if (it + DIST < n_steps) issue();
-    lds_cptr fs = smem + st * STAGE, ps = fs + BF * 64;
-#pragma unroll
-    for (int ks = 0; ks < 2; ks++) {
-      i32x4 fo[MB], po[NB];
-#pragma unroll
-      for (int mb = 0; mb < MB; mb++) fo[mb] = of.read(fs, ks, mb);
-#pragma unroll
-      for (int nb = 0; nb < NB; nb++) po[nb] = op.read(ps, ks, nb);
-#pragma unroll
-      for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-        for (int mb = 0; mb < MB; mb++) acc[mb][nb] = mfma16<T>(fo[mb], po[nb], acc[mb][nb]);
-    }
-    st = (st + 1 == NST) ? 0 : st + 1;
-    wait_tile(it + 1);
-    __syncthreads();
-  }
-
+// What is done with a tile's result.  `part`: LDS of [WF][BP] pairs (kStats).
+template <typename T, int BF, int BP, int WF, int WP, Product PROD, bool PLANES>
+__device__ __forceinline__ void finish(const ProductArgs& a, f32x4 (&acc)[BF / WF / 16][BP / WP / 16], MODA_LDS float* part, int f0, int p0, int split,
+                                       int p_count, float down, int wf, int wp, int tid) {
+  constexpr int NT = 64 * WF * WP, MB = BF / WF / 16, NB = BP / WP / 16;
+  constexpr bool FC = PROD == kGradRows || PROD == kGradWeight, PC = PROD == kGradWeight;
+  const int lane = tid & 63, n = lane & 15, q = lane >> 4;
   // four f from f_of(mb) on of p_of(nb)
-  auto f_of = [&](int mb) { return f0 + (wf * MB + mb) * 16 + (FC ? 4 * q : slot_base(q)); };
+  const int f_wave = f0 + wf * MB * 16;
+  auto f_of = [&](int mb) { return f_wave + mb * 16 + (FC ? 4 * q : slot_base(q)); };
   auto p_of = [&](int nb) { return p0 + (wp * NB + nb) * 16 + (PC ? n : slot_base(n >> 2) + (n & 3)); };
+  const bool last_f = f_wave + MB * 16 > a.f_count;  // some of the wave's f may be past the end
 
   if constexpr (PROD == kStats) {
-    MODA_LDS float* part = (MODA_LDS float*)smem;  // [WF][BP] pairs
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
       const int p = p_of(nb);
       int target = p < p_count ? (a.head ? a.target[p] : a.words.of(p)) - a.first_word : -1;
       if (target >= a.f_count) target = -1;  // of a later piece
+#pragma unroll
+      for (int mb = 0; mb < MB; mb++) acc[mb][nb] *= a.c;
+      if (last_f) {
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (f_of(mb) + i >= a.f_count) acc[mb][nb][i] = kNegInf;
+      }
+      if (__any((unsigned)(target - f_wave) < (unsigned)(MB * 16))) {
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (f_of(mb) + i == target) a.target_logit[p] = acc[mb][nb][i];
+      }
       float m = kNegInf;
 #pragma unroll
       for (int mb = 0; mb < MB; mb++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int f = f_of(mb) + i;
-          const float z = f < a.f_count ? acc[mb][nb][i] * a.c : kNegInf;
-          if (f == target) a.target_logit[p] = z;
-          acc[mb][nb][i] = z;
-          m = fmaxf(m, z);
-        }
+        m = fmaxf(fmaxf(fmaxf(m, acc[mb][nb][0]), acc[mb][nb][1]), fmaxf(acc[mb][nb][2], acc[mb][nb][3]));
       m = quad_max(m);
       const float ref = m == kNegInf ? 0.f : m;
       float s = 0.f;
@@ -293,6 +209,7 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
       for (int w = 0; w < WF; w++) s += part[2 * (w * BP + r) + 1] * fast_exp2((part[2 * (w * BP + r)] == kNegInf ? ref : part[2 * (w * BP + r)]) - ref);
       a.stats[(int64_t)(f0 / BF) * a.stats_ld + p0 + r] = float2{m, s};
     }
+    __syncthreads();  // (an item without steps brings no barrier of its own before `part` is written again)
   }
   if constexpr (PROD == kGradLogits) {
 #pragma unroll
@@ -302,14 +219,21 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
       const int target = there ? a.target[p] - a.first_word : -1;
       const float factor = there ? a.factor[p] : 0.f, lse = there ? a.lse[p] : 0.f;
 #pragma unroll
+      for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[mb][nb][i] = fast_exp2(acc[mb][nb][i] * a.c - lse);
+      if (__any((unsigned)(target - f_wave) < (unsigned)(MB * 16))) {
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[mb][nb][i] -= f_of(mb) + i == target ? 1.f : 0.f;
+      }
+#pragma unroll
       for (int mb = 0; mb < MB; mb++) {
         const int f = f_of(mb);
         float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float prob = fast_exp2(acc[mb][nb][i] * a.c - lse);
-          v[i] = f + i < a.f_count ? factor * (prob - (f + i == target ? 1.f : 0.f)) : 0.f;
-        }
+        for (int i = 0; i < 4; i++) v[i] = last_f && f + i >= a.f_count ? 0.f : factor * acc[mb][nb][i];
         if (!there || f >= a.dz_ld) continue;
         uint16_t* to = a.dz + (int64_t)p * a.dz_ld + f;
         if (PLANES) {
@@ -348,33 +272,170 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
   }
 }
 
+// WF x WP waves share a tile of BF x BP, NST stages of LDS hold 64 k of both operands each.  A workgroup stays and takes tile after tile (and
+// part after part of a split summation axis), so that the first loads of the next are on their way while a result leaves the registers: a
+// product of 32 steps otherwise spends a fifth of its time on starts and ends.
 template <typename T, int BF, int BP, int WF, int WP, int NST, Product PROD, bool PLANES>
-hipError_t launch_product_as(const ProductArgs& a, hipStream_t stream) {
+__global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductArgs a) {
+  constexpr int NT = 64 * WF * WP, MB = BF / WF / 16, NB = BP / WP / 16, DIST = NST - 1, STAGE = (BF + BP) * 64;
+  constexpr bool FC = PROD == kGradRows || PROD == kGradWeight, PC = PROD == kGradWeight;  // operands with f or p innermost
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  lds_ptr smem = (lds_ptr)smem_raw;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wf = wave % WF, wp = wave / WF;
+
+  int p_count = a.p_count, k_count = a.k_count, splits = a.splits;
+  float down = 1.f;
+  if (a.head) {
+    const int live = __builtin_amdgcn_readfirstlane(a.head->live);
+    if (PROD == kGradWeight)
+      k_count = live;
+    else
+      p_count = live;
+    if (PROD == kGradRows || PROD == kGradWeight) down = a.head->down;
+  }
+  // The workgroups of one XCD (every eighth) have neighbouring tiles at a time, of columns of eight tiles of p through all f.
+  const int tiles_f = (a.f_count + BF - 1) / BF, tiles_p = (p_count + BP - 1) / BP, tiles = tiles_f * tiles_p;
+  const int of_xcd = (tiles * splits + 7) >> 3, xcd = blockIdx.x & 7, at_once = gridDim.x >> 3;
+  const int item_end = min((xcd + 1) * of_xcd, tiles * splits), item_first = xcd * of_xcd + (int)(blockIdx.x >> 3);
+  if (item_first >= item_end) return;
+  const int steps_all = (k_count + 63) >> 6;
+
+  struct Item {
+    int f0, p0, split, first, steps;  // of the summation axis: its first step and how many (for each pair of planes)
+  };
+  auto item_of = [&](int item) {
+    Item t;
+    t.split = splits == 1 ? 0 : item / tiles;
+    const int id = item - t.split * tiles, band = id / (8 * tiles_f), in_band = id - band * 8 * tiles_f;
+    const int band_p = min(tiles_p - 8 * band, 8), f = in_band / band_p;
+    t.f0 = f * BF;
+    t.p0 = (8 * band + in_band - f * band_p) * BP;
+    t.first = (int)((int64_t)steps_all * t.split / splits);
+    t.steps = (int)((int64_t)steps_all * (t.split + 1) / splits) - t.first;
+    return t;
+  };
+
+  // the loads' side: DIST steps ahead
+  OperandLoader<FC, BF, NT> lf;
+  OperandLoader<PC, BP, NT> lp;
+  const uint16_t *fb = nullptr, *pb = nullptr;
+  int ld_st = 0, ld_pair = 0, ld_step = 0, ld_item = item_first, ld_first = 0, ld_steps = 0;
+  auto open = [&]() {
+    const Item t = item_of(ld_item);
+    lf.init(tid, (int)a.f_ld * 2, a.f_count - t.f0);
+    lp.init(tid, (int)a.p_ld * 2, p_count - t.p0);
+    fb = a.f + (FC ? (int64_t)t.f0 : (int64_t)t.f0 * a.f_ld);
+    pb = a.p + (PC ? (int64_t)t.p0 : (int64_t)t.p0 * a.p_ld);
+    ld_first = t.first;
+    ld_steps = t.steps;
+    ld_step = ld_pair = 0;
+  };
+  auto issue = [&]() {  // false: nothing is left to load
+    while (ld_step == ld_steps) {  // (an item may have no steps at all)
+      if (PLANES && ld_steps > 0 && ld_pair < 5) {
+        ld_pair++;
+        ld_step = 0;
+        break;
+      }
+      ld_item += at_once;
+      if (ld_item >= item_end) {
+        ld_item = item_end;
+        return false;
+      }
+      open();
+    }
+    lds_ptr fs = smem + ld_st * STAGE;
+    const int k0 = (ld_first + ld_step) * 64;
+    lf.load(fs, fb + (PLANES ? plane_f(ld_pair) * a.f_plane : 0), a.f_ld, k0, k_count);
+    lp.load(fs + BF * 64, pb + (PLANES ? plane_p(ld_pair) * a.p_plane : 0), a.p_ld, k0, k_count);
+    ld_st = (ld_st + 1 == NST) ? 0 : ld_st + 1;
+    ld_step++;
+    return true;
+  };
+  constexpr int LOADS = decltype(lf)::N + decltype(lp)::N;
+  typedef AsyncTileLoader<64, 64, 256> Wait;
+
+  TileOperand<FC, BF, MB> of;
+  TileOperand<PC, BP, NB> op;
+  of.init(lane, wf * MB);
+  op.init(lane, wp * NB);
+
+  open();
+  int ahead = 0;  // steps whose loads are sent and that are not worked on yet
+#pragma unroll
+  for (int j = 0; j < DIST; j++) ahead += issue();
+  if (DIST >= 2 && ahead >= 2)
+    Wait::template wait_but<LOADS>();
+  else
+    Wait::wait_all();
+  __syncthreads();
+  int st = 0;
+  for (int item = item_first; item < item_end; item += at_once) {
+    const Item t = item_of(item);
+    const int n_steps = PLANES ? 6 * t.steps : t.steps;
+    f32x4 acc[MB][NB];
+#pragma unroll
+    for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++) acc[mb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int it = 0; it < n_steps; it++) {
+      ahead += issue();
+      lds_cptr fs = smem + st * STAGE, ps = fs + BF * 64;
+#pragma unroll
+      for (int ks = 0; ks < 2; ks++) {
+        i32x4 fo[MB], po[NB];
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) fo[mb] = of.read(fs, ks, mb);
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) po[nb] = op.read(ps, ks, nb);
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+          for (int mb = 0; mb < MB; mb++) acc[mb][nb] = mfma16<T>(fo[mb], po[nb], acc[mb][nb]);
+      }
+      st = (st + 1 == NST) ? 0 : st + 1;
+      ahead--;
+      // the loads of the next step have landed; those of one behind it may be on their way, but for the first step of an item, where stores
+      // of the last result may be among what is counted
+      if (DIST >= 2 && ahead >= 2 && it > 0)
+        Wait::template wait_but<LOADS>();
+      else
+        Wait::wait_all();
+      __syncthreads();
+    }
+    finish<T, BF, BP, WF, WP, PROD, PLANES>(a, acc, (MODA_LDS float*)(smem + NST * STAGE), t.f0, t.p0, t.split, p_count, down, wf, wp, tid);
+  }
+}
+
+template <typename T, int BF, int BP, int WF, int WP, int NST, Product PROD, bool PLANES>
+hipError_t launch_product_as(const ProductArgs& a, int compute_units, hipStream_t stream) {
   static LdsAttrState state;
   const auto kernel = &product_kernel<T, BF, BP, WF, WP, NST, PROD, PLANES>;
-  const size_t lds = (size_t)NST * (BF + BP) * 128;
+  const size_t lds = (size_t)NST * (BF + BP) * 128 + (PROD == kStats ? WF * BP * 8 : 0);
   hipError_t e = allow_dynamic_lds(state, (const void*)kernel, lds);
   if (e != hipSuccess) return e;
-  const int64_t tiles = (int64_t)((a.f_count + BF - 1) / BF) * ((a.p_count + BP - 1) / BP), blocks = (tiles + 7) / 8 * 8;
-  if (blocks == 0) return hipSuccess;
-  if (blocks >= (1ll << 23)) return hipErrorInvalidValue;
-  kernel<<<dim3((unsigned)blocks, (unsigned)a.splits), 64 * WF * WP, lds, stream>>>(a);
+  const int64_t tiles = (int64_t)((a.f_count + BF - 1) / BF) * ((a.p_count + BP - 1) / BP) * a.splits;
+  if (tiles == 0) return hipSuccess;
+  if (tiles >= (1ll << 28)) return hipErrorInvalidValue;
+  const int64_t room = (int64_t)compute_units * (160 * 1024 / lds < 1 ? 1 : 160 * 1024 / lds) / 8 * 8, blocks = (tiles + 7) / 8 * 8;
+  kernel<<<(unsigned)(blocks < room || room == 0 ? blocks : room), 64 * WF * WP, lds, stream>>>(a);
   return hipGetLastError();
 }
 template <Product PROD, typename T, bool PLANES>
-hipError_t launch_product_of(const ProductArgs& a, ProductTile tile, hipStream_t stream) {
-  if (tile == kTileLarge) return launch_product_as<T, 256, 256, 2, 4, 2, PROD, PLANES>(a, stream);
-  if (tile == kTileMedium) return launch_product_as<T, 128, 128, 2, 2, 2, PROD, PLANES>(a, stream);
+hipError_t launch_product_of(const ProductArgs& a, ProductTile tile, int compute_units, hipStream_t stream) {
+  if (tile == kTileLarge) return launch_product_as<T, 256, 256, 2, 4, 2, PROD, PLANES>(a, compute_units, stream);
+  if (tile == kTileMedium) return launch_product_as<T, 128, 128, 2, 2, 2, PROD, PLANES>(a, compute_units, stream);
   if constexpr (PROD == kGradWeight)
     return hipErrorInvalidValue;  // (choose_tiling: its p are words)
   else
-    return launch_product_as<T, 128, 32, 4, 1, 3, PROD, PLANES>(a, stream);
+    return launch_product_as<T, 128, 32, 4, 1, 3, PROD, PLANES>(a, compute_units, stream);
 }
 template <Product PROD>
-hipError_t launch_product(const ProductArgs& a, int dtype, ProductTile tile, hipStream_t stream) {
-  if (dtype == MODA_HIP_FP32) return launch_product_of<PROD, BF16, true>(a, tile, stream);
-  if (dtype == MODA_HIP_FP16) return launch_product_of<PROD, FP16, false>(a, tile, stream);
-  return launch_product_of<PROD, BF16, false>(a, tile, stream);
+hipError_t launch_product(const ProductArgs& a, int dtype, ProductTile tile, int compute_units, hipStream_t stream) {
+  if (dtype == MODA_HIP_FP32) return launch_product_of<PROD, BF16, true>(a, tile, compute_units, stream);
+  if (dtype == MODA_HIP_FP16) return launch_product_of<PROD, FP16, false>(a, tile, compute_units, stream);
+  return launch_product_of<PROD, BF16, false>(a, tile, compute_units, stream);
 }
 
 }  // namespace moda

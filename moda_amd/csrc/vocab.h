@@ -233,7 +233,7 @@ struct LossPlan {
   size_t head, row_of, target, factor, lse, target_logit, counts, largest, stats, rows, weight, dz, dx_acc, dw_acc, losses, bytes;
 };
 
-constexpr int64_t kGatherBlock = 8, kCountBlock = 1024, kScanMost = 8192;
+constexpr int64_t kGatherBlock = 8, kCountBlock = 1024, kScanMost = 4096;
 constexpr int64_t kDirectRows = 128;
 
 // grid16: x lies on the 16-byte grid (its rows may be read in place); weight16: the weight does

@@ -302,9 +302,9 @@ hipError_t launch_lay_rows(const LayArgs& a, int dtype, hipStream_t stream) {
   MODA_BY_TYPE(lay_rows_kernel, dtype, blocks_for(a.rows * (a.to_ld / 8)), a);
   return hipGetLastError();
 }
-hipError_t launch_stats(const ProductArgs& a, int dtype, ProductTile tile, hipStream_t stream) { return launch_product<kStats>(a, dtype, tile, stream); }
-hipError_t launch_grad_logits(const ProductArgs& a, int dtype, ProductTile tile, hipStream_t stream) {
-  return launch_product<kGradLogits>(a, dtype, tile, stream);
+hipError_t launch_stats(const ProductArgs& a, int dtype, ProductTile tile, int compute_units, hipStream_t stream) { return launch_product<kStats>(a, dtype, tile, compute_units, stream); }
+hipError_t launch_grad_logits(const ProductArgs& a, int dtype, ProductTile tile, int compute_units, hipStream_t stream) {
+  return launch_product<kGradLogits>(a, dtype, tile, compute_units, stream);
 }
 hipError_t launch_join_stats(const JoinStatsArgs& a, hipStream_t stream) {
   // lanes enough for one round of loads where there are few rows, coalesced loads where there are many
