@@ -14,6 +14,8 @@
 // fp32 (PLANES): each operand as the sum of three bf16 (exact: 24 bits), of whose nine products the six largest are added up, the small
 // ones first; the others are below 2^-24 of the whole.  Six products of 16 bits are faster than one of the fp32 matrix instruction.
 #pragma once
+#include <type_traits>
+
 #include "../../include/moda_hip.h"
 #include "tile.h"
 #include "tile16.h"
@@ -46,18 +48,21 @@ struct ColumnLoader {
   static constexpr int N = Loader::N;
   static_assert(Loader::RPW * Loader::NW == 16, "a pass of the loads is sixteen rows");
   Loader l;
-  int voff;
+  i32x4 rs;
+  int voff, stride;
   __device__ __forceinline__ void init(int tid, int stride_bytes, int cols) {
     l.init(tid);
     const int r = l.row_in_pass, k = 8 * ((0x9C >> (2 * (r >> 2))) & 3) + (r & 3);  // slot_base(q) = 4 j  <=>  q = 0x9C >> 2 j
     voff = l.pads(cols) ? kPadOffset : k * stride_bytes + l.gchunk * 16;
+    stride = stride_bytes;
   }
   // rows [k0, k0 + 64) of `rows`, at `base`
-  __device__ __forceinline__ void load(lds_ptr tile, const uint16_t* base, int64_t ld, int k0, int rows) const {
-    const int left = rows - k0 < 64 ? rows - k0 : 64, stride_bytes = (int)ld * 2;
-    const i32x4 rs = rsrc_words(base + (int64_t)k0 * ld, left <= 0 ? 0u : (uint32_t)left * (uint32_t)stride_bytes);
-#pragma unroll
-    for (int i = 0; i < N; i++) lds_dma<16>(rs, lds_addr(tile + l.lds_elems(i)), voff, (32 * (i >> 1) + 4 * (i & 1)) * stride_bytes);
+  __device__ __forceinline__ void aim(const uint16_t* base, int64_t ld, int k0, int rows) {
+    const int left = rows - k0 < 64 ? rows - k0 : 64;
+    rs = rsrc_words(base + (int64_t)k0 * ld, left <= 0 ? 0u : (uint32_t)left * (uint32_t)stride);
+  }
+  __device__ __forceinline__ void load(lds_ptr tile, int i) const {  // the i-th of a wave's N
+    lds_dma<16>(rs, lds_addr(tile + l.lds_elems(i)), voff, (32 * (i >> 1) + 4 * (i & 1)) * stride);
   }
 };
 
@@ -67,19 +72,20 @@ struct RowLoader {
   typedef AsyncTileLoader<64, ROWS, NT> Loader;
   static constexpr int N = Loader::N;
   Loader l;
-  int voff, rows_bytes;
+  i32x4 rs;
+  int voff, now, stride, rows_bytes;
   __device__ __forceinline__ void init(int tid, int stride_bytes, int rows) {  // rows from the tile's first on
     l.init(tid);
     voff = l.row_in_pass * stride_bytes + l.gchunk * 16;
     rows_bytes = (rows < ROWS ? (rows < 0 ? 0 : rows) : ROWS) * stride_bytes;
+    stride = stride_bytes;
   }
   // columns [k0, k0 + 64) of `cols`, of the rows at `base`
-  __device__ __forceinline__ void load(lds_ptr tile, const uint16_t* base, int64_t ld, int k0, int cols) const {
-    const i32x4 rs = rsrc_words(base + k0, (uint32_t)rows_bytes);
-    const int v = l.pads(cols - k0) ? kPadOffset : voff;
-#pragma unroll
-    for (int i = 0; i < N; i++) lds_dma<16>(rs, lds_addr(tile + l.lds_elems(i)), v, l.rows_before(i) * (int)ld * 2);
+  __device__ __forceinline__ void aim(const uint16_t* base, int64_t, int k0, int cols) {
+    rs = rsrc_words(base + k0, cols > 0 ? (uint32_t)rows_bytes : 0u);
+    now = l.pads(cols - k0) ? kPadOffset : voff;
   }
+  __device__ __forceinline__ void load(lds_ptr tile, int i) const { lds_dma<16>(rs, lds_addr(tile + l.lds_elems(i)), now, l.rows_before(i) * stride); }
 };
 
 template <bool COLUMNS, int SIZE, int NT>
@@ -277,7 +283,7 @@ __device__ __forceinline__ void finish(const ProductArgs& a, f32x4 (&acc)[BF / W
 // product of 32 steps otherwise spends a fifth of its time on starts and ends.
 template <typename T, int BF, int BP, int WF, int WP, int NST, Product PROD, bool PLANES>
 __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductArgs a) {
-  constexpr int NT = 64 * WF * WP, MB = BF / WF / 16, NB = BP / WP / 16, DIST = NST - 1, STAGE = (BF + BP) * 64;
+  constexpr int NT = 64 * WF * WP, MB = BF / WF / 16, NB = BP / WP / 16, STAGE = (BF + BP) * 64;
   constexpr bool FC = PROD == kGradRows || PROD == kGradWeight, PC = PROD == kGradWeight;  // operands with f or p innermost
   extern __shared__ __align__(16) unsigned char smem_raw[];
   lds_ptr smem = (lds_ptr)smem_raw;
@@ -316,7 +322,7 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
     return t;
   };
 
-  // the loads' side: DIST steps ahead
+  // the loads' side: NST steps ahead
   OperandLoader<FC, BF, NT> lf;
   OperandLoader<PC, BP, NT> lp;
   const uint16_t *fb = nullptr, *pb = nullptr;
@@ -331,81 +337,111 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
     ld_steps = t.steps;
     ld_step = ld_pair = 0;
   };
-  auto issue = [&]() {  // false: nothing is left to load
-    while (ld_step == ld_steps) {  // (an item may have no steps at all)
+  // The next step's loads are aimed; behind the last step at nothing, which fills their place with zeros: no branch in what is timed.
+  auto aim = [&]() {
+    while (ld_step == ld_steps && ld_item < item_end) {  // (an item may have no steps at all)
       if (PLANES && ld_steps > 0 && ld_pair < 5) {
         ld_pair++;
         ld_step = 0;
         break;
       }
       ld_item += at_once;
-      if (ld_item >= item_end) {
-        ld_item = item_end;
-        return false;
-      }
-      open();
+      if (ld_item < item_end) open();
     }
-    lds_ptr fs = smem + ld_st * STAGE;
-    const int k0 = (ld_first + ld_step) * 64;
-    lf.load(fs, fb + (PLANES ? plane_f(ld_pair) * a.f_plane : 0), a.f_ld, k0, k_count);
-    lp.load(fs + BF * 64, pb + (PLANES ? plane_p(ld_pair) * a.p_plane : 0), a.p_ld, k0, k_count);
-    ld_st = (ld_st + 1 == NST) ? 0 : ld_st + 1;
-    ld_step++;
-    return true;
+    const bool more = ld_item < item_end;
+    const int k0 = more ? (ld_first + ld_step) * 64 : 0;
+    lf.aim(fb + (PLANES ? plane_f(ld_pair) * a.f_plane : 0), a.f_ld, k0, more ? k_count : 0);
+    lp.aim(pb + (PLANES ? plane_p(ld_pair) * a.p_plane : 0), a.p_ld, k0, more ? k_count : 0);
+    ld_step += more;
   };
-  constexpr int LOADS = decltype(lf)::N + decltype(lp)::N;
+  constexpr int LOADS_F = decltype(lf)::N, LOADS = LOADS_F + decltype(lp)::N;
+  auto send = [&](int i) {
+    lds_ptr to = smem + ld_st * STAGE;
+    if (i < LOADS_F)
+      lf.load(to, i);
+    else
+      lp.load(to + BF * 64, i - LOADS_F);
+  };
+  auto sent = [&]() { ld_st = (ld_st + 1 == NST) ? 0 : ld_st + 1; };
   typedef AsyncTileLoader<64, 64, 256> Wait;
 
   TileOperand<FC, BF, MB> of;
   TileOperand<PC, BP, NB> op;
   of.init(lane, wf * MB);
   op.init(lane, wp * NB);
+  // A wave's operands of half a step (32 k), read from LDS while the products of the half before are on the matrix pipe: one read between two
+  // products, in the order of use.
+  struct Half {
+    i32x4 f[MB], p[NB];
+  };
+  auto read = [&](Half& h, lds_cptr tile, int ks, int i) {
+    if (i == 0)
+      h.p[0] = op.read(tile + BF * 64, ks, 0);
+    else if (i <= MB)
+      h.f[i - 1] = of.read(tile, ks, i - 1);
+    else
+      h.p[i - MB] = op.read(tile + BF * 64, ks, i - MB);
+  };
+  constexpr int READS = MB + NB, PRODUCTS = MB * NB, APART = PRODUCTS / READS > 2 ? 2 : 1;
+  f32x4 acc[MB][NB];
+  // products of `now`, reads of `next` among them, and the loads of a step to come
+  auto half_step = [&](const Half& now, Half& next, lds_cptr tile, int ks, auto loads) {
+#pragma unroll
+    for (int j = 0; j < PRODUCTS; j++) {
+      if (j % APART == 0 && j / APART < READS) read(next, tile, ks, j / APART);
+      if (j == PRODUCTS - 1)
+#pragma unroll
+        for (int i = (PRODUCTS + APART - 1) / APART; i < READS; i++) read(next, tile, ks, i);
+      acc[j % MB][j / MB] = mfma16<T>(now.f[j % MB], now.p[j / MB], acc[j % MB][j / MB]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (decltype(loads)::value) {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++)
+          if (j == i * PRODUCTS / LOADS) send(i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
 
   open();
-  int ahead = 0;  // steps whose loads are sent and that are not worked on yet
 #pragma unroll
-  for (int j = 0; j < DIST; j++) ahead += issue();
-  if (DIST >= 2 && ahead >= 2)
-    Wait::template wait_but<LOADS>();
-  else
-    Wait::wait_all();
+  for (int j = 0; j < NST; j++) {
+    aim();
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) send(i);
+    sent();
+  }
+  Wait::wait_all();
   __syncthreads();
   int st = 0;
+  Half h0, h1;
+#pragma unroll
+  for (int i = 0; i < READS; i++) read(h0, smem, 0, i);
   for (int item = item_first; item < item_end; item += at_once) {
     const Item t = item_of(item);
     const int n_steps = PLANES ? 6 * t.steps : t.steps;
-    f32x4 acc[MB][NB];
 #pragma unroll
     for (int mb = 0; mb < MB; mb++)
 #pragma unroll
       for (int nb = 0; nb < NB; nb++) acc[mb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int it = 0; it < n_steps; it++) {
-      ahead += issue();
-      lds_cptr fs = smem + st * STAGE, ps = fs + BF * 64;
-#pragma unroll
-      for (int ks = 0; ks < 2; ks++) {
-        i32x4 fo[MB], po[NB];
-#pragma unroll
-        for (int mb = 0; mb < MB; mb++) fo[mb] = of.read(fs, ks, mb);
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++) po[nb] = op.read(ps, ks, nb);
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-          for (int mb = 0; mb < MB; mb++) acc[mb][nb] = mfma16<T>(fo[mb], po[nb], acc[mb][nb]);
-      }
+      lds_cptr tile = smem + st * STAGE;
+      half_step(h0, h1, tile, 1, std::false_type());
       st = (st + 1 == NST) ? 0 : st + 1;
-      ahead--;
-      // the loads of the next step have landed; those of one behind it may be on their way, but for the first step of an item, where stores
-      // of the last result may be among what is counted
-      if (DIST >= 2 && ahead >= 2 && it > 0)
-        Wait::template wait_but<LOADS>();
+      // the loads of the next step have landed (of those behind it too where stores of the result before are counted with them)
+      if (NST > 2 && it > 0)
+        Wait::template wait_but<(NST - 2) * LOADS>();
       else
         Wait::wait_all();
-      __syncthreads();
+      __syncthreads();  // every wave has read this step's tile, whose place the loads may have now, and sees the next one
+      lds_cptr next = smem + st * STAGE;  // (behind the last step: what is there, for nothing)
+      aim();
+      half_step(h1, h0, next, 0, std::true_type());
+      sent();
     }
     finish<T, BF, BP, WF, WP, PROD, PLANES>(a, acc, (MODA_LDS float*)(smem + NST * STAGE), t.f0, t.p0, t.split, p_count, down, wf, wp, tid);
   }
+  Wait::wait_all();  // no load outlives its workgroup's LDS
 }
 
 template <typename T, int BF, int BP, int WF, int WP, int NST, Product PROD, bool PLANES>
