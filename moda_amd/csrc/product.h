@@ -14,8 +14,6 @@
 // fp32 (PLANES): each operand as the sum of three bf16 (exact: 24 bits), of whose nine products the six largest are added up, the small
 // ones first; the others are below 2^-24 of the whole.  Six products of 16 bits are faster than one of the fp32 matrix instruction.
 #pragma once
-#include <type_traits>
-
 #include "../../include/moda_hip.h"
 #include "tile.h"
 #include "tile16.h"
@@ -41,6 +39,8 @@ __device__ __forceinline__ void three_pieces(float x, uint16_t (&piece)[3]) {
 __device__ __forceinline__ int plane_f(int i) { return (0x201100 >> (4 * (5 - i))) & 15; }
 __device__ __forceinline__ int plane_p(int i) { return (0x021010 >> (4 * (5 - i))) & 15; }
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // Rows of k of a tile whose columns are f or p: in LDS row r of a sixteen lies the k that the transposed read takes from there.
 template <int COLS, int NT>
 struct ColumnLoader {
@@ -50,16 +50,23 @@ struct ColumnLoader {
   Loader l;
   i32x4 rs;
   int voff, stride;
-  __device__ __forceinline__ void init(int tid, int stride_bytes, int cols) {
+  uint64_t at;   // of the next step's first row
+  int64_t step;  // bytes
+  __device__ __forceinline__ void begin(int tid, int64_t ld) {
     l.init(tid);
-    const int r = l.row_in_pass, k = 8 * ((0x9C >> (2 * (r >> 2))) & 3) + (r & 3);  // slot_base(q) = 4 j  <=>  q = 0x9C >> 2 j
-    voff = l.pads(cols) ? kPadOffset : k * stride_bytes + l.gchunk * 16;
-    stride = stride_bytes;
+    stride = (int)ld * 2;
+    step = 64 * (int64_t)stride;
   }
-  // rows [k0, k0 + 64) of `rows`, at `base`
-  __device__ __forceinline__ void aim(const uint16_t* base, int64_t ld, int k0, int rows) {
-    const int left = rows - k0 < 64 ? rows - k0 : 64;
-    rs = rsrc_words(base + (int64_t)k0 * ld, left <= 0 ? 0u : (uint32_t)left * (uint32_t)stride);
+  // columns f0 .. of `cols`, rows from k0 on
+  __device__ __forceinline__ void open(const uint16_t* p, int f0, int cols, int64_t ld, int k0) {
+    const int r = l.row_in_pass, k = 8 * ((0x9C >> (2 * (r >> 2))) & 3) + (r & 3);  // slot_base(q) = 4 j  <=>  q = 0x9C >> 2 j
+    voff = l.pads(cols - f0) ? kPadOffset : k * stride + l.gchunk * 16;
+    at = (uint64_t)(p + f0 + k0 * ld);
+  }
+  // the next 64 rows, of which `left` are there
+  __device__ __forceinline__ void aim(int left) {
+    rs = rsrc_words((const void*)at, (uint32_t)max(min(left, 64), 0) * (uint32_t)stride);
+    at += step;
   }
   __device__ __forceinline__ void load(lds_ptr tile, int i) const {  // the i-th of a wave's N
     lds_dma<16>(rs, lds_addr(tile + l.lds_elems(i)), voff, (32 * (i >> 1) + 4 * (i & 1)) * stride);
@@ -73,17 +80,23 @@ struct RowLoader {
   static constexpr int N = Loader::N;
   Loader l;
   i32x4 rs;
-  int voff, now, stride, rows_bytes;
-  __device__ __forceinline__ void init(int tid, int stride_bytes, int rows) {  // rows from the tile's first on
+  int voff, now, stride, bytes;
+  uint64_t at;
+  __device__ __forceinline__ void begin(int tid, int64_t ld) {
     l.init(tid);
-    voff = l.row_in_pass * stride_bytes + l.gchunk * 16;
-    rows_bytes = (rows < ROWS ? (rows < 0 ? 0 : rows) : ROWS) * stride_bytes;
-    stride = stride_bytes;
+    stride = (int)ld * 2;
+    voff = l.row_in_pass * stride + l.gchunk * 16;
   }
-  // columns [k0, k0 + 64) of `cols`, of the rows at `base`
-  __device__ __forceinline__ void aim(const uint16_t* base, int64_t, int k0, int cols) {
-    rs = rsrc_words(base + k0, cols > 0 ? (uint32_t)rows_bytes : 0u);
-    now = l.pads(cols - k0) ? kPadOffset : voff;
+  // rows f0 .. of `rows`, columns from k0 on
+  __device__ __forceinline__ void open(const uint16_t* p, int f0, int rows, int64_t ld, int k0) {
+    bytes = max(min(rows - f0, ROWS), 0) * stride;
+    at = (uint64_t)(p + f0 * ld + k0);
+  }
+  // the next 64 columns, of which `left` are there
+  __device__ __forceinline__ void aim(int left) {
+    rs = rsrc_words((const void*)at, left > 0 ? (uint32_t)bytes : 0u);
+    now = l.pads(left) ? kPadOffset : voff;
+    at += 128;
   }
   __device__ __forceinline__ void load(lds_ptr tile, int i) const { lds_dma<16>(rs, lds_addr(tile + l.lds_elems(i)), now, l.rows_before(i) * stride); }
 };
@@ -305,54 +318,51 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
   const int of_xcd = (tiles * splits + 7) >> 3, xcd = blockIdx.x & 7, at_once = gridDim.x >> 3;
   const int item_end = min((xcd + 1) * of_xcd, tiles * splits), item_first = xcd * of_xcd + (int)(blockIdx.x >> 3);
   if (item_first >= item_end) return;
-  const int steps_all = (k_count + 63) >> 6;
+  const int steps_all = (k_count + 63) >> 6, steps_of_split = splits == 1 ? steps_all : uniform(steps_all / splits);
 
   struct Item {
     int f0, p0, split, first, steps;  // of the summation axis: its first step and how many (for each pair of planes)
   };
   auto item_of = [&](int item) {
     Item t;
-    t.split = splits == 1 ? 0 : item / tiles;
-    const int id = item - t.split * tiles, band = id / (8 * tiles_f), in_band = id - band * 8 * tiles_f;
-    const int band_p = min(tiles_p - 8 * band, 8), f = in_band / band_p;
+    t.split = splits == 1 ? 0 : uniform(item / tiles);
+    const int id = item - t.split * tiles, band = uniform(id / (8 * tiles_f)), in_band = id - band * 8 * tiles_f;
+    const int band_p = min(tiles_p - 8 * band, 8), f = uniform(in_band / band_p);
     t.f0 = f * BF;
     t.p0 = (8 * band + in_band - f * band_p) * BP;
-    t.first = (int)((int64_t)steps_all * t.split / splits);
-    t.steps = (int)((int64_t)steps_all * (t.split + 1) / splits) - t.first;
+    const int part = steps_of_split, more = steps_all - part * splits;  // the first `more` parts have a step more
+    t.first = t.split * part + min(t.split, more);
+    t.steps = part + (t.split < more);
     return t;
   };
 
   // the loads' side: NST steps ahead
   OperandLoader<FC, BF, NT> lf;
   OperandLoader<PC, BP, NT> lp;
-  const uint16_t *fb = nullptr, *pb = nullptr;
-  int ld_st = 0, ld_pair = 0, ld_step = 0, ld_item = item_first, ld_first = 0, ld_steps = 0;
-  auto open = [&]() {
-    const Item t = item_of(ld_item);
-    lf.init(tid, (int)a.f_ld * 2, a.f_count - t.f0);
-    lp.init(tid, (int)a.p_ld * 2, p_count - t.p0);
-    fb = a.f + (FC ? (int64_t)t.f0 : (int64_t)t.f0 * a.f_ld);
-    pb = a.p + (PC ? (int64_t)t.p0 : (int64_t)t.p0 * a.p_ld);
-    ld_first = t.first;
-    ld_steps = t.steps;
-    ld_step = ld_pair = 0;
-  };
+  lf.begin(tid, a.f_ld);
+  lp.begin(tid, a.p_ld);
+  int ld_st = 0, ld_item = item_first - at_once, ld_pair = 5, ld_steps = 0, ld_left = 0;  // steps of the item (or pair of planes) to come, k that are there
   // The next step's loads are aimed; behind the last step at nothing, which fills their place with zeros: no branch in what is timed.
   auto aim = [&]() {
-    while (ld_step == ld_steps && ld_item < item_end) {  // (an item may have no steps at all)
-      if (PLANES && ld_steps > 0 && ld_pair < 5) {
-        ld_pair++;
-        ld_step = 0;
-        break;
+    while (ld_steps == 0 && ld_item < item_end) {  // (an item may have no steps at all)
+      ld_pair++;
+      if (!PLANES || ld_pair == 6) {
+        ld_pair = 0;
+        ld_item += at_once;
+        if (ld_item >= item_end) break;
       }
-      ld_item += at_once;
-      if (ld_item < item_end) open();
+      const Item t = item_of(ld_item);
+      const int k0 = t.first * 64;
+      lf.open(a.f + (PLANES ? plane_f(ld_pair) * a.f_plane : 0), t.f0, a.f_count, a.f_ld, k0);
+      lp.open(a.p + (PLANES ? plane_p(ld_pair) * a.p_plane : 0), t.p0, p_count, a.p_ld, k0);
+      ld_steps = t.steps;
+      ld_left = k_count - k0;
     }
-    const bool more = ld_item < item_end;
-    const int k0 = more ? (ld_first + ld_step) * 64 : 0;
-    lf.aim(fb + (PLANES ? plane_f(ld_pair) * a.f_plane : 0), a.f_ld, k0, more ? k_count : 0);
-    lp.aim(pb + (PLANES ? plane_p(ld_pair) * a.p_plane : 0), a.p_ld, k0, more ? k_count : 0);
-    ld_step += more;
+    if (ld_item >= item_end) ld_left = 0;
+    lf.aim(ld_left);
+    lp.aim(ld_left);
+    ld_left -= 64;
+    ld_steps--;
   };
   constexpr int LOADS_F = decltype(lf)::N, LOADS = LOADS_F + decltype(lp)::N;
   auto send = [&](int i) {
@@ -382,10 +392,10 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
     else
       h.p[i - MB] = op.read(tile + BF * 64, ks, i - MB);
   };
-  constexpr int READS = MB + NB, PRODUCTS = MB * NB, APART = PRODUCTS / READS > 2 ? 2 : 1;
+  constexpr int READS = MB + NB, PRODUCTS = MB * NB, APART = PRODUCTS / READS > 2 ? 2 : 1, APART2 = PRODUCTS >= 2 * LOADS ? 2 : 1;
   f32x4 acc[MB][NB];
-  // products of `now`, reads of `next` among them, and the loads of a step to come
-  auto half_step = [&](const Half& now, Half& next, lds_cptr tile, int ks, auto loads) {
+  // products of `now`, reads of `next` among them, and `others(j)` behind the j-th product
+  auto half_step = [&](const Half& now, Half& next, lds_cptr tile, int ks, auto others) {
 #pragma unroll
     for (int j = 0; j < PRODUCTS; j++) {
       if (j % APART == 0 && j / APART < READS) read(next, tile, ks, j / APART);
@@ -394,16 +404,10 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
         for (int i = (PRODUCTS + APART - 1) / APART; i < READS; i++) read(next, tile, ks, i);
       acc[j % MB][j / MB] = mfma16<T>(now.f[j % MB], now.p[j / MB], acc[j % MB][j / MB]);
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (decltype(loads)::value) {
-#pragma unroll
-        for (int i = 0; i < LOADS; i++)
-          if (j == i * PRODUCTS / LOADS) send(i);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      others(j);
     }
   };
 
-  open();
 #pragma unroll
   for (int j = 0; j < NST; j++) {
     aim();
@@ -426,7 +430,9 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
       for (int nb = 0; nb < NB; nb++) acc[mb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int it = 0; it < n_steps; it++) {
       lds_cptr tile = smem + st * STAGE;
-      half_step(h0, h1, tile, 1, std::false_type());
+      half_step(h0, h1, tile, 1, [&](int j) {
+        if (j == PRODUCTS * 3 / 4) aim();
+      });
       st = (st + 1 == NST) ? 0 : st + 1;
       // the loads of the next step have landed (of those behind it too where stores of the result before are counted with them)
       if (NST > 2 && it > 0)
@@ -435,8 +441,12 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
         Wait::wait_all();
       __syncthreads();  // every wave has read this step's tile, whose place the loads may have now, and sees the next one
       lds_cptr next = smem + st * STAGE;  // (behind the last step: what is there, for nothing)
-      aim();
-      half_step(h1, h0, next, 0, std::true_type());
+      half_step(h1, h0, next, 0, [&](int j) {  // the loads: as early as may be
+#pragma unroll
+        for (int i = 0; i < LOADS; i++)
+          if (j == (i * APART2 < PRODUCTS ? i * APART2 : PRODUCTS - 1)) send(i);
+        __builtin_amdgcn_sched_barrier(0);
+      });
       sent();
     }
     finish<T, BF, BP, WF, WP, PROD, PLANES>(a, acc, (MODA_LDS float*)(smem + NST * STAGE), t.f0, t.p0, t.split, p_count, down, wf, wp, tid);
