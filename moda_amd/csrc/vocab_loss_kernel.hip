@@ -273,8 +273,17 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const JoinSumsArgs a) {
   const int64_t rows = a.head && a.by_head ? a.head->live : a.rows;
   if (p >= rows) return;
   const float* from = a.acc + p * a.acc_ld + f;
-  f32x4 s = *(const f32x4*)from;
-  for (int i = 1; i < a.splits; i++) s += *(const f32x4*)(from + i * a.acc_split);
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  int i = 0;
+  for (; i + 8 <= a.splits; i += 8) {
+    f32x4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = *(const f32x4*)(from + (i + k) * a.acc_split);
+#pragma unroll
+    for (int k = 0; k < 8; k++) s += v[k];
+  }
+#pragma unroll 4
+  for (; i < a.splits; i++) s += *(const f32x4*)(from + i * a.acc_split);
   const float scale = a.scale * a.head->down;
   const float v[4] = {s[0] * scale, s[1] * scale, s[2] * scale, s[3] * scale};
   store_four<T, FP32_OUT>(a.out, (a.by_head ? a.row_of[p] : p) * a.out_ld + f, v, (int)min(a.width - f, (int64_t)4), a.out_vec);
