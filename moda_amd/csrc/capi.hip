@@ -1052,6 +1052,13 @@ struct VocabLoss {
       a.ld_dx = t->ld_dx;
       a.vec_dx = on_grid(t->dx, t->ld_dx, es());
       a.mean = t->reduction == MODA_HIP_LOSS_MEAN;
+      if (p.acc_rows) {
+        const moda::TileTimes& k = moda::kTileTimes[p.grad_rows.tile];
+        const int per_unit = k.at_once > 256 ? 2 : 1;
+        a.rule = {moda::tile_p(k.tile), (int)((p.rows_ld + moda::tile_f(k.tile) - 1) / moda::tile_f(k.tile)),
+                  (int)((p.piece + 63) / 64 * (p.planes == 3 ? 6 : 1)), compute_units * per_unit, p.grad_rows.splits,
+                  (float)k.step_us, (float)k.end_us, (float)(t->width * 8 / 5e6)};
+      }
       a.up = t->dtype == MODA_HIP_FP16 ? 0x1p14f : 1.f;  // (fp16: probabilities down to 2^-28 have all their bits)
     }
     return moda::launch_gather_rows(a, t->dtype, stream);
@@ -1160,6 +1167,7 @@ int moda_hip_vocab_loss_bwd(const moda_hip_vocab_loss_args* t, void* workspace, 
   const moda::LossPlan& p = v.p;
   // four results of a row are stored as one where they lie on that grid
   const auto by_four = [&](const void* at, int64_t ld) { return (uintptr_t)at % (4 * es) == 0 && ld % 4 == 0; };
+  const auto by_eight = [&](const void* at, int64_t ld) { return es == 2 && (uintptr_t)at % 16 == 0 && ld % 8 == 0 && t->width % 8 == 0; };
   MODA_TRY(v.gather());
   for (int64_t i = 0; i < p.pieces; i++) {
     moda::ProductArgs w = {};
@@ -1193,6 +1201,7 @@ int moda_hip_vocab_loss_bwd(const moda_hip_vocab_loss_args* t, void* workspace, 
         r.out = (char*)t->dx;
         r.out_ld = t->ld_dx;
         r.out_vec = by_four(t->dx, t->ld_dx);
+        r.out_by_eight = by_eight(t->dx, t->ld_dx);
       }
       MODA_TRY(moda::launch_grad_rows(r, t->dtype, p.grad_rows.tile, v.compute_units, v.stream));
     }
@@ -1214,6 +1223,7 @@ int moda_hip_vocab_loss_bwd(const moda_hip_vocab_loss_args* t, void* workspace, 
       g.out = out;
       g.out_ld = t->ld_d_weight;
       g.out_vec = by_four(out, t->ld_d_weight);
+      g.out_by_eight = by_eight(out, t->ld_d_weight);
       if (g.splits > 1) {
         g.acc = v.at<float>(p.dw_acc);
         g.acc_ld = p.acc_ld;

@@ -164,10 +164,33 @@ __device__ __forceinline__ void store_four(char* out, int64_t at, const float (&
   }
 }
 
+// The results of two neighbouring blocks of sixteen f, four f a lane as they leave the matrix instruction, rounded -> eight neighbouring f a lane:
+// those of block q >> 1 from 8 (q & 1) on.  A store then writes 64 bytes of a row, not 32.  COLUMNS: lane group q had f 4 q .., else slot_base(q) ..
+template <bool COLUMNS>
+__device__ __forceinline__ i32x4 eight_of(i32x2 a, i32x2 b, int q) {
+  i32x4 r;
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const auto half = __builtin_amdgcn_permlane32_swap(a[i], b[i], false, false);  // {a 0, a 1, b 0, b 1}, {a 2, a 3, b 2, b 3}
+    if (COLUMNS) {
+      const auto row = __builtin_amdgcn_permlane16_swap(half[0], half[1], false, false);  // {a 0, a 2, b 0, b 2}, {a 1, a 3, b 1, b 3}
+      r[i] = row[0];
+      r[2 + i] = row[1];
+    } else {  // a 0 and a 3 are neighbours, a 1 and a 2
+      const auto row = __builtin_amdgcn_permlane16_swap(half[1], half[1], false, false);
+      r[i] = half[0];
+      r[2 + i] = q & 1 ? row[0] : row[1];
+    }
+  }
+#endif
+  return r;
+}
+
 // What is done with a tile's result.  `part`: LDS of [WF][BP] pairs (kStats).
 template <typename T, int BF, int BP, int WF, int WP, Product PROD, bool PLANES>
 __device__ __forceinline__ void finish(const ProductArgs& a, f32x4 (&acc)[BF / WF / 16][BP / WP / 16], MODA_LDS float* part, int f0, int p0, int split,
-                                       int p_count, float down, int wf, int wp, int tid) {
+                                       int64_t acc_split, int p_count, float down, int wf, int wp, int tid) {
   constexpr int NT = 64 * WF * WP, MB = BF / WF / 16, NB = BP / WP / 16;
   constexpr bool FC = PROD == kGradRows || PROD == kGradWeight, PC = PROD == kGradWeight;
   const int lane = tid & 63, n = lane & 15, q = lane >> 4;
@@ -248,22 +271,30 @@ __device__ __forceinline__ void finish(const ProductArgs& a, f32x4 (&acc)[BF / W
           for (int i = 0; i < 4; i++) acc[mb][nb][i] -= f_of(mb) + i == target ? 1.f : 0.f;
       }
 #pragma unroll
-      for (int mb = 0; mb < MB; mb++) {
-        const int f = f_of(mb);
-        float v[4];
+      for (int mb = 0; mb < MB; mb += 2) {
+        i32x2 w[2][PLANES ? 3 : 1];
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = last_f && f + i >= a.f_count ? 0.f : factor * acc[mb][nb][i];
-        if (!there || f >= a.dz_ld) continue;
+        for (int h = 0; h < 2; h++) {
+          const int f = f_of(mb + h);
+          float v[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[i] = last_f && f + i >= a.f_count ? 0.f : factor * acc[mb + h][nb][i];
+          if constexpr (PLANES) {
+            uint16_t piece[4][3];
+#pragma unroll
+            for (int i = 0; i < 4; i++) three_pieces(v[i], piece[i]);
+#pragma unroll
+            for (int k = 0; k < 3; k++) w[h][k] = i32x2{piece[0][k] | piece[1][k] << 16, piece[2][k] | piece[3][k] << 16};
+          } else {
+            w[h][0] = i32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+          }
+        }
+        const int f = f_wave + (mb + (q >> 1)) * 16 + 8 * (q & 1);
         uint16_t* to = a.dz + (int64_t)p * a.dz_ld + f;
-        if (PLANES) {
-          uint16_t piece[4][3];
 #pragma unroll
-          for (int i = 0; i < 4; i++) three_pieces(v[i], piece[i]);
-#pragma unroll
-          for (int k = 0; k < 3; k++)
-            *(i32x2*)(to + k * a.dz_plane) = i32x2{piece[0][k] | piece[1][k] << 16, piece[2][k] | piece[3][k] << 16};
-        } else {
-          *(i32x2*)to = i32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+        for (int k = 0; k < (PLANES ? 3 : 1); k++) {
+          const i32x4 x = eight_of<false>(w[0][k], w[1][k], q);
+          if (there && f < a.dz_ld) *(i32x4*)(to + k * a.dz_plane) = x;
         }
       }
     }
@@ -273,19 +304,35 @@ __device__ __forceinline__ void finish(const ProductArgs& a, f32x4 (&acc)[BF / W
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
       const int p = p_of(nb);
-      if (p >= p_count) continue;
-      const int64_t row = PROD == kGradRows && !a.acc ? a.row_of[p] : p;
+      const bool there = p < p_count;
+      if (a.acc) {
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) {
+          if (!there || f_of(mb) >= a.f_count) continue;
+          f32x4* to = (f32x4*)(a.acc + split * acc_split + p * a.acc_ld + f_of(mb));
+          *to = a.add ? *to + acc[mb][nb] : acc[mb][nb];
+        }
+        continue;
+      }
+      const int64_t row = (PROD == kGradRows && there ? a.row_of[p] : p) * a.out_ld;
+#pragma unroll
+      for (int mb = 0; mb < MB; mb++) acc[mb][nb] *= scale;
+      if (!PLANES && a.out_by_eight) {
+#pragma unroll
+        for (int mb = 0; mb < MB; mb += 2) {
+          const i32x2 w[2] = {{pack2<T>(acc[mb][nb][0], acc[mb][nb][1]), pack2<T>(acc[mb][nb][2], acc[mb][nb][3])},
+                              {pack2<T>(acc[mb + 1][nb][0], acc[mb + 1][nb][1]), pack2<T>(acc[mb + 1][nb][2], acc[mb + 1][nb][3])}};
+          const i32x4 x = eight_of<true>(w[0], w[1], q);
+          const int f = f_wave + (mb + (q >> 1)) * 16 + 8 * (q & 1);
+          if (there && f < a.f_count) *(i32x4*)(a.out + (row + f) * 2) = x;
+        }
+        continue;
+      }
 #pragma unroll
       for (int mb = 0; mb < MB; mb++) {
         const int f = f_of(mb);
-        if (f >= a.f_count) continue;
-        if (a.acc) {
-          f32x4* to = (f32x4*)(a.acc + split * a.acc_split + p * a.acc_ld + f);
-          *to = a.add ? *to + acc[mb][nb] : acc[mb][nb];
-        } else {
-          const float v[4] = {acc[mb][nb][0] * scale, acc[mb][nb][1] * scale, acc[mb][nb][2] * scale, acc[mb][nb][3] * scale};
-          store_four<T, PLANES>(a.out, row * a.out_ld + f, v, a.f_count - f, a.out_vec);
-        }
+        const float v[4] = {acc[mb][nb][0], acc[mb][nb][1], acc[mb][nb][2], acc[mb][nb][3]};
+        if (there && f < a.f_count) store_four<T, PLANES>(a.out, row + f, v, a.f_count - f, a.out_vec);
       }
     }
   }
@@ -312,7 +359,9 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
     else
       p_count = live;
     if (PROD == kGradRows || PROD == kGradWeight) down = a.head->down;
+    if (PROD == kGradRows && a.acc) splits = uniform(a.head->splits);
   }
+  const int64_t acc_split = PROD == kGradRows ? p_count * a.acc_ld : a.acc_split;  // (sums of the live rows alone)
   // The workgroups of one XCD (every eighth) have neighbouring tiles at a time, of columns of eight tiles of p through all f.
   const int tiles_f = (a.f_count + BF - 1) / BF, tiles_p = (p_count + BP - 1) / BP, tiles = tiles_f * tiles_p;
   const int of_xcd = (tiles * splits + 7) >> 3, xcd = blockIdx.x & 7, at_once = gridDim.x >> 3;
@@ -449,7 +498,7 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
       });
       sent();
     }
-    finish<T, BF, BP, WF, WP, PROD, PLANES>(a, acc, (MODA_LDS float*)(smem + NST * STAGE), t.f0, t.p0, t.split, p_count, down, wf, wp, tid);
+    finish<T, BF, BP, WF, WP, PROD, PLANES>(a, acc, (MODA_LDS float*)(smem + NST * STAGE), t.f0, t.p0, t.split, acc_split, p_count, down, wf, wp, tid);
   }
   Wait::wait_all();  // no load outlives its workgroup's LDS
 }

@@ -94,11 +94,16 @@ inline EmbedGradPlan plan_embed_grad(int64_t n, int64_t vocab, int64_t width) {
 // are multiplied.
 struct LossHead {
   int live;
+  int splits;  // of the words where the gradient of the rows is added up in fp32 (SplitRule)
   float down;
 };
 
 // Rows with a target, one behind the other: their numbers, targets, factors and log sums, and the rows themselves as the products read
 // them (`planes` of 16-bit elements whose sum a row is, each [rows][x_ld], zeros behind a row's end).
+struct SplitRule {
+  int tile_p, tiles_f, steps, at_once, most;  // a tile's rows, tiles of columns, steps of 64 words, workgroups; splits that there is room for at all rows
+  float step_us, end_us, split_us;            // of a step, an item, a split of one row
+};
 struct GatherArgs {
   Words words;
   const char* x;
@@ -115,6 +120,7 @@ struct GatherArgs {
   const float *d_loss, *lse_in;
   int64_t d_loss_stride;  // 0: one for all
   float *factor, *lse;
+  SplitRule rule;
   char* dx;  // zeros for the rows without (or NULL)
   int64_t ld_dx;
   float up;  // the gradient of the logits is kept this many times as large
@@ -146,12 +152,12 @@ struct ProductArgs {
   const float *factor, *lse;
   uint16_t* dz;
   int64_t dz_ld, dz_plane;
-  float* acc;  // [splits][rows][acc_ld] in fp32, or NULL: the result itself to out
+  float* acc;  // [splits][rows][acc_ld] in fp32 (kGradRows: the live rows), or NULL: the result itself to out
   int64_t acc_ld, acc_split;
   int add;
   char* out;
   int64_t out_ld;
-  int out_vec;
+  int out_vec, out_by_eight;  // four, eight neighbouring results may be stored as one
   float scale;
 };
 
@@ -199,14 +205,15 @@ inline int tile_p(ProductTile t) { return t == kTileLarge ? 256 : t == kTileMedi
 // a start and end of each -- and where the axis is split, a launch more and the sums' way to memory and back.  Measured (8192 x 32000 x 2048,
 // bf16): a step of the large tile 1.65 us, of two medium ones on a compute unit 1.04 (alone 0.85), of the one for few rows 0.51; ends 2.5 to 4 us.
 // 1638 rows, 50257 words, width 768: 146 us by large tiles, 160 by medium ones (estimated 143, 155); 80 rows, width 512: 15.4 medium, 18.6 few.
+struct TileTimes {
+  ProductTile tile;
+  double at_once, step_us, alone_us, end_us;
+};
+constexpr TileTimes kTileTimes[3] = {{kTileLarge, 256, 1.65, 1.65, 4}, {kTileMedium, 512, 1.04, 0.85, 3}, {kTileRows, 512, 0.51, 0.45, 2.5}};
 inline Tiling choose_tiling(int64_t p, int64_t f, int64_t steps, bool may_split, bool may_few) {
-  const struct {
-    ProductTile tile;
-    double at_once, step_us, alone_us, end_us;
-  } kinds[3] = {{kTileLarge, 256, 1.65, 1.65, 4}, {kTileMedium, 512, 1.04, 0.85, 3}, {kTileRows, 512, 0.51, 0.45, 2.5}};
   Tiling best = {kTileMedium, 1};
   double least = 1e30;
-  for (const auto& k : kinds) {
+  for (const auto& k : kTileTimes) {
     if (k.tile == kTileRows && !may_few) continue;
     const int64_t tiles = ((p + tile_p(k.tile) - 1) / tile_p(k.tile)) * ((f + tile_f(k.tile) - 1) / tile_f(k.tile));
     for (int s = 1; s <= 64; s *= 2) {

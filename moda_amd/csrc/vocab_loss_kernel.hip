@@ -143,7 +143,26 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
   // The gradient of a logit is rounded to 16 bits.  The factor that rows share stays out of that, or its own rounding would be in all of them,
   // the same way: it is kept relative to the largest upstream gradient, which the products multiply by at their end.
   const float most = e > 0 ? __uint_as_float((uint32_t)e) : 1.f;
-  if (first == 0 && tid == 0) *a.head = LossHead{all, a.d_loss ? most / (a.mean ? (float)max(all, 1) : 1.f) / a.up : 1.f};
+  if (first == 0 && tid < 64) {
+    // How the words are split for the gradient of so many rows: the time of each choice, a lane a choice (choose_tiling's estimate).
+    int splits = tid + 1;
+    float us = __builtin_huge_valf();
+    if (a.rule.steps > 0 && (int64_t)splits * all <= a.rule.most * n && (splits == 1 || a.rule.steps >= 4 * splits)) {
+      const int items = (all + a.rule.tile_p - 1) / a.rule.tile_p * a.rule.tiles_f * splits;
+      us = (float)((items + a.rule.at_once - 1) / a.rule.at_once) * ((float)((a.rule.steps + splits - 1) / splits) * a.rule.step_us + a.rule.end_us) +
+           (float)splits * (float)all * a.rule.split_us;
+    }
+    for (int s = 32; s > 0; s >>= 1) {
+      const float other_us = __shfl_xor(us, s, 64);
+      const int other = __shfl_xor(splits, s, 64);
+      if (other_us < us || (other_us == us && other < splits)) {
+        us = other_us;
+        splits = other;
+      }
+    }
+    if (us == __builtin_huge_valf()) splits = 1;
+    if (tid == 0) *a.head = LossHead{all, splits, a.d_loss ? most / (a.mean ? (float)max(all, 1) : 1.f) / a.up : 1.f};
+  }
   if (tid < 64) {
     const int64_t i = first + tid;
     const int word = tid < kGatherBlock && i < n ? a.words.of(i) : -1;
@@ -272,18 +291,20 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const JoinSumsArgs a) {
   const int64_t chunks = (a.width + 3) / 4, w = (int64_t)workgroup() * 256 + threadIdx.x, p = w / chunks, f = (w - p * chunks) * 4;
   const int64_t rows = a.head && a.by_head ? a.head->live : a.rows;
   if (p >= rows) return;
+  const int splits = a.by_head ? a.head->splits : a.splits;
+  const int64_t acc_split = a.by_head ? rows * a.acc_ld : a.acc_split;
   const float* from = a.acc + p * a.acc_ld + f;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   int i = 0;
-  for (; i + 8 <= a.splits; i += 8) {
+  for (; i + 8 <= splits; i += 8) {
     f32x4 v[8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) v[k] = *(const f32x4*)(from + (i + k) * a.acc_split);
+    for (int k = 0; k < 8; k++) v[k] = *(const f32x4*)(from + (i + k) * acc_split);
 #pragma unroll
     for (int k = 0; k < 8; k++) s += v[k];
   }
 #pragma unroll 4
-  for (; i < a.splits; i++) s += *(const f32x4*)(from + i * a.acc_split);
+  for (; i < splits; i++) s += *(const f32x4*)(from + i * acc_split);
   const float scale = a.scale * a.head->down;
   const float v[4] = {s[0] * scale, s[1] * scale, s[2] * scale, s[3] * scale};
   store_four<T, FP32_OUT>(a.out, (a.by_head ? a.row_of[p] : p) * a.out_ld + f, v, (int)min(a.width - f, (int64_t)4), a.out_vec);
