@@ -30,6 +30,7 @@ from .depth_cache import DepthCache, stack_depth
 from .ops import _chunk_tokens, _tracing, parallel_moda, parallel_moda_chunk_visible
 from .paged import PagedKVCache
 from .rotary import Rotary, apply_rotary
+from .vocab import embed_tokens, linear_cross_entropy
 
 
 class DepthStream:
@@ -240,12 +241,26 @@ class MoDAStack(nn.Module):
 
     A causal stack also generates: ``prefill`` runs prompts and leaves their keys and values in a ``PagedKVCache``, ``decode`` the
     tokens that follow, each over its sequence's pages and, as in ``forward``, over the depth slots of its own earlier layers.  A captured
-    ``decode`` follows the cache's counts as they grow (pages are reserved between replays)."""
+    ``decode`` follows the cache's counts as they grow (pages are reserved between replays).
+
+    ``vocab``: a language model of that many words.  ``forward``, ``prefill`` and ``decode`` then also take tokens (int32 or int64 ``[B, N]``),
+    whose rows are ``embed_scale`` times those of ``embedding``; ``nll`` scores the rows that they return, behind the norm ``out_norm``, against
+    the words of ``head`` (``tied``: of ``embedding``); ``loss`` is both around ``forward``, for training."""
+
+    vocab: Optional[int] = None  # (of modules pickled before there was one)
 
     def __init__(self, dim, depth, num_heads, num_kv_heads, mlp_ratio=4., qkv_bias=True, is_causal=False,
-                 post_norm=False, ffn_kv=False, chunk_rows=None, rotary: Optional[Rotary] = None):
+                 post_norm=False, ffn_kv=False, chunk_rows=None, rotary: Optional[Rotary] = None, vocab: Optional[int] = None,
+                 tied: bool = True, embed_scale: float = 1.0):
         super().__init__()
         self.post_norm, self.ffn_kv = post_norm, ffn_kv
+        if vocab is not None:
+            if vocab <= 0:
+                raise ValueError(f"a vocabulary has at least one word, got {vocab}")
+            self.vocab, self.embed_scale = int(vocab), float(embed_scale)
+            self.embedding = nn.Parameter(torch.empty(vocab, dim).normal_(0.0, dim ** -0.5))
+            self.head = None if tied else nn.Parameter(torch.empty(vocab, dim).normal_(0.0, dim ** -0.5))
+            self.out_norm = nn.LayerNorm(dim, eps=1e-6)
         self.blocks = nn.ModuleList()
         for _ in range(depth):
             blk = nn.Module()
@@ -310,7 +325,28 @@ class MoDAStack(nn.Module):
         cb = 0 if attn.chunk_rows is None else _chunk_tokens(attn.moda_group_num, attn.chunk_rows)
         return _lib.host().stack_forward(x, plain[0], plain[1], attn.num_heads, attn.num_kv_heads, bool(attn.is_causal), cb, self.post_norm)
 
+    def embed(self, tokens: torch.Tensor) -> torch.Tensor:
+        """The rows ``[.., dim]`` of tokens (zeros for what is no word)."""
+        assert self.vocab is not None, "a stack of rows has no tokens: construct with vocab"
+        return embed_tokens(tokens, self.embedding, self.embed_scale)
+
+    def _rows(self, x):
+        return x if x.is_floating_point() else self.embed(x)
+
+    def nll(self, y: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, reduction: str = "none") -> torch.Tensor:
+        """The negative log-likelihood (fp32) of the words ``targets [..]`` given the rows ``y [.., dim]`` that ``forward``, ``prefill`` or ``decode``
+        returned for the tokens before them; see ``linear_cross_entropy``."""
+        assert self.vocab is not None, "a stack of rows has no vocabulary: construct with vocab"
+        return linear_cross_entropy(self.out_norm(y), self.embedding if self.head is None else self.head, targets, ignore_index=ignore_index,
+                                    reduction=reduction)
+
+    def loss(self, tokens: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, reduction: str = "mean",
+             positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``nll`` of ``targets [B, N]`` (the next words, ``ignore_index`` where there is none to learn) over ``forward(tokens)``."""
+        return self.nll(self(tokens, positions=positions), targets, ignore_index, reduction)
+
     def forward(self, x, inplace_cache: Optional[bool] = None, positions: Optional[torch.Tensor] = None):
+        x = self._rows(x)
         if inplace_cache is not False and positions is None:
             y = self._forward_native(x)
             if y is not None:
@@ -339,10 +375,11 @@ class MoDAStack(nn.Module):
 
     @torch.no_grad()
     def prefill(self, x, cache: PagedKVCache, lens: Optional[torch.Tensor] = None):
-        """Prompts ``x [batch, N, dim]``, of which the first ``lens [batch]`` (int32; none given: all ``N``) tokens are real, for the
+        """Prompts ``x [batch, N, dim]`` (or tokens), of which the first ``lens [batch]`` (int32; none given: all ``N``) tokens are real, for the
         empty sequences of ``cache`` (pages reserved): ``forward``'s result, keys and values of all layers in the cache, its
         counts advanced.  Rows behind a prompt's end hold nothing of use.  Sequences with tokens of their own (``decode`` goes on with those)
         or without pages for the prompt are an error, for which the call waits for the device (not in a captured one, which does not look)."""
+        x = self._rows(x)
         self._check_cache(x, cache)
         with torch.cuda.device_of(cache.past):
             captured = torch.cuda.is_current_stream_capturing()
@@ -360,9 +397,10 @@ class MoDAStack(nn.Module):
 
     @torch.no_grad()
     def decode(self, x, cache: PagedKVCache, lens: Optional[torch.Tensor] = None):
-        """The next tokens ``x [batch, N, dim]`` of the cache's sequences -- one each, or a few (drafted ones, pieces of a prompt),
+        """The next tokens ``x [batch, N, dim]`` (or as tokens) of the cache's sequences -- one each, or a few (drafted ones, pieces of a prompt),
         of which the first ``lens [batch]`` (int32) are real: their rows of ``forward`` over the whole sequence.  Keys and values
         go to the cache, its counts advance."""
+        x = self._rows(x)
         self._check_cache(x, cache)
         B, N, _ = x.shape
         if N == 0:

@@ -110,3 +110,15 @@ def test_no_cpu_path():
                  lambda: moda_amd.linear_cross_entropy_bwd(torch.zeros(3, 8), w, t, torch.zeros(3), torch.zeros(()))):
         with pytest.raises(RuntimeError, match="MI355X"):
             call()
+
+
+def test_stack_with_a_vocabulary():
+    plain, tied, apart = (moda_amd.MoDAStack(32, 1, 4, 2, **k) for k in ({}, {"vocab": 50}, {"vocab": 50, "tied": False}))
+    more = lambda m: sorted(set(m.state_dict()) - set(plain.state_dict()))  # noqa: E731
+    assert more(tied) == ["embedding", "out_norm.bias", "out_norm.weight"] and more(apart) == ["embedding", "head", "out_norm.bias", "out_norm.weight"]
+    with pytest.raises(ValueError, match="at least one word"):
+        moda_amd.MoDAStack(32, 1, 4, 2, vocab=0)
+    with pytest.raises(AssertionError, match="construct with vocab"):
+        plain(torch.zeros(1, 3, dtype=torch.long))
+    with pytest.raises(AssertionError, match="construct with vocab"):
+        plain.nll(torch.zeros(1, 3, 32), torch.zeros(1, 3, dtype=torch.long))
