@@ -90,7 +90,7 @@ __device__ __forceinline__ Entry entry(const SortArgs& a, int64_t i) {
   return {w < 0 ? (uint32_t)a.words.vocab : (uint32_t)w, (uint32_t)i};
 }
 
-// (The first pass clears the words' ranges besides.)
+// (The first pass clears the words' ranges besides: to look whether a range is one costs 64 K tokens on 128 K words 7 us.)
 __global__ __launch_bounds__(kSortThreads) void count_digits_kernel(const SortArgs a) {
   __shared__ uint32_t count[kDigits];
   if (!a.keys)
@@ -106,6 +106,106 @@ __global__ __launch_bounds__(kSortThreads) void count_digits_kernel(const SortAr
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) a.counts[(int64_t)blockIdx.x * kDigits + d] = count[d];
 }
 
+// How many lanes below this one have its digit, among those that are `there`; same: how many have it in all.
+__device__ __forceinline__ int rank_in_wave(int digit, bool there, int& same) {
+  uint64_t mask = __ballot(there);
+  for (int b = 0; b < kDigitBits; b++) {
+    const uint64_t set = __ballot(digit >> b & 1);
+    mask &= digit >> b & 1 ? set : ~set;
+  }
+  same = __popcll(mask);
+  return __popcll(mask & ((1ull << (threadIdx.x & 63)) - 1));
+}
+
+// Sum over the digits below that of a thread of the first kDigits; total: LDS of a number for each of their waves.
+__device__ __forceinline__ uint32_t sum_below(uint32_t count, uint32_t* total) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint32_t upto = count;  // of the digits of this wave up to this one
+  for (int s = 1; s < 64; s <<= 1) {
+    const uint32_t o = __shfl_up(upto, s, 64);
+    upto += lane >= s ? o : 0;
+  }
+  if (tid < kDigits && lane == 63) total[tid >> 6] = upto;
+  __syncthreads();
+  uint32_t lower = upto - count;
+  if (tid < kDigits)
+    for (int w = 0; w < tid >> 6; w++) lower += total[w];
+  return lower;
+}
+
+// Up to kFewTokens of them: all passes, and the words' ranges, in one workgroup (some 4 us a launch less for each pass and the ranges).
+__global__ __launch_bounds__(kSortThreads) void sort_few_kernel(const SortArgs a, int passes) {
+  constexpr int W = kSortThreads / 64;
+  __shared__ uint32_t key[kFewTokens], base[kDigits], total[kDigits / 64];
+  __shared__ uint16_t place[kFewTokens], in_wave[W][kDigits];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = (int)a.words.n;
+  Entry e[kFewRounds];
+#pragma unroll
+  for (int r = 0; r < kFewRounds; r++) {
+    const int i = r * kSortThreads + tid;
+    e[r] = i < n ? entry(a, i) : Entry{0, 0};
+  }
+  for (int p = 0; p < passes; p++) {
+    const int shift = p * kDigitBits;
+    if (tid < kDigits) base[tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kFewRounds; r++)
+      if (r * kSortThreads + tid < n) atomicAdd(&base[e[r].key >> shift & (kDigits - 1)], 1u);
+    __syncthreads();
+    const uint32_t lower = sum_below(tid < kDigits ? base[tid] : 0, total);
+    if (tid < kDigits) base[tid] = lower;
+    int to[kFewRounds];
+#pragma unroll
+    for (int r = 0; r < kFewRounds; r++) {
+      if (r * kSortThreads >= n) break;
+      for (int d = lane; d < kDigits; d += 64) in_wave[wave][d] = 0;
+      const bool there = r * kSortThreads + tid < n;
+      const int digit = e[r].key >> shift & (kDigits - 1);
+      int same;
+      const int rank = rank_in_wave(digit, there, same);
+      __syncthreads();
+      if (there && rank == 0) in_wave[wave][digit] = (uint16_t)same;
+      __syncthreads();
+      if (tid < kDigits) {  // counts of the waves -> where each begins
+        uint32_t at = base[tid];
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+          const uint32_t c = in_wave[w][tid];
+          in_wave[w][tid] = (uint16_t)at;
+          at += c;
+        }
+        base[tid] = at;
+      }
+      __syncthreads();
+      to[r] = in_wave[wave][digit] + rank;
+      __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < kFewRounds; r++)
+      if (r * kSortThreads + tid < n) {
+        key[to[r]] = e[r].key;
+        place[to[r]] = (uint16_t)e[r].place;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kFewRounds; r++) {
+      const int i = r * kSortThreads + tid;
+      if (i < n) e[r] = {key[i], place[i]};
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kFewRounds; r++) {
+    const int i = r * kSortThreads + tid;
+    if (i >= n) break;
+    a.keys_out[i] = e[r].key;
+    a.places_out[i] = e[r].place;
+    if (e[r].key >= (uint32_t)a.words.vocab) continue;
+    if (i == 0 || key[i - 1] != e[r].key) a.range[e[r].key].x = i;
+    if (i == n - 1 || key[i + 1] != e[r].key) a.range[e[r].key].y = i + 1;
+  }
+}
+
 // Where an entry goes: behind all with a lower digit, those with its own of the blocks and rounds before, and those with its own of the
 // waves and lanes before it in this round.
 __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(const SortArgs a) {
@@ -113,7 +213,7 @@ __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(const SortAr
   static_assert(kSortThreads == 2 * kDigits, "two threads a digit");
   __shared__ uint32_t base[kDigits], in_wave[W][kDigits], total[kDigits / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  uint32_t before = 0, all = 0, upto = 0;
+  uint32_t before = 0, all = 0;
   {
     uint32_t* other = &in_wave[0][0];  // what the second thread of a digit has counted
     const int d = tid & (kDigits - 1), half = (a.blocks + 1) / 2, from = tid < kDigits ? 0 : half, to = tid < kDigits ? half : a.blocks;
@@ -133,20 +233,8 @@ __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(const SortAr
       before += other[2 * d + 1];
     }
   }
-  if (tid < kDigits) {
-    upto = all;  // of the digits of this wave up to this one
-    for (int s = 1; s < 64; s <<= 1) {
-      const uint32_t o = __shfl_up(upto, s, 64);
-      upto += lane >= s ? o : 0;
-    }
-    if (lane == 63) total[wave] = upto;
-  }
-  __syncthreads();
-  if (tid < kDigits) {
-    uint32_t lower = upto - all;
-    for (int w = 0; w < wave; w++) lower += total[w];
-    base[tid] = lower + before;
-  }
+  const uint32_t lower = sum_below(tid < kDigits ? all : 0, total);
+  if (tid < kDigits) base[tid] = lower + before;
   const int64_t first = (int64_t)blockIdx.x * kSortThreads * a.rounds;
   for (int r = 0; r < a.rounds; r++) {
     for (int d = lane; d < kDigits; d += 64) in_wave[wave][d] = 0;
@@ -155,13 +243,9 @@ __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(const SortAr
     const bool there = i < a.words.n;
     const Entry e = there ? entry(a, i) : Entry{0, 0};
     const int digit = e.key >> a.shift & (kDigits - 1);
-    uint64_t same = __ballot(there);
-    for (int b = 0; b < kDigitBits; b++) {
-      const uint64_t set = __ballot(digit >> b & 1);
-      same &= digit >> b & 1 ? set : ~set;
-    }
-    const int rank = __popcll(same & ((1ull << lane) - 1));
-    if (there && rank == 0) in_wave[wave][digit] = (uint32_t)__popcll(same);
+    int same;
+    const int rank = rank_in_wave(digit, there, same);
+    if (there && rank == 0) in_wave[wave][digit] = (uint32_t)same;
     __syncthreads();
     if (tid < kDigits) {  // counts of the waves -> where each begins
       uint32_t at = base[tid];
@@ -271,7 +355,11 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const EmbedArgs a) {
   const int64_t w0 = ((int64_t)(block - a.chunk_blocks) * groups + group) * kWordsOfGroup;
   int2 run[kWordsOfGroup];
 #pragma unroll
-  for (int w = 0; w < kWordsOfGroup; w++) run[w] = w0 + w < vocab ? a.range[w0 + w] : int2{0, 0x7fffffff};
+  for (int w = 0; w < kWordsOfGroup; w++) {
+    run[w] = w0 + w < vocab ? a.range[w0 + w] : int2{0, 0x7fffffff};
+    // what the memory of a word's range held that is not there names no place of it
+    if (!a.cleared && w0 + w < vocab && ((unsigned)run[w].x >= (unsigned)n || a.keys[run[w].x] != (uint32_t)(w0 + w))) run[w] = int2{0, 0};
+  }
 #pragma unroll
   for (int w = 0; w < kWordsOfGroup; w++) {
     if (run[w].y - run[w].x > kRunRows) continue;
@@ -371,24 +459,33 @@ hipError_t launch_embed_grad(EmbedArgs& a, int dtype, bool vec, char* work, hipS
   s.range = (int2*)(work + p.range);
   s.rounds = p.rounds;
   s.blocks = p.blocks;
-  for (int i = 0; i < p.passes; i++) {
-    s.shift = i * kDigitBits;
-    s.keys = i == 0 ? nullptr : (const uint32_t*)(work + p.keys[(i - 1) & 1]);
-    s.places = i == 0 ? nullptr : (const uint32_t*)(work + p.places[(i - 1) & 1]);
-    s.keys_out = (uint32_t*)(work + p.keys[i & 1]);
-    s.places_out = (uint32_t*)(work + p.places[i & 1]);
-    count_digits_kernel<<<p.blocks, kSortThreads, 0, stream>>>(s);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    place_digits_kernel<<<p.blocks, kSortThreads, 0, stream>>>(s);
+  hipError_t e = hipSuccess;
+  if (a.words.n <= kFewTokens) {
+    s.keys_out = (uint32_t*)(work + p.keys[0]);
+    s.places_out = (uint32_t*)(work + p.places[0]);
+    if (a.words.n > 0) sort_few_kernel<<<1, kSortThreads, 0, stream>>>(s, p.passes);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    a.keys = s.keys_out;
+    a.places = s.places_out;
+  } else {
+    for (int i = 0; i < p.passes; i++) {
+      s.shift = i * kDigitBits;
+      s.keys = i == 0 ? nullptr : (const uint32_t*)(work + p.keys[(i - 1) & 1]);
+      s.places = i == 0 ? nullptr : (const uint32_t*)(work + p.places[(i - 1) & 1]);
+      s.keys_out = (uint32_t*)(work + p.keys[i & 1]);
+      s.places_out = (uint32_t*)(work + p.places[i & 1]);
+      count_digits_kernel<<<p.blocks, kSortThreads, 0, stream>>>(s);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+      place_digits_kernel<<<p.blocks, kSortThreads, 0, stream>>>(s);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    a.keys = s.keys = (const uint32_t*)(work + p.keys[(p.passes - 1) & 1]);
+    a.places = (const uint32_t*)(work + p.places[(p.passes - 1) & 1]);
+    word_ranges_kernel<<<grid_of((a.words.n + 255) / 256), 256, 0, stream>>>(s);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  a.keys = s.keys = (const uint32_t*)(work + p.keys[(p.passes - 1) & 1]);
-  a.places = (const uint32_t*)(work + p.places[(p.passes - 1) & 1]);
-  if (a.words.n > 0) word_ranges_kernel<<<grid_of((a.words.n + 255) / 256), 256, 0, stream>>>(s);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
   a.range = s.range;
+  a.cleared = a.words.n > kFewTokens;
   a.parts = (float*)(work + p.parts);
   a.part_ld = p.part_ld;
   a.chunks = (int)p.chunks;

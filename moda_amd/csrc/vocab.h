@@ -35,18 +35,20 @@ struct EmbedArgs {
   float* parts;
   int64_t part_ld;
   int chunks;
+  int cleared;  // ranges of words that are not there are empty (else whatever their memory held)
   unsigned chunk_blocks;
 };
 
 // The order of words: passes over digits of their number, lowest first, each stable.  A block of kSortThreads * rounds tokens counts its
 // digits; a second launch places them.
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits, kSortThreads = 1024, kMostSortBlocks = 128;
+constexpr int kFewRounds = 4, kFewTokens = kSortThreads * kFewRounds;  // as many one workgroup sorts by itself
 struct SortArgs {
   Words words;
   const uint32_t *keys, *places;  // NULL in the first pass: the words themselves
   uint32_t *keys_out, *places_out;
   uint32_t* counts;  // [blocks][kDigits]
-  int2* range;       // [vocab]
+  int2* range;       // [vocab]: first place and end of the words that there are
   int rounds, blocks, shift;
 };
 
@@ -66,7 +68,6 @@ inline EmbedGradPlan plan_embed_grad(int64_t n, int64_t vocab, int64_t width) {
   p.rounds = (int)((n + (int64_t)kSortThreads * kMostSortBlocks - 1) / ((int64_t)kSortThreads * kMostSortBlocks));
   if (p.rounds < 1) p.rounds = 1;
   p.blocks = (int)((n + (int64_t)kSortThreads * p.rounds - 1) / ((int64_t)kSortThreads * p.rounds));
-  if (p.blocks < 1) p.blocks = 1;  // (clears the words' ranges where there are no tokens)
   p.chunks = (n + kRunRows - 1) / kRunRows;
   p.part_ld = (width + 3) / 4 * 4;
   size_t at = 0;
