@@ -934,7 +934,7 @@ namespace {
 bool on_grid(const void* p, int64_t ld, int es) { return (uintptr_t)p % 16 == 0 && ld % (16 / es) == 0; }
 
 int check_tokens(int32_t dtype, const void* tokens, int32_t tokens64, int64_t n, int64_t vocab, int64_t width, float scale) {
-  if (!known_dtype(dtype) || n < 0 || vocab <= 0 || width <= 0 || (n > 0 && !tokens) || !(scale - scale == 0.f)) return MODA_HIP_EINVAL;
+  if (!known_dtype(dtype) || n < 0 || vocab <= 0 || width <= 0 || (n > 0 && !tokens) || !(scale * 1.5f - scale * 1.5f == 0.f)) return MODA_HIP_EINVAL;
   if ((uintptr_t)tokens % (tokens64 ? 8 : 4) != 0) return MODA_HIP_EALIGN;
   if (n >= (1ll << 30) || vocab >= (1ll << 31) - 256 || width >= (1ll << 24)) return MODA_HIP_EUNSUPPORTED;
   return MODA_HIP_OK;
@@ -1190,6 +1190,7 @@ int moda_hip_vocab_loss_bwd(const moda_hip_vocab_loss_args* t, void* workspace, 
       r.head = v.head();
       r.splits = p.grad_rows.splits;
       r.row_of = v.at<int>(p.row_of);
+      r.rows = (int)t->rows;
       r.scale = t->scale;
       if (p.acc_rows) {
         r.acc = v.at<float>(p.dx_acc);

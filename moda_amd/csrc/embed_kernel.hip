@@ -257,8 +257,8 @@ __global__ __launch_bounds__(kSortThreads) void place_digits_kernel(const SortAr
       base[tid] = at;
     }
     __syncthreads();
-    if (there) {
-      const uint32_t to = in_wave[wave][digit] + rank;
+    const uint32_t to = in_wave[wave][digit] + rank;
+    if (there && to < (uint64_t)a.words.n) {  // (tokens that change during the call make wrong results, no access out of place)
       a.keys_out[to] = e.key;
       a.places_out[to] = e.place;
     }
@@ -293,7 +293,8 @@ __device__ __forceinline__ void add_rows(const EmbedArgs& a, int first, int last
     for (int j = 0; j < VEC; j++) sum[i][j] = 0.f;
   const bits* x = (const bits*)a.weight;
   for (int b = first; b < last; b += lanes) {
-    const int place = b + sub < last ? (int)a.places[b + sub] : 0, count = min(lanes, last - b);
+    const uint32_t there = b + sub < last ? a.places[b + sub] : 0;
+    const int place = there < (uint32_t)a.words.n ? (int)there : 0, count = min(lanes, last - b);
     for (int r = 0; r < count; r += ROWS) {
       vec v[ROWS][kChunks];
 #pragma unroll

@@ -1242,7 +1242,7 @@ void check_weight(const Tensor& weight) {
   check_device(weight);
   dtype_code(weight);
 }
-void finite_scale(double scale) { CONTRACT(std::isfinite((float)scale), "scale must be finite, got ", scale); }
+void finite_scale(double scale) { CONTRACT(std::isfinite((float)scale * 1.5f), "scale must be finite, got ", scale); }
 
 Tensor embed_rows(const Tensor& tokens_in, const Tensor& weight_in, double scale) {
   check_weight(weight_in);

@@ -304,7 +304,7 @@ __device__ __forceinline__ void finish(const ProductArgs& a, f32x4 (&acc)[BF / W
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
       const int p = p_of(nb);
-      const bool there = p < p_count;
+      bool there = p < p_count;
       if (a.acc) {
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
@@ -314,7 +314,12 @@ __device__ __forceinline__ void finish(const ProductArgs& a, f32x4 (&acc)[BF / W
         }
         continue;
       }
-      const int64_t row = (PROD == kGradRows && there ? a.row_of[p] : p) * a.out_ld;
+      int r = p;
+      if (PROD == kGradRows && there) {
+        r = a.row_of[p];
+        there = (unsigned)r < (unsigned)a.rows;  // (targets that change during the call make wrong results, no access out of place)
+      }
+      const int64_t row = r * a.out_ld;
 #pragma unroll
       for (int mb = 0; mb < MB; mb++) acc[mb][nb] *= scale;
       if (!PLANES && a.out_by_eight) {

@@ -146,7 +146,7 @@ struct ProductArgs {
   float c;                        // logits in base 2
   Words words;                    // targets where there is no head
   const int *target, *row_of;
-  int first_word;
+  int first_word, rows;
   float2* stats;  // [tiles of words][rows]: largest logit, sum of the exponentials from there
   float* target_logit;
   int64_t stats_ld;

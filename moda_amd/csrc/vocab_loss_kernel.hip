@@ -254,6 +254,7 @@ __global__ __launch_bounds__(256) void join_stats_kernel(const JoinStatsArgs a) 
   float loss = (m - a.target_logit[p] + log_sum) * kLn2;  // (a target that is the likeliest word: log_sum alone, with all its bits)
   if (word < 0) lse = loss = 0.f;
   const int64_t row = a.head ? a.row_of[p] : p;
+  if ((uint64_t)row >= (uint64_t)a.words.n) return;  // (targets that change during the call)
   a.loss[row] = loss;
   a.lse[row] = lse;
 }
@@ -307,7 +308,9 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const JoinSumsArgs a) {
   for (; i < splits; i++) s += *(const f32x4*)(from + i * acc_split);
   const float scale = a.scale * a.head->down;
   const float v[4] = {s[0] * scale, s[1] * scale, s[2] * scale, s[3] * scale};
-  store_four<T, FP32_OUT>(a.out, (a.by_head ? a.row_of[p] : p) * a.out_ld + f, v, (int)min(a.width - f, (int64_t)4), a.out_vec);
+  const int64_t row = a.by_head ? a.row_of[p] : p;
+  if ((uint64_t)row >= (uint64_t)a.rows) return;  // (targets that change during the call)
+  store_four<T, FP32_OUT>(a.out, row * a.out_ld + f, v, (int)min(a.width - f, (int64_t)4), a.out_vec);
 }
 
 int64_t blocks_for(int64_t items) { return (items + 255) / 256; }

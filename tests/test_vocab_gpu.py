@@ -417,3 +417,78 @@ def test_traced_calls():
     traced = torch.jit.trace(f, (w, x, t), check_trace=False)
     other = rand(10, 32, dtype=torch.float32, seed=119)
     assert torch.equal(traced(w, other, t), f(w, other, t))
+
+
+def test_forward_mode_is_refused():
+    x, w, t = rand(4, 16, dtype=torch.float32, seed=120), rand(9, 16, dtype=torch.float32, seed=121), words(4, 9, 122)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: moda_amd.embed_tokens(t, dual), lambda: moda_amd.linear_cross_entropy(x, dual, t), lambda: moda_amd.linear_cross_entropy(dual[:4], w, t)):
+            with pytest.raises(RuntimeError):
+                call()
+
+
+def test_refusals():
+    x, w, t = rand(4, 16, dtype=torch.bfloat16, seed=123), rand(9, 16, dtype=torch.bfloat16, seed=124), words(4, 9, 125)
+    for call in (lambda: moda_amd.embed_tokens(t.float(), w), lambda: moda_amd.embed_tokens(t.cpu(), w), lambda: moda_amd.embed_tokens(t, w[0]),
+                 lambda: moda_amd.embed_tokens(t, w, math.nan), lambda: moda_amd.embed_tokens(t, w[:0]), lambda: moda_amd.embed_tokens_bwd(t, x[:3], 9),
+                 lambda: moda_amd.embed_tokens_bwd(t, x, 0), lambda: moda_amd.linear_cross_entropy(x[:, :8], w, t),
+                 lambda: moda_amd.linear_cross_entropy(x, w, t[:3]), lambda: moda_amd.linear_cross_entropy(x, w, t.short()),
+                 lambda: moda_amd.linear_cross_entropy(x, w, t, scale=math.inf), lambda: moda_amd.linear_cross_entropy(x, w.cpu().cuda()[:, None], t),
+                 lambda: moda_amd.linear_cross_entropy_bwd(x, w, t, torch.zeros(3, device="cuda"), torch.ones((), device="cuda")),
+                 lambda: moda_amd.linear_cross_entropy_bwd(x, w, t, torch.zeros(4, device="cuda"), torch.ones(4, device="cuda"))):
+        with pytest.raises(AssertionError):
+            call()
+    for call in (lambda: moda_amd.linear_cross_entropy(x.float(), w, t), lambda: moda_amd.embed_tokens(t, w.double())):
+        with pytest.raises(TypeError):
+            call()
+    with pytest.raises(ValueError, match="reduction"):
+        moda_amd.linear_cross_entropy(x, w, t, reduction="max")
+
+
+def test_offsets_past_32_bits_embedding():
+    vocab, width = (1 << 21) + 300, 1024
+    w = torch.empty(vocab, width, dtype=torch.bfloat16, device="cuda").fill_(0.25)
+    w[-40:] = rand(40, width, dtype=torch.bfloat16, seed=130)
+    t = torch.cat([torch.arange(vocab - 40, vocab, device="cuda").repeat(3), torch.tensor([0, 7, vocab], device="cuda")])
+    y = moda_amd.embed_tokens(t, w)
+    assert torch.equal(y, embed_reference(t, w, 1.0).bfloat16())
+    dy = rand(t.numel(), width, dtype=torch.bfloat16, seed=131)
+    dw = moda_amd.embed_tokens_bwd(t, dy, vocab)
+    want, sums = grad_reference(t - (vocab - 40), dy, 40, 1.0)
+    within(dw[-40:], want, want.abs() * half_step(dy.dtype) + sums * 1.01, "gradient")
+    assert torch.equal(dw[0], dy[-3]) and torch.equal(dw[7], dy[-2]) and int(dw.any(1).sum()) == 42
+
+
+def test_offsets_past_32_bits_weight():
+    vocab, width, n = (1 << 19) + 1000, 4104, 9
+    w = torch.empty(vocab, width, dtype=torch.bfloat16, device="cuda").normal_(0.0, width ** -0.5, generator=torch.Generator("cuda").manual_seed(132))
+    x = rand(n, width, dtype=torch.bfloat16, seed=133)
+    t = torch.arange(vocab - n, vocab, device="cuda")
+    loss, lse = moda_amd.linear_cross_entropy_fwd(x, w, t, reduction="none")
+    z = torch.cat([x.double() @ w[i:i + 65536].double().T for i in range(0, vocab, 65536)], 1)
+    want = torch.logsumexp(z, -1)
+    # as loss_reference's bounds, with |z| at most 8 and the sums of its terms at most width ** 0.5 times that
+    bound = 2 * (width + 8) * F * (x.double().abs() @ w[-4096:].double().abs().T).max() * 2 + (64 + vocab / 128) * F
+    within(loss, want - z[torch.arange(n), t], bound.expand(n), "loss")
+    dx, dw = moda_amd.linear_cross_entropy_bwd(x, w, t, lse, torch.ones(n, device="cuda"), reduction="none")
+    p = (z - want[:, None]).exp()
+    p[torch.arange(n), t] -= 1
+    for rows in (slice(0, 500), slice(vocab - 500, vocab)):
+        size = p[:, rows].abs().T @ x.double().abs()
+        within(dw[rows], p[:, rows].T @ x.double(), size * (2 * half_step(x.dtype) + 2 * bound + 64 * F) + smallest(x.dtype), "dw")
+    want = sum(p[:, i:i + 65536] @ w[i:i + 65536].double() for i in range(0, vocab, 65536))
+    size = sum(p[:, i:i + 65536].abs() @ w[i:i + 65536].double().abs() for i in range(0, vocab, 65536))
+    within(dx, want, size * (2 * half_step(x.dtype) + 2 * bound + vocab * F), "dx")
+
+
+def test_offsets_past_32_bits_rows():
+    n, vocab, width = 270000, 40, 8192
+    x = torch.empty(n, width, dtype=torch.bfloat16, device="cuda").normal_(0.0, 1.0, generator=torch.Generator("cuda").manual_seed(134))
+    w, t = rand(vocab, width, dtype=torch.bfloat16, seed=135, std=width ** -0.5), words(n, vocab, 136, 0.1)
+    loss, lse = moda_amd.linear_cross_entropy_fwd(x, w, t, reduction="none")
+    dx, _ = moda_amd.linear_cross_entropy_bwd(x, w, t, lse, torch.ones(n, device="cuda"), reduction="none", need_dweight=False)
+    for part in (slice(0, 300), slice(n - 300, n)):
+        ref = loss_reference(x[part], w, t[part], 1.0, -100, "none", torch.ones(300, device="cuda"))
+        within(loss[part], *ref["loss"], "loss")
+        within(dx[part], *ref["dx"], "dx")
