@@ -11,8 +11,17 @@
 //
 // f sits on the matrix instruction's A side: a lane has four neighbouring f of one p.
 //
+// Bound by the matrix pipe at the clock that the power limit leaves: 8192 rows, 32000 words, width 2048, bf16: statistics 823 us (1305
+// TFLOP/s), gradient of the logits 895, of the rows 798, of the weight 848, the pipe busy 55 to 62 % of the cycles at 2.0 to 2.1 GHz; plain library
+// products of these shapes 754, 754, 796 and 1104.  What it took (us of the four, one after the other): a workgroup for each tile, operands read
+// and then multiplied 926, 1010, 822, 934; workgroups that stay, so that the first loads of a tile are on their way during the end of the one
+// before; operands of the next half step read among the products of this one (861, 964, 836, 850: fewer cycles at a lower clock); the loads'
+// addresses advanced on the scalar unit among the products and the loads sent right behind the barrier.  Stages of 32 k, four of them: 4 - 8 %
+// slower (a barrier for half the products).  Without the tile loads at all the products took 595 to 727: what is left is there.
+//
 // fp32 (PLANES): each operand as the sum of three bf16 (exact: 24 bits), of whose nine products the six largest are added up, the small
-// ones first; the others are below 2^-24 of the whole.  Six products of 16 bits are faster than one of the fp32 matrix instruction.
+// ones first; the others are below 2^-24 of the whole.  Six products of 16 bits at 1300 TFLOP/s are faster than one of the fp32 matrix
+// instruction (150).
 #pragma once
 #include "../../include/moda_hip.h"
 #include "tile.h"
@@ -165,7 +174,8 @@ __device__ __forceinline__ void store_four(char* out, int64_t at, const float (&
 }
 
 // The results of two neighbouring blocks of sixteen f, four f a lane as they leave the matrix instruction, rounded -> eight neighbouring f a lane:
-// those of block q >> 1 from 8 (q & 1) on.  A store then writes 64 bytes of a row, not 32.  COLUMNS: lane group q had f 4 q .., else slot_base(q) ..
+// those of block q >> 1 from 8 (q & 1) on.  A store then writes 64 bytes of a row, not 32 (8192 rows, 32000 words, forward and
+// backward: 3.54 -> 3.49 ms).  COLUMNS: lane group q had f 4 q .., else slot_base(q) ..
 template <bool COLUMNS>
 __device__ __forceinline__ i32x4 eight_of(i32x2 a, i32x2 b, int q) {
   i32x4 r;

@@ -204,7 +204,7 @@ inline int tile_p(ProductTile t) { return t == kTileLarge ? 256 : t == kTileMedi
 
 // The tile whose launch takes the least time by this estimate: what the busiest workgroup does -- its tiles' steps of 64 of the summation axis, and
 // a start and end of each -- and where the axis is split, a launch more and the sums' way to memory and back.  Measured (8192 x 32000 x 2048,
-// bf16): a step of the large tile 1.65 us, of two medium ones on a compute unit 1.04 (alone 0.85), of the one for few rows 0.51; ends 2.5 to 4 us.
+// bf16): a step of the large tile 1.65 us, of two medium ones on a compute unit 1.04 (of one 0.85), of two for few rows 0.51; ends 2.5 to 4 us.
 // 1638 rows, 50257 words, width 768: 146 us by large tiles, 160 by medium ones (estimated 143, 155); 80 rows, width 512: 15.4 medium, 18.6 few.
 struct TileTimes {
   ProductTile tile;

