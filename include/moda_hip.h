@@ -438,7 +438,7 @@ int moda_hip_embed_grad(int32_t dtype, const void* tokens, int32_t tokens64, int
 
 /*
  * Cross entropy of rows x [rows, width] over the vocabulary weight [vocab, width]: logits z = scale * x weight^T (fp32, never stored),
- *   lse = log sum_v exp z[v],  loss = lse - z[target];  a row whose target is ignore_index or no word has loss 0 and lse 0, is not read
+ *   lse = log sum_v exp z[v],  loss = lse - z[target];  a row whose target is ignore_index or no word has loss 0 and lse 0 whatever it holds
  *   and has no gradient.
  * moda_hip_vocab_loss_fwd: lse [rows] fp32 in base 2 (log2 of the sum), loss fp32: [rows] (MODA_HIP_LOSS_ROWS), or one value, the sum
  * (MODA_HIP_LOSS_SUM) or the mean over the rows that have a target (MODA_HIP_LOSS_MEAN; 0 where none has).

@@ -1054,7 +1054,7 @@ struct VocabLoss {
       a.mean = t->reduction == MODA_HIP_LOSS_MEAN;
       if (p.acc_rows) {
         const moda::TileTimes& k = moda::kTileTimes[p.grad_rows.tile];
-        const int per_unit = k.at_once > 256 ? 2 : 1;
+        const int per_unit = (int)k.at_once / 256;
         a.rule = {moda::tile_p(k.tile), (int)((p.rows_ld + moda::tile_f(k.tile) - 1) / moda::tile_f(k.tile)),
                   (int)((p.piece + 63) / 64 * (p.planes == 3 ? 6 : 1)), compute_units * per_unit, p.grad_rows.splits,
                   (float)k.step_us, (float)k.end_us, (float)(t->width * 8 / 5e6)};

@@ -55,7 +55,8 @@ template <int COLS, int NT>
 struct ColumnLoader {
   typedef AsyncTileLoader<COLS, 64, NT> Loader;
   static constexpr int N = Loader::N;
-  static_assert(Loader::RPW * Loader::NW == 16, "a pass of the loads is sixteen rows");
+  static constexpr int PASS = Loader::RPW * Loader::NW;  // rows
+  static_assert(PASS == 16 || PASS == 32, "sixteens of rows, the second of two with the four k behind");
   Loader l;
   i32x4 rs;
   int voff, stride;
@@ -68,7 +69,7 @@ struct ColumnLoader {
   }
   // columns f0 .. of `cols`, rows from k0 on
   __device__ __forceinline__ void open(const uint16_t* p, int f0, int cols, int64_t ld, int k0) {
-    const int r = l.row_in_pass, k = 8 * ((0x9C >> (2 * (r >> 2))) & 3) + (r & 3);  // slot_base(q) = 4 j  <=>  q = 0x9C >> 2 j
+    const int r = l.row_in_pass, k = 8 * ((0x9C >> (2 * ((r >> 2) & 3))) & 3) + (r & 3) + 4 * (r >> 4);  // slot_base(q) = 4 j  <=>  q = 0x9C >> 2 j
     voff = l.pads(cols - f0) ? kPadOffset : k * stride + l.gchunk * 16;
     at = (uint64_t)(p + f0 + k0 * ld);
   }
@@ -78,7 +79,7 @@ struct ColumnLoader {
     at += step;
   }
   __device__ __forceinline__ void load(lds_ptr tile, int i) const {  // the i-th of a wave's N
-    lds_dma<16>(rs, lds_addr(tile + l.lds_elems(i)), voff, (32 * (i >> 1) + 4 * (i & 1)) * stride);
+    lds_dma<16>(rs, lds_addr(tile + l.lds_elems(i)), voff, (PASS == 32 ? 32 * i : 32 * (i >> 1) + 4 * (i & 1)) * stride);
   }
 };
 
@@ -472,7 +473,7 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
     }
   };
 
-#pragma unroll
+#pragma unroll 1  // (code that runs once comes from memory)
   for (int j = 0; j < NST; j++) {
     aim();
 #pragma unroll
@@ -536,6 +537,7 @@ template <Product PROD, typename T, bool PLANES>
 hipError_t launch_product_of(const ProductArgs& a, ProductTile tile, int compute_units, hipStream_t stream) {
   if (tile == kTileLarge) return launch_product_as<T, 256, 256, 2, 4, 2, PROD, PLANES>(a, compute_units, stream);
   if (tile == kTileMedium) return launch_product_as<T, 128, 128, 2, 2, 2, PROD, PLANES>(a, compute_units, stream);
+  if (tile == kTileSmall) return launch_product_as<T, 64, 64, 2, 2, 3, PROD, PLANES>(a, compute_units, stream);
   if constexpr (PROD == kGradWeight)
     return hipErrorInvalidValue;  // (choose_tiling: its p are words)
   else

@@ -193,24 +193,25 @@ struct LossTotalArgs {
   int mean;
 };
 
-// Tiles of a product: words or columns x rows.
-enum ProductTile { kTileLarge, kTileMedium, kTileRows };  // 256 x 256, 128 x 128, 128 x 32
+// Tiles of a product, f x p: 256 x 256, 128 x 128, for few rows 128 x 32, for small products 64 x 64.
+enum ProductTile { kTileLarge, kTileMedium, kTileRows, kTileSmall };
 struct Tiling {
   ProductTile tile;
   int splits;
 };
-inline int tile_f(ProductTile t) { return t == kTileLarge ? 256 : 128; }
-inline int tile_p(ProductTile t) { return t == kTileLarge ? 256 : t == kTileMedium ? 128 : 32; }
+inline int tile_f(ProductTile t) { return t == kTileLarge ? 256 : t == kTileSmall ? 64 : 128; }
+inline int tile_p(ProductTile t) { return t == kTileLarge ? 256 : t == kTileMedium ? 128 : t == kTileSmall ? 64 : 32; }
 
 // The tile whose launch takes the least time by this estimate: what the busiest workgroup does -- its tiles' steps of 64 of the summation axis, and
 // a start and end of each -- and where the axis is split, a launch more and the sums' way to memory and back.  Measured (8192 x 32000 x 2048,
-// bf16): a step of the large tile 1.65 us, of two medium ones on a compute unit 1.04 (of one 0.85), of two for few rows 0.51; ends 2.5 to 4 us.
+// bf16): a step of the large tile 1.65 us, of two medium ones on a compute unit 1.04 (of one 0.85), of two for few rows 0.51, of three
+// small ones 0.7; ends 2.5 to 4 us.
 // 1638 rows, 50257 words, width 768: 146 us by large tiles, 160 by medium ones (estimated 143, 155); 80 rows, width 512: 15.4 medium, 18.6 few.
 struct TileTimes {
   ProductTile tile;
   double at_once, step_us, alone_us, end_us;
 };
-constexpr TileTimes kTileTimes[3] = {{kTileLarge, 256, 1.65, 1.65, 4}, {kTileMedium, 512, 1.04, 0.85, 3}, {kTileRows, 512, 0.51, 0.45, 2.5}};
+constexpr TileTimes kTileTimes[4] = {{kTileLarge, 256, 1.65, 1.65, 4}, {kTileMedium, 512, 1.04, 0.85, 3}, {kTileRows, 512, 0.51, 0.45, 2.5}, {kTileSmall, 768, 0.7, 0.45, 2.5}};
 inline Tiling choose_tiling(int64_t p, int64_t f, int64_t steps, bool may_split, bool may_few) {
   Tiling best = {kTileMedium, 1};
   double least = 1e30;
@@ -244,7 +245,7 @@ struct LossPlan {
 };
 
 constexpr int64_t kGatherBlock = 8, kCountBlock = 1024, kScanMost = 4096;
-constexpr int64_t kDirectRows = 128;
+constexpr int64_t kDirectRows = 512;  // (the gather and its launch cost more than products of rows that do not count)
 
 // grid16: x lies on the 16-byte grid (its rows may be read in place); weight16: the weight does
 inline LossPlan plan_loss(int64_t n, int64_t vocab, int64_t width, bool fp32, bool grid16, bool weight16, bool backward, bool want_dx, bool want_dw,

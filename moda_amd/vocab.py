@@ -77,8 +77,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
                          reduction: str = "mean") -> torch.Tensor:
     """Cross entropy of the logits ``scale * x @ weight.T`` (fp32, in pieces of the vocabulary, never stored) for rows ``x [.., width]``
     and their ``targets [..]``: fp32, a value for each row (``reduction="none"``), their ``"sum"``, or the ``"mean"`` over the rows that have
-    a target (0 where none has).  A row whose target is ``ignore_index`` or no word has none: its loss is 0, it is not read, whatever it
-    holds, and its gradient is 0; such rows cost no products from 129 rows on and in every backward pass.
+    a target (0 where none has).  A row whose target is ``ignore_index`` or no word has none: its loss is 0 and its gradient is 0, whatever
+    it holds, and it reaches no other; such rows cost no products from 513 rows on and in every backward pass.
 
     Differentiable once in ``x`` and ``weight``.  The backward pass computes the logits again and rounds their gradient to the tensors' type
     (fp32: not at all) for the two products that read it; besides its results it needs at most some GiB.  x and weight share one dtype."""
