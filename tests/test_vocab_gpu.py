@@ -219,6 +219,16 @@ def test_loss(dtype, n, vocab, width):
         check_loss(x, w, words(n, vocab, k, none), scale, reduction=reduction, seed=k)
 
 
+# sizes that take each of the tiles (csrc/vocab.h: choose_tiling) for each of the products, whole and split over their summation axis
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("n,vocab,width", [(700, 9000, 512), (1500, 5000, 264), (8200, 1100, 2056), (4100, 2100, 2056), (1500, 12000, 1032), (5003, 9001, 520),
+                                           (20, 30000, 1024)])
+def test_loss_by_tile(dtype, n, vocab, width):
+    x, w = rand(n, width, dtype=dtype, seed=n), rand(vocab, width, dtype=dtype, seed=vocab, std=2 * width ** -0.5)
+    check_loss(x, w, words(n, vocab, 1, 0.2))
+    check_loss(x, w, words(n, vocab, 2, 0.7), 0.6, reduction="none")
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=names)
 def test_loss_layouts(dtype):
     base, wide = rand(2, 9, 10, 200, dtype=dtype, seed=20), rand(120, 200, dtype=dtype, seed=21, std=0.2)
