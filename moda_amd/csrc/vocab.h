@@ -99,12 +99,14 @@ struct LossHead {
   float down;
 };
 
-// Rows with a target, one behind the other: their numbers, targets, factors and log sums, and the rows themselves as the products read
-// them (`planes` of 16-bit elements whose sum a row is, each [rows][x_ld], zeros behind a row's end).
+// What choose_tiling's estimate needs where the device chooses the splits (vocab_loss_kernel.hip: gather_rows_kernel).
 struct SplitRule {
   int tile_p, tiles_f, steps, at_once, most;  // a tile's rows, tiles of columns, steps of 64 words, workgroups; splits that there is room for at all rows
   float step_us, end_us, split_us;            // of a step, an item, a split of one row
 };
+
+// Rows with a target, one behind the other: their numbers, targets, factors and log sums, and the rows themselves as the products read
+// them (`planes` of 16-bit elements whose sum a row is, each [rows][x_ld], zeros behind a row's end).
 struct GatherArgs {
   Words words;
   const char* x;
@@ -211,7 +213,8 @@ struct TileTimes {
   ProductTile tile;
   double at_once, step_us, alone_us, end_us;
 };
-constexpr TileTimes kTileTimes[4] = {{kTileLarge, 256, 1.65, 1.65, 4}, {kTileMedium, 512, 1.04, 0.85, 3}, {kTileRows, 512, 0.51, 0.45, 2.5}, {kTileSmall, 768, 0.7, 0.45, 2.5}};
+constexpr TileTimes kTileTimes[4] = {
+    {kTileLarge, 256, 1.65, 1.65, 4}, {kTileMedium, 512, 1.04, 0.85, 3}, {kTileRows, 512, 0.51, 0.45, 2.5}, {kTileSmall, 768, 0.7, 0.45, 2.5}};
 inline Tiling choose_tiling(int64_t p, int64_t f, int64_t steps, bool may_split, bool may_few) {
   Tiling best = {kTileMedium, 1};
   double least = 1e30;
@@ -221,7 +224,8 @@ inline Tiling choose_tiling(int64_t p, int64_t f, int64_t steps, bool may_split,
     for (int s = 1; s <= 64; s *= 2) {
       if (s > 1 && (!may_split || steps < 4 * s)) break;
       const double items = (double)tiles * s, rounds = (double)((int64_t)((items + k.at_once - 1) / k.at_once));
-      const double us = rounds * ((double)((steps + s - 1) / s) * (items <= 256 ? k.alone_us : k.step_us) + k.end_us) + (s > 1 ? 4 + (double)s * p * f * 8 / 5e6 : 0);
+      const double us = rounds * ((double)((steps + s - 1) / s) * (items <= 256 ? k.alone_us : k.step_us) + k.end_us) +
+                        (s > 1 ? 4 + (double)s * p * f * 8 / 5e6 : 0);
       if (us < least) {
         least = us;
         best = {k.tile, s};

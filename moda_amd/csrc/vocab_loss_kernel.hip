@@ -330,7 +330,8 @@ hipError_t launch_gather_rows(const GatherArgs& a, int dtype, hipStream_t stream
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  MODA_BY_TYPE(gather_rows_kernel, dtype, a.words.n > 0 ? (a.words.n + kGatherBlock - 1) / kGatherBlock : 1, a);  // (one, for the head)
+  const int64_t blocks = (a.words.n + kGatherBlock - 1) / kGatherBlock;
+  MODA_BY_TYPE(gather_rows_kernel, dtype, blocks > 0 ? blocks : 1, a);  // (one, for the head)
   return hipGetLastError();
 }
 hipError_t launch_lay_rows(const LayArgs& a, int dtype, hipStream_t stream) {
