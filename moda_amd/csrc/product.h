@@ -21,7 +21,8 @@
 //
 // fp32 (PLANES): each operand as the sum of three bf16 (exact: 24 bits), of whose nine products the six largest are added up, the small
 // ones first; the others are below 2^-24 of the whole.  Six products of 16 bits at 1300 TFLOP/s are faster than one of the fp32 matrix
-// instruction (150).
+// instruction (150).  An infinite element is its own first piece, with zeros behind, and what it makes of the small products is no number; what it
+// is worth, infinite or NaN, is the product of the first pieces, so that sums of small products that are not finite are dropped before that one.
 #pragma once
 #include "../../include/moda_hip.h"
 #include "tile.h"
@@ -495,6 +496,17 @@ __global__ __launch_bounds__(64 * WF * WP, 2) void product_kernel(const ProductA
       for (int nb = 0; nb < NB; nb++) acc[mb][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int it = 0; it < n_steps; it++) {
       lds_cptr tile = smem + st * STAGE;
+      if (PLANES && it == 5 * t.steps) {  // the first pieces are next
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+          for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const float small = acc[mb][nb][i];
+              acc[mb][nb][i] = fabsf(small) < __builtin_huge_valf() ? small : 0.f;
+            }
+      }
       half_step(h0, h1, tile, 1, [&](int j) {
         if (j == PRODUCTS * 3 / 4) aim();
       });

@@ -290,6 +290,52 @@ def test_what_is_not_finite_stays_in_its_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("n,vocab,width", [(1, 300, 64), (150, 300, 64), (700, 9000, 512), (1500, 5000, 264), (40, 300000, 1024)])
+def test_words_that_a_weight_rules_out(dtype, n, vocab, width):
+    """A weight of minus infinity in a column where every row is positive: the word's logits are minus infinity, and all else is as without the word."""
+    x, w = rand(n, width, dtype=dtype, seed=n), rand(vocab, width, dtype=dtype, seed=vocab, std=2 * width ** -0.5)
+    x[:, 5] = x[:, 5].abs() + 0.1
+    gone = torch.zeros(vocab, dtype=torch.bool, device="cuda")
+    gone[::7] = gone[-1] = True
+    kept = (~gone).nonzero()[:, 0]
+    place = words(n, kept.numel(), 3, 0.2)  # targets among the words that are left
+    t = torch.where((place >= 0) & (place < kept.numel()), kept[place.clamp(0, kept.numel() - 1)], -100)
+    left = w[kept]
+    w[gone, 5] = -math.inf
+    ref = loss_reference(x, left, torch.where(t < 0, -100, place), 1.0, -100, "none", torch.ones(n, device="cuda"))
+    loss, lse = moda_amd.linear_cross_entropy_fwd(x, w, t, reduction="none")
+    within(loss, *ref["loss"], "loss")
+    within(lse, *ref["lse"], "lse")
+    dx, dw = moda_amd.linear_cross_entropy_bwd(x, w, t, lse, torch.ones(n, device="cuda"), reduction="none")
+    assert not dw[gone].any()
+    within(dw[kept], *ref["dw"], "dw")
+    # the probability of a word that is ruled out is zero, and so is what its weights add, but for the infinite one: zero times that is NaN
+    other = torch.arange(width, device="cuda") != 5
+    within(dx[:, other], *(v[:, other] for v in ref["dx"]), "dx")
+    assert dx[t >= 0, 5].isnan().all() and not dx[t < 0].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+def test_infinite_products_keep_their_sign(dtype):
+    """A row and a weight that meet at an infinite element: what is left of the row's log sum says which way each logit went."""
+    x, w = rand(6, 64, dtype=dtype, seed=33), rand(40, 64, dtype=dtype, seed=34, std=0.3)
+    t = torch.zeros(6, dtype=torch.long, device="cuda")
+    w[:, 7] = -w[:, 7].abs() - 0.125  # (away from zero, where rounding takes an element apart)
+    x[0, 7], x[1, 7], x[2, 7], x[3, 7] = math.inf, -math.inf, math.nan, 0.0
+    z = x.double() @ w.double().T
+    loss, lse = moda_amd.linear_cross_entropy_fwd(x, w, t, reduction="none")
+    want = torch.logsumexp(z, -1) - z[:, 0]  # all minus infinity, all infinite, NaN: no number; the others are their own
+    assert torch.equal(loss.isnan(), want.isnan()) and loss[3:].isfinite().all() and loss[:3].isnan().all()
+    w[20:, 7] = 0.0
+    w[:20, 7] = -math.inf
+    x[:, 7] = x[:, 7].nan_to_num(1.0, 1.0, 1.0).abs() + 0.5
+    t += 30
+    assert moda_amd.linear_cross_entropy_fwd(x, w, t, reduction="none")[0].isfinite().all()
+    x[0, 7] = -1.0  # of infinite logits the loss is no number
+    assert moda_amd.linear_cross_entropy_fwd(x, w, t, reduction="none")[0].isnan().tolist() == [True] + [False] * 5
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
 def test_large_logits(dtype):
     """Logits of some hundreds: the likeliest word has all of the sum, and exponentials of the others leave fp32's range."""
     x, w, t = rand(140, 64, dtype=dtype, seed=38, std=8.0), rand(500, 64, dtype=dtype, seed=39, std=6.0), words(140, 500, 40)
