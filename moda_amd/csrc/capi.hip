@@ -1139,19 +1139,29 @@ int moda_hip_vocab_loss_fwd(const moda_hip_vocab_loss_args* t, void* workspace, 
   float* losses = rows_out ? t->loss : v.at<float>(v.p.losses);
   if (!v.p.direct) MODA_TRY(v.gather());
   const int64_t tile = moda::tile_f(v.p.logits.tile);
-  for (int64_t i = 0; i < v.p.pieces; i++) {
+  for (int64_t i = 0; i < v.p.pieces && t->rows > 0; i++) {
     moda::ProductArgs w = {};
     MODA_TRY(v.weights(i, w));
     moda::ProductArgs a = v.logits(i, w);
-    a.stats = v.at<float2>(v.p.stats) + i * ((v.p.piece + tile - 1) / tile) * t->rows;
+    a.stats = v.at<float2>(v.p.stats);
     a.stats_ld = t->rows;
     a.target_logit = v.at<float>(v.p.target_logit);
     MODA_TRY(moda::launch_stats(a, t->dtype, v.p.logits.tile, v.compute_units, v.stream));
+    moda::JoinStatsArgs j = {};
+    j.stats = a.stats;
+    j.target_logit = a.target_logit;
+    j.stats_ld = a.stats_ld;
+    j.tiles = (a.f_count + tile - 1) / tile;
+    j.carry = v.p.pieces > 1 ? v.at<float2>(v.p.carry) : nullptr;
+    j.first = i == 0;
+    j.last = i == v.p.pieces - 1;
+    j.head = a.head;
+    j.words = a.words;
+    j.row_of = v.at<int>(v.p.row_of);
+    j.loss = losses;
+    j.lse = t->lse;
+    MODA_TRY(moda::launch_join_stats(j, v.stream));
   }
-  const int64_t last = (v.piece_words(v.p.pieces - 1) + tile - 1) / tile;
-  moda::JoinStatsArgs j = {v.at<float2>(v.p.stats), v.at<float>(v.p.target_logit), t->rows, (v.p.pieces - 1) * ((v.p.piece + tile - 1) / tile) + last,
-                           v.head(), v.words(), v.at<int>(v.p.row_of), losses, t->lse};
-  if (t->rows > 0) MODA_TRY(moda::launch_join_stats(j, v.stream));
   if (!rows_out) MODA_TRY(moda::launch_loss_total({losses, t->loss, v.words(), v.head(), t->reduction == MODA_HIP_LOSS_MEAN}, v.stream));
   return MODA_HIP_OK;
 }

@@ -165,9 +165,11 @@ struct ProductArgs {
 };
 
 struct JoinStatsArgs {
-  const float2* stats;
+  const float2* stats;  // of one piece of the vocabulary
   const float* target_logit;
   int64_t stats_ld, tiles;
+  float2* carry;  // [rows]: of the pieces before it, then with it (or NULL: one piece is all)
+  int first, last;
   const LossHead* head;
   Words words;
   const int* row_of;
@@ -243,9 +245,9 @@ struct LossPlan {
   int64_t piece, pieces;          // words at once
   int64_t dz_ld;
   Tiling logits, grad_rows, grad_weight;
-  int64_t stat_tiles, acc_ld;
+  int64_t stat_tiles, acc_ld;  // stat_tiles: of a piece
   bool acc_rows;  // the gradient of the rows is added up in fp32
-  size_t head, row_of, target, factor, lse, target_logit, counts, largest, stats, rows, weight, dz, dx_acc, dw_acc, losses, bytes;
+  size_t head, row_of, target, factor, lse, target_logit, counts, largest, stats, carry, rows, weight, dz, dx_acc, dw_acc, losses, bytes;
 };
 
 constexpr int64_t kGatherBlock = 8, kCountBlock = 1024, kScanMost = 4096;
@@ -278,7 +280,7 @@ inline LossPlan plan_loss(int64_t n, int64_t vocab, int64_t width, bool fp32, bo
   p.dz_ld = (p.piece + 63) / 64 * 64;
   const int pairs = fp32 ? 6 : 1;
   p.logits = choose_tiling(n, p.piece, (p.k + 63) / 64 * pairs, false, true);
-  p.stat_tiles = p.pieces * ((p.piece + tile_f(p.logits.tile) - 1) / tile_f(p.logits.tile));
+  p.stat_tiles = (p.piece + tile_f(p.logits.tile) - 1) / tile_f(p.logits.tile);
   p.acc_ld = p.rows_ld;
   p.grad_rows = choose_tiling(n, width, (p.piece + 63) / 64 * pairs, true, true);
   p.grad_weight = choose_tiling(p.piece, width, (n + 63) / 64 * pairs, true, false);
@@ -300,7 +302,8 @@ inline LossPlan plan_loss(int64_t n, int64_t vocab, int64_t width, bool fp32, bo
   p.rows = take(gathers, n * p.rows_ld * 2 * p.planes);
   p.weight = take(p.copy_weight, p.piece * p.rows_ld * 2 * p.planes);
   p.target_logit = take(!backward, n * 4);
-  p.stats = take(!backward, p.stat_tiles * n * 8);
+  p.stats = take(!backward, p.stat_tiles * n * 8);  // (of a piece, which by_grid bounds: 2 GiB at most)
+  p.carry = take(!backward && p.pieces > 1, n * 8);
   p.losses = take(!backward && reduce, n * 4);
   p.dz = take(backward, n * p.dz_ld * 2 * p.planes);
   p.dx_acc = take(backward && want_dx && p.acc_rows, p.grad_rows.splits * n * p.acc_ld * 4);

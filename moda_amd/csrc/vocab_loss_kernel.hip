@@ -3,8 +3,9 @@
 //   dz[n][v] = g[n] (exp(z[n][v] - lse[n]) - [v = t_n]),  dx = s dz W,  dW = s dz^T x
 // Rows without a target are left out from the start: the others are laid one behind the other first (gather_rows_kernel), so that what is
 // in the rows left out, NaN included, reaches nothing and costs nothing.  The logits leave the registers as a largest value and a sum of
-// exponentials for every tile of words, which a second launch joins in the words' order.  The backward pass computes them once more, a piece
-// of the vocabulary at a time, and keeps that piece's gradient in 16 bits (fp32: 48) for the two products that read it.
+// exponentials for every tile of words, which a second launch joins in the words' order, behind what the pieces of the vocabulary before have
+// come to.  The backward pass computes them once more, a piece of the vocabulary at a time, and keeps that piece's gradient in 16 bits (fp32: 48)
+// for the two products that read it.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -226,6 +227,11 @@ __global__ __launch_bounds__(256) void join_stats_kernel(const JoinStatsArgs a) 
   const int rows = a.head ? a.head->live : (int)a.words.n;
   const int64_t p = (int64_t)workgroup() * ROWS + r;
   float m = kNegInf, s = 0.f;
+  if (part == 0 && p < rows && !a.first) {
+    const float2 before = a.carry[p];
+    m = before.x;
+    s = before.y;
+  }
   const auto add = [](float& m, float& s, float xm, float xs) {  // (a sum of no logit above minus infinity is zero, or NaN)
     if (xm > m) {
       s = (m == kNegInf ? s : s * fast_exp2(m - xm)) + xs;
@@ -250,6 +256,10 @@ __global__ __launch_bounds__(256) void join_stats_kernel(const JoinStatsArgs a) 
     __syncthreads();
   }
   if (part != 0 || p >= rows) return;
+  if (!a.last) {
+    a.carry[p] = float2{m, s};
+    return;
+  }
   const float log_sum = log2f(s);
   float lse = m + log_sum;
   const int word = a.head ? 0 : a.words.of(p);

@@ -83,6 +83,16 @@ def test_workspaces_stay_bounded(lib):
         assert max(sizes) < 6 << 30, sizes
 
 
+@pytest.mark.parametrize("dtype", [0, 2])
+@pytest.mark.parametrize("rows", [1, 4096, 1 << 15])
+def test_forward_workspaces_stay_bounded(lib, dtype, rows):
+    """Statistics of a piece of the vocabulary at a time (2 GiB at most, 8 bytes for each row and tile of words), and of fp32 weights a GiB laid out anew."""
+    need = lambda v: lib.moda_hip_vocab_loss_fwd_workspace_bytes(ctypes.byref(args(dtype=dtype, rows=rows, width=1024, ld_x=1024, ld_weight=1024, vocab=v)))  # noqa: E731
+    sizes = [need(v) for v in (1 << 17, 1 << 20, 1 << 24, 1 << 30)]
+    assert max(sizes) < (2 << 30) + (1 << 30) + rows * 1024 * 6 + (1 << 20), sizes
+    assert sizes[3] <= 2 * sizes[2], sizes  # pieces of 2^21 words at most
+
+
 @pytest.mark.parametrize("change,rc", [
     (dict(dtype=5), EINVAL), (dict(n=-1), EINVAL), (dict(vocab=0), EINVAL), (dict(width=0), EINVAL), (dict(tokens=None), EINVAL), (dict(at=None), EINVAL),
     (dict(out=None), EINVAL), (dict(ld_out=7), EINVAL), (dict(ld=-1), EINVAL), (dict(scale=float("nan")), EINVAL), (dict(tokens=4), EALIGN),

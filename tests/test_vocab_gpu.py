@@ -364,6 +364,31 @@ def test_many_rows_and_words(dtype, n, vocab, width):
     check_loss(x, w, words(n, vocab, 46, 0.3), reduction="mean")
 
 
+@pytest.mark.parametrize("dtype,n,vocab,width", [(torch.bfloat16, 21, (1 << 22) + 777, 8), (torch.float16, 40, (1 << 21) + 1, 20), (torch.float32, 9, 600001, 1024)], ids=str)
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_statistics_of_several_pieces(dtype, n, vocab, width, reduction):
+    """Three and more pieces of the vocabulary in the forward pass, the last of them short; targets at their borders; words whose logits are minus
+    infinity throughout a piece, and rows whose largest logits are in the first or in the last one."""
+    x, w = rand(n, width, dtype=dtype, seed=n), rand(vocab, width, dtype=dtype, seed=vocab, std=width ** -0.5)
+    x[:, 3] = x[:, 3].abs() + 0.5
+    w[100] = x[1] * 4 / x[1].float().norm()
+    w[-1] = x[2] * 4 / x[2].float().norm()
+    t = words(n, vocab, 46, 0.2)
+    t[:6] = torch.tensor([0, vocab - 1, vocab - 1, 1 << 20, (1 << 21) - 1, vocab // 2], device="cuda")
+    ref = loss_reference(x, w, t, 1.0, -100, reduction)
+    loss, lse = moda_amd.linear_cross_entropy_fwd(x, w, t, reduction=reduction)
+    within(lse, *ref["lse"], "lse")
+    within(loss, *ref["loss"], "loss")
+    # all words of the first half, whole pieces among them, ruled out
+    half = vocab // 2
+    w[:half, 3] = -math.inf
+    t[t < half] = -100
+    ref = loss_reference(x, w[half:], torch.where(t >= 0, t - half, -100), 1.0, -100, reduction)
+    loss, lse = moda_amd.linear_cross_entropy_fwd(x, w, t, reduction=reduction)
+    within(lse, *ref["lse"], "lse")
+    within(loss, *ref["loss"], "loss")
+
+
 @pytest.mark.parametrize("what", ["x", "w"])
 def test_only_one_gradient(what):
     x, w, t = rand(200, 64, dtype=torch.bfloat16, seed=47), rand(600, 64, dtype=torch.bfloat16, seed=48), words(200, 600, 49, 0.1)
