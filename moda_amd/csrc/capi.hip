@@ -1115,6 +1115,13 @@ int begin_vocab_loss(const moda_hip_vocab_loss_args* t, bool backward, void* wor
   if (!t->weight || (t->rows > 0 && (!t->x || !t->lse))) return MODA_HIP_EINVAL;
   const int es = elem_size(t->dtype);
   if ((uintptr_t)t->x % es != 0 || (uintptr_t)t->weight % es != 0 || (uintptr_t)t->lse % 4 != 0) return MODA_HIP_EALIGN;
+  if (backward) {
+    if ((t->rows > 0 && !t->d_loss) || (t->dx && t->ld_dx < t->width) || (t->d_weight && t->ld_d_weight < t->width)) return MODA_HIP_EINVAL;
+    if ((uintptr_t)t->d_loss % 4 != 0 || (uintptr_t)t->dx % es != 0 || (uintptr_t)t->d_weight % es != 0) return MODA_HIP_EALIGN;
+  } else {
+    if (!t->loss && (t->rows > 0 || t->reduction != MODA_HIP_LOSS_ROWS)) return MODA_HIP_EINVAL;
+    if ((uintptr_t)t->loss % 4 != 0) return MODA_HIP_EALIGN;
+  }
   if (v.p.bytes > 0 && (!workspace || workspace_bytes < v.p.bytes)) return MODA_HIP_EWORKSPACE;
   if ((uintptr_t)workspace % 256 != 0) return MODA_HIP_EALIGN;
   v.t = t;
@@ -1133,8 +1140,6 @@ int moda_hip_vocab_loss_fwd(const moda_hip_vocab_loss_args* t, void* workspace, 
   const int rc = begin_vocab_loss(t, false, workspace, workspace_bytes, stream, v);
   if (rc) return rc;
   const bool rows_out = t->reduction == MODA_HIP_LOSS_ROWS;
-  if (!t->loss && (t->rows > 0 || !rows_out)) return MODA_HIP_EINVAL;
-  if ((uintptr_t)t->loss % 4 != 0) return MODA_HIP_EALIGN;
   if (t->rows == 0 && rows_out) return MODA_HIP_OK;
   float* losses = rows_out ? t->loss : v.at<float>(v.p.losses);
   if (!v.p.direct) MODA_TRY(v.gather());
@@ -1171,8 +1176,6 @@ int moda_hip_vocab_loss_bwd(const moda_hip_vocab_loss_args* t, void* workspace, 
   const int rc = begin_vocab_loss(t, true, workspace, workspace_bytes, stream, v);
   if (rc) return rc;
   const int es = elem_size(t->dtype);
-  if ((t->rows > 0 && !t->d_loss) || (t->dx && t->ld_dx < t->width) || (t->d_weight && t->ld_d_weight < t->width)) return MODA_HIP_EINVAL;
-  if ((uintptr_t)t->d_loss % 4 != 0 || (uintptr_t)t->dx % es != 0 || (uintptr_t)t->d_weight % es != 0) return MODA_HIP_EALIGN;
   if (!t->dx && !t->d_weight) return MODA_HIP_OK;
   const moda::LossPlan& p = v.p;
   // four results of a row are stored as one where they lie on that grid

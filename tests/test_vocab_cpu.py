@@ -75,6 +75,15 @@ def test_backward_arguments(lib):
         assert run(**change) in (rc, -6)  # (-6: the device is asked for first)
 
 
+@pytest.mark.parametrize("which,change,rc", [
+    ("fwd", dict(loss=None), EINVAL), ("fwd", dict(loss=None, reduction=0), EINVAL), ("fwd", dict(loss=None, rows=0), EINVAL), ("fwd", dict(loss=258), EALIGN),
+    ("bwd", dict(d_loss=None), EINVAL), ("bwd", dict(ld_dx=63), EINVAL), ("bwd", dict(ld_d_weight=63), EINVAL), ("bwd", dict(dx=4097), EALIGN),
+    ("bwd", dict(d_weight=8193), EALIGN), ("bwd", dict(d_weight=8194, dtype=2), EALIGN), ("bwd", dict(d_loss=258), EALIGN)])
+def test_arguments_of_one_pass(lib, which, change, rc):
+    """Refused before anything asks for a device, so that the code is the argument's own on any machine."""
+    assert getattr(lib, "moda_hip_vocab_loss_" + which)(ctypes.byref(args(**change)), 256, 1 << 40, None) == rc
+
+
 def test_workspaces_stay_bounded(lib):
     """Of pieces: a GiB for the logits' gradient, as much for the weight laid out anew, whatever the vocabulary."""
     for dtype in (0, 2):
