@@ -1025,13 +1025,15 @@ std::pair<OptTensor, OptTensor> apply_rotary(const OptTensor& q, const OptTensor
 // paged key/value cache (moda_amd/paged.py)
 // ------------------------------------------------------------------------------------------------------------------
 
+void no_tangents(std::initializer_list<const Tensor*> xs, const char* what) {
+  const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* x : xs)
+    CONTRACT(!x->defined() || !forward || !x->_fw_grad(0).defined(), what, " has no forward-mode derivative: it would drop the tangent it is given");
+}
 void no_gradients(std::initializer_list<const Tensor*> xs, const char* what) {
-  const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
-  for (const Tensor* x : xs) {
-    if (!x->defined()) continue;
-    CONTRACT(!backward || !x->requires_grad(), what, " has no backward pass: call it under torch.no_grad()");
-    CONTRACT(!forward || !x->_fw_grad(0).defined(), what, " has no forward-mode derivative: it would drop the tangent it is given");
-  }
+  const bool backward = at::GradMode::is_enabled();
+  for (const Tensor* x : xs) CONTRACT(!x->defined() || !backward || !x->requires_grad(), what, " has no backward pass: call it under torch.no_grad()");
+  no_tangents(xs, what);
 }
 
 const int32_t* counts(const Tensor& x, const char* name, std::initializer_list<int64_t> shape, const Tensor& cache) {
@@ -1475,11 +1477,14 @@ PYBIND11_MODULE(_host, m) {
   m.def("linear_cross_entropy", &linear_cross_entropy);
   m.def("linear_cross_entropy_fwd", [](const Tensor& x, const Tensor& weight, const Tensor& targets, double scale, int64_t ignore_index, int reduction) {
     py::gil_scoped_release nogil;
+    no_tangents({&x, &weight}, "linear_cross_entropy_fwd");
     return loss_forward(*make_cross_entropy(scale, ignore_index, reduction), x, weight, targets);
   });
   m.def("linear_cross_entropy_bwd", [](const Tensor& x, const Tensor& weight, const Tensor& targets, const Tensor& lse, const Tensor& d_loss, double scale,
                                        int64_t ignore_index, int reduction, bool want_dx, bool want_dw) {
     py::gil_scoped_release nogil;
+    no_tangents({&x, &weight}, "linear_cross_entropy_bwd");
+    no_gradients({&lse, &d_loss}, "linear_cross_entropy_bwd");
     const auto r = loss_backward(*make_cross_entropy(scale, ignore_index, reduction), x, weight, targets, lse, d_loss, want_dx, want_dw);
     return std::make_pair(optional(r.first), optional(r.second));
   });

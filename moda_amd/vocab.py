@@ -92,13 +92,14 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
 def linear_cross_entropy_fwd(x, weight, targets, scale: float = 1.0, ignore_index: int = -100,
                              reduction: str = "mean") -> Tuple[torch.Tensor, torch.Tensor]:
     """``linear_cross_entropy`` with the rows' log sums: ``(loss, lse)``, lse fp32 ``[..]`` in base 2 as ``parallel_moda_fwd``'s, 0 for rows
-    without a target."""
+    without a target.  As there, no graph is recorded: x and weight count as constants (a forward-mode tangent is refused)."""
     _check_device(weight)
     return _lib.host().linear_cross_entropy_fwd(x, weight, targets, scale, ignore_index, _reduction(reduction))
 
 
 def linear_cross_entropy_bwd(x, weight, targets, lse, d_loss, scale: float = 1.0, ignore_index: int = -100, reduction: str = "mean",
                              need_dx: bool = True, need_dweight: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
-    """``(dx, dweight)`` from what ``linear_cross_entropy_fwd`` was given and returned and the loss's gradient ``d_loss`` (of its shape)."""
+    """``(dx, dweight)`` from what ``linear_cross_entropy_fwd`` was given and returned and the loss's gradient ``d_loss`` (of its shape).
+    x and weight count as constants; an lse or a d_loss that requires gradients is refused, and so is any tangent."""
     _check_device(weight)
     return _lib.host().linear_cross_entropy_bwd(x, weight, targets, lse, d_loss, scale, ignore_index, _reduction(reduction), need_dx, need_dweight)

@@ -509,6 +509,28 @@ def test_forward_mode_is_refused():
                 call()
 
 
+def test_derivatives_are_not_dropped():
+    """The two passes by themselves record nothing: what a caller could hope to differentiate is refused, but for rows and weight, which are constants."""
+    x, w, t = rand(4, 16, dtype=torch.float32, seed=120), rand(9, 16, dtype=torch.float32, seed=121), words(4, 9, 122)
+    one = torch.ones((), device="cuda")
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss, lse = moda_amd.linear_cross_entropy_fwd(xg, wg, t)
+    assert not loss.requires_grad and not lse.requires_grad
+    assert not any(g.requires_grad for g in moda_amd.linear_cross_entropy_bwd(xg, wg, t, lse, one))
+    for late in ((lse.clone().requires_grad_(), one), (lse, one.clone().requires_grad_())):
+        with pytest.raises(AssertionError, match="no backward pass"):
+            moda_amd.linear_cross_entropy_bwd(x, w, t, *late)
+        with torch.no_grad():
+            moda_amd.linear_cross_entropy_bwd(x, w, t, *late)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda a: torch.autograd.forward_ad.make_dual(a, torch.ones_like(a))  # noqa: E731
+        for call in (lambda: moda_amd.linear_cross_entropy_fwd(dual(x), w, t), lambda: moda_amd.linear_cross_entropy_fwd(x, dual(w), t),
+                     lambda: moda_amd.linear_cross_entropy_bwd(dual(x), w, t, lse, one), lambda: moda_amd.linear_cross_entropy_bwd(x, dual(w), t, lse, one),
+                     lambda: moda_amd.linear_cross_entropy_bwd(x, w, t, dual(lse), one), lambda: moda_amd.linear_cross_entropy_bwd(x, w, t, lse, dual(one))):
+            with pytest.raises(AssertionError, match="tangent"):
+                call()
+
+
 def test_refusals():
     x, w, t = rand(4, 16, dtype=torch.bfloat16, seed=123), rand(9, 16, dtype=torch.bfloat16, seed=124), words(4, 9, 125)
     for call in (lambda: moda_amd.embed_tokens(t.float(), w), lambda: moda_amd.embed_tokens(t.cpu(), w), lambda: moda_amd.embed_tokens(t, w[0]),
