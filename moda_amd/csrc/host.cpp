@@ -1228,10 +1228,10 @@ struct Rows {
   Tensor x;
   int64_t n, width, ld;
 };
-Rows rows_of(const Tensor& in, bool may_copy = true) {
+Rows rows_of(const Tensor& in) {
   const int64_t width = in.size(-1);
   Tensor x = in.dim() == 2 ? in : in.reshape({width > 0 ? in.numel() / width : 0, width});
-  if (may_copy && x.size(1) > 1 && x.stride(1) != 1) x = x.contiguous();
+  if (x.size(1) > 1 && x.stride(1) != 1) x = x.contiguous();
   return {x, x.size(0), width, x.stride(0)};
 }
 Tensor words_of(const Tensor& in, const char* name, const Tensor& beside) {
