@@ -219,7 +219,7 @@ def test_loss(dtype, n, vocab, width):
         check_loss(x, w, words(n, vocab, k, none), scale, reduction=reduction, seed=k)
 
 
-# sizes that take each of the tiles (csrc/vocab.h: choose_tiling) for each of the products, whole and split over their summation axis
+# sizes of several tiles (csrc/vocab.h: choose_tiling), whole and split over their summation axis; TILES has each of them for each of the products
 @pytest.mark.parametrize("dtype", DTYPES, ids=names)
 @pytest.mark.parametrize("n,vocab,width", [(700, 9000, 512), (1500, 5000, 264), (8200, 1100, 2056), (4100, 2100, 2056), (1500, 12000, 1032), (5003, 9001, 520),
                                            (20, 30000, 1024)])
@@ -227,6 +227,30 @@ def test_loss_by_tile(dtype, n, vocab, width):
     x, w = rand(n, width, dtype=dtype, seed=n), rand(vocab, width, dtype=dtype, seed=vocab, std=2 * width ** -0.5)
     check_loss(x, w, words(n, vocab, 1, 0.2))
     check_loss(x, w, words(n, vocab, 2, 0.7), 0.6, reduction="none")
+
+
+TILES = [  # what test_vocab_plan_cpu.py holds to take each tile, the rows read in place or not, for each product, whole and in sums
+    # up to 512 rows of 16 bits are read where they are
+    (509, 4099, 1000), (250, 13000, 520), (80, 50257, 512), (512, 66000, 1032), (511, 4099, 136), (512, 4099, 136), (513, 4099, 136), (397, 20011, 40), (5, 1100, 40),
+    # the rows' gradient as it leaves the registers and by sums, the weight's
+    (8200, 33, 1000), (3001, 33, 1032), (8200, 33, 40), (12001, 700, 40), (20001, 129, 40), (2100, 1100, 40), (2100, 1100, 72), (4100, 4099, 72), (3000, 9001, 264),
+    (8200, 129, 1032), (12000, 129, 2056), (1000, 33, 40), (1, 50257, 40), (1, 30000, 264), (513, 129, 2056),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("n,vocab,width", TILES)
+def test_loss_by_each_tile(dtype, n, vocab, width):
+    """Rows and weight inside wider ones, on the 16-byte grid; some rows without a target, which hold anything."""
+    x, w = rand(n, width + 24, dtype=dtype, seed=n)[:, 8:width + 8], rand(vocab, width + 16, dtype=dtype, seed=vocab, std=2 * width ** -0.5)[:, 16:]
+    t = words(n, vocab, 1, 0.3)
+    t[0] = vocab - 1
+    loss, dx, dw = check_loss(x, w, t, 0.8, reduction="none")
+    gone = (t < 0) | (t >= vocab)
+    assert not loss[gone].any() and not dx[gone].any()
+    x[gone] = math.nan
+    again = check_loss(x, w, t, 0.8, reduction="none")
+    assert all(torch.equal(a, b) for a, b in zip((loss, dx, dw), again))
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=names)
