@@ -2,6 +2,7 @@
 
 Tolerances are bounds on each element, from the roundings that a kernel makes: u = eps / 2 of the tensors' type for a result (and, in the
 backward pass of the cross entropy, for the gradient of a logit), 2^-24 for an fp32 operation, of which a sum of n terms has n."""
+import contextlib
 import math
 
 import pytest
@@ -473,6 +474,48 @@ def test_captured_calls_follow_their_inputs():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+def test_captured_backward():
+    """Both ends around torch's own sum, one weight for both, with autograd's engine in the capture; leaves are made in the captured step."""
+    w = rand(900, 128, dtype=torch.bfloat16, seed=73, std=0.1)
+    t, x = words(300, 900, 74, 0.2), rand(300, 128, dtype=torch.bfloat16, seed=75)
+
+    def step():
+        xg, wg = x.detach().requires_grad_(), w.detach().requires_grad_()
+        loss = moda_amd.linear_cross_entropy(xg + moda_amd.embed_tokens(t, wg, 2.0), wg, t)
+        return [loss.detach(), *torch.autograd.grad(loss, (xg, wg))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(4):
+        t.copy_(words(300, 900, 80 + k, 0.2 * k))
+        x.copy_(rand(300, 128, dtype=torch.bfloat16, seed=90 + k))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+def test_compiled_autograd():
+    """Compiled autograd runs the nodes from a graph of its own: the same bits."""
+    import torch._dynamo.compiled_autograd as compiled
+
+    x, w, t = rand(40, 64, dtype=torch.bfloat16, seed=76), rand(90, 64, dtype=torch.bfloat16, seed=77, std=0.1), words(40, 90, 78, 0.2)
+    grads = []
+    for k in range(3):
+        xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = moda_amd.linear_cross_entropy(xg + moda_amd.embed_tokens(t, wg, 2.0), wg, t, reduction="sum")
+        with compiled._enable(lambda graph: graph) if k else contextlib.nullcontext():
+            loss.backward()
+        grads.append((xg.grad, wg.grad))
+    assert all(torch.equal(a, b) for g in grads[1:] for a, b in zip(grads[0], g))
 
 
 def test_calls_on_two_streams():
