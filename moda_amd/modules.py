@@ -337,8 +337,9 @@ class MoDAStack(nn.Module):
         """The negative log-likelihood (fp32) of the words ``targets [..]`` given the rows ``y [.., dim]`` that ``forward``, ``prefill`` or ``decode``
         returned for the tokens before them; see ``linear_cross_entropy``."""
         assert self.vocab is not None, "a stack of rows has no vocabulary: construct with vocab"
-        return linear_cross_entropy(self.out_norm(y), self.embedding if self.head is None else self.head, targets, ignore_index=ignore_index,
-                                    reduction=reduction)
+        weight = self.embedding if self.head is None else self.head
+        # (autocast runs the norm in fp32, whatever its weights are in)
+        return linear_cross_entropy(self.out_norm(y).to(weight.dtype), weight, targets, ignore_index=ignore_index, reduction=reduction)
 
     def loss(self, tokens: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100, reduction: str = "mean",
              positions: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -47,6 +47,22 @@ def test_training_step(dtype, tied):
         within(got, *ref[name], name)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=names)
+@pytest.mark.parametrize("compute", [torch.bfloat16, torch.float16], ids=names)
+def test_training_step_under_autocast(dtype, compute):
+    """Parameters of any type: the norm before the loss comes out in fp32, the loss is computed in the weight's type."""
+    m = model(dtype, True)
+    tokens, targets = words(150, 517, 1, 0.1).view(2, 75), words(150, 517, 2, 0.3).view(2, 75)
+    with torch.autocast("cuda", dtype=compute):
+        loss = m.loss(tokens, targets)
+        rows = m.out_norm(m(tokens)).detach()
+    loss.backward()
+    assert rows.dtype == torch.float32 and loss.dtype == torch.float32
+    assert all(p.grad.dtype == dtype and p.grad.isfinite().all() for p in m.parameters() if p.grad is not None) and m.embedding.grad is not None
+    with torch.no_grad():
+        assert torch.equal(loss.detach(), moda_amd.linear_cross_entropy(rows.to(dtype), m.embedding, targets))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=names)
 @pytest.mark.parametrize("rotary", [True, False])
 def test_tokens_are_their_rows(dtype, rotary):
