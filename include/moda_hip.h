@@ -445,8 +445,10 @@ int moda_hip_embed_grad(int32_t dtype, const void* tokens, int32_t tokens64, int
  * moda_hip_vocab_loss_bwd: from the same arguments, lse as the forward pass left it and d_loss (fp32, [rows] or one value):
  *   dz[v] = d_loss * (exp(z[v] - lse) - [v = target]) (mean: over the number of rows that count), rounded to the tensors' type (fp32: not),
  *   dx = scale * dz weight, d_weight = scale * dz^T x (either may be NULL: not wanted).
- * dz is rounded relative to the largest |d_loss|, by which the products are multiplied (fp16: and 2^14 times as large).  The vocabulary is taken in pieces such that a piece of dz, and
- * where it has to be laid out anew (fp32, rows off the 16-byte grid or 4 MiB and more apart) of the weight, keeps within 1 GiB (256 words at least).
+ * dz is rounded relative to the largest |d_loss|, by which the products are multiplied (fp16: and 2^14 times as large, so that what is below
+ * 2^-28 of the largest |d_loss| loses bits).  The vocabulary is taken in pieces such that a piece of dz, and where it has to be laid out anew
+ * (fp32, rows off the 16-byte grid or 4 MiB and more apart) of the weight, keeps within 1 GiB (256 words at least) and the forward pass's
+ * statistics within 2.
  * Workspace of ..._workspace_bytes (which reads the sizes, strides and pointers of its arguments), 256-byte boundary, not initialised; one for
  * each call that may overlap another.  rows below 2^24, vocab below 2^31 - 256, width up to 2^16; MODA_HIP_EUNSUPPORTED otherwise.
  */

@@ -1,7 +1,9 @@
 // The matrix products of the cross entropy over a vocabulary, out[p][f] = sum_k P(p, k) F(f, k), and what is done with a result before it
 // leaves the registers:
 //   kStats        logits (f: words, p: rows, k: columns): their largest and the sum of their exponentials a row, a target's own
-//   kGradLogits   logits once more: their gradient, rounded to 16 bits (fp32: three of them)
+//   kGradLogits   logits once more: their gradient, rounded to 16 bits (fp32: three of them).  In the tensors' own type, so that the two products
+//                 that read it are ones of 16 bits: in three pieces they would be three each.  8192 x 32000 x 2048, bf16: gradients 0.0019 from 64
+//                 bits (norms), where the rounding of the results alone leaves 0.0017
 //   kGradRows     f: columns, p: rows, k: words: the gradient of the rows
 //   kGradWeight   f: columns, p: words, k: rows: the gradient of the weight
 // An operand lies in memory either with k innermost (a tile of 64 k and as many rows as the result's tile has) or with f or p innermost
@@ -11,9 +13,9 @@
 //
 // f sits on the matrix instruction's A side: a lane has four neighbouring f of one p.
 //
-// Bound by the matrix pipe at the clock that the power limit leaves: 8192 rows, 32000 words, width 2048, bf16: statistics 823 us (1305
-// TFLOP/s), gradient of the logits 895, of the rows 798, of the weight 848, the pipe busy 55 to 62 % of the cycles at 2.0 to 2.1 GHz; plain library
-// products of these shapes 754, 754, 796 and 1104.  What it took (us of the four, one after the other): a workgroup for each tile, operands read
+// Bound by the matrix pipe at the clock that the power limit leaves: 8192 rows, 32000 words, width 2048, bf16: statistics 836 us (1284
+// TFLOP/s), gradient of the logits 880, of the rows 804, of the weight 865, once the clock has settled (sixty passes in a row, the last twenty), the
+// pipe busy 55 to 62 % of the cycles at 2.0 to 2.1 GHz; plain library products of these shapes 754, 754, 796 and 1104.  What it took (us of the four, one after the other): a workgroup for each tile, operands read
 // and then multiplied 926, 1010, 822, 934; workgroups that stay, so that the first loads of a tile are on their way during the end of the one
 // before; operands of the next half step read among the products of this one (861, 964, 836, 850: fewer cycles at a lower clock); the loads'
 // addresses advanced on the scalar unit among the products and the loads sent right behind the barrier.  Stages of 32 k, four of them: 4 - 8 %

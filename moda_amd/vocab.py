@@ -78,10 +78,18 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     """Cross entropy of the logits ``scale * x @ weight.T`` (fp32, in pieces of the vocabulary, never stored) for rows ``x [.., width]``
     and their ``targets [..]``: fp32, a value for each row (``reduction="none"``), their ``"sum"``, or the ``"mean"`` over the rows that have
     a target (0 where none has).  A row whose target is ``ignore_index`` or no word has none: its loss is 0 and its gradient is 0, whatever
-    it holds, and it reaches no other; such rows cost no products from 513 rows on and in every backward pass.
+    it holds, and it reaches no other; such rows are left out of the products (but up to 512 rows of 16 bits are scored where they lie).
 
-    Differentiable once in ``x`` and ``weight``.  The backward pass computes the logits again and rounds their gradient to the tensors' type
-    (fp32: not at all) for the two products that read it; besides its results it needs at most some GiB.  x and weight share one dtype."""
+    Differentiable once in ``x`` and ``weight``, which share one dtype.  The backward pass computes the logits again and rounds their gradient to the
+    tensors' type (fp32: not at all) for the two products that read it.  fp16 keeps it relative to the largest upstream gradient of the call: what
+    is below 2^-28 of that loses bits, below 2^-39 all of them, so that with ``reduction="none"`` a row whose own upstream gradient is far below
+    another's has a coarser gradient than it would have alone (bf16 and fp32: not).
+
+    Memory besides the results, for N rows of width C.  Backward: a copy of the rows (N C elements, of 6 bytes for fp32); of the logits' gradient a piece
+    of the vocabulary of 1 GiB, or of 256 words where that is more; N C sums in fp32 where it is taken in several pieces; sums of a gradient for
+    each part of its product's summation axis where that is split (small products; together up to 2 or 3 GiB for widths above 10000); for fp32, and
+    for weights off the 16-byte grid, up to 1 GiB of weights laid out anew (256 words at least).  Forward: the same copies, and 8 bytes for each row and
+    64 to 256 words of a piece, at most 2 GiB."""
     _check_device(weight)
     r = _reduction(reduction)
     if _tracing():

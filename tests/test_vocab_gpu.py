@@ -381,6 +381,21 @@ def test_upstream_gradients_far_apart_fp16():
         within(dw, *ref["dw"], "dw")
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=names)
+@pytest.mark.parametrize("apart", [2.0 ** -12, 2.0 ** -14])
+def test_small_upstream_gradients_keep_their_bits(dtype, apart):
+    """Gradients of logits of 2^-26 of the largest upstream gradient and above have all of their bits, in fp16 too: rows far below the largest one are held
+    to the bound that they would have in a call of their own."""
+    x, w, t = rand(200, 64, dtype=dtype, seed=41), rand(400, 64, dtype=dtype, seed=42, std=0.03), words(200, 400, 43)
+    g = torch.ones(200, device="cuda")
+    small = torch.arange(0, 200, 2, device="cuda")
+    g[small] *= apart
+    _, lse = moda_amd.linear_cross_entropy_fwd(x, w, t, reduction="none")
+    dx, _ = moda_amd.linear_cross_entropy_bwd(x, w, t, lse, g, reduction="none")
+    assert (x.double() @ w.double().T).softmax(-1).min() > 2.0 ** -12
+    within(dx[small], *loss_reference(x[small], w, t[small], 1.0, -100, "none", g[small])["dx"], "dx")
+
+
 @pytest.mark.parametrize("dtype,n,vocab,width", [(torch.bfloat16, 20000, 60000, 16), (torch.float32, 40, 300000, 1024), (torch.bfloat16, 17000, 50, 24),
                                                  (torch.float16, 17000, 3000, 72)], ids=str)
 def test_many_rows_and_words(dtype, n, vocab, width):
